@@ -384,6 +384,84 @@ int rwkv_f16_gemm_applies(int64_t M, int64_t OUT, int64_t IN, int64_t out_per);
 rwkv_status rwkv_f16_gemm(const void* x, int64_t M, int64_t lda, int64_t x_group_stride, const void* w, void* y,
                           int64_t ldy, int64_t OUT, int64_t IN, int64_t out_per, int epilogue, void* stream);
 
+/* ───────────────────────── training around the recurrence ───────────────────────── */
+/* Layer norm, dense products and their gradients, which the reference leaves
+ * to MLX's autograd (RWKVBlock.swift:163-307 under valueAndGrad), and the
+ * 8-bit checkpoints their backward passes can read.  N and M (rows) may be 0
+ * and are at most 2^24.  A row pitch (ld*) counts elements; buffers without
+ * one are dense. */
+
+/* 8-bit activation checkpoint: MXINT8 of the OCP Microscaling Formats v1.0.
+ * codes int8 [N, W], W = rwkv_act8_width(D) = D rounded up to 32; scales uint8
+ * [N, W/32].  With e = floor(log2 of the group's largest magnitude): scale =
+ * e + 127 (at least 7), code = clamp(rint(x·2^(6-e)), ±127), value =
+ * code·2^(e-6).  A group with an infinity or a NaN has scale 255 and restores
+ * as NaN.  Codes beyond D are 0.  x, y: f32, bf16 or f16; D <= 2^22. */
+int64_t rwkv_act8_width(int64_t D);
+rwkv_status rwkv_act8_pack(const void* x, rwkv_dtype dt, int64_t ldx, int8_t* codes, uint8_t* scales,
+                           int64_t N, int64_t D, void* stream);
+rwkv_status rwkv_act8_unpack(const int8_t* codes, const uint8_t* scales, void* y, rwkv_dtype dt,
+                             int64_t N, int64_t D, void* stream);
+
+/* y = (x − mean)·rstd·w + b over rows of any D <= 65536.  x_dt f32, bf16 or
+ * f16; y_dt the same, or any with x_dt f32; w, b (b may be NULL) f32 or x_dt.
+ * stats [N, 2] fp32 receives (mean, rstd) where not NULL; codes and scales,
+ * both or neither, the 8-bit checkpoint of x.  y must not alias x. */
+rwkv_status rwkv_norm_fwd(const void* x, rwkv_dtype x_dt, int64_t ldx, const void* w, const void* b,
+                          rwkv_dtype w_dt, void* y, rwkv_dtype y_dt, float* stats, int8_t* codes,
+                          uint8_t* scales, int64_t N, int64_t D, float eps, void* stream);
+
+/* Gradients of rwkv_norm_fwd from its stats and either x or the checkpoint
+ * (codes and scales; then x may be NULL): dx [N, D] of x_dt, dw and db [D] of
+ * w_dt.  dx, dw, db may be NULL (db needs dw).  With dw, a workspace of
+ * rwkv_norm_bwd_workspace(N, D) bytes, 16-byte aligned.  The sums' order is
+ * fixed: the same inputs give the same bits. */
+int64_t rwkv_norm_bwd_workspace(int64_t N, int64_t D);
+rwkv_status rwkv_norm_bwd(const void* dy, rwkv_dtype y_dt, const void* x, rwkv_dtype x_dt, int64_t ldx,
+                          const int8_t* codes, const uint8_t* scales, const float* stats, const void* w,
+                          rwkv_dtype w_dt, void* dx, void* dw, void* db, int64_t N, int64_t D,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* act(z): z; relu(z)²; tanh(z); 1/(1 + e^-z). */
+typedef enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_ACT_SIGMOID = 3 } rwkv_activation;
+
+/* y = act(z) + residual, z = x·Wᵀ + bias: x [M, K], w [N, K], bias [N] (may be
+ * NULL) of dt (bf16 or f16); residual [M, N] (pitch ldr, may be NULL) and y
+ * [M, N] of y_dt (dt or f32).  fp32 sums, one rounding.  For the backward
+ * pass, each where not NULL: aux [M, N] of dt receives relu(z), tanh(z),
+ * sigmoid(z) (or z); codes and scales the 8-bit checkpoint of z.  residual may
+ * be y.  N, K <= 2^20, pitches < 2^22.  Some shapes sum ranges of K in the
+ * workspace: rwkv_linear_fwd_workspace(M, N, K) bytes, 16-byte aligned. */
+int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K);
+rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                            const void* residual, int64_t ldr, void* y, rwkv_dtype y_dt, void* aux,
+                            int8_t* codes, uint8_t* scales, rwkv_activation act, rwkv_dtype dt,
+                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
+/* dz = dy·act'(z) [M, ldz] of dt (N <= ldz < N + 8; columns from N on are
+ * written as zeros) and db = Σ_rows dz [N] of dt; either may be NULL.  dy of
+ * dy_dt (dt or f32).  z comes from kept [M, N] (the forward's aux, or with
+ * kept_is_y and relu² its y) or from the checkpoint; neither for RWKV_ACT_NONE.
+ * With db, a workspace of rwkv_linear_dact_workspace(M, N) bytes. */
+int64_t rwkv_linear_dact_workspace(int64_t M, int64_t N);
+rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, const void* kept, int kept_is_y,
+                             const int8_t* codes, const uint8_t* scales, rwkv_activation act, void* dz,
+                             int64_t ldz, void* db, rwkv_dtype dt, int64_t M, int64_t N, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* dx = dz·W [M, K] and dw = dzᵀ·x [N, K] of dt.  A pitch ldz of at least N
+ * rounded up to 8 promises zeros in dz's columns beyond N.  wgrad needs M >= 1.
+ * Workspaces as rwkv_linear_fwd's. */
+int64_t rwkv_linear_dgrad_workspace(int64_t M, int64_t N, int64_t K);
+rwkv_status rwkv_linear_dgrad(const void* dz, int64_t ldz, const void* w, int64_t ldw, void* dx, rwkv_dtype dt,
+                              int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+int64_t rwkv_linear_wgrad_workspace(int64_t M, int64_t N, int64_t K);
+rwkv_status rwkv_linear_wgrad(const void* dz, int64_t ldz, const void* x, int64_t ldx, void* dw, rwkv_dtype dt,
+                              int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
 /* ───────────────────────── x070 decode step around the hot path ───────────────────────── */
 /* fp32 activations; dense vector parameters fp32 (an fp16 file's values
  * widen exactly); low-rank matrices f16 (the reference's `lin` narrowing,

@@ -5,9 +5,10 @@ mirror of the reference's Swift API.
 
     swiftrwkv_amd.kernel     RWKVKernel API (wkv7_sequence_forward, wkv7_train_with_state, ...)
     swiftrwkv_amd.quant      RWKVQuant API (RwkvqSidecar, rwkvq_sb6_gemv, ...)
+    swiftrwkv_amd.train     layer norm, dense products and 8-bit activation checkpoints with gradients
     swiftrwkv_amd.synthetic  seeded inputs / weights of the benchmark shapes
     swiftrwkv_amd.build      builds libswiftrwkv_hip.so in-tree
 """
 from . import _lib  # noqa: F401
 
-__all__ = ["kernel", "quant", "synthetic", "build"]
+__all__ = ["kernel", "quant", "train", "synthetic", "build"]

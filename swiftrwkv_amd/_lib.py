@@ -109,6 +109,20 @@ _SIGS = {
     "rwkv_x070_seq_lora": (I, [P, L, L, P, P, P, P, P, I, L, L, L, L, I, P, P, P, P, P, P]),
     "rwkv_x070_seq_lora_split": (I, [L, L, I, L, L, L, L]),
     "rwkv_sym_gemm": (I, [P, I, L, L, L, P, P, P, P, L, L, L, I, L, I, P, L, P]),
+    "rwkv_act8_width": (L, [L]),
+    "rwkv_act8_pack": (I, [P, I, L, P, P, L, L, P]),
+    "rwkv_act8_unpack": (I, [P, P, P, I, L, L, P]),
+    "rwkv_norm_fwd": (I, [P, I, L, P, P, I, P, I, P, P, P, L, L, F, P]),
+    "rwkv_norm_bwd_workspace": (L, [L, L]),
+    "rwkv_norm_bwd": (I, [P, I, P, I, L, P, P, P, P, I, P, P, P, L, L, P, L, P]),
+    "rwkv_linear_fwd_workspace": (L, [L, L, L]),
+    "rwkv_linear_fwd": (I, [P, L, P, L, P, P, L, P, I, P, P, P, I, I, L, L, L, P, L, P]),
+    "rwkv_linear_dact_workspace": (L, [L, L]),
+    "rwkv_linear_dact": (I, [P, L, I, P, I, P, P, I, P, L, P, I, L, L, P, L, P]),
+    "rwkv_linear_dgrad_workspace": (L, [L, L, L]),
+    "rwkv_linear_dgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
+    "rwkv_linear_wgrad_workspace": (L, [L, L, L]),
+    "rwkv_linear_wgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
     "rwkv_layer_norm": (I, [P, I, P, L, P, P, P, L, L, F, P]),
     "rwkv_x070_seq_shift_mix": (I, [P, P, P, P, P, I, I, P, I, L, L, P, L, L, I, L, L, L, P]),
     "rwkv_x070_seq_tmix_pre": (I, [P] * 10 + [I, P] + [P] * 7 + [L, L, L, P]),

@@ -1,0 +1,117 @@
+// Device helpers of the training-side operators (norm.hip, linear.hip): rows
+// in chunks of 8 values of any element type and alignment, and the 8-bit
+// activation checkpoint (MXINT8 of the OCP Microscaling Formats v1.0
+// specification, written from its definition).
+//
+// A checkpoint of rows [N, D] is codes int8 [N, Dp], Dp = D rounded up to 32,
+// and one scale byte per 32 codes, [N, Dp/32].  With e = floor(log2 amax) of
+// a group (amax the largest magnitude of its 32 values), the scale byte is
+// e + 127 and code = clamp(rint(x·2^(6-e)), ±127): the value it stands for is
+// code·2^(e-6).  The step is a power of two, so x·2^(6-e) and code·2^(e-6)
+// are exact: a code depends on no rounding but rint's own (half a step, 2^-7
+// of 2^e; up to one step where |x| > 127.5 steps clamps, which keeps the
+// largest finite values from restoring as infinity), and a restored value is
+// exact in bf16, whose 8 significant bits hold 7-bit codes.  Scale bytes below
+// 7 are raised to 7, so steps are normal fp32 numbers (groups under 2^-120
+// restore with that step); 255 marks a group that held an infinity or a NaN:
+// all of it restores as NaN.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+namespace rwkv_train {
+
+constexpr int GROUP = 32;   // values per scale
+
+__host__ __device__ inline int64_t padded(int64_t d) { return (d + GROUP - 1) / GROUP * GROUP; }
+
+template <typename T>
+__device__ __forceinline__ float to_f(T x) {
+    return (float)x;
+}
+
+// Eight values from p, valid of them in range (the others 0).  Whole chunks
+// load as 16-byte pieces at whatever alignment p has (gfx950 takes any).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
+    if (valid >= 8) {
+        T raw[8];
+        __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_f(p[i]) : 0.0f;
+    }
+}
+
+// Stores the first `valid` of eight values, each rounded once to T.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
+    if (valid >= 8) {
+        T raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = (T)v[i];
+        __builtin_memcpy(p, raw, sizeof(raw));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) p[i] = (T)v[i];
+    }
+}
+
+// The step 2^(scale - 133) of a scale byte; NaN for 255.
+__device__ __forceinline__ float step_of(uint32_t scale) {
+    return __builtin_bit_cast(float, scale == 255u ? 0x7fc00000u : (scale - 6u) << 23);
+}
+
+// Scale byte of a group whose largest magnitude is amax (infinity: not finite).
+__device__ __forceinline__ uint32_t scale_of(float amax) {
+    return max(__builtin_bit_cast(uint32_t, amax) >> 23, 7u);
+}
+
+// Largest magnitude of eight values; infinity if one is infinite or a NaN.
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(v[i]);
+        m = a <= 3.402823466e38f ? fmaxf(m, a) : __builtin_inff();
+        // (once infinite it stays so: fmaxf(inf, a) = inf)
+    }
+    return m;
+}
+
+// Encodes a group's share of four neighbouring lanes (8 values each, lanes
+// 4q .. 4q+3 in column order): returns the lane's eight codes and the group's
+// scale byte.  Every lane of the quad must be active.
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t& scale) {
+    float m = amax8(v);
+    m = fmaxf(m, __shfl_xor(m, 1));
+    m = fmaxf(m, __shfl_xor(m, 2));
+    scale = scale_of(m);
+    const float inv = __builtin_bit_cast(float, (260u - min(scale, 254u)) << 23);   // 2^(133 - scale)
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float c = fminf(fmaxf(rintf(v[i] * inv), -127.0f), 127.0f);
+        w[i >> 2] |= ((uint32_t)(int)c & 0xffu) << (8 * (i & 3));
+    }
+    if (scale == 255u) w[0] = w[1] = 0u;
+    return make_uint2(w[0], w[1]);
+}
+
+// The eight values of codes c with the group's scale byte.
+__device__ __forceinline__ void decode8(uint2 c, uint32_t scale, float (&v)[8]) {
+    const float step = step_of(scale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t w = i < 4 ? c.x : c.y;
+        v[i] = (float)(int)(int8_t)(w >> (8 * (i & 3))) * step;
+    }
+}
+
+}  // namespace rwkv_train

@@ -1,0 +1,671 @@
+// Dense products with bias, activation and residual in the epilogue, and
+// their gradients, in bf16 and fp16 on the gfx950 matrix cores: the
+// projections and low-rank branches of a block in training
+// (RWKVBlock.swift:163-307) on dense weights.
+//
+//   forward   y  = act(x·Wᵀ + b) + res      x [M, K], W [N, K]
+//   dz        dz = dy·act'(z), db = Σ_rows dz
+//   input     dx = dz·W
+//   weight    dW = dzᵀ·x
+//
+// One kernel template computes C[m, n] = Σ_k A[m, k]·B[n, k] for all three:
+// an operand is either k-contiguous (x and W of the forward pass, dz of the
+// input gradient) or k-major (W of the input gradient, both operands of the
+// weight's), staged in LDS as it lies in memory.  k-contiguous rows are read
+// as 16-byte operands; k-major ones through ds_read_b64_tr_b16, which hands
+// lane i of sixteen the column i of a 4 × 16 block.  Products accumulate in
+// fp32 on v_mfma_f32_16x16x32; the epilogue works on the fp32 sums and rounds
+// once.
+//
+// Operand layout of the 16x16x32 instructions (lane l, g = l >> 4, i = l & 15):
+// A[m = i][k = 8g .. 8g+7], B[k = 8g .. 8g+7][n = i]; D[m = 4g + r][n = i].
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "act8.h"
+#include "launch.h"
+
+namespace {
+
+using namespace rwkv_train;
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int BK = 64;                   // k per stage: two 32-wide products
+constexpr int64_t MAX_LD = (1 << 22) - 8;   // a tile's byte offsets stay under 2^31
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (__is_same(T, bf16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                       c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
+                                                      0, 0, 0);
+}
+
+// ───────────────────────────── epilogue ─────────────────────────────
+
+enum { ACT_NONE = 0, ACT_RELU2 = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
+
+struct Epilogue {
+    const void* bias;     // [N] of the operands' type, or null
+    const void* res;      // [M] rows of pitch ldr, or null
+    int64_t ldr;
+    void* y;              // [M, N]
+    int wide;             // res and y are fp32 (else the operands' type)
+    void* aux;            // [M, N] of the operands' type: relu(z), tanh(z) or σ(z); or null
+    int8_t* codes;        // checkpoint of z, [M, Np]; or null
+    uint8_t* scales;
+    int act;
+    int64_t M;
+    int N;
+};
+
+// Eight neighbouring columns of a row, z without bias in v.  With codes, the
+// four lanes of a 32-column group call it together.
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int col, float (&v)[8]) {
+    const int valid = e.N - col;
+    if (e.bias) {
+        float b[8];
+        load8(reinterpret_cast<const T*>(e.bias) + col, valid, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += b[i];
+    }
+    if (e.codes) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? v[i] : 0.0f;
+        uint32_t scale;
+        const uint2 c = encode8(v, scale);
+        const int64_t np = padded(e.N), at = row * np + col;
+        if (col < np) {
+            *reinterpret_cast<uint2*>(e.codes + at) = c;
+            if ((col & 31) == 0) e.scales[at / GROUP] = (uint8_t)scale;
+        }
+    }
+    float r[8];   // the value aux keeps
+    switch (e.act) {
+        case ACT_RELU2:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                r[i] = v[i] > 0.0f || v[i] != v[i] ? v[i] : 0.0f;   // a NaN stays one
+                v[i] = r[i] * r[i];
+            }
+            break;
+        case ACT_TANH:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = r[i] = tanhf(v[i]);
+            break;
+        case ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = r[i] = 1.0f / (1.0f + __expf(-v[i]));
+            break;
+        default:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = v[i];
+    }
+    const int64_t at = row * e.N + col;
+    if (e.aux) store8(reinterpret_cast<T*>(e.aux) + at, valid, r);
+    if (e.res) {
+        float s[8];
+        if (e.wide)
+            load8(reinterpret_cast<const float*>(e.res) + row * e.ldr + col, valid, s);
+        else
+            load8(reinterpret_cast<const T*>(e.res) + row * e.ldr + col, valid, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += s[i];
+    }
+    if (e.wide)
+        store8(reinterpret_cast<float*>(e.y) + at, valid, v);
+    else
+        store8(reinterpret_cast<T*>(e.y) + at, valid, v);
+}
+
+// ───────────────────────────── operand tiles ─────────────────────────────
+
+// ROWS output rows (or columns) × BK of an operand: how a workgroup loads a
+// stage of it into registers, writes it to LDS and reads operands back.  ODD:
+// rows that are not 16-byte aligned or a k-contiguous length that 8 does not
+// divide; elsewhere buffer loads, whose range check fills what lies outside
+// the operand with zeros.
+template <typename T, bool KM, int ROWS, int THREADS, bool ODD>
+struct Tile {
+    static constexpr int P = ROWS * 8 / THREADS;   // 16-byte chunks per thread and stage
+    static constexpr int CPR = KM ? ROWS / 8 : 8;  // chunks per LDS row
+    static constexpr int STEP = THREADS / CPR;     // LDS rows a thread's chunks are apart
+    static constexpr int BYTES = ROWS * BK * 2;
+    static_assert(P >= 1 && THREADS % CPR == 0, "tile shape");
+
+    const T* p;       // operand, at the tile's first row (k-contiguous) or column (k-major)
+    int64_t ld;
+    int rows;         // rows (columns) from there to the operand's end
+    int K;
+    int c, r;         // the thread's chunk and first LDS row
+
+    __device__ __forceinline__ Tile(const void* base, int64_t ld_, int64_t at, int64_t total, int K_, int tid)
+        : p(reinterpret_cast<const T*>(base) + (KM ? at : at * ld_)), ld(ld_),
+          rows((int)min(total - at, (int64_t)(KM ? (1 << 30) : ROWS))), K(K_), c(tid % CPR), r(tid / CPR) {}
+
+    __device__ __forceinline__ void load(uint4 (&v)[P], int st) const {
+        if constexpr (ODD) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int row = r + STEP * i;
+                const int k = KM ? st * BK + row : st * BK + 8 * c;
+                const int valid = KM ? (k < K ? rows - 8 * c : 0) : (row < rows ? K - k : 0);
+                const T* q = p + (KM ? (int64_t)k * ld + 8 * c : (int64_t)row * ld + k);
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+                if (valid >= 8) {
+                    __builtin_memcpy(w, q, 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 7; ++e)
+                        if (e < valid) w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[e] << (16 * (e & 1));
+                }
+                v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else if constexpr (KM) {
+            const int left = min(BK, K - st * BK);   // rows of this stage
+            // whole dwords: one that holds a last odd column may be read
+            const int cols = (min(rows, ROWS) + 1) & ~1;
+            const int bytes = left > 0 ? (int)(((int64_t)(left - 1) * ld + cols) * 2) : 0;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(p + (left > 0 ? (int64_t)st * BK * ld : 0)), 0, bytes, 0x00020000);
+            const uint32_t o = (uint32_t)(r * (int)ld + 8 * c) * 2, step = (uint32_t)(STEP * (int)ld) * 2;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, o + i * step, 0, 0));
+        } else {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(p), 0, (int)(((int64_t)(rows - 1) * ld + K) * 2), 0x00020000);
+            const int k = st * BK + 8 * c;
+            // past the last k: an offset outside the range (also after the row steps are added)
+            const uint32_t o = k < K ? (uint32_t)(r * (int)ld + k) * 2 : 0x80000000u;
+            const uint32_t step = (uint32_t)(STEP * (int)ld) * 2;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, o + i * step, 0, 0));
+        }
+    }
+
+    // 32-byte slots of a k-major LDS row are permuted by the row, so that the
+    // eight rows a half wave reads at once lie in different banks (rows of
+    // 128 bytes: two rows share the banks' width).
+    static __device__ __forceinline__ int slot_mask(int k) {
+        return ROWS >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+    }
+
+    __device__ __forceinline__ void write(char* lds, const uint4 (&v)[P]) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int row = r + STEP * i;
+            const int at = KM ? row * ROWS * 2 + (((c >> 1) ^ slot_mask(row)) << 5) + ((c & 1) << 4)
+                              : row * 128 + ((c ^ (row & 7)) << 4);
+            *reinterpret_cast<uint4*>(lds + at) = v[i];
+        }
+    }
+
+    // The operand of rows base + 16·tile + i (i = lane & 15), k = 32·kk + 8g ..
+    // 8g + 7; base a multiple of 16.
+    static __device__ __forceinline__ uint4 frag(char* lds, int base, int tile, int kk, int lane) {
+        const int g = lane >> 4, i = lane & 15;
+        if constexpr (KM) {
+            typedef __attribute__((address_space(3))) s16x4* lptr;
+            const int k = 32 * kk + 8 * g + (i >> 2);
+            const int s = slot_mask(k);   // the same for k + 4 (bit 2 takes no part)
+            const int col = (((base >> 4) + tile) ^ s) * 32 + (i & 3) * 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(lds + k * ROWS * 2 + col));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(lds + (k + 4) * ROWS * 2 + col));
+            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(uint4, v);
+        } else {
+            const int row = base + 16 * tile + i;
+            return *reinterpret_cast<const uint4*>(lds + row * 128 + (((4 * kk + g) ^ (row & 7)) << 4));
+        }
+    }
+};
+
+struct GemmArgs {
+    const void* a;
+    int64_t lda;          // k-contiguous: [M][lda]; k-major: [K][lda]
+    const void* b;
+    int64_t ldb;
+    int64_t M;
+    int N, K;
+    int KB;               // rows of a k-major B: K, or less where A's last columns are padding zeros
+    int splits, per;      // K ranges of `per` stages each; > 1: fp32 sums into part [splits][M][N]
+    float* part;
+    Epilogue e;
+};
+
+template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, bool ODD>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void gemm_kernel(GemmArgs g) {
+    constexpr int BM = 16 * WM * AM, BN = 16 * WN * AN, THREADS = 64 * WM * WN;
+    using TileA = Tile<T, AKM, BM, THREADS, ODD>;
+    using TileB = Tile<T, BKM, BN, THREADS, ODD>;
+    constexpr int STAGE = TileA::BYTES + TileB::BYTES;
+    constexpr int EROW = 16 * AN + 4;   // floats per staged row of the epilogue
+    static_assert(WM * WN * 16 * EROW * 4 <= 2 * STAGE, "epilogue staging");
+    __shared__ __align__(16) char lds[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // Tiles in groups of 4 row blocks × every column block, column-major
+    // within a group; XCD x (workgroups x, x + 8, ...) takes a contiguous run
+    // of that order, so its workgroups share operand blocks in its L2.
+    const int ntm = (int)((g.M + BM - 1) / BM), ntn = (g.N + BN - 1) / BN, total = ntm * ntn;
+    const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3;
+    const int t = xcd * (total >> 3) + min(xcd, total & 7) + loc;
+    const int grp = t / (4 * ntn), first = 4 * grp, gm = min(4, ntm - first);
+    const int rr = t - grp * 4 * ntn;
+    const int64_t m0 = (int64_t)(first + rr % gm) * BM;
+    const int n0 = (rr / gm) * BN;
+    const int nst = (g.K + BK - 1) / BK;
+    const int st0 = blockIdx.y * g.per, st1 = min(nst, st0 + g.per);
+
+    const TileA ta(g.a, g.lda, m0, g.M, g.K, tid);
+    const TileB tb(g.b, g.ldb, n0, g.N, g.KB, tid);
+    const int wm = wave % WM, wn = wave / WM;
+    f32x4 acc[AM][AN];
+#pragma unroll
+    for (int i = 0; i < AM; ++i)
+#pragma unroll
+        for (int j = 0; j < AN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    uint4 va[TileA::P], vb[TileB::P];
+    ta.load(va, st0);
+    tb.load(vb, st0);
+    ta.write(lds, va);
+    tb.write(lds + TileA::BYTES, vb);
+    ta.load(va, st0 + 1);
+    tb.load(vb, st0 + 1);
+    __syncthreads();
+    for (int st = st0; st < st1; ++st) {
+        char* cur = lds + ((st - st0) & 1) * STAGE;
+        char* nxt = lds + ((st - st0 + 1) & 1) * STAGE;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            uint4 av[AM], bv[AN];
+#pragma unroll
+            for (int j = 0; j < AN; ++j) bv[j] = TileB::frag(cur + TileA::BYTES, wn * AN * 16, j, kk, lane);
+#pragma unroll
+            for (int i = 0; i < AM; ++i) av[i] = TileA::frag(cur, wm * AM * 16, i, kk, lane);
+            if (kk == 1) {   // the next stage's chunks, then the loads of the one after
+                ta.write(nxt, va);
+                tb.write(nxt + TileA::BYTES, vb);
+                ta.load(va, st + 2);
+                tb.load(vb, st + 2);
+            }
+#pragma unroll
+            for (int i = 0; i < AM; ++i)
+#pragma unroll
+                for (int j = 0; j < AN; ++j) acc[i][j] = mfma<T>(av[i], bv[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+
+    // Epilogue: 16 rows at a time through the wave's own LDS, so that a lane
+    // gets eight neighbouring columns.
+    const int gq = lane >> 4, li = lane & 15;
+    float* stage = reinterpret_cast<float*>(lds) + wave * 16 * EROW;
+    constexpr int LPR = 2 * AN, RPP = 64 / LPR;   // lanes per row, rows per pass
+#pragma unroll
+    for (int i = 0; i < AM; ++i) {
+#pragma unroll
+        for (int j = 0; j < AN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) stage[(4 * gq + q) * EROW + 16 * j + li] = acc[i][j][q];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int ps = 0; ps < 16 / RPP; ++ps) {
+            const int rloc = ps * RPP + lane / LPR, cl = 8 * (lane % LPR);
+            const int64_t row = m0 + (wm * AM + i) * 16 + rloc;
+            const int col = n0 + wn * AN * 16 + cl;
+            if (row >= g.M) continue;
+            float v[8];
+            const float4 lo = *reinterpret_cast<const float4*>(stage + rloc * EROW + cl);
+            const float4 hi = *reinterpret_cast<const float4*>(stage + rloc * EROW + cl + 4);
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+            if (g.splits > 1)
+                store8(g.part + ((int64_t)blockIdx.y * g.M + row) * g.N + col, g.N - col, v);
+            else
+                finish8<T>(g.e, row, col, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Sums the K ranges in order and finishes: a thread per 8 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void split_reduce_kernel(const float* part, int splits, Epilogue e) {
+    const int cpr = (int)(padded(e.N) / 8);
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / cpr;
+    if (row >= e.M) return;   // whole quads: cpr is a multiple of 4
+    const int col = 8 * (int)(i - row * cpr), valid = e.N - col;
+    float v[8] = {};
+    for (int s = 0; s < splits; ++s) {
+        float p[8];
+        load8(part + ((int64_t)s * e.M + row) * e.N + col, valid, p);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += p[k];
+    }
+    finish8<T>(e, row, col, v);
+}
+
+// ───────────────────────────── dz and the bias gradient ─────────────────────────────
+
+struct DactArgs {
+    const void* dy;
+    int64_t lddy;
+    int dy32;
+    const void* kept;       // [M, N]: y = relu(z)² (from_y), or what the forward's aux holds; null: codes or no activation
+    int from_y;
+    const int8_t* codes;    // checkpoint of z
+    const uint8_t* scales;
+    int act;
+    void* dz;               // [M, ldz] or null
+    int64_t ldz;            // >= N; columns from N on are written as zeros
+    float* part;            // [gridDim.y][N] column sums, or null
+    int64_t M;
+    int N;
+};
+
+// dz = dy·act'(z) in chunks of 8 columns: TX chunks across, 256/TX rows down
+// a block, rows strided over gridDim.y.
+template <typename T>
+__global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
+    __shared__ float sums[256 * 8];
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, TY = 256 / TX;
+    const int col = 8 * (blockIdx.x * TX + tx), valid = a.N - col;
+    float s[8] = {};
+    if (col < a.ldz || valid > 0) {
+        for (int64_t row = (int64_t)blockIdx.y * TY + ty; row < a.M; row += (int64_t)gridDim.y * TY) {
+            float d[8];
+            if (a.dy32)
+                load8(reinterpret_cast<const float*>(a.dy) + row * a.lddy + col, valid, d);
+            else
+                load8(reinterpret_cast<const T*>(a.dy) + row * a.lddy + col, valid, d);
+            if (a.act != ACT_NONE) {
+                float z[8];
+                if (a.codes) {
+                    const int64_t at = row * padded(a.N) + col;
+                    if (valid > 0)
+                        decode8(*reinterpret_cast<const uint2*>(a.codes + at), a.scales[at / GROUP], z);
+                    else
+                        for (int i = 0; i < 8; ++i) z[i] = 0.0f;
+                } else {
+                    load8(reinterpret_cast<const T*>(a.kept) + row * a.N + col, valid, z);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float m;
+                    if (a.act == ACT_RELU2) {
+                        const float r = a.from_y ? sqrtf(z[i]) : (z[i] > 0.0f || z[i] != z[i] ? z[i] : 0.0f);
+                        m = 2.0f * r;
+                    } else if (a.act == ACT_TANH) {
+                        const float h = a.codes ? tanhf(z[i]) : z[i];
+                        m = 1.0f - h * h;
+                    } else {
+                        const float h = a.codes ? 1.0f / (1.0f + __expf(-z[i])) : z[i];
+                        m = h * (1.0f - h);
+                    }
+                    d[i] = i < valid ? d[i] * m : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += d[i];
+            if (a.dz) store8(reinterpret_cast<T*>(a.dz) + row * a.ldz + col, (int)min(a.ldz - col, (int64_t)8), d);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[i * 256 + threadIdx.x] = s[i];
+    __syncthreads();
+    if (ty != 0) return;
+    for (int r = 1; r < TY; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] += sums[i * 256 + r * TX + tx];
+    if (valid > 0) store8(a.part + (int64_t)blockIdx.y * a.N + col, valid, s);
+}
+
+// Column sums of part [G][N], in order within 16 interleaved runs of rows.
+template <typename T>
+__global__ __launch_bounds__(256) void bias_reduce_kernel(const float* part, int G, int N, T* out) {
+    __shared__ float s[16][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const int col = blockIdx.x * 16 + c;
+    float t = 0.0f;
+    if (col < N) {
+#pragma unroll 8
+        for (int g = r; g < G; g += 16) t += part[(int64_t)g * N + col];
+    }
+    s[r][c] = t;
+    __syncthreads();
+    if (r != 0 || col >= N) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += s[i][c];
+    out[col] = (T)sum;
+}
+
+rwkv_status status_of(const char* what) {
+    const hipError_t e = hipGetLastError();
+    RWKV_REQUIRE(e == hipSuccess, RWKV_E_HIP, "%s: %s", what, hipGetErrorString(e));
+    return RWKV_OK;
+}
+
+// ───────────────────────────── routes ─────────────────────────────
+
+struct Route {
+    int tile;       // output tile edge
+    int splits, per;
+};
+
+int64_t tiles_of(int64_t M, int64_t N, int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); }
+
+Route route_of(int64_t M, int64_t N, int64_t K, bool odd) {
+    const int nst = (int)((K + BK - 1) / BK);
+    Route r{64, 1, nst};
+    if (!odd && tiles_of(M, N, 256) >= 200) r.tile = 256;
+    else if (tiles_of(M, N, 128) >= 200) r.tile = 128;
+    const int64_t tiles = tiles_of(M, N, r.tile);
+    int s = 1;
+    if (tiles < 256) s = (int)std::min<int64_t>(std::min<int64_t>(512 / tiles, (nst + 3) / 4), 32);
+    if (s > 1) {
+        r.per = (nst + s - 1) / s;
+        r.splits = (nst + r.per - 1) / r.per;
+    }
+    return r;
+}
+
+int64_t route_workspace(const Route& r, int64_t M, int64_t N) {
+    return r.splits > 1 ? (int64_t)r.splits * M * N * 4 : 0;
+}
+
+template <typename T, bool AKM, bool BKM, bool ODD>
+void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)tiles_of(g.M, g.N, r.tile), (unsigned)r.splits);
+    if constexpr (!ODD) {
+        if (r.tile == 256) {
+            rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 4, 8, 4, ODD>, grid, dim3(512), s, g);
+            return;
+        }
+    }
+    if (r.tile == 128)
+        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 4, 4, ODD>, grid, dim3(256), s, g);
+    else
+        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 2, 2, ODD>, grid, dim3(256), s, g);
+}
+
+// C = A·Bᵀ by the route of its sizes, then the epilogue.
+rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, void* workspace, int64_t bytes,
+                     hipStream_t s) {
+    const bool aligned = (uintptr_t)g.a % 16 == 0 && (uintptr_t)g.b % 16 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0;
+    const bool odd = !aligned || ((!akm || !bkm) && g.K % 8 != 0);
+    const Route r = route_of(g.M, g.N, g.K, odd);
+    RWKV_REQUIRE(tiles_of(g.M, g.N, r.tile) < (int64_t(1) << 31), RWKV_E_SHAPE, "%s: too many output tiles", what);
+    const int64_t need = route_workspace(r, g.M, g.N);
+    RWKV_REQUIRE(need == 0 || (workspace && bytes >= need && (uintptr_t)workspace % 16 == 0), RWKV_E_SHAPE,
+                 "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need);
+    g.splits = r.splits;
+    g.per = r.per;
+    g.part = r.splits > 1 ? (float*)workspace : nullptr;
+    auto by_layout = [&](auto type, auto o) {
+        using T = decltype(type);
+        constexpr bool O = decltype(o)::value;
+        if (!akm && !bkm) gemm_launch_tile<T, false, false, O>(r, g, s);
+        else if (!akm) gemm_launch_tile<T, false, true, O>(r, g, s);
+        else gemm_launch_tile<T, true, true, O>(r, g, s);
+        if (r.splits > 1) {
+            const int64_t chunks = g.M * (padded(g.N) / 8);
+            rwkv::launch(split_reduce_kernel<T>, dim3((unsigned)((chunks + 255) / 256)), dim3(256), s, g.part, r.splits,
+                         g.e);
+        }
+    };
+    if (dt == RWKV_BF16 && odd) by_layout(bf16{}, std::true_type{});
+    else if (dt == RWKV_BF16) by_layout(bf16{}, std::false_type{});
+    else if (odd) by_layout(f16{}, std::true_type{});
+    else by_layout(f16{}, std::false_type{});
+    return status_of(what);
+}
+
+// For either kind of alignment (the pointers are not known yet).
+int64_t gemm_workspace(int64_t M, int64_t N, int64_t K) {
+    if (M == 0) return 0;
+    return std::max(route_workspace(route_of(M, N, K, false), M, N), route_workspace(route_of(M, N, K, true), M, N));
+}
+
+bool shape_ok(int64_t M, int64_t N, int64_t K) {
+    return M >= 0 && M <= (1 << 24) && N >= 1 && N <= (1 << 20) && K >= 1 && K <= (1 << 20);
+}
+bool half_ok(int dt) { return dt == RWKV_BF16 || dt == RWKV_F16; }
+bool ld_ok(int64_t ld, int64_t cols) { return ld >= cols && ld <= MAX_LD; }
+
+// Blocks down the rows of dact_kernel (each adds one partial row of db).
+void dact_geometry(int64_t M, int64_t N, int& TX, int& gx, int& gy) {
+    const int64_t chunks = (N + 7) / 8;
+    TX = 1;
+    while (TX < 64 && TX < chunks) TX *= 2;
+    gx = (int)((chunks + TX - 1) / TX);
+    const int ty = 256 / TX;
+    gy = (int)std::max<int64_t>(1, std::min<int64_t>((M + ty - 1) / ty, std::max(1, 2048 / gx)));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K) {
+    return shape_ok(M, N, K) ? gemm_workspace(M, N, K) : 0;
+}
+
+rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                            const void* residual, int64_t ldr, void* y, rwkv_dtype y_dt, void* aux, int8_t* codes,
+                            uint8_t* scales, rwkv_activation act, rwkv_dtype dt, int64_t M, int64_t N, int64_t K,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+    RWKV_REQUIRE(half_ok(dt) && (y_dt == dt || y_dt == RWKV_F32), RWKV_E_DTYPE, "linear_fwd: types %d, output %d",
+                 (int)dt, (int)y_dt);
+    RWKV_REQUIRE(act >= 0 && act <= ACT_SIGMOID, RWKV_E_UNSUPPORTED, "linear_fwd: activation %d", (int)act);
+    RWKV_REQUIRE(shape_ok(M, N, K) && ld_ok(ldx, K) && ld_ok(ldw, K) && (!residual || ldr >= N), RWKV_E_SHAPE,
+                 "linear_fwd: M=%lld N=%lld K=%lld ldx=%lld ldw=%lld ldr=%lld", (long long)M, (long long)N,
+                 (long long)K, (long long)ldx, (long long)ldw, (long long)ldr);
+    RWKV_REQUIRE(M == 0 || (x && w && y), RWKV_E_NULL, "linear_fwd: null buffer");
+    RWKV_REQUIRE(!codes == !scales, RWKV_E_NULL, "linear_fwd: codes and scales go together");
+    if (M == 0) return RWKV_OK;
+    GemmArgs g{};
+    g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)N, g.K = g.KB = (int)K;
+    g.e = Epilogue{bias, residual, ldr, y, y_dt == RWKV_F32, aux, codes, scales, (int)act, M, (int)N};
+    return gemm_run("linear_fwd", false, false, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int64_t rwkv_linear_dact_workspace(int64_t M, int64_t N) {
+    if (!shape_ok(M, N, 1)) return 0;
+    int TX, gx, gy;
+    dact_geometry(M, N, TX, gx, gy);
+    return (int64_t)gy * N * 4;
+}
+
+rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, const void* kept, int kept_is_y,
+                             const int8_t* codes, const uint8_t* scales, rwkv_activation act, void* dz, int64_t ldz,
+                             void* db, rwkv_dtype dt, int64_t M, int64_t N, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+    RWKV_REQUIRE(half_ok(dt) && (dy_dt == dt || dy_dt == RWKV_F32), RWKV_E_DTYPE, "linear_dact: types %d, dy %d",
+                 (int)dt, (int)dy_dt);
+    RWKV_REQUIRE(act >= 0 && act <= ACT_SIGMOID && (!kept_is_y || act == ACT_RELU2), RWKV_E_UNSUPPORTED,
+                 "linear_dact: activation %d, kept_is_y %d", (int)act, kept_is_y);
+    RWKV_REQUIRE(shape_ok(M, N, 1) && lddy >= N && (!dz || (ldz >= N && ldz < N + 8)), RWKV_E_SHAPE,
+                 "linear_dact: M=%lld N=%lld lddy=%lld ldz=%lld", (long long)M, (long long)N, (long long)lddy,
+                 (long long)ldz);
+    RWKV_REQUIRE(!codes == !scales && !(codes && kept), RWKV_E_NULL,
+                 "linear_dact: codes and scales go together, without kept");
+    RWKV_REQUIRE(M == 0 || (dy && (act == ACT_NONE || kept || codes)), RWKV_E_NULL, "linear_dact: null buffer");
+    int TX, gx, gy;
+    dact_geometry(M, N, TX, gx, gy);
+    RWKV_REQUIRE(!db || (workspace && workspace_bytes >= (int64_t)gy * N * 4 && (uintptr_t)workspace % 16 == 0),
+                 RWKV_E_SHAPE, "linear_dact: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                 (long long)gy * N * 4);
+    if (!db && !dz) return RWKV_OK;
+    const hipStream_t s = (hipStream_t)stream;
+    const DactArgs a{dy, lddy, dy_dt == RWKV_F32, kept, kept_is_y, codes, scales, (int)act, dz, dz ? ldz : N,
+                     db ? (float*)workspace : nullptr, M, (int)N};
+    const dim3 grid((unsigned)gx, (unsigned)gy), bgrid((unsigned)((N + 15) / 16));
+    if (dt == RWKV_BF16) {
+        rwkv::launch(dact_kernel<bf16>, grid, dim3(256), s, a, TX);
+        if (db) rwkv::launch(bias_reduce_kernel<bf16>, bgrid, dim3(256), s, (const float*)workspace, gy, (int)N, (bf16*)db);
+    } else {
+        rwkv::launch(dact_kernel<f16>, grid, dim3(256), s, a, TX);
+        if (db) rwkv::launch(bias_reduce_kernel<f16>, bgrid, dim3(256), s, (const float*)workspace, gy, (int)N, (f16*)db);
+    }
+    return status_of("linear_dact launch");
+}
+
+int64_t rwkv_linear_dgrad_workspace(int64_t M, int64_t N, int64_t K) {
+    return shape_ok(M, N, K) ? gemm_workspace(M, K, N) : 0;
+}
+
+rwkv_status rwkv_linear_dgrad(const void* dz, int64_t ldz, const void* w, int64_t ldw, void* dx, rwkv_dtype dt,
+                              int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+    RWKV_REQUIRE(half_ok(dt), RWKV_E_DTYPE, "linear_dgrad: dtype %d", (int)dt);
+    RWKV_REQUIRE(shape_ok(M, N, K) && ld_ok(ldz, N) && ld_ok(ldw, K), RWKV_E_SHAPE,
+                 "linear_dgrad: M=%lld N=%lld K=%lld ldz=%lld ldw=%lld", (long long)M, (long long)N, (long long)K,
+                 (long long)ldz, (long long)ldw);
+    RWKV_REQUIRE(M == 0 || (dz && w && dx), RWKV_E_NULL, "linear_dgrad: null buffer");
+    if (M == 0) return RWKV_OK;
+    GemmArgs g{};
+    // the pitch's columns beyond N hold zeros (rwkv_linear_dact writes them),
+    // and W has no rows there: contract over the multiple of 8
+    const int64_t kk = ldz >= (N + 7) / 8 * 8 ? (N + 7) / 8 * 8 : N;
+    g.a = dz, g.lda = ldz, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)K, g.K = (int)kk, g.KB = (int)N;
+    g.e = Epilogue{nullptr, nullptr, 0, dx, 0, nullptr, nullptr, nullptr, ACT_NONE, M, (int)K};
+    return gemm_run("linear_dgrad", false, true, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int64_t rwkv_linear_wgrad_workspace(int64_t M, int64_t N, int64_t K) {
+    return shape_ok(M, N, K) && M > 0 ? gemm_workspace(N, K, M) : 0;
+}
+
+rwkv_status rwkv_linear_wgrad(const void* dz, int64_t ldz, const void* x, int64_t ldx, void* dw, rwkv_dtype dt,
+                              int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+    RWKV_REQUIRE(half_ok(dt), RWKV_E_DTYPE, "linear_wgrad: dtype %d", (int)dt);
+    RWKV_REQUIRE(shape_ok(M, N, K) && M >= 1 && ld_ok(ldz, N) && ld_ok(ldx, K), RWKV_E_SHAPE,
+                 "linear_wgrad: M=%lld N=%lld K=%lld ldz=%lld ldx=%lld", (long long)M, (long long)N, (long long)K,
+                 (long long)ldz, (long long)ldx);
+    RWKV_REQUIRE(dz && x && dw, RWKV_E_NULL, "linear_wgrad: null buffer");
+    GemmArgs g{};
+    g.a = dz, g.lda = ldz, g.b = x, g.ldb = ldx, g.M = N, g.N = (int)K, g.K = g.KB = (int)M;
+    g.e = Epilogue{nullptr, nullptr, 0, dw, 0, nullptr, nullptr, nullptr, ACT_NONE, N, (int)K};
+    return gemm_run("linear_wgrad", true, true, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"
