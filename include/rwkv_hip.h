@@ -429,26 +429,27 @@ typedef enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_AC
  * NULL) of dt (bf16 or f16); residual [M, N] (pitch ldr, may be NULL) and y
  * [M, N] of y_dt (dt or f32).  fp32 sums, one rounding.  For the backward
  * pass, each where not NULL: aux [M, N] of dt receives relu(z), tanh(z),
- * sigmoid(z) (or z); codes and scales the 8-bit checkpoint of z.  residual may
- * be y.  N, K <= 2^20, pitches < 2^22.  Some shapes sum ranges of K in the
+ * sigmoid(z) (or z); rem [M, N] the next 8 bits of aux, without aux of a y of
+ * dt without residual; codes and scales the 8-bit checkpoint of z.  aux needs
+ * rem.  residual may be y.  N, K <= 2^20, pitches < 2^22.  Some shapes sum ranges of K in the
  * workspace: rwkv_linear_fwd_workspace(M, N, K) bytes, 16-byte aligned. */
 int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K);
 rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                             const void* residual, int64_t ldr, void* y, rwkv_dtype y_dt, void* aux,
-                            int8_t* codes, uint8_t* scales, rwkv_activation act, rwkv_dtype dt,
+                            uint8_t* rem, int8_t* codes, uint8_t* scales, rwkv_activation act, rwkv_dtype dt,
                             int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                             void* stream);
 
 /* dz = dy·act'(z) [M, ldz] of dt (N <= ldz < N + 8; columns from N on are
  * written as zeros) and db = Σ_rows dz [N] of dt; either may be NULL.  dy of
  * dy_dt (dt or f32).  z comes from kept [M, N] (the forward's aux, or with
- * kept_is_y and relu² its y) or from the checkpoint; neither for RWKV_ACT_NONE.
+ * kept_is_y and relu² its y) and rem, its remainders, or from the checkpoint; neither for RWKV_ACT_NONE.
  * With db, a workspace of rwkv_linear_dact_workspace(M, N) bytes. */
 int64_t rwkv_linear_dact_workspace(int64_t M, int64_t N);
-rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, const void* kept, int kept_is_y,
-                             const int8_t* codes, const uint8_t* scales, rwkv_activation act, void* dz,
-                             int64_t ldz, void* db, rwkv_dtype dt, int64_t M, int64_t N, void* workspace,
-                             int64_t workspace_bytes, void* stream);
+rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, const void* kept,
+                             const uint8_t* rem, int kept_is_y, const int8_t* codes, const uint8_t* scales,
+                             rwkv_activation act, void* dz, int64_t ldz, void* db, rwkv_dtype dt, int64_t M,
+                             int64_t N, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* dx = dz·W [M, K] and dw = dzᵀ·x [N, K] of dt.  A pitch ldz of at least N
  * rounded up to 8 promises zeros in dz's columns beyond N.  wgrad needs M >= 1.

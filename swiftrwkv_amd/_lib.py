@@ -116,9 +116,9 @@ _SIGS = {
     "rwkv_norm_bwd_workspace": (L, [L, L]),
     "rwkv_norm_bwd": (I, [P, I, P, I, L, P, P, P, P, I, P, P, P, L, L, P, L, P]),
     "rwkv_linear_fwd_workspace": (L, [L, L, L]),
-    "rwkv_linear_fwd": (I, [P, L, P, L, P, P, L, P, I, P, P, P, I, I, L, L, L, P, L, P]),
+    "rwkv_linear_fwd": (I, [P, L, P, L, P, P, L, P, I, P, P, P, P, I, I, L, L, L, P, L, P]),
     "rwkv_linear_dact_workspace": (L, [L, L]),
-    "rwkv_linear_dact": (I, [P, L, I, P, I, P, P, I, P, L, P, I, L, L, P, L, P]),
+    "rwkv_linear_dact": (I, [P, L, I, P, P, I, P, P, I, P, L, P, I, L, L, P, L, P]),
     "rwkv_linear_dgrad_workspace": (L, [L, L, L]),
     "rwkv_linear_dgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
     "rwkv_linear_wgrad_workspace": (L, [L, L, L]),

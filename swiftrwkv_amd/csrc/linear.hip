@@ -56,6 +56,42 @@ __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
 
 enum { ACT_NONE = 0, ACT_RELU2 = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
 
+// What the forward pass keeps of an activation has 8 bits more than the 16 of
+// its type: the backward pass takes 1 − h² and the like from it, where 16 bits
+// alone would cost more than the rounding of dz does.  v and its rounding a
+// are neighbours in the order of fp32 bit patterns, so the difference of the
+// patterns, rounded to its upper 8 bits (a few at the type's subnormals
+// clamp), is what a lacks: 16 (bf16) or 18 (fp16) bits in all.
+template <typename T>
+__device__ __forceinline__ uint32_t rem_of(float v, T a) {
+    constexpr int SH = __is_same(T, bf16) ? 8 : 5;
+    const float f = (float)a;
+    const int d = (int)(__builtin_bit_cast(uint32_t, v) - __builtin_bit_cast(uint32_t, f));
+    const int q = min(max((d + (1 << (SH - 1))) >> SH, -128), 127);
+    return fabsf(f) <= 3.402823466e38f ? (uint32_t)q & 0xffu : 0u;
+}
+
+template <typename T>
+__device__ __forceinline__ float with_rem(float a, uint32_t rem) {
+    constexpr int SH = __is_same(T, bf16) ? 8 : 5;
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) + (uint32_t)((int)(int8_t)rem * (1 << SH)));
+}
+
+// Remainders of eight values, valid of them stored.
+template <typename T>
+__device__ __forceinline__ void store_rem8(uint8_t* p, int valid, const float (&v)[8]) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= rem_of(v[i], (T)v[i]) << (8 * (i & 3));
+    if (valid >= 8) {
+        __builtin_memcpy(p, w, 8);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+}
+
 struct Epilogue {
     const void* bias;     // [N] of the operands' type, or null
     const void* res;      // [M] rows of pitch ldr, or null
@@ -63,6 +99,7 @@ struct Epilogue {
     void* y;              // [M, N]
     int wide;             // res and y are fp32 (else the operands' type)
     void* aux;            // [M, N] of the operands' type: relu(z), tanh(z) or σ(z); or null
+    uint8_t* rem;         // [M, N]: the next 8 bits of aux, without aux of y; or null
     int8_t* codes;        // checkpoint of z, [M, Np]; or null
     uint8_t* scales;
     int act;
@@ -115,6 +152,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int col,
     }
     const int64_t at = row * e.N + col;
     if (e.aux) store8(reinterpret_cast<T*>(e.aux) + at, valid, r);
+    if (e.rem) store_rem8<T>(e.rem + at, valid, e.aux ? r : v);
     if (e.res) {
         float s[8];
         if (e.wide)
@@ -363,11 +401,27 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const float* part, in
 
 // ───────────────────────────── dz and the bias gradient ─────────────────────────────
 
+// Adds the remainders of eight values.
+template <typename T>
+__device__ __forceinline__ void load_rem8(const uint8_t* p, int valid, float (&v)[8]) {
+    uint32_t w[2] = {0u, 0u};
+    if (valid >= 8) {
+        __builtin_memcpy(w, p, 8);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = with_rem<T>(v[i], (w[i >> 2] >> (8 * (i & 3))) & 0xffu);
+}
+
 struct DactArgs {
     const void* dy;
     int64_t lddy;
     int dy32;
     const void* kept;       // [M, N]: y = relu(z)² (from_y), or what the forward's aux holds; null: codes or no activation
+    const uint8_t* rem;     // [M, N]: its next 8 bits
     int from_y;
     const int8_t* codes;    // checkpoint of z
     const uint8_t* scales;
@@ -404,6 +458,7 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
                         for (int i = 0; i < 8; ++i) z[i] = 0.0f;
                 } else {
                     load8(reinterpret_cast<const T*>(a.kept) + row * a.N + col, valid, z);
+                    load_rem8<T>(a.rem + row * a.N + col, valid, z);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -569,8 +624,8 @@ int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K) {
 }
 
 rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
-                            const void* residual, int64_t ldr, void* y, rwkv_dtype y_dt, void* aux, int8_t* codes,
-                            uint8_t* scales, rwkv_activation act, rwkv_dtype dt, int64_t M, int64_t N, int64_t K,
+                            const void* residual, int64_t ldr, void* y, rwkv_dtype y_dt, void* aux, uint8_t* rem,
+                            int8_t* codes, uint8_t* scales, rwkv_activation act, rwkv_dtype dt, int64_t M, int64_t N, int64_t K,
                             void* workspace, int64_t workspace_bytes, void* stream) {
     RWKV_REQUIRE(half_ok(dt) && (y_dt == dt || y_dt == RWKV_F32), RWKV_E_DTYPE, "linear_fwd: types %d, output %d",
                  (int)dt, (int)y_dt);
@@ -580,10 +635,13 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
                  (long long)K, (long long)ldx, (long long)ldw, (long long)ldr);
     RWKV_REQUIRE(M == 0 || (x && w && y), RWKV_E_NULL, "linear_fwd: null buffer");
     RWKV_REQUIRE(!codes == !scales, RWKV_E_NULL, "linear_fwd: codes and scales go together");
+    RWKV_REQUIRE(!aux || rem, RWKV_E_NULL, "linear_fwd: aux without its remainders");
+    RWKV_REQUIRE(!rem || aux || (y_dt == dt && !residual), RWKV_E_UNSUPPORTED,
+                 "linear_fwd: remainders of a y of another type, or with a residual in it");
     if (M == 0) return RWKV_OK;
     GemmArgs g{};
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)N, g.K = g.KB = (int)K;
-    g.e = Epilogue{bias, residual, ldr, y, y_dt == RWKV_F32, aux, codes, scales, (int)act, M, (int)N};
+    g.e = Epilogue{bias, residual, ldr, y, y_dt == RWKV_F32, aux, rem, codes, scales, (int)act, M, (int)N};
     return gemm_run("linear_fwd", false, false, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -594,9 +652,9 @@ int64_t rwkv_linear_dact_workspace(int64_t M, int64_t N) {
     return (int64_t)gy * N * 4;
 }
 
-rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, const void* kept, int kept_is_y,
-                             const int8_t* codes, const uint8_t* scales, rwkv_activation act, void* dz, int64_t ldz,
-                             void* db, rwkv_dtype dt, int64_t M, int64_t N, void* workspace, int64_t workspace_bytes,
+rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, const void* kept,
+                             const uint8_t* rem, int kept_is_y, const int8_t* codes, const uint8_t* scales,
+                             rwkv_activation act, void* dz, int64_t ldz, void* db, rwkv_dtype dt, int64_t M, int64_t N, void* workspace, int64_t workspace_bytes,
                              void* stream) {
     RWKV_REQUIRE(half_ok(dt) && (dy_dt == dt || dy_dt == RWKV_F32), RWKV_E_DTYPE, "linear_dact: types %d, dy %d",
                  (int)dt, (int)dy_dt);
@@ -607,6 +665,7 @@ rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, con
                  (long long)ldz);
     RWKV_REQUIRE(!codes == !scales && !(codes && kept), RWKV_E_NULL,
                  "linear_dact: codes and scales go together, without kept");
+    RWKV_REQUIRE(!kept == !rem, RWKV_E_NULL, "linear_dact: kept and its remainders go together");
     RWKV_REQUIRE(M == 0 || (dy && (act == ACT_NONE || kept || codes)), RWKV_E_NULL, "linear_dact: null buffer");
     int TX, gx, gy;
     dact_geometry(M, N, TX, gx, gy);
@@ -615,7 +674,7 @@ rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, con
                  (long long)gy * N * 4);
     if (!db && !dz) return RWKV_OK;
     const hipStream_t s = (hipStream_t)stream;
-    const DactArgs a{dy, lddy, dy_dt == RWKV_F32, kept, kept_is_y, codes, scales, (int)act, dz, dz ? ldz : N,
+    const DactArgs a{dy, lddy, dy_dt == RWKV_F32, kept, rem, kept_is_y, codes, scales, (int)act, dz, dz ? ldz : N,
                      db ? (float*)workspace : nullptr, M, (int)N};
     const dim3 grid((unsigned)gx, (unsigned)gy), bgrid((unsigned)((N + 15) / 16));
     if (dt == RWKV_BF16) {
@@ -646,7 +705,7 @@ rwkv_status rwkv_linear_dgrad(const void* dz, int64_t ldz, const void* w, int64_
     // and W has no rows there: contract over the multiple of 8
     const int64_t kk = ldz >= (N + 7) / 8 * 8 ? (N + 7) / 8 * 8 : N;
     g.a = dz, g.lda = ldz, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)K, g.K = (int)kk, g.KB = (int)N;
-    g.e = Epilogue{nullptr, nullptr, 0, dx, 0, nullptr, nullptr, nullptr, ACT_NONE, M, (int)K};
+    g.e = Epilogue{nullptr, nullptr, 0, dx, 0, nullptr, nullptr, nullptr, nullptr, ACT_NONE, M, (int)K};
     return gemm_run("linear_dgrad", false, true, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -664,7 +723,7 @@ rwkv_status rwkv_linear_wgrad(const void* dz, int64_t ldz, const void* x, int64_
     RWKV_REQUIRE(dz && x && dw, RWKV_E_NULL, "linear_wgrad: null buffer");
     GemmArgs g{};
     g.a = dz, g.lda = ldz, g.b = x, g.ldb = ldx, g.M = N, g.N = (int)K, g.K = g.KB = (int)M;
-    g.e = Epilogue{nullptr, nullptr, 0, dw, 0, nullptr, nullptr, nullptr, ACT_NONE, N, (int)K};
+    g.e = Epilogue{nullptr, nullptr, 0, dw, 0, nullptr, nullptr, nullptr, nullptr, ACT_NONE, N, (int)K};
     return gemm_run("linear_wgrad", true, true, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
 }
 

@@ -417,6 +417,28 @@ def test_streams_and_repeats():
     assert all(torch.equal(p, q) for p, q in zip(here, there))
 
 
+def test_what_autograd_refuses():
+    case("norm and linear: gradients of gradients, a kept tensor changed in place, a second backward pass")
+    g = gen(14)
+    x = randn(g, 6, 64, dtype=BF).requires_grad_(True)
+    w, lw = randn(g, 32, 64, dtype=BF).requires_grad_(True), torch.ones(64, device=DEV)
+    for f in (lambda: train.layer_norm(x, lw), lambda: train.linear(x, w, activation="tanh")):
+        y = f()
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+        with pytest.raises(RuntimeError, match="gradients of its gradients"):
+            torch.autograd.grad(dx.float().sum(), x)
+        y = f()
+        y.backward(torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="second time"):
+            y.backward(torch.ones_like(y))
+    y = train.linear(x, w, activation="tanh")
+    with torch.no_grad():
+        y.mul_(2)                            # tanh's gradient reads y
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape
+
+
 def test_forward_in_a_graph():
     case("norm, linear and checkpoint captured into a graph, replayed between eager work")
     g = gen(13)

@@ -55,7 +55,7 @@ def test_norm_entries_refuse():
 def test_linear_entries_refuse():
     lib = _lib.lib()
     fwd = lambda **k: [k.get("x", D), k.get("ldx", 8), D, k.get("ldw", 8), None, k.get("res"), k.get("ldr", 0), D,  # noqa: E731
-                       k.get("ydt", 1), None, k.get("codes"), None, k.get("act", 0), k.get("dt", 1), k.get("M", 2),
+                       k.get("ydt", 1), k.get("aux"), k.get("rem"), k.get("codes"), None, k.get("act", 0), k.get("dt", 1), k.get("M", 2),
                        k.get("N", 4), k.get("K", 8), k.get("ws"), k.get("wsn", 0), None]
     refused(DTYPE, "rwkv_linear_fwd", *fwd(dt=0, ydt=0))
     refused(DTYPE, "rwkv_linear_fwd", *fwd(ydt=2))
@@ -68,6 +68,9 @@ def test_linear_entries_refuse():
     refused(SHAPE, "rwkv_linear_fwd", *fwd(res=D, ldr=3))
     refused(NULL, "rwkv_linear_fwd", *fwd(x=None))
     refused(NULL, "rwkv_linear_fwd", *fwd(codes=D))
+    refused(NULL, "rwkv_linear_fwd", *fwd(aux=D))            # without remainders
+    refused(UNSUP, "rwkv_linear_fwd", *fwd(rem=D, ydt=0))    # remainders of an fp32 y
+    refused(UNSUP, "rwkv_linear_fwd", *fwd(rem=D, res=D, ldr=4))
     refused(0, "rwkv_linear_fwd", *fwd(M=0, x=None))
     # a shape that sums ranges of K refuses a workspace that is short
     M, N, K = 256, 64, 16384
@@ -80,9 +83,10 @@ def test_linear_entries_refuse():
         refused(NULL, entry, None, 8, D, 8, D, 1, 8, 8, 8, None, 0, None)
     refused(SHAPE, "rwkv_linear_wgrad", D, 8, D, 8, D, 1, 0, 8, 8, None, 0, None)   # no rows to sum
     refused(SHAPE, "rwkv_linear_wgrad", D, M, D, N, D, 1, K, M, N, D, need // 2 - 4, None)
-    dact = lambda **k: [D, k.get("ld", 8), k.get("dydt", 1), k.get("kept"), k.get("isy", 0), k.get("codes"), k.get("scales"),  # noqa: E731
+    dact = lambda **k: [D, k.get("ld", 8), k.get("dydt", 1), k.get("kept"), k.get("rem", k.get("kept")), k.get("isy", 0), k.get("codes"), k.get("scales"),  # noqa: E731
                         k.get("act", 0), D, k.get("ldz", 8), k.get("db"), 1, 2, 8, None, 0, None]
     refused(NULL, "rwkv_linear_dact", *dact(act=1))                      # nothing kept
+    refused(NULL, "rwkv_linear_dact", *dact(act=1, kept=D, rem=None))
     refused(NULL, "rwkv_linear_dact", *dact(act=1, kept=D, codes=D, scales=D))
     refused(UNSUP, "rwkv_linear_dact", *dact(act=2, kept=D, isy=1))
     refused(SHAPE, "rwkv_linear_dact", *dact(ldz=16))
