@@ -105,6 +105,7 @@ struct Epilogue {
     int act;
     int64_t M;
     int N;
+    bool plain;           // y alone, of the operands' type
 };
 
 // Eight neighbouring columns of a row, z without bias in v.  With codes, the
@@ -285,14 +286,53 @@ struct GemmArgs {
     Epilogue e;
 };
 
+// A wave's 16·AM × 16·AN products, RC row tiles at a time through its own
+// 16·RC · EROW floats of LDS, so that a lane gets eight neighbouring columns.
+template <int AN>
+constexpr int EROW = 16 * AN + 4;   // floats per staged row
+
+template <typename T, int AM, int AN, int RC>
+__device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc)[AM][AN], float* stage, int64_t row0,
+                                            int col0, int lane) {
+    static_assert(AM % RC == 0, "row tiles per pass");
+    constexpr int LPR = 2 * AN, RPP = 64 / LPR;   // lanes per row, rows per step
+    const int gq = lane >> 4, li = lane & 15;
+    const int cl = 8 * (lane % LPR), col = col0 + cl;
+#pragma unroll
+    for (int h = 0; h < AM / RC; ++h) {
+#pragma unroll
+        for (int i = 0; i < RC; ++i)
+#pragma unroll
+            for (int j = 0; j < AN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    stage[(16 * i + 4 * gq + q) * EROW<AN> + 16 * j + li] = acc[h * RC + i][j][q];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int rloc = lane / LPR; rloc < 16 * RC; rloc += RPP) {
+            const int64_t row = row0 + h * 16 * RC + rloc;
+            if (row >= g.M) break;
+            float v[8];
+            const float4 lo = *reinterpret_cast<const float4*>(stage + rloc * EROW<AN> + cl);
+            const float4 hi = *reinterpret_cast<const float4*>(stage + rloc * EROW<AN> + cl + 4);
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+            if (g.splits > 1)
+                store8(g.part + ((int64_t)blockIdx.y * g.M + row) * g.N + col, g.N - col, v);
+            else
+                finish8<T>(g.e, row, col, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, bool ODD>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void gemm_kernel(GemmArgs g) {
     constexpr int BM = 16 * WM * AM, BN = 16 * WN * AN, THREADS = 64 * WM * WN;
     using TileA = Tile<T, AKM, BM, THREADS, ODD>;
     using TileB = Tile<T, BKM, BN, THREADS, ODD>;
     constexpr int STAGE = TileA::BYTES + TileB::BYTES;
-    constexpr int EROW = 16 * AN + 4;   // floats per staged row of the epilogue
-    static_assert(WM * WN * 16 * EROW * 4 <= 2 * STAGE, "epilogue staging");
+    static_assert(WM * WN * 32 * EROW<AN> * 4 <= 2 * STAGE, "epilogue staging");
     __shared__ __align__(16) char lds[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // Tiles in groups of 4 row blocks × every column block, column-major
@@ -349,36 +389,311 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void gemm_kernel
         __syncthreads();
     }
 
-    // Epilogue: 16 rows at a time through the wave's own LDS, so that a lane
-    // gets eight neighbouring columns.
-    const int gq = lane >> 4, li = lane & 15;
-    float* stage = reinterpret_cast<float*>(lds) + wave * 16 * EROW;
-    constexpr int LPR = 2 * AN, RPP = 64 / LPR;   // lanes per row, rows per pass
+    finish_tile<T, AM, AN, 2>(g, acc, reinterpret_cast<float*>(lds) + wave * 32 * EROW<AN>, m0 + wm * AM * 16,
+                              n0 + wn * AN * 16, lane);
+}
+
+// ───────────────────────────── whole tiles: loads straight into LDS ─────────────────────────────
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes per lane from a buffer into LDS at `at` + 16·lane (bytes, uniform).
+// The compiler does not know of these loads: whoever reads the LDS bytes waits
+// for vmcnt first.  Offsets outside the buffer store zeros.
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t at, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(at), "v"(off), "s"(rsrc));
+}
+
+__device__ __forceinline__ i32x4 rsrc_of(uint64_t base, uint32_t bytes) {
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)base), __builtin_amdgcn_readfirstlane((int)(base >> 32) & 0xffff),
+                 __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+
+// ROWS × BK of an operand with 16-byte aligned rows, as Tile lays it out.  A
+// load covers 1024 LDS bytes; the permutation of the LDS layout is applied to
+// the global addresses its lanes read.
+template <typename T, bool KM, int ROWS, int WAVES>
+struct DmaTile {
+    static constexpr int P = ROWS / 8 / WAVES;       // loads per wave and stage
+    static constexpr int KR = KM ? 512 / ROWS : 0;   // k rows per load
+    static constexpr int BYTES = ROWS * BK * 2;
+    static_assert(P >= 1, "tile shape");
+    using Read = Tile<T, KM, ROWS, 64 * WAVES, false>;
+
+    uint64_t p;        // the tile's first row (k-contiguous) or column (k-major)
+    int64_t ld;
+    int rows, K;       // rows (columns) from there to the operand's end, at most ROWS; the operand's k
+    uint32_t off[2];   // the lane's byte offset in its first (and, k-major, odd) loads
+    uint32_t step;     // bytes between loads
+    int c;             // k-contiguous: the lane's k within a stage
+
+    __device__ __forceinline__ DmaTile(const void* base, int64_t ld_, int wave, int lane)
+        : p((uint64_t)base), ld(ld_), rows(0), K(0) {
+        if constexpr (KM) {
 #pragma unroll
-    for (int i = 0; i < AM; ++i) {
-#pragma unroll
-        for (int j = 0; j < AN; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) stage[(4 * gq + q) * EROW + 16 * j + li] = acc[i][j][q];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int ps = 0; ps < 16 / RPP; ++ps) {
-            const int rloc = ps * RPP + lane / LPR, cl = 8 * (lane % LPR);
-            const int64_t row = m0 + (wm * AM + i) * 16 + rloc;
-            const int col = n0 + wn * AN * 16 + cl;
-            if (row >= g.M) continue;
-            float v[8];
-            const float4 lo = *reinterpret_cast<const float4*>(stage + rloc * EROW + cl);
-            const float4 hi = *reinterpret_cast<const float4*>(stage + rloc * EROW + cl + 4);
-            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-            if (g.splits > 1)
-                store8(g.part + ((int64_t)blockIdx.y * g.M + row) * g.N + col, g.N - col, v);
-            else
-                finish8<T>(g.e, row, col, v);
+            for (int o = 0; o < 2; ++o) {
+                const int k = (o * WAVES + wave) * KR + lane / (ROWS / 8), pos = lane % (ROWS / 8);
+                const int chunk = (((pos >> 1) ^ Read::slot_mask(k)) << 1) | (pos & 1);
+                off[o] = (uint32_t)(k * (int)ld + 8 * chunk) * 2;
+            }
+            step = (uint32_t)(2 * WAVES * KR * (int)ld) * 2;
+            c = 0;
+        } else {
+            const int r = wave * 8 + (lane >> 3);
+            c = 8 * ((lane & 7) ^ (r & 7));
+            off[0] = off[1] = (uint32_t)(r * (int)ld + c) * 2;
+            step = (uint32_t)(8 * WAVES * (int)ld) * 2;
         }
-        __builtin_amdgcn_wave_barrier();
     }
+
+    __device__ __forceinline__ void start(const void* base, int64_t at, int64_t total, int K_) {
+        p = (uint64_t)base + (uint64_t)(KM ? at : at * ld) * 2;
+        rows = (int)min(total - at, (int64_t)ROWS);
+        K = K_;
+    }
+
+    __device__ __forceinline__ i32x4 stage(int st) const {
+        if constexpr (KM) {
+            const int left = min(BK, K - st * BK), cols = (rows + 1) & ~1;
+            return rsrc_of(p + (uint64_t)st * BK * (uint64_t)ld * 2,
+                           left > 0 ? (uint32_t)(((int64_t)(left - 1) * ld + cols) * 2) : 0u);
+        } else {
+            const int left = K - st * BK;
+            return rsrc_of(p + (uint64_t)st * BK * 2, left > 0 ? (uint32_t)(((int64_t)(rows - 1) * ld + left) * 2) : 0u);
+        }
+    }
+    // past the last k: an offset outside the range, also after the steps are added
+    __device__ __forceinline__ uint32_t lane_off(int st, int odd) const {
+        if constexpr (KM) return off[odd];
+        else return st * BK + c < K ? off[0] : 0x80000000u;
+    }
+    // load j of the wave: LDS byte within the tile, and what to add to the lane's offset
+    static __device__ __forceinline__ uint32_t at(int j, int wave) { return (uint32_t)(j * WAVES + wave) * 1024; }
+    __device__ __forceinline__ uint32_t add(int j) const { return KM ? (uint32_t)(j >> 1) * step : (uint32_t)j * step; }
+};
+
+// The tile of workgroup `id`: tiles in groups of 4 row blocks × every column
+// block, column-major within a group; XCD x (workgroups x, x + 8, ...) takes a
+// contiguous run of that order, so its workgroups share operand blocks in its
+// L2.
+__device__ __forceinline__ void tile_of(int id, int ntm, int ntn, int& tm, int& tn) {
+    const int total = ntm * ntn, xcd = id & 7, loc = id >> 3;
+    const int t = xcd * (total >> 3) + min(xcd, total & 7) + loc;
+    const int grp = t / (4 * ntn), first = 4 * grp, gm = min(4, ntm - first);
+    const int rr = t - grp * 4 * ntn;
+    tm = first + rr % gm;
+    tn = rr / gm;
+}
+
+// Lanes of odd 16-lane rows of a and of even ones of b change places.
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    const T2 v = {(T)a, (T)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+enum { EPI_PLAIN, EPI_PART, EPI_FULL };
+
+// C = A·Bᵀ on whole tiles.  A workgroup walks the work items (tile, K range)
+// blockIdx.x, + gridDim.x, ...; its loads run two stages ahead of the products
+// straight through the items' ends.  A stage is two halves of 32 k: while the
+// matrix cores work on one half's operands the other's are read, so within
+// a stage there is one barrier, after the first half: every wave has then
+// read the stage's buffer, which the second half refills, and the next
+// stage's loads are done.
+//
+// The products are taken as (B tile)·(A tile)ᵀ, so that a lane holds four
+// neighbouring columns of a row: columns 16j + 4g .. + 3 of row 16i + (l & 15).
+template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, int EPI>
+__global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
+    constexpr int BM = 16 * WM * AM, BN = 16 * WN * AN, W = WM * WN;
+    using DA = DmaTile<T, AKM, BM, W>;
+    using DB = DmaTile<T, BKM, BN, W>;
+    using TileA = typename DA::Read;
+    using TileB = typename DB::Read;
+    constexpr uint32_t STAGE = DA::BYTES + DB::BYTES;
+    constexpr int NM = AM * AN, NF = AM + AN, ND = DA::P + DB::P;
+    constexpr int CPR = 4 * AN;   // 16-byte chunks of a staged row of the epilogue
+    __shared__ __align__(1024) char lds[2 * STAGE + (EPI == EPI_FULL ? W * 16 * CPR * 16 : 0)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ntm = (int)((g.M + BM - 1) / BM), ntn = (g.N + BN - 1) / BN, tiles = ntm * ntn, items = tiles * g.splits;
+    const int nst = (g.K + BK - 1) / BK;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const int wm = wave % WM, wn = wave / WM;
+
+    // the loader: item, stage and the descriptors of its tile
+    DA da(g.a, g.lda, wave, lane);
+    DB db(g.b, g.ldb, wave, lane);
+    int l_item = blockIdx.x, l_st = 0, l_end = 0;
+    auto l_start = [&] {
+        if (l_item < items) {
+            const int split = l_item / tiles;
+            int tm, tn;
+            tile_of(l_item - split * tiles, ntm, ntn, tm, tn);
+            da.start(g.a, (int64_t)tm * BM, g.M, g.K);
+            db.start(g.b, (int64_t)tn * BN, g.N, g.KB);
+            l_st = split * g.per;
+            l_end = min(nst, l_st + g.per);
+        } else {
+            da.K = db.K = 0;   // nothing left: loads out of range
+            l_st = 0;
+            l_end = 1 << 30;
+        }
+    };
+    i32x4 ra, rb;
+    uint32_t oa[2], ob[2];
+    auto l_stage = [&] {
+        ra = da.stage(l_st);
+        rb = db.stage(l_st);
+        oa[0] = da.lane_off(l_st, 0);
+        oa[1] = da.lane_off(l_st, 1);
+        ob[0] = db.lane_off(l_st, 0);
+        ob[1] = db.lane_off(l_st, 1);
+        if (++l_st == l_end) {
+            l_item += gridDim.x;
+            l_start();
+        }
+    };
+    auto load = [&](uint32_t buf, int j) {
+        if (j < DA::P)
+            load_to_lds(ra, base + buf + DA::at(j, wave), oa[j & 1] + da.add(j));
+        else
+            load_to_lds(rb, base + buf + DA::BYTES + DB::at(j - DA::P, wave), ob[(j - DA::P) & 1] + db.add(j - DA::P));
+    };
+
+    f32x4 acc[AM][AN];
+    uint4 av[2][AM], bv[2][AN];
+    auto read = [&](int set, int kk, uint32_t buf, int f) {
+        if (f < AN) bv[set][f] = TileB::frag(lds + buf + DA::BYTES, wn * AN * 16, f, kk, lane);
+        else av[set][f - AN] = TileA::frag(lds + buf, wm * AM * 16, f - AN, kk, lane);
+    };
+    l_start();
+    l_stage();
+#pragma unroll
+    for (int j = 0; j < ND; ++j) load(0, j);
+    l_stage();
+#pragma unroll
+    for (int j = 0; j < ND; ++j) load(STAGE, j);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ND) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int f = 0; f < NF; ++f) read(0, 0, 0, f);
+    uint32_t cur = 0;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int split = item / tiles;
+        int tm, tn;
+        tile_of(item - split * tiles, ntm, ntn, tm, tn);
+        const int count = min(nst, (split + 1) * g.per) - split * g.per;
+#pragma unroll
+        for (int i = 0; i < AM; ++i)
+#pragma unroll
+            for (int j = 0; j < AN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int st = 0; st < count; ++st) {
+            // first half: products of k 0..31, operands of k 32..63
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                if (m % (NM / NF) == 0 && m / (NM / NF) < NF) read(1, 1, cur, m / (NM / NF));
+                acc[m / AN][m % AN] = mfma<T>(bv[0][m % AN], av[0][m / AN], acc[m / AN][m % AN]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            l_stage();
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                if (m % (NM / NF) == 0 && m / (NM / NF) < NF) read(0, 0, cur ^ STAGE, m / (NM / NF));
+                if (m % (NM / ND) == 0 && m / (NM / ND) < ND) load(cur, m / (NM / ND));
+                acc[m / AN][m % AN] = mfma<T>(bv[1][m % AN], av[1][m / AN], acc[m / AN][m % AN]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            cur ^= STAGE;
+        }
+
+        const int64_t row0 = (int64_t)tm * BM + wm * AM * 16;
+        const int col0 = tn * BN + wn * AN * 16, gq = lane >> 4, li = lane & 15;
+        if constexpr (EPI == EPI_PLAIN) {
+            // neighbouring lanes' fours become eights
+#pragma unroll
+            for (int i = 0; i < AM; ++i) {
+                __builtin_amdgcn_sched_barrier(0);   // a row tile's addresses at a time
+                const int64_t row = row0 + 16 * i + li;
+#pragma unroll
+                for (int j = 0; j < AN; j += 2) {
+                    uint32_t x0 = pack2<T>(acc[i][j][0], acc[i][j][1]), x1 = pack2<T>(acc[i][j][2], acc[i][j][3]);
+                    uint32_t y0 = pack2<T>(acc[i][j + 1][0], acc[i][j + 1][1]), y1 = pack2<T>(acc[i][j + 1][2], acc[i][j + 1][3]);
+                    swap16(x0, y0);
+                    swap16(x1, y1);
+                    const int col = col0 + 16 * (j + (gq & 1)) + 8 * (gq >> 1), valid = g.N - col;
+                    if (row >= g.M) continue;
+                    T* y = reinterpret_cast<T*>(g.e.y) + row * g.N + col;
+                    const uint32_t w[4] = {x0, x1, y0, y1};
+                    if (valid >= 8) {
+                        __builtin_memcpy(y, w, 16);
+                    } else {
+#pragma unroll 1
+                        for (int e = 0; e < valid; ++e) {
+                            const uint32_t d = e < 4 ? (e < 2 ? x0 : x1) : (e < 6 ? y0 : y1);
+                            reinterpret_cast<uint16_t*>(y)[e] = (uint16_t)(d >> (16 * (e & 1)));
+                        }
+                    }
+                }
+            }
+        } else if constexpr (EPI == EPI_PART) {
+#pragma unroll
+            for (int i = 0; i < AM; ++i) {
+                const int64_t row = row0 + 16 * i + li;
+                if (row >= g.M) continue;
+                float* p = g.part + ((int64_t)split * g.M + row) * g.N;
+#pragma unroll
+                for (int j = 0; j < AN; ++j) {
+                    const int col = col0 + 16 * j + 4 * gq, valid = g.N - col;
+                    if (valid >= 4) {
+                        __builtin_memcpy(p + col, &acc[i][j], 16);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 3; ++e)
+                            if (e < valid) p[col + e] = acc[i][j][e];
+                    }
+                }
+            }
+        } else {
+            // sixteen rows at a time through LDS of the wave's own; a rolled
+            // loop, as the finishing code is long
+            float4* const own = reinterpret_cast<float4*>(lds + 2 * STAGE) + wave * 16 * CPR;
+#pragma unroll 1
+            for (int i = 0; i < AM; ++i) {
+#pragma unroll
+                for (int k = 0; k < AM; ++k) {
+                    if (i != k) continue;
+#pragma unroll
+                    for (int j = 0; j < AN; ++j)
+                        own[li * CPR + ((4 * j + gq) ^ li)] = make_float4(acc[k][j][0], acc[k][j][1], acc[k][j][2], acc[k][j][3]);
+                }
+                __builtin_amdgcn_wave_barrier();
+                constexpr int LPR = CPR / 2, RPP = 64 / LPR;   // lanes per row, rows per step
+#pragma unroll
+                for (int ps = 0; ps < 16 / RPP; ++ps) {
+                    const int r = ps * RPP + lane / LPR, q = lane % LPR;
+                    const float4 lo = own[r * CPR + ((2 * q) ^ r)], hi = own[r * CPR + ((2 * q + 1) ^ r)];
+                    float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                    if (row0 + 16 * i + r < g.M) finish8<T>(g.e, row0 + 16 * i + r, col0 + 8 * q, v);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads of stages that do not come still write LDS
 }
 
 // Sums the K ranges in order and finishes: a thread per 8 columns.
@@ -551,7 +866,14 @@ void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)tiles_of(g.M, g.N, r.tile), (unsigned)r.splits);
     if constexpr (!ODD) {
         if (r.tile == 256) {
-            rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 4, 8, 4, ODD>, grid, dim3(512), s, g);
+            // one workgroup per CU (its LDS) walks the items
+            const dim3 cus((unsigned)std::min<int64_t>(tiles_of(g.M, g.N, r.tile) * r.splits, 256));
+            if (r.splits > 1)
+                rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, 8, 8, EPI_PART>, cus, dim3(256), s, g);
+            else if (g.e.plain)
+                rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, 8, 8, EPI_PLAIN>, cus, dim3(256), s, g);
+            else if constexpr (!AKM && !BKM)
+                rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, 8, 8, EPI_FULL>, cus, dim3(256), s, g);
             return;
         }
     }
@@ -573,6 +895,7 @@ rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, v
                  "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need);
     g.splits = r.splits;
     g.per = r.per;
+    g.e.plain = !g.e.bias && !g.e.res && !g.e.wide && !g.e.aux && !g.e.rem && !g.e.codes && g.e.act == ACT_NONE;
     g.part = r.splits > 1 ? (float*)workspace : nullptr;
     auto by_layout = [&](auto type, auto o) {
         using T = decltype(type);
