@@ -68,40 +68,38 @@ __device__ __forceinline__ float step_of(uint32_t scale) {
     return __builtin_bit_cast(float, scale == 255u ? 0x7fc00000u : (scale - 6u) << 23);
 }
 
-// Scale byte of a group whose largest magnitude is amax (infinity: not finite).
-__device__ __forceinline__ uint32_t scale_of(float amax) {
-    return max(__builtin_bit_cast(uint32_t, amax) >> 23, 7u);
+// Scale byte of a group whose largest magnitude has the bits amax (255:
+// infinity or NaN, whose patterns are the largest).
+__device__ __forceinline__ uint32_t scale_of(uint32_t amax) { return max(amax >> 23, 7u); }
+
+// Bits of the largest magnitude of eight values.
+__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+    return m;
 }
 
-// Largest magnitude of eight values; infinity if one is infinite or a NaN.
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(v[i]);
-        m = a <= 3.402823466e38f ? fmaxf(m, a) : __builtin_inff();
-        // (once infinite it stays so: fmaxf(inf, a) = inf)
-    }
-    return m;
+// The low bytes of four dwords.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
 }
 
 // Encodes a group's share of four neighbouring lanes (8 values each, lanes
 // 4q .. 4q+3 in column order): returns the lane's eight codes and the group's
 // scale byte.  Every lane of the quad must be active.
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t& scale) {
-    float m = amax8(v);
-    m = fmaxf(m, __shfl_xor(m, 1));
-    m = fmaxf(m, __shfl_xor(m, 2));
+    uint32_t m = amax8(v);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 2));
     scale = scale_of(m);
     const float inv = __builtin_bit_cast(float, (260u - min(scale, 254u)) << 23);   // 2^(133 - scale)
-    uint32_t w[2] = {0u, 0u};
+    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(rintf(v[i] * inv), -127.0f), 127.0f);
-        w[i >> 2] |= ((uint32_t)(int)c & 0xffu) << (8 * (i & 3));
-    }
-    if (scale == 255u) w[0] = w[1] = 0u;
-    return make_uint2(w[0], w[1]);
+    for (int i = 0; i < 8; ++i)   // 1.5·2^23 rounds to an integer, in the low byte as two's complement
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_fmed3f(v[i] * inv, -127.0f, 127.0f) + 12582912.0f);
+    const bool bad = scale == 255u;
+    return make_uint2(bad ? 0u : low_bytes(w[0], w[1], w[2], w[3]), bad ? 0u : low_bytes(w[4], w[5], w[6], w[7]));
 }
 
 // The eight values of codes c with the group's scale byte.

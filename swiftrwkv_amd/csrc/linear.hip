@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "act8.h"
 #include "launch.h"
@@ -59,16 +60,44 @@ enum { ACT_NONE = 0, ACT_RELU2 = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
 // What the forward pass keeps of an activation has 8 bits more than the 16 of
 // its type: the backward pass takes 1 − h² and the like from it, where 16 bits
 // alone would cost more than the rounding of dz does.  v and its rounding a
-// are neighbours in the order of fp32 bit patterns, so the difference of the
-// patterns, rounded to its upper 8 bits (a few at the type's subnormals
-// clamp), is what a lacks: 16 (bf16) or 18 (fp16) bits in all.
+// are neighbours in the order of fp32 bit patterns; the upper 8 bits of the
+// patterns' difference are what a lacks: 16 (bf16) or 18 (fp16) bits in all.
+
+// Eight values rounded to T, packed.  bf16 takes ties away from zero: what is
+// lost is then the low half of the pattern, read as a signed number.  (A NaN's
+// low half is zero here: it comes of 16-bit operands.)
 template <typename T>
-__device__ __forceinline__ uint32_t rem_of(float v, T a) {
-    constexpr int SH = __is_same(T, bf16) ? 8 : 5;
-    const float f = (float)a;
-    const int d = (int)(__builtin_bit_cast(uint32_t, v) - __builtin_bit_cast(uint32_t, f));
-    const int q = min(max((d + (1 << (SH - 1))) >> SH, -128), 127);
-    return fabsf(f) <= 3.402823466e38f ? (uint32_t)q & 0xffu : 0u;
+__device__ __forceinline__ uint4 round8(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (__is_same(T, bf16)) {
+            w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, v[2 * i + 1]) + 0x8000u,
+                                         __builtin_bit_cast(uint32_t, v[2 * i]) + 0x8000u, 0x07060302u);
+        } else {
+            typedef T T2 __attribute__((ext_vector_type(2)));
+            w[i] = __builtin_bit_cast(uint32_t, T2{(T)v[2 * i], (T)v[2 * i + 1]});
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The next 8 bits of the eight values that round8 rounded.
+template <typename T>
+__device__ __forceinline__ uint2 rem8(const float (&v)[8]) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = __builtin_bit_cast(uint32_t, v[i]);
+        if constexpr (__is_same(T, bf16)) {
+            w[i] = bits >> 8;
+        } else {   // at the type's subnormals the difference is larger: it clamps; an infinity keeps none
+            const float f = (float)(T)v[i];
+            const int q = min(max((int)(bits - __builtin_bit_cast(uint32_t, f)) >> 5, -128), 127);
+            w[i] = fabsf(f) <= 65504.0f ? (uint32_t)q : 0u;
+        }
+    }
+    return make_uint2(low_bytes(w[0], w[1], w[2], w[3]), low_bytes(w[4], w[5], w[6], w[7]));
 }
 
 template <typename T>
@@ -77,19 +106,39 @@ __device__ __forceinline__ float with_rem(float a, uint32_t rem) {
     return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) + (uint32_t)((int)(int8_t)rem * (1 << SH)));
 }
 
-// Remainders of eight values, valid of them stored.
-template <typename T>
-__device__ __forceinline__ void store_rem8(uint8_t* p, int valid, const float (&v)[8]) {
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= rem_of(v[i], (T)v[i]) << (8 * (i & 3));
+// The first `valid` of eight packed 16-bit values, or bytes.
+__device__ __forceinline__ void store_raw(void* p, int valid, uint4 w) {
     if (valid >= 8) {
-        __builtin_memcpy(p, w, 8);
+        __builtin_memcpy(p, &w, 16);
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < valid) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+#pragma unroll 1
+        for (int i = 0; i < valid; ++i) {
+            const uint32_t d = i < 4 ? (i < 2 ? w.x : w.y) : (i < 6 ? w.z : w.w);
+            reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(d >> (16 * (i & 1)));
+        }
     }
+}
+__device__ __forceinline__ void store_raw(uint8_t* p, int valid, uint2 w) {
+    if (valid >= 8) {
+        __builtin_memcpy(p, &w, 8);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < valid; ++i) p[i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    }
+}
+
+// tanh: the odd Taylor polynomial to x^11 where |x| < 0.35 (the next term is
+// under 2^-26 of x), else (1 − t)/(1 + t), t = e^(−2|x|).
+__device__ __forceinline__ float tanh_of(float x) {
+    const float s = x * x;
+    const float p = x * (1.0f + s * (-1.0f / 3 + s * (2.0f / 15 + s * (-17.0f / 315 + s * (62.0f / 2835 + s * (-1382.0f / 155925))))));
+    const float t = __builtin_amdgcn_exp2f(fabsf(x) * -2.885390081777927f);
+    const float q = __builtin_copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+    return fabsf(x) < 0.35f ? p : q;
+}
+
+__device__ __forceinline__ float sigmoid_of(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
 struct Epilogue {
@@ -108,65 +157,96 @@ struct Epilogue {
     bool plain;           // y alone, of the operands' type
 };
 
-// Eight neighbouring columns of a row, z without bias in v.  With codes, the
+// Eight neighbouring columns of each of C rows row, row + step, ..., z without
+// bias in v.  Every flag is looked at once for all of them.  With codes, the
 // four lanes of a 32-column group call it together.
-template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int col, float (&v)[8]) {
+template <typename T, int C>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t row, int step, int col, float (&v)[C][8]) {
     const int valid = e.N - col;
     if (e.bias) {
         float b[8];
         load8(reinterpret_cast<const T*>(e.bias) + col, valid, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += b[i];
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] += b[i];
     }
     if (e.codes) {
+        const int64_t np = padded(e.N);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < valid ? v[i] : 0.0f;
-        uint32_t scale;
-        const uint2 c = encode8(v, scale);
-        const int64_t np = padded(e.N), at = row * np + col;
-        if (col < np) {
-            *reinterpret_cast<uint2*>(e.codes + at) = c;
-            if ((col & 31) == 0) e.scales[at / GROUP] = (uint8_t)scale;
+        for (int c = 0; c < C; ++c) {
+            if (valid < 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] = i < valid ? v[c][i] : 0.0f;
+            }
+            uint32_t scale;
+            const uint2 code = encode8(v[c], scale);
+            if (col < np && row + c * step < e.M) {
+                const int64_t at = (row + c * step) * np + col;
+                *reinterpret_cast<uint2*>(e.codes + at) = code;
+                if ((col & 31) == 0) e.scales[at / GROUP] = (uint8_t)scale;
+            }
         }
     }
-    float r[8];   // the value aux keeps
-    switch (e.act) {
-        case ACT_RELU2:
+    const int64_t at = row * e.N + col, pitch = (int64_t)step * e.N;
+    if (e.act == ACT_RELU2) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                r[i] = v[i] > 0.0f || v[i] != v[i] ? v[i] : 0.0f;   // a NaN stays one
-                v[i] = r[i] * r[i];
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] < 0.0f ? 0.0f : v[c][i];   // a NaN stays one
+    } else if (e.act == ACT_TANH) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = tanh_of(v[c][i]);
+    } else if (e.act == ACT_SIGMOID) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = sigmoid_of(v[c][i]);
+    }
+    if (e.aux) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (row + c * step < e.M) {
+                store_raw(reinterpret_cast<T*>(e.aux) + at + c * pitch, valid, round8<T>(v[c]));
+                store_raw(e.rem + at + c * pitch, valid, rem8<T>(v[c]));
             }
-            break;
-        case ACT_TANH:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = r[i] = tanhf(v[i]);
-            break;
-        case ACT_SIGMOID:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = r[i] = 1.0f / (1.0f + __expf(-v[i]));
-            break;
-        default:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = v[i];
     }
-    const int64_t at = row * e.N + col;
-    if (e.aux) store8(reinterpret_cast<T*>(e.aux) + at, valid, r);
-    if (e.rem) store_rem8<T>(e.rem + at, valid, e.aux ? r : v);
+    if (e.act == ACT_RELU2) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] *= v[c][i];
+    }
+    if (e.rem && !e.aux) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (row + c * step < e.M) store_raw(e.rem + at + c * pitch, valid, rem8<T>(v[c]));
+    }
     if (e.res) {
-        float s[8];
-        if (e.wide)
-            load8(reinterpret_cast<const float*>(e.res) + row * e.ldr + col, valid, s);
-        else
-            load8(reinterpret_cast<const T*>(e.res) + row * e.ldr + col, valid, s);
+        float s[C][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += s[i];
+        for (int c = 0; c < C; ++c) {
+            const int64_t from = min(row + c * step, e.M - 1) * e.ldr + col;   // all C loads before their use
+            if (e.wide)
+                load8(reinterpret_cast<const float*>(e.res) + from, valid, s[c]);
+            else
+                load8(reinterpret_cast<const T*>(e.res) + from, valid, s[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] += s[c][i];
     }
-    if (e.wide)
-        store8(reinterpret_cast<float*>(e.y) + at, valid, v);
-    else
-        store8(reinterpret_cast<T*>(e.y) + at, valid, v);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (row + c * step >= e.M) continue;
+        if (e.wide)
+            store8(reinterpret_cast<float*>(e.y) + at + c * pitch, valid, v[c]);
+        else
+            store_raw(reinterpret_cast<T*>(e.y) + at + c * pitch, valid, round8<T>(v[c]));
+    }
 }
 
 // ───────────────────────────── operand tiles ─────────────────────────────
@@ -308,19 +388,26 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc
                 for (int q = 0; q < 4; ++q)
                     stage[(16 * i + 4 * gq + q) * EROW<AN> + 16 * j + li] = acc[h * RC + i][j][q];
         __builtin_amdgcn_wave_barrier();
+        constexpr int C = 16 * RC / RPP < 4 ? 16 * RC / RPP : 4;   // rows of a lane per round
 #pragma unroll 1
-        for (int rloc = lane / LPR; rloc < 16 * RC; rloc += RPP) {
+        for (int rloc = lane / LPR; rloc < 16 * RC; rloc += C * RPP) {
             const int64_t row = row0 + h * 16 * RC + rloc;
-            if (row >= g.M) break;
-            float v[8];
-            const float4 lo = *reinterpret_cast<const float4*>(stage + rloc * EROW<AN> + cl);
-            const float4 hi = *reinterpret_cast<const float4*>(stage + rloc * EROW<AN> + cl + 4);
-            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-            if (g.splits > 1)
-                store8(g.part + ((int64_t)blockIdx.y * g.M + row) * g.N + col, g.N - col, v);
-            else
-                finish8<T>(g.e, row, col, v);
+            float v[C][8];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float4 lo = *reinterpret_cast<const float4*>(stage + (rloc + c * RPP) * EROW<AN> + cl);
+                const float4 hi = *reinterpret_cast<const float4*>(stage + (rloc + c * RPP) * EROW<AN> + cl + 4);
+                v[c][0] = lo.x; v[c][1] = lo.y; v[c][2] = lo.z; v[c][3] = lo.w;
+                v[c][4] = hi.x; v[c][5] = hi.y; v[c][6] = hi.z; v[c][7] = hi.w;
+            }
+            if (g.splits > 1) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    if (row + c * RPP < g.M)
+                        store8(g.part + ((int64_t)blockIdx.y * g.M + row + c * RPP) * g.N + col, g.N - col, v[c]);
+            } else {
+                finish<T, C>(g.e, row, RPP, col, v);
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -397,13 +484,21 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void gemm_kernel
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes per lane from a buffer into LDS at `at` + 16·lane (bytes, uniform).
-// The compiler does not know of these loads: whoever reads the LDS bytes waits
-// for vmcnt first.  Offsets outside the buffer store zeros.
-__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t at, uint32_t off) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(at), "v"(off), "s"(rsrc));
+// 16 bytes per lane from a buffer into LDS at m0 + 16·lane (bytes).  The
+// compiler does not know of these loads: whoever reads the LDS bytes waits for
+// vmcnt first.  Offsets outside the buffer store zeros.  m0 is set a product
+// earlier (an instruction has to lie between); nothing else here uses it.
+template <int ADD>
+__device__ __forceinline__ void lds_target(uint32_t at) {
+    asm volatile("s_add_u32 m0, %0, %1" ::"s"(at), "n"(ADD) : "scc");
+}
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off) {
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc));
+}
+
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
 }
 
 __device__ __forceinline__ i32x4 rsrc_of(uint64_t base, uint32_t bytes) {
@@ -422,56 +517,56 @@ struct DmaTile {
     static_assert(P >= 1, "tile shape");
     using Read = Tile<T, KM, ROWS, 64 * WAVES, false>;
 
-    uint64_t p;        // the tile's first row (k-contiguous) or column (k-major)
+    i32x4 r;           // the stage's part of the tile
     int64_t ld;
-    int rows, K;       // rows (columns) from there to the operand's end, at most ROWS; the operand's k
-    uint32_t off[2];   // the lane's byte offset in its first (and, k-major, odd) loads
-    uint32_t step;     // bytes between loads
+    int k, cols;       // k from the stage's start to the operand's end; k-major: columns, to whole dwords
+    uint32_t x;        // k-contiguous: sends offsets past the last k out of range
+    uint32_t off[P];   // the lane's byte offset of each load
     int c;             // k-contiguous: the lane's k within a stage
 
-    __device__ __forceinline__ DmaTile(const void* base, int64_t ld_, int wave, int lane)
-        : p((uint64_t)base), ld(ld_), rows(0), K(0) {
-        if constexpr (KM) {
+    __device__ __forceinline__ DmaTile(int64_t ld_, int wave, int lane) : r{}, ld(ld_), k(0), cols(0), x(0), c(0) {
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const int k = (o * WAVES + wave) * KR + lane / (ROWS / 8), pos = lane % (ROWS / 8);
+        for (int j = 0; j < P; ++j) {   // LDS bytes 1024·(j·WAVES + wave) of the tile
+            if constexpr (KM) {
+                const int k = (j * WAVES + wave) * KR + lane / (ROWS / 8), pos = lane % (ROWS / 8);
                 const int chunk = (((pos >> 1) ^ Read::slot_mask(k)) << 1) | (pos & 1);
-                off[o] = (uint32_t)(k * (int)ld + 8 * chunk) * 2;
+                off[j] = (uint32_t)(k * (int)ld + 8 * chunk) * 2;
+            } else {
+                const int r = (j * WAVES + wave) * 8 + (lane >> 3);
+                c = 8 * ((lane & 7) ^ (r & 7));   // (r & 7 is the same for every j)
+                off[j] = (uint32_t)(r * (int)ld + c) * 2;
             }
-            step = (uint32_t)(2 * WAVES * KR * (int)ld) * 2;
-            c = 0;
-        } else {
-            const int r = wave * 8 + (lane >> 3);
-            c = 8 * ((lane & 7) ^ (r & 7));
-            off[0] = off[1] = (uint32_t)(r * (int)ld + c) * 2;
-            step = (uint32_t)(8 * WAVES * (int)ld) * 2;
         }
     }
 
-    __device__ __forceinline__ void start(const void* base, int64_t at, int64_t total, int K_) {
-        p = (uint64_t)base + (uint64_t)(KM ? at : at * ld) * 2;
-        rows = (int)min(total - at, (int64_t)ROWS);
-        K = K_;
+    // Row (column) `at` of `total`, stage st of an operand of K.
+    __device__ __forceinline__ void start(const void* base, int64_t at, int64_t total, int K, int st) {
+        const int rows = (int)min(total - at, (int64_t)ROWS);
+        k = K - st * BK;
+        // a dword that holds a last odd column may be read whole
+        cols = (rows + 1) & ~1;
+        const uint64_t p = (uint64_t)base + (KM ? (uint64_t)at + (uint64_t)st * BK * (uint64_t)ld : (uint64_t)at * ld + (uint64_t)st * BK) * 2;
+        r = rsrc_of(p, k <= 0 ? 0u : KM ? bytes() : (uint32_t)(((int64_t)(rows - 1) * ld + k) * 2));
+        x = beyond();
     }
+    __device__ __forceinline__ void end() { k = 0, r[2] = 0; }   // loads out of range from here on
 
-    __device__ __forceinline__ i32x4 stage(int st) const {
-        if constexpr (KM) {
-            const int left = min(BK, K - st * BK), cols = (rows + 1) & ~1;
-            return rsrc_of(p + (uint64_t)st * BK * (uint64_t)ld * 2,
-                           left > 0 ? (uint32_t)(((int64_t)(left - 1) * ld + cols) * 2) : 0u);
-        } else {
-            const int left = K - st * BK;
-            return rsrc_of(p + (uint64_t)st * BK * 2, left > 0 ? (uint32_t)(((int64_t)(rows - 1) * ld + left) * 2) : 0u);
-        }
+    // To the next stage, in steps that fit between products.
+    __device__ __forceinline__ void next_base() {
+        const uint64_t p = ((uint64_t)(uint32_t)r[1] << 32 | (uint32_t)r[0]) + (KM ? (uint64_t)BK * (uint64_t)ld * 2 : BK * 2);
+        r[0] = (int)(uint32_t)p;
+        r[1] = (int)(p >> 32);
+        k -= BK;
     }
-    // past the last k: an offset outside the range, also after the steps are added
-    __device__ __forceinline__ uint32_t lane_off(int st, int odd) const {
-        if constexpr (KM) return off[odd];
-        else return st * BK + c < K ? off[0] : 0x80000000u;
+    __device__ __forceinline__ void next_bytes() {
+        if constexpr (KM) r[2] = k >= BK ? r[2] : k > 0 ? (int)bytes() : 0;
+        else r[2] = k > 0 ? r[2] - BK * 2 : 0;
     }
-    // load j of the wave: LDS byte within the tile, and what to add to the lane's offset
-    static __device__ __forceinline__ uint32_t at(int j, int wave) { return (uint32_t)(j * WAVES + wave) * 1024; }
-    __device__ __forceinline__ uint32_t add(int j) const { return KM ? (uint32_t)(j >> 1) * step : (uint32_t)j * step; }
+    __device__ __forceinline__ void next_beyond() { x = beyond(); }
+
+private:
+    __device__ __forceinline__ uint32_t bytes() const { return (uint32_t)(((int64_t)(min(k, BK) - 1) * ld + cols) * 2); }
+    __device__ __forceinline__ uint32_t beyond() const { return KM || c < k ? 0u : 0x80000000u; }
 };
 
 // The tile of workgroup `id`: tiles in groups of 4 row blocks × every column
@@ -506,10 +601,12 @@ enum { EPI_PLAIN, EPI_PART, EPI_FULL };
 // C = A·Bᵀ on whole tiles.  A workgroup walks the work items (tile, K range)
 // blockIdx.x, + gridDim.x, ...; its loads run two stages ahead of the products
 // straight through the items' ends.  A stage is two halves of 32 k: while the
-// matrix cores work on one half's operands the other's are read, so within
-// a stage there is one barrier, after the first half: every wave has then
-// read the stage's buffer, which the second half refills, and the next
-// stage's loads are done.
+// matrix cores work on one half's operands the other's are read.  After two
+// thirds of the first half every wave has read the stage's buffer, which is
+// refilled from there on; at three eighths of the second half the next stage's
+// loads have to be done.  One wave per SIMD issues everything, so whatever is
+// not a product stands between products a few instructions at a time: the
+// loader's step to the next stage in one piece cost 8 % of the kernel.
 //
 // The products are taken as (B tile)·(A tile)ᵀ, so that a lane holds four
 // neighbouring columns of a row: columns 16j + 4g .. + 3 of row 16i + (l & 15).
@@ -522,6 +619,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     using TileB = typename DB::Read;
     constexpr uint32_t STAGE = DA::BYTES + DB::BYTES;
     constexpr int NM = AM * AN, NF = AM + AN, ND = DA::P + DB::P;
+    // Within a stage's 2·NM products: operands are read beside every RM-th
+    // product from the half's start (from MB in the second half), loads are
+    // issued beside every LM-th from MA in the first half on, spread as far as
+    // they go: the texture path takes 64 bytes a cycle, half of a stage's time.
+    constexpr int RM = NM / 2 / NF, MA = NM * 11 / 16, MB = NM * 3 / 8, LM = (2 * NM - MA) / ND;
+    static_assert(RM * NF <= MA && MB + RM * NF <= NM && MA + LM * ND <= 2 * NM, "places of a stage");
+    constexpr int SM = MA / 6;   // the loader's steps: beside every SM-th before MA
+    static_assert(RM * NF <= MA && MB + RM * NF <= NM && MA + LM * ND <= 2 * NM, "places of a stage");
     constexpr int CPR = 4 * AN;   // 16-byte chunks of a staged row of the epilogue
     __shared__ __align__(1024) char lds[2 * STAGE + (EPI == EPI_FULL ? W * 16 * CPR * 16 : 0)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -530,44 +635,51 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const int wm = wave % WM, wn = wave / WM;
 
-    // the loader: item, stage and the descriptors of its tile
-    DA da(g.a, g.lda, wave, lane);
-    DB db(g.b, g.ldb, wave, lane);
-    int l_item = blockIdx.x, l_st = 0, l_end = 0;
-    auto l_start = [&] {
+    // the loader: its item, the stages left of it, and the operands' parts of
+    // its stage; a step to the next stage has six parts
+    DA da(g.lda, wave, lane);
+    DB db(g.ldb, wave, lane);
+    int l_item = blockIdx.x, l_left = 0;
+    auto start = [&] {
         if (l_item < items) {
-            const int split = l_item / tiles;
+            const int split = l_item / tiles, st = split * g.per;
             int tm, tn;
             tile_of(l_item - split * tiles, ntm, ntn, tm, tn);
-            da.start(g.a, (int64_t)tm * BM, g.M, g.K);
-            db.start(g.b, (int64_t)tn * BN, g.N, g.KB);
-            l_st = split * g.per;
-            l_end = min(nst, l_st + g.per);
+            da.start(g.a, (int64_t)tm * BM, g.M, g.K, st);
+            db.start(g.b, (int64_t)tn * BN, g.N, g.KB, st);
+            l_left = min(nst, st + g.per) - st;
         } else {
-            da.K = db.K = 0;   // nothing left: loads out of range
-            l_st = 0;
-            l_end = 1 << 30;
+            da.end();
+            db.end();
+            l_left = 1 << 30;
         }
     };
-    i32x4 ra, rb;
-    uint32_t oa[2], ob[2];
-    auto l_stage = [&] {
-        ra = da.stage(l_st);
-        rb = db.stage(l_st);
-        oa[0] = da.lane_off(l_st, 0);
-        oa[1] = da.lane_off(l_st, 1);
-        ob[0] = db.lane_off(l_st, 0);
-        ob[1] = db.lane_off(l_st, 1);
-        if (++l_st == l_end) {
-            l_item += gridDim.x;
-            l_start();
-        }
+    auto step = [&](auto part) {
+        if constexpr (part == 0) da.next_base();
+        if constexpr (part == 1) da.next_bytes();
+        if constexpr (part == 2) db.next_base();
+        if constexpr (part == 3) db.next_bytes();
+        if constexpr (part == 4) da.next_beyond(), db.next_beyond();
+        if constexpr (part == 5)
+            if (--l_left == 0) {
+                l_item += gridDim.x;
+                start();
+            }
     };
-    auto load = [&](uint32_t buf, int j) {
-        if (j < DA::P)
-            load_to_lds(ra, base + buf + DA::at(j, wave), oa[j & 1] + da.add(j));
-        else
-            load_to_lds(rb, base + buf + DA::BYTES + DB::at(j - DA::P, wave), ob[(j - DA::P) & 1] + db.add(j - DA::P));
+    // load j of a wave into its buffer: target and load
+    auto target = [&](uint32_t buf, auto j) {
+        lds_target<(j < DA::P ? 0 : DA::BYTES) + (j < DA::P ? j : j - DA::P) * W * 1024>(base + buf + wave * 1024);
+    };
+    auto load = [&](auto j) {
+        if constexpr (j < DA::P) load_to_lds(da.r, AKM ? da.off[j] : da.off[j] | da.x);
+        else load_to_lds(db.r, BKM ? db.off[j - DA::P] : db.off[j - DA::P] | db.x);
+    };
+    auto load_all = [&](uint32_t buf) {
+        unrolled([&](auto j) {
+            target(buf, j);
+            asm volatile("s_nop 0");
+            load(j);
+        }, std::make_integer_sequence<int, ND>{});
     };
 
     f32x4 acc[AM][AN];
@@ -576,13 +688,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
         if (f < AN) bv[set][f] = TileB::frag(lds + buf + DA::BYTES, wn * AN * 16, f, kk, lane);
         else av[set][f - AN] = TileA::frag(lds + buf, wm * AM * 16, f - AN, kk, lane);
     };
-    l_start();
-    l_stage();
-#pragma unroll
-    for (int j = 0; j < ND; ++j) load(0, j);
-    l_stage();
-#pragma unroll
-    for (int j = 0; j < ND; ++j) load(STAGE, j);
+    start();
+    load_all(0);
+    unrolled(step, std::make_integer_sequence<int, 6>{});
+    load_all(STAGE);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ND) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -599,24 +708,43 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
 #pragma unroll
             for (int j = 0; j < AN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int st = 0; st < count; ++st) {
-            // first half: products of k 0..31, operands of k 32..63
-#pragma unroll
-            for (int m = 0; m < NM; ++m) {
-                if (m % (NM / NF) == 0 && m / (NM / NF) < NF) read(1, 1, cur, m / (NM / NF));
+            unrolled([&](auto m) {
+                if constexpr (m == MA) {   // every wave has read this stage's buffer
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                if constexpr (m % SM == SM - 1 && m / SM < 6) step(std::integral_constant<int, m / SM>{});
+                constexpr bool dma = m >= MA && (m - MA) % LM == 0 && (m - MA) / LM < ND;
+                if constexpr (dma) {
+                    target(cur, std::integral_constant<int, (m - MA) / LM>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if constexpr (m % RM == 0 && m / RM < NF) read(1, 1, cur, m / RM);
                 acc[m / AN][m % AN] = mfma<T>(bv[0][m % AN], av[0][m / AN], acc[m / AN][m % AN]);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            l_stage();
-#pragma unroll
-            for (int m = 0; m < NM; ++m) {
-                if (m % (NM / NF) == 0 && m / (NM / NF) < NF) read(0, 0, cur ^ STAGE, m / (NM / NF));
-                if (m % (NM / ND) == 0 && m / (NM / ND) < ND) load(cur, m / (NM / ND));
+                if constexpr (dma) load(std::integral_constant<int, (m - MA) / LM>{});
+                __builtin_amdgcn_sched_barrier(0);
+            }, std::make_integer_sequence<int, NM>{});
+            unrolled([&](auto m) {
+                constexpr int at = NM + m - MA;   // loads' place
+                if constexpr (m == MB) {   // the next stage's loads are done in every wave
+                    constexpr int issued = (at + LM - 1) / LM < ND ? (at + LM - 1) / LM : ND;
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(issued) : "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                constexpr bool dma = at % LM == 0 && at / LM < ND;
+                if constexpr (dma) {
+                    target(cur, std::integral_constant<int, at / LM>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if constexpr (m >= MB && (m - MB) % RM == 0 && (m - MB) / RM < NF) read(0, 0, cur ^ STAGE, (m - MB) / RM);
                 acc[m / AN][m % AN] = mfma<T>(bv[1][m % AN], av[1][m / AN], acc[m / AN][m % AN]);
                 __builtin_amdgcn_sched_barrier(0);
-            }
+                if constexpr (dma) load(std::integral_constant<int, at / LM>{});
+                __builtin_amdgcn_sched_barrier(0);
+            }, std::make_integer_sequence<int, NM>{});
             cur ^= STAGE;
         }
 
@@ -682,13 +810,17 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
                 }
                 __builtin_amdgcn_wave_barrier();
                 constexpr int LPR = CPR / 2, RPP = 64 / LPR;   // lanes per row, rows per step
+                constexpr int C = 16 / RPP;
+                const int q = lane % LPR;
+                float v[C][8];
 #pragma unroll
-                for (int ps = 0; ps < 16 / RPP; ++ps) {
-                    const int r = ps * RPP + lane / LPR, q = lane % LPR;
+                for (int c = 0; c < C; ++c) {
+                    const int r = c * RPP + lane / LPR;
                     const float4 lo = own[r * CPR + ((2 * q) ^ r)], hi = own[r * CPR + ((2 * q + 1) ^ r)];
-                    float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                    if (row0 + 16 * i + r < g.M) finish8<T>(g.e, row0 + 16 * i + r, col0 + 8 * q, v);
+                    v[c][0] = lo.x; v[c][1] = lo.y; v[c][2] = lo.z; v[c][3] = lo.w;
+                    v[c][4] = hi.x; v[c][5] = hi.y; v[c][6] = hi.z; v[c][7] = hi.w;
                 }
+                finish<T, C>(g.e, row0 + 16 * i + lane / LPR, RPP, col0 + 8 * q, v);
                 __builtin_amdgcn_wave_barrier();
             }
         }
@@ -704,14 +836,15 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const float* part, in
     const int64_t row = i / cpr;
     if (row >= e.M) return;   // whole quads: cpr is a multiple of 4
     const int col = 8 * (int)(i - row * cpr), valid = e.N - col;
-    float v[8] = {};
+    float v[1][8] = {};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         float p[8];
         load8(part + ((int64_t)s * e.M + row) * e.N + col, valid, p);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += p[k];
+        for (int k = 0; k < 8; ++k) v[0][k] += p[k];
     }
-    finish8<T>(e, row, col, v);
+    finish<T, 1>(e, row, 1, col, v);
 }
 
 // ───────────────────────────── dz and the bias gradient ─────────────────────────────
@@ -749,51 +882,67 @@ struct DactArgs {
 };
 
 // dz = dy·act'(z) in chunks of 8 columns: TX chunks across, 256/TX rows down
-// a block, rows strided over gridDim.y.
+// a block, rows strided over gridDim.y, four of them loaded at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
+    constexpr int U = 4;
     __shared__ float sums[256 * 8];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, TY = 256 / TX;
     const int col = 8 * (blockIdx.x * TX + tx), valid = a.N - col;
+    const int64_t step = (int64_t)gridDim.y * TY, np = padded(a.N);
     float s[8] = {};
     if (col < a.ldz || valid > 0) {
-        for (int64_t row = (int64_t)blockIdx.y * TY + ty; row < a.M; row += (int64_t)gridDim.y * TY) {
-            float d[8];
-            if (a.dy32)
-                load8(reinterpret_cast<const float*>(a.dy) + row * a.lddy + col, valid, d);
-            else
-                load8(reinterpret_cast<const T*>(a.dy) + row * a.lddy + col, valid, d);
-            if (a.act != ACT_NONE) {
-                float z[8];
-                if (a.codes) {
-                    const int64_t at = row * padded(a.N) + col;
-                    if (valid > 0)
-                        decode8(*reinterpret_cast<const uint2*>(a.codes + at), a.scales[at / GROUP], z);
-                    else
-                        for (int i = 0; i < 8; ++i) z[i] = 0.0f;
-                } else {
-                    load8(reinterpret_cast<const T*>(a.kept) + row * a.N + col, valid, z);
-                    load_rem8<T>(a.rem + row * a.N + col, valid, z);
-                }
+        for (int64_t first = (int64_t)blockIdx.y * TY + ty; first < a.M; first += U * step) {
+            float d[U][8], z[U][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float m;
-                    if (a.act == ACT_RELU2) {
-                        const float r = a.from_y ? sqrtf(z[i]) : (z[i] > 0.0f || z[i] != z[i] ? z[i] : 0.0f);
-                        m = 2.0f * r;
-                    } else if (a.act == ACT_TANH) {
-                        const float h = a.codes ? tanhf(z[i]) : z[i];
-                        m = 1.0f - h * h;
-                    } else {
-                        const float h = a.codes ? 1.0f / (1.0f + __expf(-z[i])) : z[i];
-                        m = h * (1.0f - h);
-                    }
-                    d[i] = i < valid ? d[i] * m : 0.0f;
+            for (int u = 0; u < U; ++u) {   // rows past the end: the first again, without a store
+                const int64_t row = first + u * step < a.M ? first + u * step : first;
+                if (a.dy32)
+                    load8(reinterpret_cast<const float*>(a.dy) + row * a.lddy + col, valid, d[u]);
+                else
+                    load8(reinterpret_cast<const T*>(a.dy) + row * a.lddy + col, valid, d[u]);
+                if (a.act == ACT_NONE) continue;
+                if (a.codes) {
+                    const int64_t at = row * np + (valid > 0 ? col : 0);
+                    decode8(*reinterpret_cast<const uint2*>(a.codes + at), a.scales[at / GROUP], z[u]);
+                } else {
+                    load8(reinterpret_cast<const T*>(a.kept) + row * a.N + col, valid, z[u]);
+                    load_rem8<T>(a.rem + row * a.N + col, valid, z[u]);
                 }
             }
+            // the factor of dy
+            if (a.act == ACT_RELU2 && a.from_y) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += d[i];
-            if (a.dz) store8(reinterpret_cast<T*>(a.dz) + row * a.ldz + col, (int)min(a.ldz - col, (int64_t)8), d);
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[u][i] *= 2.0f * __builtin_amdgcn_sqrtf(z[u][i]);
+            } else if (a.act == ACT_RELU2) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[u][i] *= z[u][i] < 0.0f ? 0.0f : 2.0f * z[u][i];   // a NaN stays one
+            } else if (a.act != ACT_NONE) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float h = z[u][i];
+                        if (a.codes) h = a.act == ACT_TANH ? tanh_of(h) : sigmoid_of(h);
+                        d[u][i] *= a.act == ACT_TANH ? 1.0f - h * h : h * (1.0f - h);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t row = first + u * step;
+                if (row >= a.M) continue;
+                if (valid < 8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[u][i] = i < valid ? d[u][i] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] += d[u][i];
+                if (a.dz) store8(reinterpret_cast<T*>(a.dz) + row * a.ldz + col, (int)min(a.ldz - col, (int64_t)8), d[u]);
+            }
         }
     }
     if (!a.part) return;
