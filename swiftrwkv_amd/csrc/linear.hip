@@ -361,19 +361,57 @@ struct GemmArgs {
     int64_t M;
     int N, K;
     int KB;               // rows of a k-major B: K, or less where A's last columns are padding zeros
-    int splits, per;      // K ranges of `per` stages each; > 1: fp32 sums into part [splits][M][N]
+    int full;             // tiles taken whole; the others in `splits` K ranges of `per` stages each,
+    int splits, per;      //   fp32 sums into part [splits][tiles - full][tile]
     float* part;
     Epilogue e;
 };
 
+// Tile `id`: tiles in groups of 4 row blocks × every column
+// block, column-major within a group; XCD x (workgroups x, x + 8, ...) takes a
+// contiguous run of that order, so its workgroups share operand blocks in its
+// L2.
+__device__ __forceinline__ void tile_of(int id, int ntm, int ntn, int& tm, int& tn) {
+    const int total = ntm * ntn, xcd = id & 7, loc = id >> 3;
+    const int t = xcd * (total >> 3) + min(xcd, total & 7) + loc;
+    const int grp = t / (4 * ntn), first = 4 * grp, gm = min(4, ntm - first);
+    const int rr = t - grp * 4 * ntn;
+    tm = first + rr % gm;
+    tn = rr / gm;
+}
+
+// A workgroup's piece: a tile, and the stages of it.
+struct Item {
+    int tm, tn, st0, st1;
+    int part;   // index of its partial tile; -1: the tile is whole
+};
+__device__ __forceinline__ Item item_of(const GemmArgs& g, int id, int ntm, int ntn) {
+    const int rest = ntm * ntn - g.full, nst = (g.K + BK - 1) / BK;
+    Item it;
+    if (id < g.full) {
+        tile_of(id, ntm, ntn, it.tm, it.tn);
+        it.st0 = 0, it.st1 = nst, it.part = -1;
+    } else {
+        it.part = id - g.full;
+        const int split = it.part / rest;
+        tile_of(g.full + it.part - split * rest, ntm, ntn, it.tm, it.tn);
+        it.st0 = split * g.per, it.st1 = min(nst, it.st0 + g.per);
+    }
+    return it;
+}
+__device__ __forceinline__ int items_of(const GemmArgs& g, int ntm, int ntn) {
+    return g.full + (ntm * ntn - g.full) * g.splits;
+}
+
 // A wave's 16·AM × 16·AN products, RC row tiles at a time through its own
-// 16·RC · EROW floats of LDS, so that a lane gets eight neighbouring columns.
+// 16·RC · EROW floats of LDS, so that a lane gets eight neighbouring columns;
+// or into the wave's place in a partial tile, if there is one.
 template <int AN>
 constexpr int EROW = 16 * AN + 4;   // floats per staged row
 
 template <typename T, int AM, int AN, int RC>
 __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc)[AM][AN], float* stage, int64_t row0,
-                                            int col0, int lane) {
+                                            int col0, int lane, float* part, int pitch) {
     static_assert(AM % RC == 0, "row tiles per pass");
     constexpr int LPR = 2 * AN, RPP = 64 / LPR;   // lanes per row, rows per step
     const int gq = lane >> 4, li = lane & 15;
@@ -400,11 +438,10 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc
                 v[c][0] = lo.x; v[c][1] = lo.y; v[c][2] = lo.z; v[c][3] = lo.w;
                 v[c][4] = hi.x; v[c][5] = hi.y; v[c][6] = hi.z; v[c][7] = hi.w;
             }
-            if (g.splits > 1) {
+            if (part) {
 #pragma unroll
                 for (int c = 0; c < C; ++c)
-                    if (row + c * RPP < g.M)
-                        store8(g.part + ((int64_t)blockIdx.y * g.M + row + c * RPP) * g.N + col, g.N - col, v[c]);
+                    if (row + c * RPP < g.M) store8(part + (h * 16 * RC + rloc + c * RPP) * pitch + cl, 8, v[c]);
             } else {
                 finish<T, C>(g.e, row, RPP, col, v);
             }
@@ -422,18 +459,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void gemm_kernel
     static_assert(WM * WN * 32 * EROW<AN> * 4 <= 2 * STAGE, "epilogue staging");
     __shared__ __align__(16) char lds[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // Tiles in groups of 4 row blocks × every column block, column-major
-    // within a group; XCD x (workgroups x, x + 8, ...) takes a contiguous run
-    // of that order, so its workgroups share operand blocks in its L2.
-    const int ntm = (int)((g.M + BM - 1) / BM), ntn = (g.N + BN - 1) / BN, total = ntm * ntn;
-    const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3;
-    const int t = xcd * (total >> 3) + min(xcd, total & 7) + loc;
-    const int grp = t / (4 * ntn), first = 4 * grp, gm = min(4, ntm - first);
-    const int rr = t - grp * 4 * ntn;
-    const int64_t m0 = (int64_t)(first + rr % gm) * BM;
-    const int n0 = (rr / gm) * BN;
-    const int nst = (g.K + BK - 1) / BK;
-    const int st0 = blockIdx.y * g.per, st1 = min(nst, st0 + g.per);
+    const int ntm = (int)((g.M + BM - 1) / BM), ntn = (g.N + BN - 1) / BN, tiles = ntm * ntn;
+    const Item it = item_of(g, blockIdx.x, ntm, ntn);
+    const int64_t m0 = (int64_t)it.tm * BM;
+    const int n0 = it.tn * BN;
+    const int st0 = it.st0, st1 = it.st1;
 
     const TileA ta(g.a, g.lda, m0, g.M, g.K, tid);
     const TileB tb(g.b, g.ldb, n0, g.N, g.KB, tid);
@@ -476,8 +506,9 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void gemm_kernel
         __syncthreads();
     }
 
+    float* const part = it.part < 0 ? nullptr : g.part + (int64_t)it.part * BM * BN + wm * AM * 16 * BN + wn * AN * 16;
     finish_tile<T, AM, AN, 2>(g, acc, reinterpret_cast<float*>(lds) + wave * 32 * EROW<AN>, m0 + wm * AM * 16,
-                              n0 + wn * AN * 16, lane);
+                              n0 + wn * AN * 16, lane, part, BN);
 }
 
 // ───────────────────────────── whole tiles: loads straight into LDS ─────────────────────────────
@@ -509,7 +540,7 @@ __device__ __forceinline__ i32x4 rsrc_of(uint64_t base, uint32_t bytes) {
 // ROWS × BK of an operand with 16-byte aligned rows, as Tile lays it out.  A
 // load covers 1024 LDS bytes; the permutation of the LDS layout is applied to
 // the global addresses its lanes read.
-template <typename T, bool KM, int ROWS, int WAVES>
+template <typename T, bool KM, int ROWS, int WAVES, bool FEW>
 struct DmaTile {
     static constexpr int P = ROWS / 8 / WAVES;       // loads per wave and stage
     static constexpr int KR = KM ? 512 / ROWS : 0;   // k rows per load
@@ -521,22 +552,30 @@ struct DmaTile {
     int64_t ld;
     int k, cols;       // k from the stage's start to the operand's end; k-major: columns, to whole dwords
     uint32_t x;        // k-contiguous: sends offsets past the last k out of range
-    uint32_t off[P];   // the lane's byte offset of each load
+    // the lane's byte offset of each load; FEW: of the first, odd and even, where
+    // registers are short (k-major)
+    uint32_t off[FEW && KM ? 2 : P];
     int c;             // k-contiguous: the lane's k within a stage
 
     __device__ __forceinline__ DmaTile(int64_t ld_, int wave, int lane) : r{}, ld(ld_), k(0), cols(0), x(0), c(0) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {   // LDS bytes 1024·(j·WAVES + wave) of the tile
             if constexpr (KM) {
-                const int k = (j * WAVES + wave) * KR + lane / (ROWS / 8), pos = lane % (ROWS / 8);
-                const int chunk = (((pos >> 1) ^ Read::slot_mask(k)) << 1) | (pos & 1);
-                off[j] = (uint32_t)(k * (int)ld + 8 * chunk) * 2;
+                if (FEW && j > 1) continue;
+                const int kr = (j * WAVES + wave) * KR + lane / (ROWS / 8), pos = lane % (ROWS / 8);
+                const int chunk = (((pos >> 1) ^ Read::slot_mask(kr)) << 1) | (pos & 1);
+                off[j] = (uint32_t)(kr * (int)ld + 8 * chunk) * 2;
             } else {
-                const int r = (j * WAVES + wave) * 8 + (lane >> 3);
-                c = 8 * ((lane & 7) ^ (r & 7));   // (r & 7 is the same for every j)
-                off[j] = (uint32_t)(r * (int)ld + c) * 2;
+                const int row = (j * WAVES + wave) * 8 + (lane >> 3);
+                c = 8 * ((lane & 7) ^ (row & 7));   // the same for every j
+                off[j] = (uint32_t)(row * (int)ld + c) * 2;
             }
         }
+    }
+    template <int j>
+    __device__ __forceinline__ uint32_t at() const {
+        if constexpr (FEW && KM) return off[j & 1] + (uint32_t)((j >> 1) * 2 * WAVES * KR * (int)ld) * 2;
+        else return KM ? off[j] : off[j] | x;
     }
 
     // Row (column) `at` of `total`, stage st of an operand of K.
@@ -569,37 +608,10 @@ private:
     __device__ __forceinline__ uint32_t beyond() const { return KM || c < k ? 0u : 0x80000000u; }
 };
 
-// The tile of workgroup `id`: tiles in groups of 4 row blocks × every column
-// block, column-major within a group; XCD x (workgroups x, x + 8, ...) takes a
-// contiguous run of that order, so its workgroups share operand blocks in its
-// L2.
-__device__ __forceinline__ void tile_of(int id, int ntm, int ntn, int& tm, int& tn) {
-    const int total = ntm * ntn, xcd = id & 7, loc = id >> 3;
-    const int t = xcd * (total >> 3) + min(xcd, total & 7) + loc;
-    const int grp = t / (4 * ntn), first = 4 * grp, gm = min(4, ntm - first);
-    const int rr = t - grp * 4 * ntn;
-    tm = first + rr % gm;
-    tn = rr / gm;
-}
-
-// Lanes of odd 16-lane rows of a and of even ones of b change places.
-__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    typedef T T2 __attribute__((ext_vector_type(2)));
-    const T2 v = {(T)a, (T)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
-
 enum { EPI_PLAIN, EPI_PART, EPI_FULL };
 
-// C = A·Bᵀ on whole tiles.  A workgroup walks the work items (tile, K range)
-// blockIdx.x, + gridDim.x, ...; its loads run two stages ahead of the products
+// C = A·Bᵀ.  A workgroup walks the items (tile, K range) blockIdx.x,
+// + gridDim.x, ...; its loads run two stages ahead of the products
 // straight through the items' ends.  A stage is two halves of 32 k: while the
 // matrix cores work on one half's operands the other's are read.  After two
 // thirds of the first half every wave has read the stage's buffer, which is
@@ -613,8 +625,8 @@ enum { EPI_PLAIN, EPI_PART, EPI_FULL };
 template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     constexpr int BM = 16 * WM * AM, BN = 16 * WN * AN, W = WM * WN;
-    using DA = DmaTile<T, AKM, BM, W>;
-    using DB = DmaTile<T, BKM, BN, W>;
+    using DA = DmaTile<T, AKM, BM, W, EPI == EPI_PART>;
+    using DB = DmaTile<T, BKM, BN, W, EPI == EPI_PART>;
     using TileA = typename DA::Read;
     using TileB = typename DB::Read;
     constexpr uint32_t STAGE = DA::BYTES + DB::BYTES;
@@ -628,10 +640,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     constexpr int SM = MA / 6;   // the loader's steps: beside every SM-th before MA
     static_assert(RM * NF <= MA && MB + RM * NF <= NM && MA + LM * ND <= 2 * NM, "places of a stage");
     constexpr int CPR = 4 * AN;   // 16-byte chunks of a staged row of the epilogue
-    __shared__ __align__(1024) char lds[2 * STAGE + (EPI == EPI_FULL ? W * 16 * CPR * 16 : 0)];
+    __shared__ __align__(1024) char lds[2 * STAGE + (EPI == EPI_PART ? 0 : W * 16 * CPR * 16)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int ntm = (int)((g.M + BM - 1) / BM), ntn = (g.N + BN - 1) / BN, tiles = ntm * ntn, items = tiles * g.splits;
-    const int nst = (g.K + BK - 1) / BK;
+    const int ntm = (int)((g.M + BM - 1) / BM), ntn = (g.N + BN - 1) / BN;
+    // the whole tiles, or the pieces of the others
+    const int first = (EPI == EPI_PART ? g.full : 0) + blockIdx.x, items = EPI == EPI_PART ? items_of(g, ntm, ntn) : g.full;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const int wm = wave % WM, wn = wave / WM;
 
@@ -639,15 +652,13 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     // its stage; a step to the next stage has six parts
     DA da(g.lda, wave, lane);
     DB db(g.ldb, wave, lane);
-    int l_item = blockIdx.x, l_left = 0;
+    int l_item = first, l_left = 0;
     auto start = [&] {
         if (l_item < items) {
-            const int split = l_item / tiles, st = split * g.per;
-            int tm, tn;
-            tile_of(l_item - split * tiles, ntm, ntn, tm, tn);
-            da.start(g.a, (int64_t)tm * BM, g.M, g.K, st);
-            db.start(g.b, (int64_t)tn * BN, g.N, g.KB, st);
-            l_left = min(nst, st + g.per) - st;
+            const Item it = item_of(g, l_item, ntm, ntn);
+            da.start(g.a, (int64_t)it.tm * BM, g.M, g.K, it.st0);
+            db.start(g.b, (int64_t)it.tn * BN, g.N, g.KB, it.st0);
+            l_left = it.st1 - it.st0;
         } else {
             da.end();
             db.end();
@@ -671,8 +682,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
         lds_target<(j < DA::P ? 0 : DA::BYTES) + (j < DA::P ? j : j - DA::P) * W * 1024>(base + buf + wave * 1024);
     };
     auto load = [&](auto j) {
-        if constexpr (j < DA::P) load_to_lds(da.r, AKM ? da.off[j] : da.off[j] | da.x);
-        else load_to_lds(db.r, BKM ? db.off[j - DA::P] : db.off[j - DA::P] | db.x);
+        if constexpr (j < DA::P) load_to_lds(da.r, da.template at<j>());
+        else load_to_lds(db.r, db.template at<j - DA::P>());
     };
     auto load_all = [&](uint32_t buf) {
         unrolled([&](auto j) {
@@ -698,11 +709,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) read(0, 0, 0, f);
     uint32_t cur = 0;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int split = item / tiles;
-        int tm, tn;
-        tile_of(item - split * tiles, ntm, ntn, tm, tn);
-        const int count = min(nst, (split + 1) * g.per) - split * g.per;
+    for (int item = first; item < items; item += gridDim.x) {
+        const Item it = item_of(g, item, ntm, ntn);
+        const int count = it.st1 - it.st0;
 #pragma unroll
         for (int i = 0; i < AM; ++i)
 #pragma unroll
@@ -748,52 +757,20 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
             cur ^= STAGE;
         }
 
-        const int64_t row0 = (int64_t)tm * BM + wm * AM * 16;
-        const int col0 = tn * BN + wn * AN * 16, gq = lane >> 4, li = lane & 15;
-        if constexpr (EPI == EPI_PLAIN) {
-            // neighbouring lanes' fours become eights
+        int l = lane;
+        asm volatile("" : "+v"(l));   // addresses are formed here, not kept over the products
+        const int64_t row0 = (int64_t)it.tm * BM + wm * AM * 16;
+        const int col0 = it.tn * BN + wn * AN * 16, gq = l >> 4, li = l & 15;
+        if constexpr (EPI == EPI_PART) {
+            float* p = g.part + (int64_t)it.part * BM * BN + (wm * AM * 16 + li) * BN + wn * AN * 16 + 4 * gq;
+            int left = (int)min(g.M - row0, (int64_t)BM) - li;   // rows from the lane's on
 #pragma unroll
-            for (int i = 0; i < AM; ++i) {
-                __builtin_amdgcn_sched_barrier(0);   // a row tile's addresses at a time
-                const int64_t row = row0 + 16 * i + li;
+            for (int i = 0; i < AM; ++i, left -= 16, p += 16 * BN) {
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" : "+v"(p), "+v"(left));   // stepped, not formed ahead
+                if (left <= 0) continue;
 #pragma unroll
-                for (int j = 0; j < AN; j += 2) {
-                    uint32_t x0 = pack2<T>(acc[i][j][0], acc[i][j][1]), x1 = pack2<T>(acc[i][j][2], acc[i][j][3]);
-                    uint32_t y0 = pack2<T>(acc[i][j + 1][0], acc[i][j + 1][1]), y1 = pack2<T>(acc[i][j + 1][2], acc[i][j + 1][3]);
-                    swap16(x0, y0);
-                    swap16(x1, y1);
-                    const int col = col0 + 16 * (j + (gq & 1)) + 8 * (gq >> 1), valid = g.N - col;
-                    if (row >= g.M) continue;
-                    T* y = reinterpret_cast<T*>(g.e.y) + row * g.N + col;
-                    const uint32_t w[4] = {x0, x1, y0, y1};
-                    if (valid >= 8) {
-                        __builtin_memcpy(y, w, 16);
-                    } else {
-#pragma unroll 1
-                        for (int e = 0; e < valid; ++e) {
-                            const uint32_t d = e < 4 ? (e < 2 ? x0 : x1) : (e < 6 ? y0 : y1);
-                            reinterpret_cast<uint16_t*>(y)[e] = (uint16_t)(d >> (16 * (e & 1)));
-                        }
-                    }
-                }
-            }
-        } else if constexpr (EPI == EPI_PART) {
-#pragma unroll
-            for (int i = 0; i < AM; ++i) {
-                const int64_t row = row0 + 16 * i + li;
-                if (row >= g.M) continue;
-                float* p = g.part + ((int64_t)split * g.M + row) * g.N;
-#pragma unroll
-                for (int j = 0; j < AN; ++j) {
-                    const int col = col0 + 16 * j + 4 * gq, valid = g.N - col;
-                    if (valid >= 4) {
-                        __builtin_memcpy(p + col, &acc[i][j], 16);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 3; ++e)
-                            if (e < valid) p[col + e] = acc[i][j][e];
-                    }
-                }
+                for (int j = 0; j < AN; ++j) *reinterpret_cast<f32x4*>(p + 16 * j) = acc[i][j];
             }
         } else {
             // sixteen rows at a time through LDS of the wave's own; a rolled
@@ -809,18 +786,26 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
                         own[li * CPR + ((4 * j + gq) ^ li)] = make_float4(acc[k][j][0], acc[k][j][1], acc[k][j][2], acc[k][j][3]);
                 }
                 __builtin_amdgcn_wave_barrier();
-                constexpr int LPR = CPR / 2, RPP = 64 / LPR;   // lanes per row, rows per step
-                constexpr int C = 16 / RPP;
-                const int q = lane % LPR;
+                constexpr int LPR = CPR / 2, RPP = 64 / LPR, C = 16 / RPP;   // lanes per row, rows per step
+                const int q = l % LPR;
                 float v[C][8];
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const int r = c * RPP + lane / LPR;
+                    const int r = c * RPP + l / LPR;
                     const float4 lo = own[r * CPR + ((2 * q) ^ r)], hi = own[r * CPR + ((2 * q + 1) ^ r)];
                     v[c][0] = lo.x; v[c][1] = lo.y; v[c][2] = lo.z; v[c][3] = lo.w;
                     v[c][4] = hi.x; v[c][5] = hi.y; v[c][6] = hi.z; v[c][7] = hi.w;
                 }
-                finish<T, C>(g.e, row0 + 16 * i + lane / LPR, RPP, col0 + 8 * q, v);
+                const int64_t row = row0 + 16 * i + l / LPR;
+                const int col = col0 + 8 * q;
+                if constexpr (EPI == EPI_FULL) {
+                    finish<T, C>(g.e, row, RPP, col, v);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < C; ++c)
+                        if (row + c * RPP < g.M)
+                            store_raw(reinterpret_cast<T*>(g.e.y) + (row + c * RPP) * g.N + col, g.N - col, round8<T>(v[c]));
+                }
                 __builtin_amdgcn_wave_barrier();
             }
         }
@@ -828,23 +813,28 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads of stages that do not come still write LDS
 }
 
-// Sums the K ranges in order and finishes: a thread per 8 columns.
+// Sums the K ranges of the tiles from g.full on, in order, and finishes them:
+// a thread per 8 columns.
 template <typename T>
-__global__ __launch_bounds__(256) void split_reduce_kernel(const float* part, int splits, Epilogue e) {
-    const int cpr = (int)(padded(e.N) / 8);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = i / cpr;
-    if (row >= e.M) return;   // whole quads: cpr is a multiple of 4
-    const int col = 8 * (int)(i - row * cpr), valid = e.N - col;
+__global__ __launch_bounds__(256) void split_reduce_kernel(GemmArgs g, int BM, int BN, int ntm, int ntn) {
+    const int rest = ntm * ntn - g.full, per = BM * BN / 8 / 256;   // blocks per tile
+    const int t = blockIdx.x / per, at = (blockIdx.x - t * per) * 256 + threadIdx.x;
+    int tm, tn;
+    tile_of(g.full + t, ntm, ntn, tm, tn);
+    const int r = at / (BN / 8), c = 8 * (at - r * (BN / 8));
+    const int64_t row = (int64_t)tm * BM + r;
+    if (row >= g.M) return;   // whole quads: a row's chunks
+    const int col = tn * BN + c;
+    const float* p = g.part + ((int64_t)t * BM + r) * BN + c;
     float v[1][8] = {};
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        float p[8];
-        load8(part + ((int64_t)s * e.M + row) * e.N + col, valid, p);
+    for (int s = 0; s < g.splits; ++s) {
+        float q[8];
+        load8(p + (int64_t)s * rest * BM * BN, 8, q);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[0][k] += p[k];
+        for (int k = 0; k < 8; ++k) v[0][k] += q[k];
     }
-    finish<T, 1>(e, row, 1, col, v);
+    finish<T, 1>(g.e, row, 1, col, v);
 }
 
 // ───────────────────────────── dz and the bias gradient ─────────────────────────────
@@ -985,49 +975,88 @@ rwkv_status status_of(const char* what) {
 // ───────────────────────────── routes ─────────────────────────────
 
 struct Route {
-    int tile;       // output tile edge
-    int splits, per;
+    int bm, bn;       // output tile
+    int64_t full;     // tiles taken whole
+    int splits, per;  // K ranges of the others
 };
 
-int64_t tiles_of(int64_t M, int64_t N, int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); }
+int64_t tiles_of(int64_t M, int64_t N, int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
 
+// Microseconds of the output tiles, fitted to 3186 timings of 216 sizes (16 ..
+// 8192 rows, 96 .. 8192 columns, K 512 .. 8192), each tile in 1 .. 32 ranges of
+// K: a CU that takes n pieces of `stages` each needs
+//   start·⌈n / fit⌉ + stages·(first + more·(n − 1))·(1 + 0.23·share of busy CUs).
+// The cheapest of the four is 0.8 % behind the fastest one measured, in the mean.
+struct Shape {
+    int bm, bn, fit;
+    double start, first, more;
+};
+constexpr Shape SHAPES[] = {{256, 256, 1, 8.5, 1.10, 1.15}, {256, 128, 1, 2.8, 0.70, 0.73},
+                            {128, 128, 2, 1.8, 0.41, 0.40}, {64, 64, 4, 0.3, 0.245, 0.152}};
+
+double pieces_cost(const Shape& s, int64_t pieces, int stages) {
+    if (pieces == 0) return 0;
+    const int64_t n = (pieces + 255) / 256;
+    const double busy = std::min(1.0, pieces / 256.0);
+    return s.start * ((n + s.fit - 1) / s.fit) + stages * (s.first + s.more * (n - 1)) * (1 + 0.23 * busy);
+}
+
+// The tile, and how many of its tiles are taken whole: all; or whole rounds of
+// the 256 CUs, with the rest in ranges of K, for whose sums a second launch
+// (3.3 us) reads and writes 4 bytes a value and range at 6.4 TB/s.
 Route route_of(int64_t M, int64_t N, int64_t K, bool odd) {
     const int nst = (int)((K + BK - 1) / BK);
-    Route r{64, 1, nst};
-    if (!odd && tiles_of(M, N, 256) >= 200) r.tile = 256;
-    else if (tiles_of(M, N, 128) >= 200) r.tile = 128;
-    const int64_t tiles = tiles_of(M, N, r.tile);
-    int s = 1;
-    if (tiles < 256) s = (int)std::min<int64_t>(std::min<int64_t>(512 / tiles, (nst + 3) / 4), 32);
-    if (s > 1) {
-        r.per = (nst + s - 1) / s;
-        r.splits = (nst + r.per - 1) / r.per;
+    Route best{};
+    double least = 1e300;
+    for (const Shape& s : SHAPES) {
+        if (odd && s.bm == 256) continue;   // its loads want aligned rows
+        const int64_t tiles = tiles_of(M, N, s.bm, s.bn);
+        const double whole = pieces_cost(s, tiles, nst);
+        if (whole < least) least = whole, best = Route{s.bm, s.bn, tiles, 1, nst};
+        const int64_t round = s.fit > 1 ? tiles : 256, full = odd || tiles < 256 ? 0 : tiles / round * round, rest = tiles - full;
+        if (rest == 0 || rest > 256) continue;
+        const double before = full ? pieces_cost(s, full, nst) + 4 : 0;
+        for (int split = 2; split <= 32 && split * 2 <= nst; split = split < 4 ? split + 1 : split * 2) {
+            const int per = (nst + split - 1) / split, splits = (nst + per - 1) / per;
+            const double t = before + pieces_cost(s, rest * splits, per) + 3.3 + (double)(rest * splits) * s.bm * s.bn * 8 / 6.4e6;
+            if (t < least) least = t, best = Route{s.bm, s.bn, full, splits, per};
+        }
     }
-    return r;
+    return best;
 }
 
 int64_t route_workspace(const Route& r, int64_t M, int64_t N) {
-    return r.splits > 1 ? (int64_t)r.splits * M * N * 4 : 0;
+    const int64_t rest = tiles_of(M, N, r.bm, r.bn) - r.full;
+    return rest * r.splits * r.bm * r.bn * 4;
+}
+
+// The whole tiles, then the pieces of the others, on at most `fit` workgroups
+// (what the LDS of 256 CUs holds).
+template <typename T, bool AKM, bool BKM, int AM, int AN>
+void gemm_launch_dma(int fit, const GemmArgs& g, int64_t items, hipStream_t s) {
+    const dim3 whole((unsigned)std::min<int64_t>(g.full, fit)), pieces((unsigned)std::min<int64_t>(items - g.full, fit));
+    if (g.full > 0) {
+        if constexpr (!AKM && !BKM) {
+            if (g.e.plain) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN>, whole, dim3(256), s, g);
+            else rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_FULL>, whole, dim3(256), s, g);
+        } else {
+            rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN>, whole, dim3(256), s, g);
+        }
+    }
+    if (items > g.full) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PART>, pieces, dim3(256), s, g);
 }
 
 template <typename T, bool AKM, bool BKM, bool ODD>
 void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
-    const dim3 grid((unsigned)tiles_of(g.M, g.N, r.tile), (unsigned)r.splits);
+    const int64_t items = g.full + (tiles_of(g.M, g.N, r.bm, r.bn) - g.full) * g.splits;
+    const dim3 grid((unsigned)items);
     if constexpr (!ODD) {
-        if (r.tile == 256) {
-            // one workgroup per CU (its LDS) walks the items
-            const dim3 cus((unsigned)std::min<int64_t>(tiles_of(g.M, g.N, r.tile) * r.splits, 256));
-            if (r.splits > 1)
-                rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, 8, 8, EPI_PART>, cus, dim3(256), s, g);
-            else if (g.e.plain)
-                rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, 8, 8, EPI_PLAIN>, cus, dim3(256), s, g);
-            else if constexpr (!AKM && !BKM)
-                rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, 8, 8, EPI_FULL>, cus, dim3(256), s, g);
-            return;
-        }
+        if (r.bm == 256 && r.bn == 256) return gemm_launch_dma<T, AKM, BKM, 8, 8>(256, g, items, s);
+        if (r.bm == 256) return gemm_launch_dma<T, AKM, BKM, 8, 4>(256, g, items, s);
+        if (r.bm == 128) return gemm_launch_dma<T, AKM, BKM, 4, 4>(512, g, items, s);
     }
-    if (r.tile == 128)
-        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 4, 4, ODD>, grid, dim3(256), s, g);
+    if (r.bm == 128)
+        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 4, 4, true>, grid, dim3(256), s, g);
     else
         rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 2, 2, ODD>, grid, dim3(256), s, g);
 }
@@ -1038,25 +1067,25 @@ rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, v
     const bool aligned = (uintptr_t)g.a % 16 == 0 && (uintptr_t)g.b % 16 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0;
     const bool odd = !aligned || ((!akm || !bkm) && g.K % 8 != 0);
     const Route r = route_of(g.M, g.N, g.K, odd);
-    RWKV_REQUIRE(tiles_of(g.M, g.N, r.tile) < (int64_t(1) << 31), RWKV_E_SHAPE, "%s: too many output tiles", what);
+    const int64_t tiles = tiles_of(g.M, g.N, r.bm, r.bn), rest = tiles - r.full;
+    RWKV_REQUIRE(r.full + rest * r.splits < (int64_t(1) << 22), RWKV_E_SHAPE, "%s: too many output tiles", what);
     const int64_t need = route_workspace(r, g.M, g.N);
     RWKV_REQUIRE(need == 0 || (workspace && bytes >= need && (uintptr_t)workspace % 16 == 0), RWKV_E_SHAPE,
                  "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need);
+    g.full = (int)r.full;
     g.splits = r.splits;
     g.per = r.per;
+    g.part = (float*)workspace;
     g.e.plain = !g.e.bias && !g.e.res && !g.e.wide && !g.e.aux && !g.e.rem && !g.e.codes && g.e.act == ACT_NONE;
-    g.part = r.splits > 1 ? (float*)workspace : nullptr;
     auto by_layout = [&](auto type, auto o) {
         using T = decltype(type);
         constexpr bool O = decltype(o)::value;
         if (!akm && !bkm) gemm_launch_tile<T, false, false, O>(r, g, s);
         else if (!akm) gemm_launch_tile<T, false, true, O>(r, g, s);
         else gemm_launch_tile<T, true, true, O>(r, g, s);
-        if (r.splits > 1) {
-            const int64_t chunks = g.M * (padded(g.N) / 8);
-            rwkv::launch(split_reduce_kernel<T>, dim3((unsigned)((chunks + 255) / 256)), dim3(256), s, g.part, r.splits,
-                         g.e);
-        }
+        if (rest > 0)
+            rwkv::launch(split_reduce_kernel<T>, dim3((unsigned)(rest * (r.bm * r.bn / 2048))), dim3(256), s, g, r.bm, r.bn,
+                         (int)((g.M + r.bm - 1) / r.bm), (int)((g.N + r.bn - 1) / r.bn));
     };
     if (dt == RWKV_BF16 && odd) by_layout(bf16{}, std::true_type{});
     else if (dt == RWKV_BF16) by_layout(bf16{}, std::false_type{});
