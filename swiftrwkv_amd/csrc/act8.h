@@ -48,6 +48,29 @@ __device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
     }
 }
 
+// Eight values as loaded, to be converted later: a row that is on its way
+// while another is worked on.
+template <typename T>
+struct Raw8 {
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, int valid) {
+        if (valid >= 8) {
+            __builtin_memcpy(q, p, sizeof(q));
+        } else {
+            T t[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = i < valid ? p[i] : (T)0.0f;
+            __builtin_memcpy(q, t, sizeof(q));
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        T t[8];
+        __builtin_memcpy(t, q, sizeof(q));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f(t[i]);
+    }
+};
+
 // Stores the first `valid` of eight values, each rounded once to T.
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {

@@ -1003,8 +1003,10 @@ double pieces_cost(const Shape& s, int64_t pieces, int stages) {
 
 // The tile, and how many of its tiles are taken whole: all; or whole rounds of
 // the 256 CUs, with the rest in ranges of K, for whose sums a second launch
-// (3.3 us) reads and writes 4 bytes a value and range at 6.4 TB/s.
-Route route_of(int64_t M, int64_t N, int64_t K, bool odd) {
+// (3.3 us) reads and writes 4 bytes a value and range at 6.4 TB/s.  km: both
+// operands k-major, for which the largest tile has no kernel for ranges (it
+// would spill registers, whose reloads wait for every load before them).
+Route route_of(int64_t M, int64_t N, int64_t K, bool odd, bool km) {
     const int nst = (int)((K + BK - 1) / BK);
     Route best{};
     double least = 1e300;
@@ -1014,7 +1016,7 @@ Route route_of(int64_t M, int64_t N, int64_t K, bool odd) {
         const double whole = pieces_cost(s, tiles, nst);
         if (whole < least) least = whole, best = Route{s.bm, s.bn, tiles, 1, nst};
         const int64_t round = s.fit > 1 ? tiles : 256, full = odd || tiles < 256 ? 0 : tiles / round * round, rest = tiles - full;
-        if (rest == 0 || rest > 256) continue;
+        if (rest == 0 || rest > 256 || (km && s.bn == 256)) continue;
         const double before = full ? pieces_cost(s, full, nst) + 4 : 0;
         for (int split = 2; split <= 32 && split * 2 <= nst; split = split < 4 ? split + 1 : split * 2) {
             const int per = (nst + split - 1) / split, splits = (nst + per - 1) / per;
@@ -1043,7 +1045,8 @@ void gemm_launch_dma(int fit, const GemmArgs& g, int64_t items, hipStream_t s) {
             rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN>, whole, dim3(256), s, g);
         }
     }
-    if (items > g.full) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PART>, pieces, dim3(256), s, g);
+    if constexpr (!(AKM && BKM && AN == 8))
+        if (items > g.full) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PART>, pieces, dim3(256), s, g);
 }
 
 template <typename T, bool AKM, bool BKM, bool ODD>
@@ -1066,7 +1069,7 @@ rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, v
                      hipStream_t s) {
     const bool aligned = (uintptr_t)g.a % 16 == 0 && (uintptr_t)g.b % 16 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0;
     const bool odd = !aligned || ((!akm || !bkm) && g.K % 8 != 0);
-    const Route r = route_of(g.M, g.N, g.K, odd);
+    const Route r = route_of(g.M, g.N, g.K, odd, akm && bkm);
     const int64_t tiles = tiles_of(g.M, g.N, r.bm, r.bn), rest = tiles - r.full;
     RWKV_REQUIRE(r.full + rest * r.splits < (int64_t(1) << 22), RWKV_E_SHAPE, "%s: too many output tiles", what);
     const int64_t need = route_workspace(r, g.M, g.N);
@@ -1095,9 +1098,9 @@ rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, v
 }
 
 // For either kind of alignment (the pointers are not known yet).
-int64_t gemm_workspace(int64_t M, int64_t N, int64_t K) {
+int64_t gemm_workspace(int64_t M, int64_t N, int64_t K, bool km) {
     if (M == 0) return 0;
-    return std::max(route_workspace(route_of(M, N, K, false), M, N), route_workspace(route_of(M, N, K, true), M, N));
+    return std::max(route_workspace(route_of(M, N, K, false, km), M, N), route_workspace(route_of(M, N, K, true, km), M, N));
 }
 
 bool shape_ok(int64_t M, int64_t N, int64_t K) {
@@ -1121,7 +1124,7 @@ void dact_geometry(int64_t M, int64_t N, int& TX, int& gx, int& gy) {
 extern "C" {
 
 int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K) {
-    return shape_ok(M, N, K) ? gemm_workspace(M, N, K) : 0;
+    return shape_ok(M, N, K) ? gemm_workspace(M, N, K, false) : 0;
 }
 
 rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -1189,7 +1192,7 @@ rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, con
 }
 
 int64_t rwkv_linear_dgrad_workspace(int64_t M, int64_t N, int64_t K) {
-    return shape_ok(M, N, K) ? gemm_workspace(M, K, N) : 0;
+    return shape_ok(M, N, K) ? gemm_workspace(M, K, N, false) : 0;
 }
 
 rwkv_status rwkv_linear_dgrad(const void* dz, int64_t ldz, const void* w, int64_t ldw, void* dx, rwkv_dtype dt,
@@ -1211,7 +1214,7 @@ rwkv_status rwkv_linear_dgrad(const void* dz, int64_t ldz, const void* w, int64_
 }
 
 int64_t rwkv_linear_wgrad_workspace(int64_t M, int64_t N, int64_t K) {
-    return shape_ok(M, N, K) && M > 0 ? gemm_workspace(N, K, M) : 0;
+    return shape_ok(M, N, K) && M > 0 ? gemm_workspace(N, K, M, true) : 0;
 }
 
 rwkv_status rwkv_linear_wgrad(const void* dz, int64_t ldz, const void* x, int64_t ldx, void* dw, rwkv_dtype dt,

@@ -70,62 +70,87 @@ __device__ __forceinline__ void load_w(const void* w, int w32, int col, int vali
 }
 
 // TPR threads hold one row in registers, thread t the 8-value chunks
-// t + TPR·j, j < NV.
+// t + TPR·j, j < NV, and walk the rows blockIdx.x·RPB + threadIdx.x / TPR,
+// + gridDim.x·RPB, ...: up to 16384 columns w and b stay in registers from row
+// to row (fp32 weights are four times a bf16 row's bytes) and the next row is
+// loaded while one is worked on.
 template <typename TX, typename TY, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd_kernel(NormFwd a) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    constexpr bool HOLD = NV <= 4;
     __shared__ float part[2][16];
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (row >= a.N) return;   // whole waves; no row shares a barrier where RPB > 1
-    const TX* xr = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
-    float v[NV][8];
-    float s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int col = 8 * (t + TPR * j);
-        load8(xr + col, a.D - col, v[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[j][i];
-    const float mean = row_sum<TPR>(s, part, 0) / (float)a.D;
-    float q = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int col = 8 * (t + TPR * j);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float d = v[j][i] - mean;
-            q += col + i < a.D ? d * d : 0.0f;
-        }
-    }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, part, 1) / (float)a.D + a.eps);
-    if (a.stats && t == 0) {
-        a.stats[2 * row] = mean;
-        a.stats[2 * row + 1] = rstd;
-    }
-    TY* yr = reinterpret_cast<TY*>(a.y) + row * a.D;
+    const TX* x = reinterpret_cast<const TX*>(a.x);
     const int64_t dp = padded(a.D);
+    float w[HOLD ? NV : 1][8], b[HOLD ? NV : 1][8];
+    Raw8<TX> next[NV];
+    auto load_row = [&](int64_t r) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int col = 8 * (t + TPR * j), valid = a.D - col;
-        if (a.codes && col < dp) {   // whole quads: dp is a multiple of 32
-            uint32_t scale;
-            const uint2 c = encode8(v[j], scale);
-            *reinterpret_cast<uint2*>(a.codes + row * dp + col) = c;
-            if ((t & 3) == 0) a.scales[(row * dp + col) / GROUP] = (uint8_t)scale;
+        for (int j = 0; j < NV; ++j) next[j].load(x + r * a.ldx + 8 * (t + TPR * j), a.D - 8 * (t + TPR * j));
+    };
+    if constexpr (HOLD) {
+        load_row(row);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = 8 * (t + TPR * j);
+            load_w<TX>(a.w, a.w32, col, a.D - col, w[j]);
+            if (a.b) load_w<TX>(a.b, a.w32, col, a.D - col, b[j]);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[j][i] = 0.0f;
         }
-        if (valid > 0) {
-            float w[8], y[8];
-            load_w<TX>(a.w, a.w32, col, valid, w);
+    }
+    for (; row < a.N; row += step) {
+        float v[NV][8];
+        float s = 0.0f;
+        if constexpr (!HOLD) load_row(row);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = (v[j][i] - mean) * rstd * w[i];
-            if (a.b) {
-                load_w<TX>(a.b, a.w32, col, valid, w);
+        for (int j = 0; j < NV; ++j) next[j].get(v[j]);
+        if (HOLD && row + step < a.N) load_row(row + step);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] += w[i];
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[j][i];
+        const float mean = row_sum<TPR>(s, part, 0) / (float)a.D;
+        float q = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = 8 * (t + TPR * j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = v[j][i] - mean;
+                q += col + i < a.D ? d * d : 0.0f;
+            }
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, part, 1) / (float)a.D + a.eps);
+        if (a.stats && t == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mean, rstd);
+        TY* yr = reinterpret_cast<TY*>(a.y) + row * a.D;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = 8 * (t + TPR * j), valid = a.D - col;
+            if (a.codes && col < dp) {   // whole quads: dp is a multiple of 32
+                uint32_t scale;
+                const uint2 c = encode8(v[j], scale);
+                *reinterpret_cast<uint2*>(a.codes + row * dp + col) = c;
+                if ((t & 3) == 0) a.scales[(row * dp + col) / GROUP] = (uint8_t)scale;
+            }
+            if (valid <= 0) continue;
+            float y[8];
+            if constexpr (HOLD) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = (v[j][i] - mean) * rstd * w[j][i] + b[j][i];
+            } else {
+                load_w<TX>(a.w, a.w32, col, valid, w[0]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = (v[j][i] - mean) * rstd * w[0][i];
+                if (a.b) {
+                    load_w<TX>(a.b, a.w32, col, valid, w[0]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] += w[0][i];
+                }
             }
             store8(yr + col, valid, y);
         }
@@ -148,49 +173,74 @@ struct NormBwd {
 };
 
 // Block b walks the rows b·RPB + threadIdx.x / TPR, + gridDim.x·RPB, ...; a
-// thread's columns never change, so their dw / db sums stay in its registers
-// until the end, where the block's row groups add theirs in order.
+// thread's columns never change, so w and their dw / db sums stay in its
+// registers until the end, where the block's row groups add theirs in order.
+// The next row is loaded while one is worked on.
 template <typename TX, typename TY, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd_kernel(NormBwd a) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    constexpr bool HOLD = NV <= 4;
     __shared__ float part[4][16];
     __shared__ float sums[RPB > 1 ? 2 * TPR * NV * 8 : 1];
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-    const int64_t dp = padded(a.D);
+    const int64_t dp = padded(a.D), step = (int64_t)gridDim.x * RPB;
     float dw[NV][8] = {}, db[NV][8] = {};
-    int slot = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPB + grp; row < a.N; row += (int64_t)gridDim.x * RPB) {
-        const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
-        float xh[NV][8], g[NV][8];
-        float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int col = 8 * (t + TPR * j), valid = a.D - col;
-            if (valid <= 0) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) xh[j][i] = g[j][i] = 0.0f;
-                continue;
-            }
-            load8(reinterpret_cast<const TY*>(a.dy) + row * a.D + col, valid, g[j]);
-            if (a.codes) {
-                const int64_t at = row * dp + col;
-                decode8(*reinterpret_cast<const uint2*>(a.codes + at), a.scales[at / GROUP], xh[j]);
-            } else {
-                load8(reinterpret_cast<const TX*>(a.x) + row * a.ldx + col, valid, xh[j]);
-            }
-        }
+    float w[HOLD ? NV : 1][8];
+    Raw8<TY> gr[NV];
+    Raw8<TX> xr[NV];   // or codes in its first half and the scale behind
+    float mean_n = 0.0f, rstd_n = 0.0f;
+    auto load_row = [&](int64_t row) {
+        const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+        mean_n = st.x, rstd_n = st.y;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = 8 * (t + TPR * j), valid = a.D - col;
             if (valid <= 0) continue;
-            float w[8];
-            load_w<TX>(a.w, a.w32, col, valid, w);
+            gr[j].load(reinterpret_cast<const TY*>(a.dy) + row * a.D + col, valid);
+            if (a.codes) {
+                const int64_t at = row * dp + col;
+                const uint2 c = *reinterpret_cast<const uint2*>(a.codes + at);
+                xr[j].q[0] = make_uint4(c.x, c.y, a.scales[at / GROUP], 0u);
+            } else {
+                xr[j].load(reinterpret_cast<const TX*>(a.x) + row * a.ldx + col, valid);
+            }
+        }
+    };
+    int64_t row = (int64_t)blockIdx.x * RPB + grp;
+    if constexpr (HOLD) {
+        if (row < a.N) load_row(row);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load_w<TX>(a.w, a.w32, 8 * (t + TPR * j), a.D - 8 * (t + TPR * j), w[j]);
+    }
+    int slot = 0;
+    for (; row < a.N; row += step) {
+        if constexpr (!HOLD) load_row(row);
+        const float mean = mean_n, rstd = rstd_n;
+        float xh[NV][8], g[NV][8];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (a.D - 8 * (t + TPR * j) <= 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) xh[j][i] = g[j][i] = 0.0f;
+                continue;
+            }
+            gr[j].get(g[j]);
+            if (a.codes) decode8(make_uint2(xr[j].q[0].x, xr[j].q[0].y), xr[j].q[0].z, xh[j]);
+            else xr[j].get(xh[j]);
+        }
+        if (HOLD && row + step < a.N) load_row(row + step);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = 8 * (t + TPR * j), valid = a.D - col;
+            if (valid <= 0) continue;
+            if constexpr (!HOLD) load_w<TX>(a.w, a.w32, col, valid, w[0]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 xh[j][i] = i < valid ? (xh[j][i] - mean) * rstd : 0.0f;
                 dw[j][i] += g[j][i] * xh[j][i];
                 db[j][i] += g[j][i];
-                g[j][i] *= w[i];
+                g[j][i] *= w[HOLD ? j : 0][i];
                 s1 += g[j][i];
                 s2 += g[j][i] * xh[j][i];
             }
@@ -305,40 +355,43 @@ rwkv_status status_of(const char* what) {
     return RWKV_OK;
 }
 
-// Blocks of the backward pass: two per CU, or one per RPB rows of a small
-// call.  Each writes one partial row of dw and db.
+// Blocks of the backward pass: three per CU of 256 threads, two and one of
+// more; or one per RPB rows of a small call.  Each writes one partial row of
+// dw and db.
 int norm_bwd_blocks(int64_t N, int64_t D) {
-    const int rpb = D <= 2048 ? 4 : 1;
-    return (int)std::min<int64_t>((N + rpb - 1) / rpb, 512);
+    const int rpb = D <= 1024 ? 4 : 1, full = D <= 4096 ? 768 : D <= 8192 ? 512 : 256;
+    return (int)std::min<int64_t>((N + rpb - 1) / rpb, full);
 }
+
+// One wave per row up to 1024 columns, then a block: a thread holds 8 or 16
+// values of a row (the backward pass keeps five times as many registers).
+#define RWKV_NORM_WIDTHS(RUN)                      \
+    if (a.D <= 512) RUN(256, 64, 1)                \
+    else if (a.D <= 1024) RUN(256, 64, 2)          \
+    else if (a.D <= 2048) RUN(256, 256, 1)         \
+    else if (a.D <= 4096) RUN(256, 256, 2)         \
+    else if (a.D <= 8192) RUN(512, 512, 2)         \
+    else if (a.D <= 16384) RUN(1024, 1024, 2)      \
+    else RUN(1024, 1024, 8)
 
 template <typename TX, typename TY>
 void norm_fwd_launch(const NormFwd& a, hipStream_t s) {
-    const dim3 rows4((unsigned)((a.N + 3) / 4)), rows1((unsigned)a.N);
-#define RWKV_NORM(grid, threads, TPR, NV) rwkv::launch(norm_fwd_kernel<TX, TY, TPR, NV>, grid, dim3(threads), s, a)
-    if (a.D <= 512) RWKV_NORM(rows4, 256, 64, 1);
-    else if (a.D <= 1024) RWKV_NORM(rows4, 256, 64, 2);
-    else if (a.D <= 2048) RWKV_NORM(rows4, 256, 64, 4);
-    else if (a.D <= 4096) RWKV_NORM(rows1, 256, 256, 2);
-    else if (a.D <= 8192) RWKV_NORM(rows1, 256, 256, 4);
-    else if (a.D <= 16384) RWKV_NORM(rows1, 256, 256, 8);
-    else RWKV_NORM(rows1, 1024, 1024, 8);
-#undef RWKV_NORM
+    // rows beyond a full chip's are walked
+    const int64_t blocks = a.D <= 1024 ? (a.N + 3) / 4 : a.N, full = a.D <= 4096 ? 2048 : a.D <= 8192 ? 1024 : 512;
+    const dim3 grid((unsigned)std::min(blocks, full));
+#define RUN(threads, TPR, NV) rwkv::launch(norm_fwd_kernel<TX, TY, TPR, NV>, grid, dim3(threads), s, a);
+    RWKV_NORM_WIDTHS(RUN)
+#undef RUN
 }
 
 template <typename TX, typename TY>
 void norm_bwd_launch(const NormBwd& a, hipStream_t s) {
     const dim3 grid((unsigned)norm_bwd_blocks(a.N, a.D));
-#define RWKV_NORM(threads, TPR, NV) rwkv::launch(norm_bwd_kernel<TX, TY, TPR, NV>, grid, dim3(threads), s, a)
-    if (a.D <= 512) RWKV_NORM(256, 64, 1);
-    else if (a.D <= 1024) RWKV_NORM(256, 64, 2);
-    else if (a.D <= 2048) RWKV_NORM(256, 64, 4);
-    else if (a.D <= 4096) RWKV_NORM(256, 256, 2);
-    else if (a.D <= 8192) RWKV_NORM(256, 256, 4);
-    else if (a.D <= 16384) RWKV_NORM(256, 256, 8);
-    else RWKV_NORM(1024, 1024, 8);
-#undef RWKV_NORM
+#define RUN(threads, TPR, NV) rwkv::launch(norm_bwd_kernel<TX, TY, TPR, NV>, grid, dim3(threads), s, a);
+    RWKV_NORM_WIDTHS(RUN)
+#undef RUN
 }
+#undef RWKV_NORM_WIDTHS
 
 // Input and output types a norm takes: the same, or fp32 into 16 bits.
 bool norm_types(int x, int y) { return rwkv::dtype_ok(x) && rwkv::dtype_ok(y) && (x == y || x == RWKV_F32); }
