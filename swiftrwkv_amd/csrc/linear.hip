@@ -872,10 +872,11 @@ struct DactArgs {
 };
 
 // dz = dy·act'(z) in chunks of 8 columns: TX chunks across, 256/TX rows down
-// a block, rows strided over gridDim.y, four of them loaded at a time.
+// a block, rows strided over gridDim.y, two of them loaded at a time
+// (8192 x 8192 bf16 relu² from y: 4.96 TB/s; four at a time, on fewer waves, 3.97).
 template <typename T>
 __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
-    constexpr int U = 4;
+    constexpr int U = 2;
     __shared__ float sums[256 * 8];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, TY = 256 / TX;
     const int col = 8 * (blockIdx.x * TX + tx), valid = a.N - col;
@@ -885,8 +886,13 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
         for (int64_t first = (int64_t)blockIdx.y * TY + ty; first < a.M; first += U * step) {
             float d[U][8], z[U][8];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {   // rows past the end: the first again, without a store
-                const int64_t row = first + u * step < a.M ? first + u * step : first;
+            for (int u = 0; u < U; ++u) {
+                const int64_t row = first + u * step;
+                if (row >= a.M) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[u][i] = z[u][i] = 0.0f;
+                    continue;
+                }
                 if (a.dy32)
                     load8(reinterpret_cast<const float*>(a.dy) + row * a.lddy + col, valid, d[u]);
                 else
@@ -1109,14 +1115,15 @@ bool shape_ok(int64_t M, int64_t N, int64_t K) {
 bool half_ok(int dt) { return dt == RWKV_BF16 || dt == RWKV_F16; }
 bool ld_ok(int64_t ld, int64_t cols) { return ld >= cols && ld <= MAX_LD; }
 
-// Blocks down the rows of dact_kernel (each adds one partial row of db).
-void dact_geometry(int64_t M, int64_t N, int& TX, int& gx, int& gy) {
+// Blocks of dact_kernel: 2048 at most, half of that with db, to which each
+// block down the rows adds one partial row.
+void dact_geometry(int64_t M, int64_t N, bool db, int& TX, int& gx, int& gy) {
     const int64_t chunks = (N + 7) / 8;
     TX = 1;
     while (TX < 64 && TX < chunks) TX *= 2;
     gx = (int)((chunks + TX - 1) / TX);
     const int ty = 256 / TX;
-    gy = (int)std::max<int64_t>(1, std::min<int64_t>((M + ty - 1) / ty, std::max(1, 2048 / gx)));
+    gy = (int)std::max<int64_t>(1, std::min<int64_t>((M + ty - 1) / ty, std::max(1, (db ? 1024 : 2048) / gx)));
 }
 
 }  // namespace
@@ -1152,7 +1159,7 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
 int64_t rwkv_linear_dact_workspace(int64_t M, int64_t N) {
     if (!shape_ok(M, N, 1)) return 0;
     int TX, gx, gy;
-    dact_geometry(M, N, TX, gx, gy);
+    dact_geometry(M, N, true, TX, gx, gy);
     return (int64_t)gy * N * 4;
 }
 
@@ -1172,7 +1179,7 @@ rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, con
     RWKV_REQUIRE(!kept == !rem, RWKV_E_NULL, "linear_dact: kept and its remainders go together");
     RWKV_REQUIRE(M == 0 || (dy && (act == ACT_NONE || kept || codes)), RWKV_E_NULL, "linear_dact: null buffer");
     int TX, gx, gy;
-    dact_geometry(M, N, TX, gx, gy);
+    dact_geometry(M, N, db != nullptr, TX, gx, gy);
     RWKV_REQUIRE(!db || (workspace && workspace_bytes >= (int64_t)gy * N * 4 && (uintptr_t)workspace % 16 == 0),
                  RWKV_E_SHAPE, "linear_dact: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                  (long long)gy * N * 4);
