@@ -837,6 +837,77 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(GemmArgs g, int BM, i
     finish<T, 1>(g.e, row, 1, col, v);
 }
 
+// ───────────────────────────── a few rows ─────────────────────────────
+
+// x [M <= 16, K] through W: a block takes 16·NT columns (rows of W), its eight
+// waves every eighth 32 of k, straight from memory into the products' operands
+// (any alignment), the next U of each on their way under U products; their
+// sums meet in LDS, in order.
+template <typename T, int NT>
+__global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
+    constexpr int WAVES = 8, U = 8 / NT;
+    __shared__ __align__(16) float sums[WAVES][16][16 * NT + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i = lane & 15;
+    const int n0 = blockIdx.x * 16 * NT, steps = (g.K + 31) / 32;
+    const T* xr = reinterpret_cast<const T*>(g.a) + (int64_t)min(i, (int)g.M - 1) * g.lda;
+    const T* wr[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) wr[t] = reinterpret_cast<const T*>(g.b) + (int64_t)min(n0 + 16 * t + i, g.N - 1) * g.ldb;
+    auto chunk = [&](const T* p, int k) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (k + 8 <= g.K) {
+            __builtin_memcpy(&v, p + k, 16);
+        } else if (k < g.K) {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            for (int e = 0; e < 7; ++e)
+                if (k + e < g.K) w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[k + e] << (16 * (e & 1));
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return v;
+    };
+    uint4 w[NT][U], x[U];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (s + WAVES * u) * 32 + 8 * q;
+            x[u] = chunk(xr, k);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) w[t][u] = chunk(wr[t], k);
+        }
+    };
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    load(wave);
+    for (int s = wave; s < steps; s += WAVES * U) {
+        uint4 cw[NT][U], cx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            cx[u] = x[u];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) cw[t][u] = w[t][u];
+        }
+        if (s + WAVES * U < steps) load(s + WAVES * U);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t] = mfma<T>(cw[t][u], cx[u], acc[t]);
+    }
+    // (rows of x from M on are the last one again, columns from N on W's last row)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<f32x4*>(&sums[wave][i][16 * t + 4 * q]) = acc[t];
+    __syncthreads();
+    if (threadIdx.x >= 32 * NT) return;
+    const int m = threadIdx.x / (2 * NT), c = 8 * (threadIdx.x % (2 * NT));
+    float v[1][8] = {};
+#pragma unroll
+    for (int r = 0; r < WAVES; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[0][e] += sums[r][m][c + e];
+    finish<T, 1>(g.e, m, 1, n0 + c, v);   // stores rows under M
+}
+
 // ───────────────────────────── dz and the bias gradient ─────────────────────────────
 
 // Adds the remainders of eight values.
@@ -1070,9 +1141,24 @@ void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
         rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 2, 2, ODD>, grid, dim3(256), s, g);
 }
 
+// Few rows with a K that is one trip to memory (1 x 4096 x 1024: 4.0 us, by
+// 64 x 64 tiles 7), or with two blocks of columns per CU (16 x 14336 x 4096: 38
+// us, by tiles 45).  Between, x's loads cost as much as W's and ranges of K are
+// faster (16 x 4096 x 14336: 36 us, by tiles 29).
+bool rows16_applies(int64_t M, int64_t N, int64_t K) { return M <= 16 && (K <= 1024 || N >= 8192); }
+
 // C = A·Bᵀ by the route of its sizes, then the epilogue.
 rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, void* workspace, int64_t bytes,
                      hipStream_t s) {
+    if (!akm && !bkm && rows16_applies(g.M, g.N, g.K)) {
+        const int nt = g.e.codes ? 2 : 1;   // a group of codes is 32 columns
+        const dim3 grid((unsigned)((g.N + 16 * nt - 1) / (16 * nt)));
+        if (dt == RWKV_BF16 && nt == 1) rwkv::launch(rows16_kernel<bf16, 1>, grid, dim3(512), s, g);
+        else if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 2>, grid, dim3(512), s, g);
+        else if (nt == 1) rwkv::launch(rows16_kernel<f16, 1>, grid, dim3(512), s, g);
+        else rwkv::launch(rows16_kernel<f16, 2>, grid, dim3(512), s, g);
+        return status_of(what);
+    }
     const bool aligned = (uintptr_t)g.a % 16 == 0 && (uintptr_t)g.b % 16 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0;
     const bool odd = !aligned || ((!akm || !bkm) && g.K % 8 != 0);
     const Route r = route_of(g.M, g.N, g.K, odd, akm && bkm);
@@ -1131,7 +1217,7 @@ void dact_geometry(int64_t M, int64_t N, bool db, int& TX, int& gx, int& gy) {
 extern "C" {
 
 int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K) {
-    return shape_ok(M, N, K) ? gemm_workspace(M, N, K, false) : 0;
+    return shape_ok(M, N, K) && !rows16_applies(M, N, K) ? gemm_workspace(M, N, K, false) : 0;
 }
 
 rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
