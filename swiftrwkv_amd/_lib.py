@@ -117,6 +117,7 @@ _SIGS = {
     "rwkv_norm_bwd": (I, [P, I, P, I, L, P, P, P, P, I, P, P, P, L, L, P, L, P]),
     "rwkv_linear_fwd_workspace": (L, [L, L, L]),
     "rwkv_linear_fwd": (I, [P, L, P, L, P, P, L, P, I, P, P, P, P, I, I, L, L, L, P, L, P]),
+    "rwkv_linear_pad": (I, [P, L, P, L, L, P]),
     "rwkv_linear_dact_workspace": (L, [L, L]),
     "rwkv_linear_dact": (I, [P, L, I, P, P, I, P, P, I, P, L, P, I, L, L, P, L, P]),
     "rwkv_linear_dgrad_workspace": (L, [L, L, L]),

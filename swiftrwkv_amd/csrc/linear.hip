@@ -908,6 +908,27 @@ __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     finish<T, 1>(g.e, m, 1, n0 + c, v);   // stores rows under M
 }
 
+// ───────────────────────────── rows of whole chunks ─────────────────────────────
+
+// Rows of D 16-bit values into rows of cpr chunks of 8, zeros behind: a thread
+// per chunk.
+__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* x, int64_t ldx, uint4* y, int64_t chunks, int cpr, int D) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= chunks) return;
+    const int64_t row = i / cpr;
+    const int col = 8 * (int)(i - row * cpr), valid = D - col;
+    const uint16_t* p = x + row * ldx + col;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (valid >= 8) {
+        __builtin_memcpy(w, p, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < valid) w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+    }
+    y[i] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // ───────────────────────────── dz and the bias gradient ─────────────────────────────
 
 // Adds the remainders of eight values.
@@ -1071,11 +1092,12 @@ struct Shape {
 constexpr Shape SHAPES[] = {{256, 256, 1, 8.5, 1.10, 1.15}, {256, 128, 1, 2.8, 0.70, 0.73},
                             {128, 128, 2, 1.8, 0.41, 0.40}, {64, 64, 4, 0.3, 0.245, 0.152}};
 
-double pieces_cost(const Shape& s, int64_t pieces, int stages) {
+double pieces_cost(const Shape& s, int64_t pieces, int stages, bool odd) {
     if (pieces == 0) return 0;
     const int64_t n = (pieces + 255) / 256;
     const double busy = std::min(1.0, pieces / 256.0);
-    return s.start * ((n + s.fit - 1) / s.fit) + stages * (s.first + s.more * (n - 1)) * (1 + 0.23 * busy);
+    const double wait = odd ? 0.9 : 0.0;   // misaligned rows: a stage's loads wait for one another
+    return s.start * ((n + s.fit - 1) / s.fit) + stages * (s.first + wait + s.more * (n - 1)) * (1 + 0.23 * busy);
 }
 
 // The tile, and how many of its tiles are taken whole: all; or whole rounds of
@@ -1090,14 +1112,14 @@ Route route_of(int64_t M, int64_t N, int64_t K, bool odd, bool km) {
     for (const Shape& s : SHAPES) {
         if (odd && s.bm == 256) continue;   // its loads want aligned rows
         const int64_t tiles = tiles_of(M, N, s.bm, s.bn);
-        const double whole = pieces_cost(s, tiles, nst);
+        const double whole = pieces_cost(s, tiles, nst, odd);
         if (whole < least) least = whole, best = Route{s.bm, s.bn, tiles, 1, nst};
         const int64_t round = s.fit > 1 ? tiles : 256, full = odd || tiles < 256 ? 0 : tiles / round * round, rest = tiles - full;
         if (rest == 0 || rest > 256 || (km && s.bn == 256)) continue;
-        const double before = full ? pieces_cost(s, full, nst) + 4 : 0;
+        const double before = full ? pieces_cost(s, full, nst, odd) + 4 : 0;
         for (int split = 2; split <= 32 && split * 2 <= nst; split = split < 4 ? split + 1 : split * 2) {
             const int per = (nst + split - 1) / split, splits = (nst + per - 1) / per;
-            const double t = before + pieces_cost(s, rest * splits, per) + 3.3 + (double)(rest * splits) * s.bm * s.bn * 8 / 6.4e6;
+            const double t = before + pieces_cost(s, rest * splits, per, odd) + 3.3 + (double)(rest * splits) * s.bm * s.bn * 8 / 6.4e6;
             if (t < least) least = t, best = Route{s.bm, s.bn, full, splits, per};
         }
     }
@@ -1240,6 +1262,18 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)N, g.K = g.KB = (int)K;
     g.e = Epilogue{bias, residual, ldr, y, y_dt == RWKV_F32, aux, rem, codes, scales, (int)act, M, (int)N};
     return gemm_run("linear_fwd", false, false, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+rwkv_status rwkv_linear_pad(const void* x, int64_t ldx, void* y, int64_t N, int64_t D, void* stream) {
+    RWKV_REQUIRE(N >= 0 && N <= (1 << 24) && D >= 1 && D <= (1 << 20) && ldx >= D, RWKV_E_SHAPE,
+                 "linear_pad: N=%lld D=%lld ldx=%lld", (long long)N, (long long)D, (long long)ldx);
+    RWKV_REQUIRE(N == 0 || (x && y && (uintptr_t)y % 16 == 0), RWKV_E_NULL, "linear_pad: null or misaligned buffer");
+    if (N == 0) return RWKV_OK;
+    const int64_t cpr = (D + 7) / 8, chunks = N * cpr, blocks = (chunks + 255) / 256;
+    RWKV_REQUIRE(blocks < (int64_t(1) << 31), RWKV_E_SHAPE, "linear_pad: %lld values", (long long)(N * D));
+    rwkv::launch(pad_kernel, dim3((unsigned)blocks), dim3(256), (hipStream_t)stream, (const uint16_t*)x, ldx, (uint4*)y, chunks,
+                 (int)cpr, (int)D);
+    return status_of("linear_pad launch");
 }
 
 int64_t rwkv_linear_dact_workspace(int64_t M, int64_t N) {

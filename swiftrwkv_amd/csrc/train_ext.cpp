@@ -130,6 +130,16 @@ Rows rows_of(const Tensor& x, bool dense = false) {
     return {x.detach().contiguous(), N, D, D};
 }
 
+// Rows for the products: 16-byte aligned ones as they lie, others as a copy
+// whose width is rounded up to 8, with zeros behind.
+Rows aligned_rows(Rows r) {
+    if (r.D % 8 == 0 && r.ld % 8 == 0 && (uintptr_t)r.p() % 16 == 0) return r;
+    const int64_t W = (r.D + 7) / 8 * 8;
+    Tensor t = empty({r.N, W}, r.t.scalar_type(), r.t.device());
+    check(rwkv_linear_pad(r.p(), r.ld, t.data_ptr(), r.N, r.D, stream_of(r.t)));
+    return {std::move(t), r.N, W, W};
+}
+
 struct Ws {
     Tensor t;
     int64_t bytes;
@@ -347,7 +357,7 @@ struct LinearNode : Node {
         int64_t ldz = dy.ld;
         // dy itself serves as dz unless it has to be multiplied, narrowed, or
         // laid out in whole 16-byte chunks (with zeros behind an odd N)
-        const bool own_z = need_z && (act != 0 || y_dt != dt || N % 8 || dy.ld % 8);
+        const bool own_z = need_z && (act != 0 || y_dt != dt || N % 8 || dy.ld % 8 || (uintptr_t)dy.p() % 16);
         if (own_z) {
             ldz = (N + 7) / 8 * 8;
             dzt = empty({M, ldz}, dt, dev);
@@ -371,8 +381,9 @@ struct LinearNode : Node {
         if (need_w && M == 0) {
             out[1] = at::zeros({N, K}, wt.options());
         } else if (need_w) {
-            const Tensor xt = x8 ? unpack(xc.unpack(self), xs.unpack(self), {M, K}, dt) : x.unpack(self);
-            const Rows xr = rows_of(xt);
+            // codes hold zeros up to a multiple of 32
+            const Tensor xt = x8 ? unpack(xc.unpack(self), xs.unpack(self), {M, (K + 7) / 8 * 8}, dt) : x.unpack(self);
+            const Rows xr = rows_of(xt);   // (columns from K on, of a padded x, are not asked for)
             out[1] = empty({N, K}, dt, dev);
             check(rwkv_linear_wgrad(cptr(dzt), ldz, xr.p(), xr.ld, ptr(out[1]), dt_of(dt), M, N, K, ws.p(), ws.bytes, s));
         }
@@ -438,7 +449,10 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const auto dev = x.device();
     const Guard guard(dev);
-    const Rows xr = rows_of(x), wr = rows_of(w);
+    const Rows x0 = rows_of(x), w0 = rows_of(w);
+    // a few rows are read as they lie
+    const bool pad = x0.N > 16;
+    const Rows xr = pad ? aligned_rows(x0) : x0, wr = pad ? aligned_rows(w0) : w0;
     const Tensor bc = !b.defined() || b.is_contiguous() ? b : b.detach().contiguous();
     Rows rr{};
     if (res.defined()) rr = rows_of(res);
@@ -452,10 +466,11 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!from_y) aux = empty({M, N}, dt, dev);
     }
     if (z8) z = codes_for(M, N, dev);
-    const Ws ws(rwkv_linear_fwd_workspace(M, N, K), dev);
+    const int64_t KK = xr.D;   // K, or K rounded up to 8 in both
+    const Ws ws(rwkv_linear_fwd_workspace(M, N, KK), dev);
     check(rwkv_linear_fwd(xr.p(), xr.ld, wr.p(), wr.ld, cptr(bc), rr.t.defined() ? rr.p() : nullptr, rr.ld, ptr(y),
                           dt_of(yt), ptr(aux), ptr<uint8_t>(rem), ptr<int8_t>(z.codes), ptr<uint8_t>(z.scales),
-                          (rwkv_activation)act, dt_of(dt), M, N, K, ws.p(), ws.bytes, stream_of(x)));
+                          (rwkv_activation)act, dt_of(dt), M, N, KK, ws.p(), ws.bytes, stream_of(x)));
     if (train) {
         node->x_shape = x.sizes().vec();
         node->y_shape.assign(ysize.begin(), ysize.end());
@@ -470,7 +485,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->w = SavedVariable(wr.t, false);
         if (wants(w)) {
             if (keep8) {
-                const Codes c = pack(xr);
+                const Codes c = pack(x0);
                 node->xc = SavedVariable(c.codes, false);
                 node->xs = SavedVariable(c.scales, false);
             } else {

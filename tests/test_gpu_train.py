@@ -326,6 +326,55 @@ def test_linear_large(M, N, K):
     run_linear(M, N, K, HF, "tanh", True, None, True, seed=1)
 
 
+@pytest.mark.parametrize("M,N,K", [
+    (16, 512, 1024), (16, 33, 1023), (9, 8192, 1100), (16, 8200, 2056), (17, 512, 1024),   # few rows, and one more
+    (2048, 4096, 640), (1024, 8192, 320),                                                  # 256 x 128 tiles
+    (4096, 4096, 328), (4864, 4096, 1032), (5120, 4096, 4096),                             # 256 x 256, whole rounds and a rest
+    (512, 384, 8192), (130, 250, 6000),                                                    # ranges of K
+    (300, 200, 1021), (2050, 1030, 515)])                                                  # rows that are padded
+def test_linear_routes(M, N, K):
+    run_linear(M, N, K, BF, "tanh", True, None, False)
+    run_linear(M, N, K, HF, "relu2", False, F32, (M + K) % 3 == 0, seed=2)
+    run_linear(M, N, K, BF, "none", False, None, False, seed=3)
+
+
+def test_linear_misaligned_rows_and_gradients():
+    """x, W and dy as views that start between 16-byte chunks, of one width."""
+    case("linear: misaligned views of x, W and dy")
+    g = gen(21)
+    for M, N, K in ((40, 96, 128), (10, 96, 128), (70, 64, 200)):
+        x, w = randn(g, M, K + 8, dtype=BF)[:, 1:K + 1], randn(g, N, K + 8, dtype=BF, scale=0.1)[:, 3:K + 3]
+        dy = randn(g, M, N + 8, dtype=BF)[:, 5:N + 5]
+        xa, wa = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = train.linear(xa, wa)
+        dx, dw = torch.autograd.grad(y, (xa, wa), dy)
+        X, W, DY = x.double(), w.double(), dy.double()
+        check("y", y.detach(), X @ W.t(), E24 * (K + 32) * (X.abs() @ W.abs().t()))
+        check("dx", dx, DY @ W, E24 * (N + 32) * (DY.abs() @ W.abs()))
+        check("dw", dw, DY.t() @ X, E24 * (M + 32) * (DY.abs().t() @ X.abs()))
+
+
+def test_kept_activation_has_eight_more_bits():
+    """tanh's and relu²'s gradients through an fp32 residual, whose dy of 1
+    shows the slope before its rounding to dz: db sums it in fp32.  One row:
+    db = slope, off by its own rounding, the kept value's 2^-16 (bf16) or
+    2^-18 (fp16) of the activation and the fp32 function."""
+    for dt, bits in ((BF, 2.0 ** -16), (HF, 2.0 ** -18)):
+        for act, res in (("tanh", False), ("tanh", True), ("sigmoid", False), ("relu2", False), ("relu2", True)):
+            case(f"kept {act} {dt} residual {res}")
+            g = gen(5)
+            x, w = randn(g, 1, 64, dtype=dt), randn(g, 640, 64, dtype=dt, scale=0.2)
+            b = torch.zeros(640, device=DEV, dtype=dt, requires_grad=True)
+            r = torch.zeros(1, 640, device=DEV) if res else None
+            y = train.linear(x, w, b, act, r)
+            db, = torch.autograd.grad(y, b, torch.ones_like(y))
+            z = (x.double() @ w.double().t())[0]
+            bz = E24 * 96 * (x.double().abs() @ w.double().abs().t())[0]
+            a = ACT[act](z)
+            kept_off = {"tanh": 2 * a.abs() * a.abs(), "sigmoid": a, "relu2": 2 * z.clamp(min=0)}[act] * bits
+            check("slope", db, SLOPE[act](z), kept_off + 2 * bz + FUNC * (1 + a.abs()) + TINY[dt] * 2)
+
+
 def test_linear_layouts_and_needs():
     case("linear: views, 3-D, no rows, single gradients")
     g = gen(11)

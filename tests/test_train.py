@@ -82,6 +82,10 @@ def test_linear_entries_refuse():
         refused(SHAPE, entry, D, 7, D, 8, D, 1, 8, 8, 8, None, 0, None)
         refused(NULL, entry, None, 8, D, 8, D, 1, 8, 8, 8, None, 0, None)
     refused(SHAPE, "rwkv_linear_wgrad", D, 8, D, 8, D, 1, 0, 8, 8, None, 0, None)   # no rows to sum
+    refused(SHAPE, "rwkv_linear_pad", D, 6, D, 2, 7, None)
+    refused(SHAPE, "rwkv_linear_pad", D, 7, D, -1, 7, None)
+    refused(NULL, "rwkv_linear_pad", D, 7, D + 8, 2, 7, None)      # misaligned output
+    refused(0, "rwkv_linear_pad", None, 7, None, 0, 7, None)
     refused(SHAPE, "rwkv_linear_wgrad", D, M, D, N, D, 1, K, M, N, D, need // 2 - 4, None)
     dact = lambda **k: [D, k.get("ld", 8), k.get("dydt", 1), k.get("kept"), k.get("rem", k.get("kept")), k.get("isy", 0), k.get("codes"), k.get("scales"),  # noqa: E731
                         k.get("act", 0), D, k.get("ldz", 8), k.get("db"), 1, 2, 8, None, 0, None]
