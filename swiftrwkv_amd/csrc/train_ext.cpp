@@ -1,8 +1,8 @@
 // Python module _train: the training-side operators (norm.hip, linear.hip) as
 // torch functions with their gradients.  The C ABI does the work; this is the
 // argument checks, the allocations and the autograd nodes around it, which in
-// Python cost 112 us for a small layer norm with its gradients.  Engine and
-// threads of torch's own autograd take 50 of them either way.
+// Python cost 112 us for a small layer norm with its gradients and 10 for one
+// without; here 57 to 67, of which torch's engine and its threads take 50, and 5.
 //
 // The reference forms these operators from MLX operations under valueAndGrad
 // (RWKVBlock.swift:163-307).
@@ -450,8 +450,9 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto dev = x.device();
     const Guard guard(dev);
     const Rows x0 = rows_of(x), w0 = rows_of(w);
-    // a few rows are read as they lie
-    const bool pad = x0.N > 16;
+    // small products are read as they lie: two more launches and buffers take
+    // the host 10 us, about what the pass loses on the GPU at 2^30 products
+    const bool pad = (double)x0.N * N * K >= 1073741824.0;
     const Rows xr = pad ? aligned_rows(x0) : x0, wr = pad ? aligned_rows(w0) : w0;
     const Tensor bc = !b.defined() || b.is_contiguous() ? b : b.detach().contiguous();
     Rows rr{};

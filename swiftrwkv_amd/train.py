@@ -104,9 +104,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     run on the matrix cores.  For it an activation keeps 1 byte per value where
     y tells the rest (without a residual; float16 relu² apart), else 3.  keep8:
     x and, under an activation, z are kept in 8 bits instead.  With no gradient
-    needed nothing is kept.  More than 16 rows run on copies of x and weight
-    whose rows are whole 16-byte chunks where K or the alignment is not (and a
-    backward pass keeps those)."""
+    needed nothing is kept.  From M·N·K = 2^30 on, x and weight whose rows are not
+    whole 16-byte chunks (K not a multiple of 8, or misaligned) are copied into
+    such rows first, and a backward pass keeps the copies."""
     return (_ext or extension()).linear(x, weight, bias, activation, residual, keep8)
 
 

@@ -331,7 +331,7 @@ def test_linear_large(M, N, K):
     (2048, 4096, 640), (1024, 8192, 320),                                                  # 256 x 128 tiles
     (4096, 4096, 328), (4864, 4096, 1032), (5120, 4096, 4096),                             # 256 x 256, whole rounds and a rest
     (512, 384, 8192), (130, 250, 6000),                                                    # ranges of K
-    (300, 200, 1021), (2050, 1030, 515)])                                                  # rows that are padded
+    (300, 200, 1021), (2050, 1030, 515), (1100, 1030, 1001), (20, 14000, 4099)])           # odd rows, the last three padded
 def test_linear_routes(M, N, K):
     run_linear(M, N, K, BF, "tanh", True, None, False)
     run_linear(M, N, K, HF, "relu2", False, F32, (M + K) % 3 == 0, seed=2)
