@@ -275,28 +275,38 @@ struct Tile {
     int rows;         // rows (columns) from there to the operand's end
     int K;
     int c, r;         // the thread's chunk and first LDS row
+    bool whole;       // the operand's rows hold a chunk
 
     __device__ __forceinline__ Tile(const void* base, int64_t ld_, int64_t at, int64_t total, int K_, int tid)
         : p(reinterpret_cast<const T*>(base) + (KM ? at : at * ld_)), ld(ld_),
-          rows((int)min(total - at, (int64_t)(KM ? (1 << 30) : ROWS))), K(K_), c(tid % CPR), r(tid / CPR) {}
+          rows((int)min(total - at, (int64_t)(KM ? (1 << 30) : ROWS))), K(K_), c(tid % CPR), r(tid / CPR),
+          whole((KM ? total : (int64_t)K_) >= 8) {}
 
     __device__ __forceinline__ void load(uint4 (&v)[P], int st) const {
         if constexpr (ODD) {
+            // A chunk that would pass the row's end is loaded as the row's last
+            // whole one (fix() moves its values): every load is unconditional
+            // and none is looked at before it is written to LDS.
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int row = r + STEP * i;
-                const int k = KM ? st * BK + row : st * BK + 8 * c;
-                const int valid = KM ? (k < K ? rows - 8 * c : 0) : (row < rows ? K - k : 0);
-                const T* q = p + (KM ? (int64_t)k * ld + 8 * c : (int64_t)row * ld + k);
-                uint32_t w[4] = {0u, 0u, 0u, 0u};
-                if (valid >= 8) {
-                    __builtin_memcpy(w, q, 16);
-                } else {
+                for (int i = 0; i < P; ++i) {
+                    const int row = r + STEP * i;
+                    const T* q = p + (KM ? (int64_t)min(st * BK + row, K - 1) * ld : (int64_t)min(row, rows - 1) * ld) + from(st);
+                    __builtin_memcpy(&v[i], q, 16);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int row = r + STEP * i;
+                    const int k = KM ? st * BK + row : st * BK + 8 * c;
+                    const int valid = KM ? (k < K ? rows - 8 * c : 0) : (row < rows ? K - k : 0);
+                    const T* q = p + (KM ? (int64_t)k * ld + 8 * c : (int64_t)row * ld + k);
+                    uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
                     for (int e = 0; e < 7; ++e)
                         if (e < valid) w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[e] << (16 * (e & 1));
+                    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                v[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         } else if constexpr (KM) {
             const int left = min(BK, K - st * BK);   // rows of this stage
@@ -319,6 +329,27 @@ struct Tile {
 #pragma unroll
             for (int i = 0; i < P; ++i)
                 v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, o + i * step, 0, 0));
+        }
+    }
+
+    // Column (of a k-major row, or k) at which the thread's chunk is loaded.
+    __device__ __forceinline__ int from(int st) const { return KM ? min(8 * c, rows - 8) : min(st * BK + 8 * c, K - 8); }
+
+    // Stage st's chunks as loaded into what they stand for: zeros past the end.
+    __device__ __forceinline__ void fix(uint4 (&v)[P], int st) const {
+        if constexpr (!ODD) return;
+        const bool tail = (st + 1) * BK > K;
+        if (!whole || !(tail || (KM && rows < ROWS))) return;
+        const int moved = (KM ? 8 * c : st * BK + 8 * c) - from(st);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            uint64_t lo = (uint64_t)v[i].y << 32 | v[i].x, hi = (uint64_t)v[i].w << 32 | v[i].z;
+            if (moved >= 4) lo = hi, hi = 0;
+            const int sh = 16 * (moved & 3);
+            lo = lo >> sh | (hi << 1) << (63 - sh);
+            hi >>= sh;
+            if (moved >= 8 || (KM && st * BK + r + STEP * i >= K)) lo = hi = 0;
+            v[i] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
         }
     }
 
@@ -483,6 +514,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     uint4 va[TileA::P], vb[TileB::P];
     ta.load(va, st0);
     tb.load(vb, st0);
+    ta.fix(va, st0);
+    tb.fix(vb, st0);
     ta.write(lds, va);
     tb.write(lds + TileA::BYTES, vb);
     ta.load(va, st0 + 1);
@@ -499,6 +532,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 #pragma unroll
             for (int i = 0; i < AM; ++i) av[i] = TileA::frag(cur, wm * AM * 16, i, kk, lane);
             if (kk == 1) {   // the next stage's chunks, then the loads of the one after
+                ta.fix(va, st + 1);
+                tb.fix(vb, st + 1);
                 ta.write(nxt, va);
                 tb.write(nxt + TileA::BYTES, vb);
                 ta.load(va, st + 2);
@@ -1102,7 +1137,7 @@ double pieces_cost(const Shape& s, int64_t pieces, int stages, bool odd) {
     if (pieces == 0) return 0;
     const int64_t n = (pieces + 255) / 256;
     const double busy = std::min(1.0, pieces / 256.0);
-    const double wait = odd ? 0.9 : 0.0;   // misaligned rows: a stage's loads wait for one another
+    const double wait = odd ? 0.25 : 0.0;   // misaligned loads take longer
     return s.start * ((n + s.fit - 1) / s.fit) + stages * (s.first + wait + s.more * (n - 1)) * (1 + 0.23 * busy);
 }
 
