@@ -431,8 +431,10 @@ typedef enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_AC
  * pass, each where not NULL: aux [M, N] of dt receives relu(z), tanh(z),
  * sigmoid(z) (or z); rem [M, N] the next 8 bits of aux, without aux of a y of
  * dt without residual; codes and scales the 8-bit checkpoint of z.  aux needs
- * rem.  residual may be y.  N, K <= 2^20, pitches < 2^22.  Some shapes sum ranges of K in the
- * workspace: rwkv_linear_fwd_workspace(M, N, K) bytes, 16-byte aligned. */
+ * rem.  residual may be y.  N, K <= 2^20; ldx and ldw (and below ldz) at most
+ * RWKV_LINEAR_MAX_PITCH.  Some shapes sum ranges of K in the workspace:
+ * rwkv_linear_fwd_workspace(M, N, K) bytes, 16-byte aligned. */
+#define RWKV_LINEAR_MAX_PITCH ((1 << 22) - 8)
 int64_t rwkv_linear_fwd_workspace(int64_t M, int64_t N, int64_t K);
 rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                             const void* residual, int64_t ldr, void* y, rwkv_dtype y_dt, void* aux,

@@ -47,7 +47,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BK = 64;                   // k per stage: two 32-wide products
-constexpr int64_t MAX_LD = (1 << 22) - 8;   // a tile's byte offsets stay under 2^31
+constexpr int64_t MAX_LD = RWKV_LINEAR_MAX_PITCH;   // a tile's byte offsets stay under 2^31
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {

@@ -130,6 +130,13 @@ Rows rows_of(const Tensor& x, bool dense = false) {
     return {x.detach().contiguous(), N, D, D};
 }
 
+// Operands of the products, which take rows up to a pitch; others are copied.
+Rows product_rows(const Tensor& x) {
+    Rows r = rows_of(x);
+    if (r.ld > RWKV_LINEAR_MAX_PITCH) r = {r.t.detach().contiguous(), r.N, r.D, r.D};
+    return r;
+}
+
 // Rows for the products: 16-byte aligned ones as they lie, others as a copy
 // whose width is rounded up to 8, with zeros behind.
 Rows aligned_rows(Rows r) {
@@ -351,13 +358,15 @@ struct LinearNode : Node {
         if (need_r) out[res_at] = dyt;
         if (!need_x && !need_w && !need_b) return once(std::move(out), *this, "linear");
         const Rows dy = rows_of(dyt);
-        const Rows wr = rows_of(wt);
+        const Rows wr = product_rows(wt);
         const bool need_z = need_x || need_w;
         Tensor dzt = dy.t;
         int64_t ldz = dy.ld;
-        // dy itself serves as dz unless it has to be multiplied, narrowed, or
-        // laid out in whole 16-byte chunks (with zeros behind an odd N)
-        const bool own_z = need_z && (act != 0 || y_dt != dt || N % 8 || dy.ld % 8 || (uintptr_t)dy.p() % 16);
+        // dy itself serves as dz unless it has to be multiplied, narrowed,
+        // brought closer together, or laid out in whole 16-byte chunks (with
+        // zeros behind an odd N)
+        const bool own_z = need_z && (act != 0 || y_dt != dt || N % 8 || dy.ld % 8 || (uintptr_t)dy.p() % 16 ||
+                                      dy.ld > RWKV_LINEAR_MAX_PITCH);
         if (own_z) {
             ldz = (N + 7) / 8 * 8;
             dzt = empty({M, ldz}, dt, dev);
@@ -383,7 +392,7 @@ struct LinearNode : Node {
         } else if (need_w) {
             // codes hold zeros up to a multiple of 32
             const Tensor xt = x8 ? unpack(xc.unpack(self), xs.unpack(self), {M, (K + 7) / 8 * 8}, dt) : x.unpack(self);
-            const Rows xr = rows_of(xt);   // (columns from K on, of a padded x, are not asked for)
+            const Rows xr = product_rows(xt);   // (columns from K on, of a padded x, are not asked for)
             out[1] = empty({N, K}, dt, dev);
             check(rwkv_linear_wgrad(cptr(dzt), ldz, xr.p(), xr.ld, ptr(out[1]), dt_of(dt), M, N, K, ws.p(), ws.bytes, s));
         }
@@ -449,7 +458,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const auto dev = x.device();
     const Guard guard(dev);
-    const Rows x0 = rows_of(x), w0 = rows_of(w);
+    const Rows x0 = product_rows(x), w0 = product_rows(w);
     // small products are read as they lie: two more launches and buffers take
     // the host 10 us, about what the pass loses on the GPU at 2^30 products
     const bool pad = (double)x0.N * N * K >= 1073741824.0;

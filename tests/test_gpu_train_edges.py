@@ -1,0 +1,69 @@
+"""Training-side operators on the GPU where layout, value or use is out of the
+ordinary.  Tolerances: half a step, finfo.eps / 2, per rounding to 16 bits;
+2^-24 per fp32 operation; what a test adds to these it derives."""
+import sys
+
+import pytest
+import torch
+
+from swiftrwkv_amd import _lib, train
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def case(msg):
+    print(f"[case] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (scale * torch.randn(shape, generator=g, device=DEV)).to(dtype)
+
+
+# ───────────────────────────── rows far apart ─────────────────────────────
+
+def last_rows(t, step):
+    """t's rows as the last rows of t.shape[0] blocks, `step` values apart."""
+    rows, width = t.shape
+    buf = torch.zeros(rows * step + 8, dtype=t.dtype, device=t.device)
+    v = buf.as_strided((rows, width), (step, 1), 8)
+    v.copy_(t)
+    return v
+
+
+LIMIT = 1 << 22   # values between rows up to which the products read them in place, 8 fewer
+
+
+@pytest.mark.parametrize("step", [LIMIT - 8, LIMIT, LIMIT + 104])
+@pytest.mark.parametrize("M,N,K", [(4, 8, 96), (20, 16, 104)])
+def test_rows_far_apart(M, N, K, step):
+    """x, W and dy with any distance between rows: what copies of them give."""
+    case(f"linear {M} x {N} x {K}, rows {step} values apart")
+    g = gen(M + N)
+    x, w, dy = randn(g, M, K, dtype=BF), randn(g, N, K, dtype=BF, scale=0.1), randn(g, M, N, dtype=BF)
+    for act, keep8 in (("none", False), ("tanh", False), ("none", True)):
+        got = []
+        for xv, wv, dv in ((x, w, dy), (last_rows(x, step), last_rows(w, step), last_rows(dy, step))):
+            a, b = xv.detach().requires_grad_(True), wv.detach().requires_grad_(True)
+            y = train.linear(a, b, activation=act, keep8=keep8)
+            got.append([y.detach(), *torch.autograd.grad(y, (a, b), dv)])
+        assert all(torch.equal(p, q) for p, q in zip(*got)), (act, keep8)
+
+
+def test_last_token_of_a_long_batch():
+    case("linear and channel_mix on the last token's rows of a long batch")
+    h = torch.zeros(4, 8200, 512, device=DEV, dtype=BF)
+    h[:, -1] = randn(gen(1), 4, 512, dtype=BF)
+    w = randn(gen(2), 64, 512, dtype=BF, scale=0.05)
+    assert h[:, -1].stride(0) >= LIMIT
+    assert torch.equal(train.linear(h[:, -1], w), train.linear(h[:, -1].contiguous(), w))
+    one = torch.ones(512, device=DEV)
+    with torch.no_grad():
+        _, last = train.channel_mix(h, one, None, one, w, w.t().contiguous())
+    assert torch.equal(train.linear(last, w), train.linear(last.contiguous(), w))
