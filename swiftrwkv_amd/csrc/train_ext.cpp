@@ -186,13 +186,17 @@ Tensor unpack(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, 
     return y;
 }
 
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
 // Gradients of gradients: the kernels leave no graph, so a graph through
-// their results raises instead of missing a term.
-variable_list once(variable_list&& g, const Node& node, const char* what) {
+// their results raises instead of missing a term, on the way to every input
+// and to what dy was made of.
+variable_list once(variable_list&& g, const Tensor& dy, const Node& node, const char* what) {
     if (!at::GradMode::is_enabled()) return std::move(g);
+    torch::autograd::edge_list edges(node.next_edges());
+    if (wants(dy)) edges.push_back(torch::autograd::impl::gradient_edge(dy));
     const std::shared_ptr<Node> err(
-        new torch::autograd::Error(std::string(what) + ": gradients of its gradients are not available",
-                                    torch::autograd::edge_list(node.next_edges())),   // on the way to every input
+        new torch::autograd::Error(std::string(what) + ": gradients of its gradients are not available", std::move(edges)),
         torch::autograd::deleteNode);
     for (Tensor& t : g)
         if (t.defined()) {
@@ -201,8 +205,6 @@ variable_list once(variable_list&& g, const Node& node, const char* what) {
         }
     return std::move(g);
 }
-
-bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // ───────────────────────────── layer norm ─────────────────────────────
 
@@ -245,7 +247,7 @@ struct NormNode : Node {
         check(rwkv_norm_bwd(dy.p(), dt_of(y_dt), keep8 ? nullptr : xr.p(), dt_of(x_dt), ld, ptr<int8_t>(ct),
                             ptr<uint8_t>(sc), ptr<float>(st), ptr(wt), dt_of(wt.scalar_type()), ptr(out[0]), ptr(dw),
                             need_b ? ptr(out[2]) : nullptr, N, D, ws.p(), ws.bytes, stream_of(st)));
-        return once(std::move(out), *this, "layer_norm");
+        return once(std::move(out), grads[0], *this, "layer_norm");
     }
 };
 
@@ -356,7 +358,7 @@ struct LinearNode : Node {
         const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(y_shape, wt.options().dtype(y_dt));
         variable_list out(num_outputs());
         if (need_r) out[res_at] = dyt;
-        if (!need_x && !need_w && !need_b) return once(std::move(out), *this, "linear");
+        if (!need_x && !need_w && !need_b) return once(std::move(out), grads[0], *this, "linear");
         const Rows dy = rows_of(dyt);
         const Rows wr = product_rows(wt);
         const bool need_z = need_x || need_w;
@@ -396,7 +398,7 @@ struct LinearNode : Node {
             out[1] = empty({N, K}, dt, dev);
             check(rwkv_linear_wgrad(cptr(dzt), ldz, xr.p(), xr.ld, ptr(out[1]), dt_of(dt), M, N, K, ws.p(), ws.bytes, s));
         }
-        return once(std::move(out), *this, "linear");
+        return once(std::move(out), grads[0], *this, "linear");
     }
 };
 

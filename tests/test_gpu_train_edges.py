@@ -67,3 +67,25 @@ def test_last_token_of_a_long_batch():
     with torch.no_grad():
         _, last = train.channel_mix(h, one, None, one, w, w.t().contiguous())
     assert torch.equal(train.linear(last, w), train.linear(last.contiguous(), w))
+
+
+# ───────────────────────────── gradients of gradients ─────────────────────────────
+
+def test_gradients_of_gradients_by_way_of_dy():
+    """dx depends on dy: a second derivative that reaches dy's own inputs, and
+    none of the operator's, raises instead of leaving its term out."""
+    case("norm and linear: second derivatives through dy")
+    g = gen(14)
+    x, w, lw = randn(g, 6, 64, dtype=BF).requires_grad_(True), randn(g, 32, 64, dtype=BF), torch.ones(64, device=DEV)
+    for f in (lambda: train.layer_norm(x, lw), lambda: train.linear(x, w), lambda: train.linear(x, w, activation="tanh"),
+              lambda: train.linear(x, w, None, "none", torch.zeros(6, 32, device=DEV, dtype=BF))):
+        y = f()
+        v = torch.ones_like(y).requires_grad_(True)
+        dx, = torch.autograd.grad((v * y).float().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="gradients of its gradients"):
+            torch.autograd.grad(dx.float().sum() + v.float().sum(), v)
+    # one that reads no gradient is as before
+    y = train.linear(x, w)
+    v = torch.ones_like(y).requires_grad_(True)
+    dv, = torch.autograd.grad((v * y).float().sum(), v, create_graph=True)
+    assert torch.equal(dv, y)
