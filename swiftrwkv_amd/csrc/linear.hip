@@ -66,12 +66,14 @@ enum { ACT_NONE = 0, ACT_RELU2 = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
 // What the forward pass keeps of an activation has 8 bits more than the 16 of
 // its type: the backward pass takes 1 − h² and the like from it, where 16 bits
 // alone would cost more than the rounding of dz does.  v and its rounding a
-// are neighbours in the order of fp32 bit patterns; the upper 8 bits of the
-// patterns' difference are what a lacks: 16 (bf16) or 18 (fp16) bits in all.
+// are neighbours in the order of fp32 bit patterns; the patterns' difference,
+// to the nearest of the steps that 8 bits hold, is what a lacks: 16 (bf16) or
+// 18 (fp16) bits in all, errors either way.  (128 steps clamp to 127: one value
+// in 256 is off by up to a step, the others by half of one, and none comes to
+// lie halfway between two values of the type, from where it would go to the
+// even one whichever side it was on.)
 
-// Eight values rounded to T, packed.  bf16 takes ties away from zero: what is
-// lost is then the low half of the pattern, read as a signed number.  (A NaN's
-// low half is zero here: it comes of 16-bit operands.)
+// Eight values rounded to T, packed.  bf16 takes ties away from zero.
 template <typename T>
 __device__ __forceinline__ uint4 round8(const float (&v)[8]) {
     uint32_t w[4];
@@ -88,18 +90,21 @@ __device__ __forceinline__ uint4 round8(const float (&v)[8]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The next 8 bits of the eight values that round8 rounded.
+// The next 8 bits of the eight values, a what round8 made of them.  (A NaN's
+// are any: it stays one.)
 template <typename T>
-__device__ __forceinline__ uint2 rem8(const float (&v)[8]) {
+__device__ __forceinline__ uint2 rem8(const float (&v)[8], uint4 a) {
     uint32_t w[8];
+    const uint32_t r[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t bits = __builtin_bit_cast(uint32_t, v[i]);
         if constexpr (__is_same(T, bf16)) {
-            w[i] = bits >> 8;
+            const uint32_t at = i & 1 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16;
+            w[i] = (uint32_t)min(max((int)(bits - at + 0x80u) >> 8, -127), 127);
         } else {   // at the type's subnormals the difference is larger: it clamps; an infinity keeps none
-            const float f = (float)(T)v[i];
-            const int q = min(max((int)(bits - __builtin_bit_cast(uint32_t, f)) >> 5, -128), 127);
+            const float f = (float)__builtin_bit_cast(T, (uint16_t)(r[i / 2] >> (16 * (i & 1))));
+            const int q = min(max((int)(bits - __builtin_bit_cast(uint32_t, f) + 16u) >> 5, -127), 127);
             w[i] = fabsf(f) <= 65504.0f ? (uint32_t)q : 0u;
         }
     }
@@ -215,8 +220,9 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t row, int step,
 #pragma unroll
         for (int c = 0; c < C; ++c)
             if (row + c * step < e.M) {
-                store_raw(reinterpret_cast<T*>(e.aux) + at + c * pitch, valid, round8<T>(v[c]));
-                store_raw(e.rem + at + c * pitch, valid, rem8<T>(v[c]));
+                const uint4 a = round8<T>(v[c]);
+                store_raw(reinterpret_cast<T*>(e.aux) + at + c * pitch, valid, a);
+                store_raw(e.rem + at + c * pitch, valid, rem8<T>(v[c], a));
             }
     }
     if (e.act == ACT_RELU2) {
@@ -228,7 +234,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t row, int step,
     if (e.rem && !e.aux) {
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (row + c * step < e.M) store_raw(e.rem + at + c * pitch, valid, rem8<T>(v[c]));
+            if (row + c * step < e.M) store_raw(e.rem + at + c * pitch, valid, rem8<T>(v[c], round8<T>(v[c])));
     }
     if (e.res) {
         float s[C][8];
