@@ -427,7 +427,7 @@ typedef enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_AC
 
 /* y = act(z) + residual, z = x·Wᵀ + bias: x [M, K], w [N, K], bias [N] (may be
  * NULL) of dt (bf16 or f16); residual [M, N] (pitch ldr, may be NULL) and y
- * [M, N] of y_dt (dt or f32).  fp32 sums, one rounding.  For the backward
+ * [M, N] of y_dt (dt or f32).  fp32 sums, one rounding, ties to even.  For the backward
  * pass, each where not NULL: aux [M, N] of dt receives relu(z), tanh(z),
  * sigmoid(z) (or z); rem [M, N] the next 8 bits of aux, without aux of a y of
  * dt without residual; codes and scales the 8-bit checkpoint of z.  aux needs

@@ -73,20 +73,13 @@ enum { ACT_NONE = 0, ACT_RELU2 = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
 // lie halfway between two values of the type, from where it would go to the
 // even one whichever side it was on.)
 
-// Eight values rounded to T, packed.  bf16 takes ties away from zero.
+// Eight values rounded to T (ties to even), packed.
 template <typename T>
 __device__ __forceinline__ uint4 round8(const float (&v)[8]) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (__is_same(T, bf16)) {
-            w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, v[2 * i + 1]) + 0x8000u,
-                                         __builtin_bit_cast(uint32_t, v[2 * i]) + 0x8000u, 0x07060302u);
-        } else {
-            typedef T T2 __attribute__((ext_vector_type(2)));
-            w[i] = __builtin_bit_cast(uint32_t, T2{(T)v[2 * i], (T)v[2 * i + 1]});
-        }
-    }
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, T2{(T)v[2 * i], (T)v[2 * i + 1]});
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 

@@ -115,3 +115,39 @@ def test_kept_relu_is_not_one_sided(dt, bias, res):
     mean = ((db.double() - want) / (2 * z))[on].mean().item()
     print(f"  mean {mean / bias:.3f} of the bound", flush=True)
     assert abs(mean) <= bias
+
+
+# ───────────────────────────── rounding ─────────────────────────────
+
+@pytest.mark.parametrize("M,N,K", [(5, 64, 8), (64, 96, 8), (33, 31, 9), (1, 40, 2048), (600, 640, 8), (4096, 4096, 8),
+                                   (16, 128, 8192)])
+def test_bf16_results_round_ties_to_even(M, N, K):
+    """Rows with two values that are not zero: exact sums, rounded as torch
+    rounds, ties to even, on each of the products' routes."""
+    case(f"ties of bf16 results {M} x {N} x {K}")
+    g = gen(M + N + K)
+    pow2 = lambda *s: torch.exp2(torch.randint(-9, 1, s, generator=g, device=DEV).float())  # noqa: E731
+    x, w, dy = (torch.zeros(s, device=DEV) for s in ((M, K), (N, K), (M, N)))
+    x[:, 0], x[:, K - 1] = 1.0, pow2(M)
+    w[:, 0], w[:, K - 1] = 1.0 + torch.randint(0, 128, (N,), generator=g, device=DEV) / 128, pow2(N)
+    dy[:, 0], dy[:, N - 1] = 1.0, pow2(M)
+    dy[0], dy[M - 1] = 1.0, pow2(N)
+    r = (1.0 + torch.randint(0, 128, (M, N), generator=g, device=DEV) / 128).to(BF)
+    x, w, dy = (v.to(BF).requires_grad_(True) for v in (x, w, dy))
+    even = lambda v: v.float().to(BF)  # noqa: E731  (the sums are exact in fp32)
+    X, W, DY = (v.detach().double() for v in (x, w, dy))
+    y = train.linear(x, w)
+    assert torch.equal(y, even(X @ W.t()))
+    z = X @ W.t()
+    yr = train.linear(x.detach(), w.detach(), None, "none", r)
+    exact = z.float().double() == z
+    assert exact.all() and torch.equal(yr, even(z + r.double()))
+    h = train.linear(x.detach(), w.detach(), None, "relu2")
+    sq = (z.float() * z.float())    # relu² is a product in fp32
+    assert torch.equal(h, sq.to(BF))
+    dx, dw = torch.autograd.grad(y, (x, w), dy.detach())
+    # rows of two terms each
+    assert torch.equal(dx[1:-1], even(DY @ W)[1:-1]) and torch.equal(dw[1:-1], even(DY.t() @ X)[1:-1])
+    ties = (z + r.double()).float()
+    low = ties.view(torch.int32) & 0xffff
+    assert (low == 0x8000).any()   # there are ties among them
