@@ -428,9 +428,9 @@ typedef enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_AC
 /* y = act(z) + residual, z = x·Wᵀ + bias: x [M, K], w [N, K], bias [N] (may be
  * NULL) of dt (bf16 or f16); residual [M, N] (pitch ldr, may be NULL) and y
  * [M, N] of y_dt (dt or f32).  fp32 sums, one rounding, ties to even.  For the backward
- * pass, each where not NULL: aux [M, N] of dt receives relu(z), tanh(z),
- * sigmoid(z) (or z); rem [M, N] the next 8 bits of aux, without aux of a y of
- * dt without residual; codes and scales the 8-bit checkpoint of z.  aux needs
+ * pass, each where not NULL: aux [M, N] of dt receives relu(z) with relu²,
+ * else z; rem [M, N] the next 8 bits of aux, without aux those of relu²'s y (of
+ * dt, without residual); codes and scales the 8-bit checkpoint of z.  aux needs
  * rem.  residual may be y.  N, K <= 2^20; ldx and ldw (and below ldz) at most
  * RWKV_LINEAR_MAX_PITCH.  Some shapes sum ranges of K in the workspace:
  * rwkv_linear_fwd_workspace(M, N, K) bytes, 16-byte aligned. */

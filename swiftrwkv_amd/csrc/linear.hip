@@ -63,9 +63,11 @@ __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
 
 enum { ACT_NONE = 0, ACT_RELU2 = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
 
-// What the forward pass keeps of an activation has 8 bits more than the 16 of
-// its type: the backward pass takes 1 − h² and the like from it, where 16 bits
-// alone would cost more than the rounding of dz does.  v and its rounding a
+// What the forward pass keeps for an activation's slope: relu(z), or y for
+// bf16 relu², whose root it is; for tanh and sigmoid z, as their values say
+// nothing of a slope near zero (1 − h² of a bf16 tanh is 0 from z = 3.5 on).  It
+// has 8 bits more than the 16 of its type, which alone would cost more than
+// the rounding of dz does.  v and its rounding a
 // are neighbours in the order of fp32 bit patterns; the patterns' difference,
 // to the nearest of the steps that 8 bits hold, is what a lacks: 16 (bf16) or
 // 18 (fp16) bits in all, errors either way.  (128 steps clamp to 127: one value
@@ -145,14 +147,26 @@ __device__ __forceinline__ float sigmoid_of(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
+// Slopes by t = e^(−2|z|) and e^(−|z|), as precise near zero as elsewhere:
+// 1 − tanh² = 4t/(1 + t)², σ(1 − σ) = t/(1 + t)².
+__device__ __forceinline__ float tanh_slope(float z) {
+    const float t = __builtin_amdgcn_exp2f(fabsf(z) * -2.885390081777927f), r = __builtin_amdgcn_rcpf(1.0f + t);
+    return 4.0f * t * r * r;
+}
+
+__device__ __forceinline__ float sigmoid_slope(float z) {
+    const float t = __builtin_amdgcn_exp2f(fabsf(z) * -1.4426950408889634f), r = __builtin_amdgcn_rcpf(1.0f + t);
+    return t * r * r;
+}
+
 struct Epilogue {
     const void* bias;     // [N] of the operands' type, or null
     const void* res;      // [M] rows of pitch ldr, or null
     int64_t ldr;
     void* y;              // [M, N]
     int wide;             // res and y are fp32 (else the operands' type)
-    void* aux;            // [M, N] of the operands' type: relu(z), tanh(z) or σ(z); or null
-    uint8_t* rem;         // [M, N]: the next 8 bits of aux, without aux of y; or null
+    void* aux;            // [M, N] of the operands' type: relu(z) with relu², else z; or null
+    uint8_t* rem;         // [M, N]: the next 8 bits of aux, without aux of relu²'s y; or null
     int8_t* codes;        // checkpoint of z, [M, Np]; or null
     uint8_t* scales;
     int act;
@@ -198,16 +212,6 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t row, int step,
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] < 0.0f ? 0.0f : v[c][i];   // a NaN stays one
-    } else if (e.act == ACT_TANH) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[c][i] = tanh_of(v[c][i]);
-    } else if (e.act == ACT_SIGMOID) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[c][i] = sigmoid_of(v[c][i]);
     }
     if (e.aux) {
 #pragma unroll
@@ -223,6 +227,16 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t row, int step,
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[c][i] *= v[c][i];
+    } else if (e.act == ACT_TANH) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = tanh_of(v[c][i]);
+    } else if (e.act == ACT_SIGMOID) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = sigmoid_of(v[c][i]);
     }
     if (e.rem && !e.aux) {
 #pragma unroll
@@ -1053,11 +1067,7 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float h = z[u][i];
-                        if (a.codes) h = a.act == ACT_TANH ? tanh_of(h) : sigmoid_of(h);
-                        d[u][i] *= a.act == ACT_TANH ? 1.0f - h * h : h * (1.0f - h);
-                    }
+                    for (int i = 0; i < 8; ++i) d[u][i] *= a.act == ACT_TANH ? tanh_slope(z[u][i]) : sigmoid_slope(z[u][i]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -1295,8 +1305,8 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
     RWKV_REQUIRE(M == 0 || (x && w && y), RWKV_E_NULL, "linear_fwd: null buffer");
     RWKV_REQUIRE(!codes == !scales, RWKV_E_NULL, "linear_fwd: codes and scales go together");
     RWKV_REQUIRE(!aux || rem, RWKV_E_NULL, "linear_fwd: aux without its remainders");
-    RWKV_REQUIRE(!rem || aux || (y_dt == dt && !residual), RWKV_E_UNSUPPORTED,
-                 "linear_fwd: remainders of a y of another type, or with a residual in it");
+    RWKV_REQUIRE(!rem || aux || (act == ACT_RELU2 && y_dt == dt && !residual), RWKV_E_UNSUPPORTED,
+                 "linear_fwd: remainders of a y that is not relu(z)^2, of another type, or with a residual in it");
     if (M == 0) return RWKV_OK;
     GemmArgs g{};
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)N, g.K = g.KB = (int)K;

@@ -328,13 +328,17 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 constexpr int RELU2 = RWKV_ACT_RELU2;
 
-// Keeps x (or its checkpoint), W, and of the activation, with 8 bits more than
-// the type's 16: nothing for "none"; y for bfloat16 relu² without a residual
-// (relu(z) = √y); tanh or σ where y is that; else an extra buffer of relu(z),
-// tanh(z) or σ(z) (float16 relu² too: its squares underflow early); or with
-// keep8 the 8-bit checkpoint of z.
+// Keeps x (or its checkpoint), W, and for the activation's slope, with 8 bits
+// more than the type's 16: nothing for "none"; y for bfloat16 relu² without a
+// residual (relu(z) = √y); else an extra buffer of relu(z) (float16 relu² too:
+// its squares underflow early) or, for tanh and sigmoid, of z; or with keep8
+// the 8-bit checkpoint of z.  A result of tanh and sigmoid without a residual
+// that was changed in place is refused, as torch does for its own, though only
+// the count of its changes is kept.
 struct LinearNode : Node {
     SavedVariable x, xc, xs, w, kept, rem, zc, zs;
+    c10::VariableVersion y_version;
+    int64_t y_was = -1;   // its value after the forward pass, if it is looked at
     std::vector<int64_t> x_shape, y_shape, res_shape;
     at::ScalarType dt, y_dt;
     int64_t M, N, K;
@@ -353,6 +357,8 @@ struct LinearNode : Node {
                    need_r = res_at >= 0 && task_should_compute_output(res_at);
         const auto self = shared_from_this();
         const Tensor wt = w.unpack(self);
+        TORCH_CHECK(y_was < 0 || (int64_t)y_version.current_version() == y_was,
+                    "linear: its result has been modified by an inplace operation before the backward pass");
         const auto dev = wt.device();
         const Guard guard(dev);
         const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(y_shape, wt.options().dtype(y_dt));
@@ -381,7 +387,7 @@ struct LinearNode : Node {
         if (need_b) out[bias_at] = empty({N}, dt, dev);
         if (own_z || need_b) {
             const Tensor k = kept.unpack(self), r = rem.unpack(self), c = zc.unpack(self), sc = zs.unpack(self);
-            check(rwkv_linear_dact(dy.p(), dy.ld, dt_of(y_dt), cptr(k), ptr<uint8_t>(r), from_y && act == RELU2,
+            check(rwkv_linear_dact(dy.p(), dy.ld, dt_of(y_dt), cptr(k), ptr<uint8_t>(r), from_y,
                                    ptr<int8_t>(c), ptr<uint8_t>(sc), (rwkv_activation)act, own_z ? ptr(dzt) : nullptr,
                                    ldz, need_b ? ptr(out[bias_at]) : nullptr, dt_of(dt), M, N, ws.p(), ws.bytes, s));
         }
@@ -470,7 +476,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (res.defined()) rr = rows_of(res);
     const int64_t M = xr.N;
     const bool z8 = train && keep8 && act != 0;
-    const bool from_y = train && !z8 && act != 0 && !res.defined() && !(act == RELU2 && dt == at::kHalf);
+    const bool from_y = train && !z8 && act == RELU2 && !res.defined() && dt == at::kBFloat16;
     Tensor y = empty(ysize, yt, dev), aux, rem;
     Codes z;
     if (train && act != 0 && !z8) {
@@ -512,6 +518,10 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (aux.defined()) node->kept = SavedVariable(aux, false);
         torch::autograd::set_history(y, node);
         if (from_y) node->kept = SavedVariable(y, true);
+        if (aux.defined() && act != RELU2 && !res.defined()) {
+            node->y_version = y.unsafeGetTensorImpl()->version_counter();
+            node->y_was = node->y_version.current_version();
+        }
     }
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS

@@ -101,8 +101,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     float32 is added after the activation; the result has its type (x's
     without one).  Products accumulate in fp32 and the result is rounded once.
     The gradient of z is rounded to x's type before its two products, as they
-    run on the matrix cores.  For it an activation keeps 1 byte per value where
-    y tells the rest (without a residual; float16 relu² apart), else 3.  keep8:
+    run on the matrix cores.  For it an activation keeps 3 bytes per value
+    (bfloat16 relu² without a residual 1, beside y).  keep8:
     x and, under an activation, z are kept in 8 bits instead.  With no gradient
     needed nothing is kept.  From M·N·K = 2^30 on, x and weight whose rows are not
     whole 16-byte chunks (K not a multiple of 8, or misaligned) are copied into

@@ -151,3 +151,55 @@ def test_bf16_results_round_ties_to_even(M, N, K):
     ties = (z + r.double()).float()
     low = ties.view(torch.int32) & 0xffff
     assert (low == 0x8000).any()   # there are ties among them
+
+
+def slope64(act, z):
+    if act == "tanh":
+        return 1 / torch.cosh(z) ** 2
+    return torch.sigmoid(z) * torch.sigmoid(-z) if act == "sigmoid" else 2 * z.clamp(min=0)
+
+
+FUNC = 2.0 ** -20   # relative error of the fp32 e^z (a few units in the last place), for arguments about 1
+
+
+def swept(dt, n, top):
+    """z from −top to top as the product of x [1, 8] and w [n, 8] in two parts, exact in fp32 but for one sum."""
+    z = torch.linspace(-top, top, n, device=DEV, dtype=torch.float64)
+    w = torch.zeros(n, 8, device=DEV, dtype=dt)
+    w[:, 0] = z.to(dt)
+    w[:, 1] = ((z - w[:, 0].double()) * 64).to(dt)
+    x = torch.zeros(1, 8, device=DEV, dtype=dt)
+    x[0, 0], x[0, 1] = 1.0, 2.0 ** -6
+    return x, w, (x.double() @ w.double().t())[0]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("act", ["tanh", "sigmoid"])
+@pytest.mark.parametrize("how", ["alone", "residual", "keep8"])
+def test_slope_where_the_activation_saturates(act, dt, how):
+    """The slope keeps its relative precision as it goes to zero.  What is kept
+    of z has 16 (bf16) or 18 (fp16) significant bits, to half a step, to one
+    where the remainder's byte clamps: 2^-15 and 2^-17 of z, of which the slope
+    takes at most 2|z| (tanh), |z| (sigmoid); from the 8-bit checkpoint z is
+    what its codes stand for.  The sum z and e^z add 2^-24·2|z|, FUNC·(1 + |z|).
+    One row: the bias gradient is dy·slope, rounded once (dy keeps fp16's off
+    its subnormals)."""
+    case(f"slope of {act} {dt} {how}, z to 16")
+    x, w, z = swept(dt, 4096, 16.0)
+    b = torch.zeros(4096, device=DEV, dtype=dt, requires_grad=True)
+    res = torch.zeros(1, 4096, device=DEV, dtype=dt) if how == "residual" else None
+    y = train.linear(x, w, b, act, res, keep8=how == "keep8")
+    scale = 2.0 ** 14 if dt == HF else 1.0
+    db, = torch.autograd.grad(y, b, torch.full_like(y, scale))
+    kept = 2.0 ** -15 if dt == BF else 2.0 ** -17
+    if how == "keep8":
+        zf = z.float()   # the fp32 sum that the checkpoint is taken of
+        z, kept = train.checkpoint8(zf).restore().double(), 0.0
+    ref = slope64(act, z) * scale
+    tiny = 2.0 ** -25 if dt == HF else 0.0
+    rel = 2 * z.abs() * (kept + 2.0 ** -24) + FUNC * (1 + z.abs())
+    u = torch.finfo(dt).eps / 2
+    bound = ref * (rel + rel ** 2) * (1 + u) + u * ref + tiny
+    worst = ((db.double() - ref).abs() / bound).max().item()
+    print(f"  worst error {worst:.3f} of its bound", flush=True)
+    assert worst <= 1.0
