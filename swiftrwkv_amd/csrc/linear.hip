@@ -1357,7 +1357,9 @@ rwkv_status rwkv_linear_dact(const void* dy, int64_t lddy, rwkv_dtype dy_dt, con
     const hipStream_t s = (hipStream_t)stream;
     const DactArgs a{dy, lddy, dy_dt == RWKV_F32, kept, rem, kept_is_y, codes, scales, (int)act, dz, dz ? ldz : N,
                      db ? (float*)workspace : nullptr, M, (int)N};
-    const dim3 grid((unsigned)gx, (unsigned)gy), bgrid((unsigned)((N + 15) / 16));
+    // a pitch may reach into the chunk after N's last: its zeros are written too
+    const unsigned across = (unsigned)((a.ldz + 8 * TX - 1) / (8 * TX));
+    const dim3 grid(across, (unsigned)gy), bgrid((unsigned)((N + 15) / 16));
     if (dt == RWKV_BF16) {
         rwkv::launch(dact_kernel<bf16>, grid, dim3(256), s, a, TX);
         if (db) rwkv::launch(bias_reduce_kernel<bf16>, bgrid, dim3(256), s, (const float*)workspace, gy, (int)N, (bf16*)db);

@@ -203,3 +203,26 @@ def test_slope_where_the_activation_saturates(act, dt, how):
     worst = ((db.double() - ref).abs() / bound).max().item()
     print(f"  worst error {worst:.3f} of its bound", flush=True)
     assert worst <= 1.0
+
+
+# ───────────────────────────── the padding columns of dz ─────────────────────────────
+
+@pytest.mark.parametrize("N", [1, 3, 8, 16, 64, 505, 512, 513, 2048])
+def test_padding_columns_of_dz_are_zeros(N):
+    """rwkv_linear_dact writes zeros into every column from N to its pitch."""
+    case(f"dact {N} columns, every pitch")
+    L = _lib.lib()
+    M = 37
+    s = torch.cuda.current_stream().cuda_stream
+    dy = randn(gen(N), M, N, dtype=BF)
+    ws = torch.empty(L.rwkv_linear_dact_workspace(M, N), dtype=torch.uint8, device=DEV)
+    for ldz in range(N, N + 8):
+        for with_db in (False, True):
+            dz = torch.full((M, ldz), float("nan"), device=DEV, dtype=BF)
+            db = torch.full((N,), float("nan"), device=DEV, dtype=BF)
+            _lib.check(L.rwkv_linear_dact(dy.data_ptr(), N, 1, None, None, 0, None, None, 0, dz.data_ptr(), ldz,
+                                          db.data_ptr() if with_db else None, 1, M, N, ws.data_ptr(), ws.numel(), s))
+            assert torch.equal(dz[:, :N], dy) and not dz[:, N:].any(), (ldz, with_db)
+            if with_db:
+                off = 2.0 ** -24 * 64 * dy.double().abs().sum(0) + 2.0 ** -8 * dy.double().sum(0).abs() + 2.0 ** -133
+                assert ((db.double() - dy.double().sum(0)).abs() <= off).all()
