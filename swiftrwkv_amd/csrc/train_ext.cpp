@@ -84,6 +84,14 @@ Tensor tensor_arg(PyObject* o, const char* what, bool optional = false) {
     return t;
 }
 
+// A result without a tangent would read as a derivative of zero; for a
+// gradient's input as for the call's.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what,
+                                    ": forward-mode derivatives are not available");
+}
+
 void need_device(const Tensor& x, const char* what) {
     if (!x.is_cuda())
         raise(PyExc_ValueError, std::string(what) + " must live on a ROCm device, got " + x.device().str());
@@ -224,6 +232,7 @@ struct NormNode : Node {
     variable_list apply(variable_list&& grads) override {
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1),
                    need_b = num_outputs() > 2 && task_should_compute_output(2);
+        no_tangent("layer_norm", {&grads[0]});
         const auto self = shared_from_this();
         const Tensor st = stats.unpack(self), wt = w.unpack(self), xt = x.unpack(self), ct = codes.unpack(self),
                      sc = scales.unpack(self);
@@ -257,6 +266,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 6) raise(PyExc_TypeError, "layer_norm: six arguments");
     const Tensor x = tensor_arg(a[0], "layer_norm: x");
     Tensor w = tensor_arg(a[1], "layer_norm: weight"), b = tensor_arg(a[2], "layer_norm: bias", true);
+    no_tangent("layer_norm", {&x, &w, &b});
     const double eps = PyFloat_AsDouble(a[3]);
     if (PyErr_Occurred()) throw python_error();
     const auto xt = x.scalar_type();
@@ -355,6 +365,7 @@ struct LinearNode : Node {
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1),
                    need_b = bias_at >= 0 && task_should_compute_output(bias_at),
                    need_r = res_at >= 0 && task_should_compute_output(res_at);
+        no_tangent("linear", {&grads[0]});
         const auto self = shared_from_this();
         const Tensor wt = w.unpack(self);
         TORCH_CHECK(y_was < 0 || (int64_t)y_version.current_version() == y_was,
@@ -416,6 +427,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 6) raise(PyExc_TypeError, "linear: six arguments");
     const Tensor x = tensor_arg(a[0], "linear: x"), w = tensor_arg(a[1], "linear: weight"),
                  b = tensor_arg(a[2], "linear: bias", true), res = tensor_arg(a[4], "linear: residual", true);
+    no_tangent("linear", {&x, &w, &b, &res});
     const auto dt = x.scalar_type();
     if (dt == at::kFloat) raise(PyExc_TypeError, "linear: x must be bfloat16 or float16, got float32");
     const char* name = PyUnicode_Check(a[3]) ? PyUnicode_AsUTF8(a[3]) : nullptr;

@@ -226,3 +226,23 @@ def test_padding_columns_of_dz_are_zeros(N):
             if with_db:
                 off = 2.0 ** -24 * 64 * dy.double().abs().sum(0) + 2.0 ** -8 * dy.double().sum(0).abs() + 2.0 ** -133
                 assert ((db.double() - dy.double().sum(0)).abs() <= off).all()
+
+
+# ───────────────────────────── forward mode ─────────────────────────────
+
+def test_forward_mode_derivatives_are_refused():
+    case("norm and linear: a tangent on the device")
+    x, w, one = randn(gen(1), 4, 64, dtype=BF), randn(gen(2), 8, 64, dtype=BF), torch.ones(64, device=DEV)
+    r = torch.zeros(4, 8, device=DEV)
+    fa = torch.autograd.forward_ad
+    with fa.dual_level():
+        dual = lambda t: fa.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (lambda: train.layer_norm(dual(x), one), lambda: train.layer_norm(x, one, dual(one)),
+                  lambda: train.linear(x, dual(w)), lambda: train.linear(x, w, None, "none", dual(r))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+        assert train.linear(x, w).shape == (4, 8)   # no tangent among its inputs
+        leaf = x.detach().requires_grad_(True)
+        for y in (train.layer_norm(leaf, one), train.linear(leaf, w), train.linear(leaf, w, activation="tanh")):
+            with pytest.raises(NotImplementedError, match="forward-mode"):   # and of a gradient
+                torch.autograd.grad(y, leaf, dual(torch.ones_like(y)))

@@ -87,3 +87,19 @@ def test_restore_checks():
             bad.restore()
     with pytest.raises(TypeError, match="restore to float32"):
         make().restore(torch.float64)
+
+
+CALLS = {"layer_norm": lambda a, b: train.layer_norm(a, b[0]), "linear": lambda a, b: train.linear(a, b)}
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(name, which):
+    """A result without a tangent would read as a derivative of zero."""
+    args = [t(2, 8), t(4, 8)]
+    with torch.autograd.forward_ad.dual_level():
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match=f"{name}: forward-mode"):
+            CALLS[name](*args)
+    with pytest.raises(ValueError, match=DEVICE):   # the level is closed
+        CALLS[name](t(2, 8), t(4, 8))
