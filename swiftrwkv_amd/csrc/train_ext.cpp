@@ -19,6 +19,8 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <algorithm>
 #include <cstring>
@@ -90,6 +92,21 @@ void no_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
     for (const Tensor* t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what,
                                     ": forward-mode derivatives are not available");
+}
+
+// Calls here go past torch's dispatcher: a traced one would be a constant, and
+// a tensor of a transform or of a class with a dispatch of its own is not the
+// memory that it stands for.
+void plain_call(const char* what, std::initializer_list<const Tensor*> inputs) {
+    using c10::DispatchKey;
+    using c10::impl::TorchDispatchModeKey;
+    constexpr c10::DispatchKeySet wrapped({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
+                                           DispatchKey::FuncTorchGradWrapper});
+    bool ok = !c10::impl::tls_is_dispatch_key_included(DispatchKey::Tracer);
+    for (const TorchDispatchModeKey k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        ok = ok && !c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
+    for (const Tensor* t : inputs) ok = ok && (!t->defined() || !t->key_set().has_any(wrapped));
+    TORCH_CHECK_NOT_IMPLEMENTED(ok, what, ": not available under tracing or function transforms");
 }
 
 void need_device(const Tensor& x, const char* what) {
@@ -266,6 +283,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 6) raise(PyExc_TypeError, "layer_norm: six arguments");
     const Tensor x = tensor_arg(a[0], "layer_norm: x");
     Tensor w = tensor_arg(a[1], "layer_norm: weight"), b = tensor_arg(a[2], "layer_norm: bias", true);
+    plain_call("layer_norm", {&x, &w, &b});
     no_tangent("layer_norm", {&x, &w, &b});
     const double eps = PyFloat_AsDouble(a[3]);
     if (PyErr_Occurred()) throw python_error();
@@ -427,6 +445,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 6) raise(PyExc_TypeError, "linear: six arguments");
     const Tensor x = tensor_arg(a[0], "linear: x"), w = tensor_arg(a[1], "linear: weight"),
                  b = tensor_arg(a[2], "linear: bias", true), res = tensor_arg(a[4], "linear: residual", true);
+    plain_call("linear", {&x, &w, &b, &res});
     no_tangent("linear", {&x, &w, &b, &res});
     const auto dt = x.scalar_type();
     if (dt == at::kFloat) raise(PyExc_TypeError, "linear: x must be bfloat16 or float16, got float32");
@@ -545,6 +564,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_checkpoint8(PyObject*, PyObject* o) {
     HANDLE_TH_ERRORS
     const Tensor x = tensor_arg(o, "checkpoint8: x");
+    plain_call("checkpoint8", {&x});
     if (x.dim() < 1 || x.size(-1) < 1)
         raise(PyExc_ValueError, "checkpoint8: x must have a last axis of at least 1, got " + shape_of(x));
     need_device(x, "checkpoint8: x");
@@ -564,6 +584,7 @@ PyObject* py_restore8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 4 || !THPVariable_Check(a[0]) || !THPVariable_Check(a[1]) || !PyTuple_Check(a[2]))
         raise(PyExc_TypeError, "restore8: codes, scales, shape, dtype");
     const Tensor codes = THPVariable_Unpack(a[0]), scales = THPVariable_Unpack(a[1]);
+    plain_call("restore8", {&codes, &scales});
     if (!THPDtype_Check(a[3]) || !float_ok(reinterpret_cast<THPDtype*>(a[3])->scalar_type))
         raise(PyExc_TypeError, "checkpoints restore to float32, bfloat16 or float16");
     c10::SmallVector<int64_t, 6> shape;

@@ -103,3 +103,25 @@ def test_forward_mode_derivatives_are_refused(name, which):
             CALLS[name](*args)
     with pytest.raises(ValueError, match=DEVICE):   # the level is closed
         CALLS[name](t(2, 8), t(4, 8))
+
+
+TRACED = {**CALLS, "checkpoint8": lambda a, b: train.checkpoint8(a).codes}
+
+
+@pytest.mark.parametrize("name", TRACED)
+def test_transforms_and_tracing_are_refused(name):
+    """A traced call would be a constant, a transformed one has no memory."""
+    f = lambda a: TRACED[name](a, t(4, 8))  # noqa: E731
+    with pytest.raises(NotImplementedError, match=f"{name}: .*transforms"):
+        torch.vmap(f)(t(3, 2, 8))
+    with pytest.raises(NotImplementedError, match=f"{name}: .*transforms"):
+        torch.func.vjp(f, t(2, 8))
+    with pytest.raises(NotImplementedError, match=f"{name}: .*tracing"):
+        torch.jit.trace(f, t(2, 8), check_trace=False)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for mode in ("real", "fake"):
+        with pytest.raises(NotImplementedError, match=f"{name}: .*tracing"):
+            make_fx(f, tracing_mode=mode)(t(2, 8))
+    with torch._subclasses.FakeTensorMode() as m:
+        with pytest.raises(NotImplementedError, match=f"{name}: .*tracing"):
+            f(m.from_tensor(t(2, 8)))
