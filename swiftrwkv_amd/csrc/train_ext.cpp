@@ -76,6 +76,12 @@ bool float_ok(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 |
 
 rwkv_dtype dt_of(at::ScalarType t) { return t == at::kFloat ? RWKV_F32 : t == at::kBFloat16 ? RWKV_BF16 : RWKV_F16; }
 
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();   // an array of several, say
+    return v == 1;
+}
+
 // The tensor behind an argument; undefined for None where that is allowed.
 Tensor tensor_arg(PyObject* o, const char* what, bool optional = false) {
     if (optional && o == Py_None) return {};
@@ -293,7 +299,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!THPDtype_Check(a[4])) raise(PyExc_TypeError, "layer_norm: out_dtype must be a torch.dtype");
         yt = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
     }
-    const bool keep8 = PyObject_IsTrue(a[5]) == 1;
+    const bool keep8 = truth(a[5]);
     if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > MAX_D)
         raise(PyExc_ValueError, "layer_norm: the last axis must hold 1 to 65536 values, got " + shape_of(x));
     const int64_t D = x.size(-1);
@@ -454,7 +460,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; name && i < 4; ++i)
         if (std::strcmp(name, ACTIVATIONS[i]) == 0) act = i;
     if (act < 0) raise(PyExc_ValueError, std::string("linear: activation '") + (name ? name : "?") + "' is none of none, relu2, tanh, sigmoid");
-    const bool keep8 = PyObject_IsTrue(a[5]) == 1;
+    const bool keep8 = truth(a[5]);
     if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1) || w.numel() == 0)
         raise(PyExc_ValueError, "linear: x " + shape_of(x) + " and weight " + shape_of(w) + " must be [..., K] and [N, K]");
     const int64_t N = w.size(0), K = w.size(1);

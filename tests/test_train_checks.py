@@ -125,3 +125,10 @@ def test_transforms_and_tracing_are_refused(name):
     with torch._subclasses.FakeTensorMode() as m:
         with pytest.raises(NotImplementedError, match=f"{name}: .*tracing"):
             f(m.from_tensor(t(2, 8)))
+
+
+def test_keep8_has_to_have_a_truth_value():
+    """An argument whose truth value raises: its own error, no call."""
+    for f in (lambda k: train.layer_norm(t(2, 8), t(8), keep8=k), lambda k: train.linear(t(2, 8), t(4, 8), keep8=k)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            f(torch.zeros(2))
