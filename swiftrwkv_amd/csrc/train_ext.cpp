@@ -504,9 +504,13 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto dev = x.device();
     const Guard guard(dev);
     const Rows x0 = product_rows(x), w0 = product_rows(w);
-    // small products are read as they lie: two more launches and buffers take
-    // the host 10 us, about what the pass loses on the GPU at 2^30 products
-    const bool pad = (double)x0.N * N * K >= 1073741824.0;
+    // Aligned copies, for all three products.  Not for small ones: two more
+    // launches and buffers take the host 10 us, about what the pass loses on the
+    // GPU at 2^30 products.  Nor for few rows, where W's copy costs more than
+    // the product: 64 rows through 14000 x 4099 bf16 as they lie 51 us forward,
+    // 112 backward; copied 69 (39 of them the copies) and 80; 128 rows 50 and
+    // 132, 74 and 101; 512 rows 117 and 251, 104 and 176.
+    const bool pad = x0.N > 128 && (double)x0.N * N * K >= 1073741824.0;
     const Rows xr = pad ? aligned_rows(x0) : x0, wr = pad ? aligned_rows(w0) : w0;
     const Tensor bc = !b.defined() || b.is_contiguous() ? b : b.detach().contiguous();
     Rows rr{};

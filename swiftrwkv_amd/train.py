@@ -104,9 +104,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     run on the matrix cores.  For it an activation keeps 3 bytes per value
     (bfloat16 relu² without a residual 1, beside y).  keep8:
     x and, under an activation, z are kept in 8 bits instead.  With no gradient
-    needed nothing is kept.  From M·N·K = 2^30 on, x and weight whose rows are not
-    whole 16-byte chunks (K not a multiple of 8, or misaligned) are copied into
-    such rows first, and a backward pass keeps the copies."""
+    needed nothing is kept.  With more than 128 rows and from M·N·K = 2^30 on, x and
+    weight whose rows are not whole 16-byte chunks (K not a multiple of 8, or
+    misaligned) are copied into such rows first, and a backward pass keeps the
+    copies."""
     return (_ext or extension()).linear(x, weight, bias, activation, residual, keep8)
 
 

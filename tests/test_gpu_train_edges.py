@@ -246,3 +246,25 @@ def test_forward_mode_derivatives_are_refused():
         for y in (train.layer_norm(leaf, one), train.linear(leaf, w), train.linear(leaf, w, activation="tanh")):
             with pytest.raises(NotImplementedError, match="forward-mode"):   # and of a gradient
                 torch.autograd.grad(y, leaf, dual(torch.ones_like(y)))
+
+
+# ───────────────────────────── odd rows ─────────────────────────────
+
+def test_few_rows_copy_no_weights():
+    """A few rows through a W whose rows are not whole chunks: W is read as it
+    lies, on every call, not copied into aligned rows first."""
+    w = randn(gen(1), 8192, 8195, dtype=BF, scale=0.01)
+    for M in (1, 16, 17, 40):
+        case(f"memory of a product {M} x 8192 x 8195")
+        x = randn(gen(M), M, 8195, dtype=BF)
+        with torch.no_grad():
+            train.linear(x, w)
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            y = train.linear(x, w)
+            used = torch.cuda.max_memory_allocated() - before
+        assert used < w.numel() * 2 / 2, (M, used)
+        z = x.double() @ w.double().t()
+        off = 2.0 ** -24 * (8195 + 32) * (x.double().abs() @ w.double().abs().t())
+        assert ((y.double() - z).abs() <= 2.0 ** -8 * z.abs() + off * (1 + 2.0 ** -8)).all()
