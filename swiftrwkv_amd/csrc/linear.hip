@@ -692,7 +692,6 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     constexpr int RM = NM / 2 / NF, MA = NM * 11 / 16, MB = NM * 3 / 8, LM = (2 * NM - MA) / ND;
     static_assert(RM * NF <= MA && MB + RM * NF <= NM && MA + LM * ND <= 2 * NM, "places of a stage");
     constexpr int SM = MA / 6;   // the loader's steps: beside every SM-th before MA
-    static_assert(RM * NF <= MA && MB + RM * NF <= NM && MA + LM * ND <= 2 * NM, "places of a stage");
     constexpr int CPR = 4 * AN;   // 16-byte chunks of a staged row of the epilogue
     __shared__ __align__(1024) char lds[2 * STAGE + (EPI == EPI_PART ? 0 : W * 16 * CPR * 16)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1135,6 +1134,8 @@ int64_t tiles_of(int64_t M, int64_t N, int bm, int bn) { return ((M + bm - 1) / 
 // K: a CU that takes n pieces of `stages` each needs
 //   start·⌈n / fit⌉ + stages·(first + more·(n − 1))·(1 + 0.23·share of busy CUs).
 // The cheapest of the four is 0.8 % behind the fastest one measured, in the mean.
+// A K below 512, which lies outside the fit, costs more than this says: output
+// bytes have no term (8192 x 2048 x 96 by 64 x 64 tiles: 7.4 us here, 21 measured).
 struct Shape {
     int bm, bn, fit;
     double start, first, more;
@@ -1213,10 +1214,17 @@ void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
         rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 2, 2, ODD>, grid, dim3(256), s, g);
 }
 
-// Few rows with a K that is one trip to memory (1 x 4096 x 1024: 4.0 us, by
-// 64 x 64 tiles 7), or with two blocks of columns per CU (16 x 14336 x 4096: 38
-// us, by tiles 45).  Between, x's loads cost as much as W's and ranges of K are
-// faster (16 x 4096 x 14336: 36 us, by tiles 29).
+// Few rows with a short K (a wave's loads on their way at once hold 2048 of it,
+// 1024 with codes), or with two blocks of columns per CU; elsewhere x's loads
+// cost as much as W's and ranges of K are faster.  us by rows16_kernel, by 64 x
+// 64 tiles (bf16, back to back, W from memory):
+//   N      K      1 row        16 rows          N      K      1 row       16 rows
+//   1024   1024   4.4,  8.4     4.9,  8.5       4096   4096   9.0, 16.3   11.8, 16.8
+//   4096   1024   4.7,  9.3     5.1,  8.6       4096   8192  18.9, 19.3   22.7, 19.7
+//   8192   2048  10.6, 22.8    12.5, 22.7      14336   4096  26.5, 45.1   38.9, 45.3
+//   8192    512   6.6,  5.7     7.0,  5.7      14336   8192  54.8, 51.5   76.6, 53.3
+// The rule errs both ways: K = 2048 of fewer columns would gain as well (4096 x
+// 2048 6.4 and 11.3), and from N = 6144 on a K of 512, or one of 8192, loses.
 bool rows16_applies(int64_t M, int64_t N, int64_t K) { return M <= 16 && (K <= 1024 || N >= 8192); }
 
 // C = A·Bᵀ by the route of its sizes, then the epilogue.
