@@ -1016,7 +1016,10 @@ struct DactArgs {
     int N;
 };
 
-// dz = dy·act'(z) in chunks of 8 columns: TX chunks across, 256/TX rows down
+// dz = dy·act'(z), rounded to the operands' type: both products that read it run
+// on 16-bit matrix instructions, and 32 bits would cost them twice the time or
+// more.  dx and dW are off by √2 of a 16-bit result's own rounding for it; db sums
+// the values before.  In chunks of 8 columns: TX chunks across, 256/TX rows down
 // a block, rows strided over gridDim.y, two of them loaded at a time
 // (8192 x 8192 bf16 relu² from y: 4.96 TB/s; four at a time, on fewer waves, 3.97).
 template <typename T>

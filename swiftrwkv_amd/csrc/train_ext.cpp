@@ -2,7 +2,8 @@
 // torch functions with their gradients.  The C ABI does the work; this is the
 // argument checks, the allocations and the autograd nodes around it, which in
 // Python cost 112 us for a small layer norm with its gradients and 10 for one
-// without; here 57 to 67, of which torch's engine and its threads take 50, and 5.
+// without; here 32 or 55 to 67, by process, most of it torch's engine and its
+// threads, and 5.
 //
 // The reference forms these operators from MLX operations under valueAndGrad
 // (RWKVBlock.swift:163-307).

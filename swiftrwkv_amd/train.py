@@ -8,8 +8,8 @@ Sources/RWKVModel/RWKVBlock.swift:163-307); here each is hand-written kernels
 behind the C ABI.  channel_mix runs them together as one block half.
 
 Tensors live on a ROCm device; results and gradients come back in the types
-of the arguments.  Leading axes are rows; a last axis that is not contiguous is
-copied first.  Checks, allocations and autograd nodes are native code
+of the arguments.  Leading axes are rows, at most 2^24; a last axis that is not
+contiguous is copied first.  Checks, allocations and autograd nodes are native code
 (csrc/train_ext.cpp).  Gradients of gradients, forward-mode derivatives, tracing
 and function transforms raise.  There is no CPU fallback: a missing library raises.
 """
