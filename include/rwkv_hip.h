@@ -470,6 +470,82 @@ rwkv_status rwkv_linear_wgrad(const void* dz, int64_t ldz, const void* x, int64_
                               int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                               void* stream);
 
+/* Dropout's random numbers.  Element (row, col) of rows [N, D] is kept iff its
+ * 16-bit number is at least threshold (round(65536·p); 0 keeps everything,
+ * 65536 nothing); kept values are multiplied by 65536 / (65536 − threshold),
+ * dropped ones are zero, infinities and NaN too.  The numbers of columns 8c ..
+ * 8c + 7 are the 128 bits, low half of a word first, of Philox4x32-10 (Salmon,
+ * Moraes, Dror, Shaw 2011) for the key (seed, low word first) and the counter
+ * (c, row, offset, low word first).  With seed_dev (device) the seed is read
+ * there when the kernel runs. */
+typedef struct {
+    uint64_t seed;
+    const int64_t* seed_dev;
+    uint64_t offset;
+    int32_t threshold;
+} rwkv_drop;
+
+/* y = drop(x) + residual: x [N, D] of x_dt, residual (pitch ldr, may be NULL)
+ * and y [N, D] of y_dt; the types are alike or one of them is f32.  The
+ * gradient of x is the same call on dy.  D <= 2^22. */
+rwkv_status rwkv_dropout(const void* x, rwkv_dtype x_dt, int64_t ldx, const void* residual, int64_t ldr, void* y,
+                         rwkv_dtype y_dt, const rwkv_drop* drop, int64_t N, int64_t D, void* stream);
+
+/* The end of one block and the start of the next, rows of D <= 8192:
+ *   x' = x + scale·drop(gate·LN(o; post_weight, post_bias)),  h = LN(x'; weight, bias)
+ * x [N, D] of x_dt (f32 or dt), o and gate of dt, vectors [D] of w_dt (f32 or
+ * dt).  gate, post_weight (no norm of o), post_bias, scale and bias may be
+ * NULL. */
+typedef struct {
+    const void *x, *o, *gate;
+    int64_t ldx, ldo, ldg;
+    rwkv_dtype x_dt, dt, w_dt;
+    const void *post_weight, *post_bias, *scale, *weight, *bias;
+    float post_eps, eps;
+    rwkv_drop drop;
+    int64_t N, D;
+} rwkv_join;
+
+/* xs = x' [N, D] of x_dt, h [N, D] of dt; stats [N, 4] fp32 (mean and rstd of o
+ * and of x'; 16-byte aligned) where not NULL.  xs may be x where ldx = D; no
+ * other output may alias an input. */
+rwkv_status rwkv_join_fwd(const rwkv_join* args, void* xs, void* h, float* stats, void* stream);
+
+/* Gradients from x' as stored and the stats (args->x is not read, args->o only
+ * with gate, post_weight or scale): dxs [N, D]
+ * of x_dt and dh [N, D] of dt, each NULL for zeros; dx of x_dt, dout and dgate
+ * of dt, vectors' gradients of w_dt, each NULL where not wanted.  For those of
+ * vectors a workspace of rwkv_join_bwd_workspace(N, D) bytes, 16-byte aligned.
+ * The sums' order is fixed. */
+int64_t rwkv_join_bwd_workspace(int64_t N, int64_t D);
+rwkv_status rwkv_join_bwd(const rwkv_join* args, const void* xs, const float* stats, const void* dxs, const void* dh,
+                          void* dx, void* dout, void* dgate, void* dweight, void* dbias, void* dpost_weight,
+                          void* dpost_bias, void* dscale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The recurrence's tail in training (rwkv_wkv_tail's formula, heads of 64):
+ *   y = (LN_head(o)·weight + bias + (Σ_head r·k·r_k)·v)·gate
+ * over rows [N, 64 H], H <= 1024: o of o_dt (f32 or dt), r, k, v, gate and y of dt, r_k,
+ * weight and bias [64 H] of w_dt (f32 or dt). */
+typedef struct {
+    const void *o, *r, *k, *v, *gate;
+    int64_t ldo, ldr, ldk, ldv, ldg;
+    rwkv_dtype o_dt, dt, w_dt;
+    const void *r_k, *weight, *bias;
+    float eps;
+    int64_t N, H;
+} rwkv_tail;
+
+rwkv_status rwkv_tail_fwd(const rwkv_tail* args, void* y, void* stream);
+
+/* Gradients, dense rows in the types of what they belong to, each NULL where
+ * not wanted (dr_k, dweight and dbias go together and take a workspace of
+ * rwkv_tail_bwd_workspace(N, H) bytes, 16-byte aligned).  dy [N] rows of dt,
+ * pitch lddy.  The sums' order is fixed. */
+int64_t rwkv_tail_bwd_workspace(int64_t N, int64_t H);
+rwkv_status rwkv_tail_bwd(const rwkv_tail* args, const void* dy, int64_t lddy, void* dout, void* dr, void* dk, void* dv,
+                          void* dgate, void* dr_k, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
 /* ───────────────────────── x070 decode step around the hot path ───────────────────────── */
 /* fp32 activations; dense vector parameters fp32 (an fp16 file's values
  * widen exactly); low-rank matrices f16 (the reference's `lin` narrowing,

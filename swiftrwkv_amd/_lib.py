@@ -60,6 +60,26 @@ class ModelDesc(ctypes.Structure):
                 ("head_size", L), ("vocab_size", L)]
 
 
+class Drop(ctypes.Structure):
+    """rwkv_drop: dropout's random numbers."""
+    _fields_ = [("seed", ctypes.c_uint64), ("seed_dev", P), ("offset", ctypes.c_uint64), ("threshold", ctypes.c_int32)]
+
+
+class Join(ctypes.Structure):
+    """rwkv_join: the operands of a block join."""
+    _fields_ = ([(n, P) for n in ("x", "o", "gate")] + [(n, L) for n in ("ldx", "ldo", "ldg")] +
+                [(n, I) for n in ("x_dt", "dt", "w_dt")] +
+                [(n, P) for n in ("post_weight", "post_bias", "scale", "weight", "bias")] +
+                [("post_eps", F), ("eps", F), ("drop", Drop), ("N", L), ("D", L)])
+
+
+class Tail(ctypes.Structure):
+    """rwkv_tail: the operands of the recurrence's tail."""
+    _fields_ = ([(n, P) for n in ("o", "r", "k", "v", "gate")] + [(n, L) for n in ("ldo", "ldr", "ldk", "ldv", "ldg")] +
+                [(n, I) for n in ("o_dt", "dt", "w_dt")] + [(n, P) for n in ("r_k", "weight", "bias")] +
+                [("eps", F), ("N", L), ("H", L)])
+
+
 # name → (restype, argtypes)
 _SIGS = {
     "rwkv_abi_version": (I, []),
@@ -124,6 +144,13 @@ _SIGS = {
     "rwkv_linear_dgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
     "rwkv_linear_wgrad_workspace": (L, [L, L, L]),
     "rwkv_linear_wgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
+    "rwkv_dropout": (I, [P, I, L, P, L, P, I, ctypes.POINTER(Drop), L, L, P]),
+    "rwkv_join_fwd": (I, [ctypes.POINTER(Join), P, P, P, P]),
+    "rwkv_join_bwd_workspace": (L, [L, L]),
+    "rwkv_join_bwd": (I, [ctypes.POINTER(Join)] + [P] * 13 + [L, P]),
+    "rwkv_tail_fwd": (I, [ctypes.POINTER(Tail), P, P]),
+    "rwkv_tail_bwd_workspace": (L, [L, L]),
+    "rwkv_tail_bwd": (I, [ctypes.POINTER(Tail), P, L] + [P] * 9 + [L, P]),
     "rwkv_layer_norm": (I, [P, I, P, L, P, P, P, L, L, F, P]),
     "rwkv_x070_seq_shift_mix": (I, [P, P, P, P, P, I, I, P, I, L, L, P, L, L, I, L, L, L, P]),
     "rwkv_x070_seq_tmix_pre": (I, [P] * 10 + [I, P] + [P] * 7 + [L, L, L, P]),

@@ -20,7 +20,7 @@ EXT = os.path.join(PKG, "_train.so")
 ARCH = os.environ.get("SWIFTRWKV_ARCH", "gfx950")
 
 HIP_SOURCES = ["wkv7.hip", "wkv7_chunked.hip", "rwkvq.hip", "x070.hip", "gemm.hip", "gemv_mfma.hip", "prefill.hip",
-               "norm.hip", "linear.hip"]
+               "norm.hip", "linear.hip", "block.hip"]
 HOST_SOURCES = ["host.cpp", "manifest.cpp"]
 
 # Packed-FP32 VALU ops are disabled for every device compile.

@@ -1,4 +1,4 @@
-// Python module _train: the training-side operators (norm.hip, linear.hip) as
+// Python module _train: the training-side operators (norm.hip, linear.hip, block.hip) as
 // torch functions with their gradients.  The C ABI does the work; this is the
 // argument checks, the allocations and the autograd nodes around it, which in
 // Python cost 112 us for a small layer norm with its gradients and 10 for one
@@ -24,6 +24,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -223,10 +224,11 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // Gradients of gradients: the kernels leave no graph, so a graph through
 // their results raises instead of missing a term, on the way to every input
 // and to what dy was made of.
-variable_list once(variable_list&& g, const Tensor& dy, const Node& node, const char* what) {
+variable_list once(variable_list&& g, std::initializer_list<const Tensor*> dys, const Node& node, const char* what) {
     if (!at::GradMode::is_enabled()) return std::move(g);
     torch::autograd::edge_list edges(node.next_edges());
-    if (wants(dy)) edges.push_back(torch::autograd::impl::gradient_edge(dy));
+    for (const Tensor* dy : dys)
+        if (wants(*dy)) edges.push_back(torch::autograd::impl::gradient_edge(*dy));
     const std::shared_ptr<Node> err(
         new torch::autograd::Error(std::string(what) + ": gradients of its gradients are not available", std::move(edges)),
         torch::autograd::deleteNode);
@@ -236,6 +238,9 @@ variable_list once(variable_list&& g, const Tensor& dy, const Node& node, const 
             torch::autograd::set_history(t, err);
         }
     return std::move(g);
+}
+variable_list once(variable_list&& g, const Tensor& dy, const Node& node, const char* what) {
+    return once(std::move(g), {&dy}, node, what);
 }
 
 // ───────────────────────────── layer norm ─────────────────────────────
@@ -569,6 +574,405 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ───────────────────────────── dropout ─────────────────────────────
+
+// A probability and the two numbers that name its draw; the seed from a tensor
+// is read by the kernels, so a captured call takes what it holds at the replay.
+struct DropArgs {
+    rwkv_drop d{};
+    Tensor seed;
+};
+
+uint64_t count_arg(PyObject* o, const char* what) {
+    if (PyLong_Check(o)) {
+        const uint64_t v = PyLong_AsUnsignedLongLong(o);
+        if (!PyErr_Occurred()) return v;
+        PyErr_Clear();
+    }
+    raise(PyLong_Check(o) ? PyExc_ValueError : PyExc_TypeError, std::string(what) + " must be an integer of 0 to 2^64 - 1");
+}
+
+// p, seed and offset, before anything is known of the device
+DropArgs drop_args(PyObject* p, PyObject* seed, PyObject* offset, const std::string& what) {
+    DropArgs r;
+    const double v = PyFloat_AsDouble(p);
+    if (PyErr_Occurred()) throw python_error();
+    if (!(v >= 0.0 && v <= 1.0)) raise(PyExc_ValueError, what + ": p must be 0 to 1, got " + std::to_string(v));
+    r.d.threshold = (int32_t)std::nearbyint(v * 65536.0);
+    r.d.offset = count_arg(offset, (what + ": offset").c_str());
+    if (THPVariable_Check(seed)) {
+        r.seed = THPVariable_Unpack(seed);
+        if (r.seed.scalar_type() != at::kLong || r.seed.numel() != 1)
+            raise(PyExc_TypeError, what + ": a seed tensor holds one int64, got " + shape_of(r.seed) + " " + type_of(r.seed.scalar_type()));
+    } else {
+        r.d.seed = count_arg(seed, (what + ": seed").c_str());
+    }
+    return r;
+}
+
+// The call's argument; t, the seed's tensor, outlives it.
+const rwkv_drop drop_of(const rwkv_drop& d, const Tensor& t) {
+    rwkv_drop r = d;
+    if (t.defined()) r.seed_dev = static_cast<const int64_t*>(t.const_data_ptr());
+    return r;
+}
+
+// Keeps nothing but the numbers' names: the backward pass draws them again.
+struct DropoutNode : Node {
+    SavedVariable seed;
+    rwkv_drop drop;
+    std::vector<int64_t> shape;
+    at::ScalarType x_dt, y_dt;
+    c10::Device dev{at::kCUDA};
+
+    std::string name() const override { return "DropoutBackward"; }
+    void release_variables() override { seed.reset_data(); }
+
+    variable_list apply(variable_list&& grads) override {
+        const bool need_x = task_should_compute_output(0), need_r = num_outputs() > 1 && task_should_compute_output(1);
+        no_tangent("dropout", {&grads[0]});
+        const Tensor st = seed.unpack(shared_from_this());
+        const Guard guard(dev);
+        const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(shape, at::TensorOptions().dtype(y_dt).device(dev));
+        variable_list out(num_outputs());
+        if (need_r) out[1] = dyt;
+        if (need_x) {
+            const Rows dy = rows_of(dyt);
+            out[0] = empty(shape, x_dt, dev);
+            const rwkv_drop d = drop_of(drop, st);
+            check(rwkv_dropout(dy.p(), dt_of(y_dt), dy.ld, nullptr, 0, ptr(out[0]), dt_of(x_dt), &d, dy.N, dy.D, stream_of(dyt)));
+        }
+        return once(std::move(out), grads[0], *this, "dropout");
+    }
+};
+
+// dropout(x, p, seed, offset, residual)
+PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5) raise(PyExc_TypeError, "dropout: five arguments");
+    const Tensor x = tensor_arg(a[0], "dropout: x"), res = tensor_arg(a[4], "dropout: residual", true);
+    const DropArgs drop = drop_args(a[1], a[2], a[3], "dropout");
+    plain_call("dropout", {&x, &res, &drop.seed});
+    no_tangent("dropout", {&x, &res});
+    const auto xt = x.scalar_type(), yt = res.defined() ? res.scalar_type() : xt;
+    if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > (1 << 22))
+        raise(PyExc_ValueError, "dropout: the last axis must hold 1 to 2^22 values, got " + shape_of(x));
+    if (yt != xt && yt != at::kFloat)
+        raise(PyExc_TypeError, std::string("dropout: residual must be ") + type_of(xt) + " or float32, got " + type_of(yt));
+    if (res.defined() && res.sizes() != x.sizes())
+        raise(PyExc_ValueError, "dropout: residual must be " + shape_of(x) + ", got " + shape_of(res));
+    need_device(x, "dropout: x");
+    if (res.defined()) same_device(x, res, "dropout: residual");
+    if (drop.seed.defined()) same_device(x, drop.seed, "dropout: seed");
+
+    std::shared_ptr<DropoutNode> node;
+    if (at::GradMode::is_enabled() && (wants(x) || wants(res))) {
+        node = std::shared_ptr<DropoutNode>(new DropoutNode(), torch::autograd::deleteNode);
+        node->set_next_edges(res.defined() ? torch::autograd::collect_next_edges(x, res) : torch::autograd::collect_next_edges(x));
+    }
+    const Guard guard(x.device());
+    const Rows xr = rows_of(x);
+    Rows rr{};
+    if (res.defined()) rr = rows_of(res);
+    Tensor y = empty(x.sizes(), yt, x.device());
+    const rwkv_drop d = drop_of(drop.d, drop.seed);
+    check(rwkv_dropout(xr.p(), dt_of(xt), xr.ld, rr.t.defined() ? rr.p() : nullptr, rr.ld, ptr(y), dt_of(yt), &d, xr.N, xr.D,
+                       stream_of(x)));
+    if (node) {
+        if (drop.seed.defined()) node->seed = SavedVariable(drop.seed, false);
+        node->drop = drop.d;
+        node->shape = x.sizes().vec();
+        node->x_dt = xt;
+        node->y_dt = yt;
+        node->dev = x.device();
+        torch::autograd::set_history(y, node);
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// ───────────────────────────── block join ─────────────────────────────
+
+// The vectors of a call, [D] each (or `also`), of one type: float32 or `dt`.
+struct Vector {
+    const char* name;
+    Tensor t;   // as given
+    Tensor c;   // contiguous
+};
+
+at::ScalarType vectors_of(std::initializer_list<Vector*> all, const std::string& what, const Tensor& x, at::ScalarType dt,
+                          int64_t D) {
+    const auto wt = (*all.begin())->t.scalar_type();
+    for (Vector* v : all) {
+        if (!v->t.defined()) continue;
+        if (v->t.dim() != 1 || v->t.size(0) != D)
+            raise(PyExc_ValueError, what + ": " + v->name + " must be [" + std::to_string(D) + "], got " + shape_of(v->t));
+        if (v->t.scalar_type() != wt || (wt != at::kFloat && wt != dt))
+            raise(PyExc_TypeError, what + ": " + v->name + " is " + type_of(v->t.scalar_type()) + "; the vectors share float32 or " +
+                                       type_of(dt));
+    }
+    need_device(x, (what + ": x").c_str());
+    for (Vector* v : all)
+        if (v->t.defined()) {
+            same_device(x, v->t, (what + ": " + v->name).c_str());
+            v->c = v->t.is_contiguous() ? v->t : v->t.detach().contiguous();
+        }
+    return wt;
+}
+
+// Keeps x' (its own result), the statistics, and o and gate where they reach a
+// gradient.
+struct JoinNode : Node {
+    enum { X, O, GATE, W, B, PW, PB, SC, INPUTS };
+    SavedVariable xs, stats, seed, in[INPUTS];   // (X unused)
+    rwkv_drop drop;
+    int at[INPUTS];                              // an input's gradient among the outputs, or -1
+    std::vector<int64_t> shape;
+    at::ScalarType x_dt, dt, w_dt;
+    int64_t N, D;
+    float post_eps, eps;
+
+    std::string name() const override { return "BlockJoinBackward"; }
+
+    void release_variables() override {
+        for (SavedVariable* v : {&xs, &stats, &seed}) v->reset_data();
+        for (SavedVariable& v : in) v.reset_data();
+    }
+
+    variable_list apply(variable_list&& grads) override {
+        no_tangent("block_join", {&grads[0], &grads[1]});
+        const auto self = shared_from_this();
+        const Tensor x1 = xs.unpack(self), st = stats.unpack(self), sd = seed.unpack(self);
+        Tensor t[INPUTS];
+        for (int i = O; i < INPUTS; ++i) t[i] = in[i].unpack(self);
+        const auto dev = st.device();
+        const Guard guard(dev);
+        Rows o{}, g{}, dx{}, dh{};
+        if (t[O].defined()) o = rows_of(t[O]);
+        if (t[GATE].defined()) g = rows_of(t[GATE]);
+        if (grads[0].defined()) dx = rows_of(grads[0], true);
+        if (grads[1].defined()) dh = rows_of(grads[1], true);
+        const auto opt = [](const Rows& r) { return r.t.defined() ? r.p() : nullptr; };
+        variable_list out(num_outputs());
+        void* d[INPUTS] = {};
+        bool sums = false;
+        for (int i = 0; i < INPUTS; ++i) {
+            if (at[i] < 0 || !task_should_compute_output(at[i])) continue;
+            Tensor& r = out[at[i]];
+            r = i < W ? empty(shape, i == X ? x_dt : dt, dev) : empty({D}, w_dt, dev);
+            d[i] = ptr(r);
+            sums = sums || i >= W;
+        }
+        const rwkv_join a{nullptr, opt(o), opt(g), 0, o.ld, g.ld, dt_of(x_dt), dt_of(dt), dt_of(w_dt), cptr(t[PW]), cptr(t[PB]),
+                          cptr(t[SC]), cptr(t[W]), nullptr, post_eps, eps, drop_of(drop, sd), N, D};
+        const Ws ws(sums ? rwkv_join_bwd_workspace(N, D) : 0, dev);
+        check(rwkv_join_bwd(&a, cptr(x1), ptr<float>(st), opt(dx), opt(dh), d[X], d[O], d[GATE], d[W], d[B], d[PW], d[PB], d[SC],
+                            ws.p(), ws.bytes, stream_of(st)));
+        return once(std::move(out), {&grads[0], &grads[1]}, *this, "block_join");
+    }
+};
+
+// block_join(x, o, weight, bias, post_weight, post_bias, gate, scale, p, seed, offset, eps, post_eps): (x', h)
+PyObject* py_block_join(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 13) raise(PyExc_TypeError, "block_join: thirteen arguments");
+    const Tensor x = tensor_arg(a[0], "block_join: x"), o = tensor_arg(a[1], "block_join: o"),
+                 gate = tensor_arg(a[6], "block_join: gate", true);
+    Vector w{"weight", tensor_arg(a[2], "block_join: weight"), {}}, b{"bias", tensor_arg(a[3], "block_join: bias", true), {}},
+        pw{"post_weight", tensor_arg(a[4], "block_join: post_weight", true), {}},
+        pb{"post_bias", tensor_arg(a[5], "block_join: post_bias", true), {}},
+        sc{"scale", tensor_arg(a[7], "block_join: scale", true), {}};
+    const DropArgs drop = drop_args(a[8], a[9], a[10], "block_join");
+    const double eps = PyFloat_AsDouble(a[11]);
+    if (PyErr_Occurred()) throw python_error();
+    const double post_eps = PyFloat_AsDouble(a[12]);
+    if (PyErr_Occurred()) throw python_error();
+    plain_call("block_join", {&x, &o, &gate, &w.t, &b.t, &pw.t, &pb.t, &sc.t, &drop.seed});
+    no_tangent("block_join", {&x, &o, &gate, &w.t, &b.t, &pw.t, &pb.t, &sc.t});
+    if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > 8192)
+        raise(PyExc_ValueError, "block_join: the last axis must hold 1 to 8192 values, got " + shape_of(x));
+    const int64_t D = x.size(-1);
+    const auto xt = x.scalar_type(), dt = o.scalar_type();
+    if (o.sizes() != x.sizes() || (gate.defined() && gate.sizes() != x.sizes()))
+        raise(PyExc_ValueError, "block_join: o " + shape_of(o) + (gate.defined() ? " and gate " + shape_of(gate) : "") + " must be " + shape_of(x) + " as x");
+    if (xt != dt && xt != at::kFloat)
+        raise(PyExc_TypeError, std::string("block_join: x must be float32 or ") + type_of(dt) + " as o, got " + type_of(xt));
+    if (gate.defined() && gate.scalar_type() != dt)
+        raise(PyExc_TypeError, std::string("block_join: gate is ") + type_of(gate.scalar_type()) + ", o " + type_of(dt));
+    if (pb.t.defined() && !pw.t.defined()) raise(PyExc_ValueError, "block_join: post_bias without post_weight");
+    const auto wt = vectors_of({&w, &b, &pw, &pb, &sc}, "block_join", x, dt, D);
+    same_device(x, o, "block_join: o");
+    if (gate.defined()) same_device(x, gate, "block_join: gate");
+    if (drop.seed.defined()) same_device(x, drop.seed, "block_join: seed");
+
+    const Tensor* const inputs[JoinNode::INPUTS] = {&x, &o, &gate, &w.t, &b.t, &pw.t, &pb.t, &sc.t};
+    bool train = false;
+    for (const Tensor* t : inputs) train = train || wants(*t);
+    train = train && at::GradMode::is_enabled();
+    std::shared_ptr<JoinNode> node;
+    if (train) {
+        node = std::shared_ptr<JoinNode>(new JoinNode(), torch::autograd::deleteNode);
+        torch::autograd::edge_list edges;
+        for (int i = 0; i < JoinNode::INPUTS; ++i) {
+            node->at[i] = inputs[i]->defined() ? (int)edges.size() : -1;
+            if (inputs[i]->defined()) edges.push_back(wants(*inputs[i]) ? torch::autograd::impl::gradient_edge(*inputs[i]) : torch::autograd::Edge());
+        }
+        node->set_next_edges(std::move(edges));
+    }
+    const auto dev = x.device();
+    const Guard guard(dev);
+    const Rows xr = rows_of(x), orr = rows_of(o);
+    Rows g{};
+    if (gate.defined()) g = rows_of(gate);
+    Tensor xs = empty(x.sizes(), xt, dev), h = empty(x.sizes(), dt, dev), st;
+    if (train) st = empty({xr.N, 4}, at::kFloat, dev);
+    const rwkv_join j{xr.p(), orr.p(), g.t.defined() ? g.p() : nullptr, xr.ld, orr.ld, g.ld, dt_of(xt), dt_of(dt), dt_of(wt),
+                      cptr(pw.c), cptr(pb.c), cptr(sc.c), cptr(w.c), cptr(b.c), (float)post_eps, (float)eps,
+                      drop_of(drop.d, drop.seed), xr.N, D};
+    check(rwkv_join_fwd(&j, ptr(xs), ptr(h), ptr<float>(st), stream_of(x)));
+    if (train) {
+        node->drop = drop.d;
+        node->shape = x.sizes().vec();
+        node->x_dt = xt;
+        node->dt = dt;
+        node->w_dt = wt;
+        node->N = xr.N;
+        node->D = D;
+        node->eps = (float)eps;
+        node->post_eps = (float)post_eps;
+        if (drop.seed.defined()) node->seed = SavedVariable(drop.seed, false);
+        node->stats = SavedVariable(st, false);
+        if (gate.defined() || pw.t.defined() || sc.t.defined()) node->in[JoinNode::O] = SavedVariable(orr.t, false);
+        if (gate.defined()) node->in[JoinNode::GATE] = SavedVariable(g.t, false);
+        node->in[JoinNode::W] = SavedVariable(w.c, false);
+        if (pw.c.defined()) node->in[JoinNode::PW] = SavedVariable(pw.c, false);
+        if (pb.c.defined()) node->in[JoinNode::PB] = SavedVariable(pb.c, false);
+        if (sc.c.defined()) node->in[JoinNode::SC] = SavedVariable(sc.c, false);
+        torch::autograd::set_history(std::vector<Tensor>{xs, h}, node);
+        node->xs = SavedVariable(xs, true);
+    }
+    PyObject* r = PyTuple_New(2);
+    if (!r) throw python_error();
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(xs)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(h)));
+    return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// ───────────────────────────── the recurrence's tail ─────────────────────────────
+
+struct TailNode : Node {
+    enum { O, R, K, V, GATE, RK, W, B, INPUTS };
+    SavedVariable in[INPUTS];
+    std::vector<int64_t> shape, rk_shape;
+    at::ScalarType o_dt, dt, w_dt;
+    int64_t N, H;
+    float eps;
+
+    std::string name() const override { return "WkvTailBackward"; }
+
+    void release_variables() override {
+        for (SavedVariable& v : in) v.reset_data();
+    }
+
+    variable_list apply(variable_list&& grads) override {
+        no_tangent("wkv_tail", {&grads[0]});
+        const auto self = shared_from_this();
+        Tensor t[INPUTS];
+        Rows r[RK];
+        for (int i = 0; i < INPUTS; ++i) t[i] = in[i].unpack(self);
+        const auto dev = t[O].device();
+        const Guard guard(dev);
+        for (int i = 0; i < RK; ++i) r[i] = rows_of(t[i]);
+        const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(shape, t[R].options());
+        const Rows dy = rows_of(dyt);
+        variable_list out(INPUTS);
+        void* d[INPUTS] = {};
+        bool sums = false;
+        for (int i = RK; i < INPUTS; ++i) sums = sums || task_should_compute_output(i);
+        for (int i = 0; i < INPUTS; ++i) {
+            if (i < RK ? !task_should_compute_output(i) : !sums) continue;   // the three sums go together
+            out[i] = i < RK ? empty(shape, i == O ? o_dt : dt, dev) : empty(i == RK ? at::IntArrayRef(rk_shape) : at::IntArrayRef(shape.back()), w_dt, dev);
+            d[i] = ptr(out[i]);
+        }
+        const rwkv_tail a{r[O].p(), r[R].p(), r[K].p(), r[V].p(), r[GATE].p(), r[O].ld, r[R].ld, r[K].ld, r[V].ld, r[GATE].ld,
+                          dt_of(o_dt), dt_of(dt), dt_of(w_dt), cptr(t[RK]), cptr(t[W]), cptr(t[B]), eps, N, H};
+        const Ws ws(sums ? rwkv_tail_bwd_workspace(N, H) : 0, dev);
+        check(rwkv_tail_bwd(&a, dy.p(), dy.ld, d[O], d[R], d[K], d[V], d[GATE], d[RK], d[W], d[B], ws.p(), ws.bytes,
+                            stream_of(dyt)));
+        for (int i = RK; i < INPUTS; ++i)
+            if (!task_should_compute_output(i)) out[i] = Tensor();
+        return once(std::move(out), grads[0], *this, "wkv_tail");
+    }
+};
+
+// wkv_tail(o, r, k, v, r_k, gate, weight, bias, eps)
+PyObject* py_wkv_tail(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9) raise(PyExc_TypeError, "wkv_tail: nine arguments");
+    const Tensor in[5] = {tensor_arg(a[0], "wkv_tail: o"), tensor_arg(a[1], "wkv_tail: r"), tensor_arg(a[2], "wkv_tail: k"),
+                          tensor_arg(a[3], "wkv_tail: v"), tensor_arg(a[5], "wkv_tail: gate")};
+    const char* const names[5] = {"o", "r", "k", "v", "gate"};
+    const Tensor &o = in[0], &r = in[1];
+    const Tensor rk0 = tensor_arg(a[4], "wkv_tail: r_k");
+    Vector w{"weight", tensor_arg(a[6], "wkv_tail: weight"), {}}, b{"bias", tensor_arg(a[7], "wkv_tail: bias"), {}}, rk{"r_k", rk0, {}};
+    const double eps = PyFloat_AsDouble(a[8]);
+    if (PyErr_Occurred()) throw python_error();
+    plain_call("wkv_tail", {&in[0], &in[1], &in[2], &in[3], &in[4], &rk0, &w.t, &b.t});
+    no_tangent("wkv_tail", {&in[0], &in[1], &in[2], &in[3], &in[4], &rk0, &w.t, &b.t});
+    if (o.dim() < 1 || o.size(-1) < 64 || o.size(-1) % 64 || o.size(-1) > 65536)
+        raise(PyExc_ValueError, "wkv_tail: the last axis must hold 1 to 1024 heads of 64, got " + shape_of(o));
+    const int64_t C = o.size(-1);
+    const auto ot = o.scalar_type(), dt = r.scalar_type();
+    for (int i = 1; i < 5; ++i) {
+        if (in[i].sizes() != o.sizes())
+            raise(PyExc_ValueError, std::string("wkv_tail: ") + names[i] + " must be " + shape_of(o) + " as o, got " + shape_of(in[i]));
+        if (in[i].scalar_type() != dt)
+            raise(PyExc_TypeError, std::string("wkv_tail: ") + names[i] + " is " + type_of(in[i].scalar_type()) + ", r " + type_of(dt));
+    }
+    if (ot != dt && ot != at::kFloat)
+        raise(PyExc_TypeError, std::string("wkv_tail: o must be float32 or ") + type_of(dt) + " as r, got " + type_of(ot));
+    if (rk0.dim() == 2 && rk0.size(0) == C / 64 && rk0.size(1) == 64) rk.t = rk0.detach().reshape({C});
+    const auto wt = vectors_of({&w, &b, &rk}, "wkv_tail", o, dt, C);
+    for (int i = 1; i < 5; ++i) same_device(o, in[i], (std::string("wkv_tail: ") + names[i]).c_str());
+
+    const Tensor* const inputs[TailNode::INPUTS] = {&in[0], &in[1], &in[2], &in[3], &in[4], &rk0, &w.t, &b.t};
+    bool train = false;
+    for (const Tensor* t : inputs) train = train || wants(*t);
+    train = train && at::GradMode::is_enabled();
+    std::shared_ptr<TailNode> node;
+    if (train) {
+        node = std::shared_ptr<TailNode>(new TailNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(in[0], in[1], in[2], in[3], in[4], rk0, w.t, b.t));
+    }
+    const auto dev = o.device();
+    const Guard guard(dev);
+    Rows rows[5];
+    for (int i = 0; i < 5; ++i) rows[i] = rows_of(in[i]);
+    Tensor y = empty(o.sizes(), dt, dev);
+    const rwkv_tail j{rows[0].p(), rows[1].p(), rows[2].p(), rows[3].p(), rows[4].p(), rows[0].ld, rows[1].ld, rows[2].ld,
+                      rows[3].ld, rows[4].ld, dt_of(ot), dt_of(dt), dt_of(wt), cptr(rk.c), cptr(w.c), cptr(b.c), (float)eps,
+                      rows[0].N, C / 64};
+    check(rwkv_tail_fwd(&j, ptr(y), stream_of(o)));
+    if (train) {
+        for (int i = 0; i < 5; ++i) node->in[i] = SavedVariable(rows[i].t, false);
+        node->in[TailNode::RK] = SavedVariable(rk.c, false);
+        node->in[TailNode::W] = SavedVariable(w.c, false);
+        node->in[TailNode::B] = SavedVariable(b.c, false);
+        node->shape = o.sizes().vec();
+        node->rk_shape = rk0.sizes().vec();
+        node->o_dt = ot;
+        node->dt = dt;
+        node->w_dt = wt;
+        node->N = rows[0].N;
+        node->H = C / 64;
+        node->eps = (float)eps;
+        torch::autograd::set_history(y, node);
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // ───────────────────────────── checkpoints ─────────────────────────────
 
 // checkpoint8(x): (codes, scales)
@@ -628,6 +1032,9 @@ PyObject* py_set_error(PyObject*, PyObject* type) {
 PyMethodDef methods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))py_layer_norm, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))py_linear, METH_FASTCALL, nullptr},
+    {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
+    {"block_join", (PyCFunction)(void (*)(void))py_block_join, METH_FASTCALL, nullptr},
+    {"wkv_tail", (PyCFunction)(void (*)(void))py_wkv_tail, METH_FASTCALL, nullptr},
     {"checkpoint8", py_checkpoint8, METH_O, nullptr},
     {"restore8", (PyCFunction)(void (*)(void))py_restore8, METH_FASTCALL, nullptr},
     {"set_error", py_set_error, METH_O, nullptr},

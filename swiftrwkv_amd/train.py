@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import importlib
 import os
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -109,6 +109,63 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     misaligned) are copied into such rows first, and a backward pass keeps the
     copies."""
     return (_ext or extension()).linear(x, weight, bias, activation, residual, keep8)
+
+
+# ───────────────────────────── around a block ─────────────────────────────
+
+def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *, offset: int = 0,
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """drop(x) + residual, differentiable in both.  x float32, bfloat16 or
+    float16 (last axis at most 2^22); residual of x's type or float32; the
+    result has its type (x's without one).
+
+    A value is dropped, and then zero whatever it was, where its 16-bit random
+    number is under t = round(65536·p); the others are multiplied by
+    65536/(65536 − t).  The numbers come from Philox4x32-10 with the key `seed`
+    and a counter of the value's row and column in [rows, last axis] and
+    `offset`: the same (seed, offset) gives the same mask whatever the type,
+    strides or device, so every call of a step has an offset of its own.  The
+    mask is never stored; the backward pass draws it again.  seed 0 to 2^64 − 1,
+    or an int64 tensor of one value on x's device, which the kernels read as
+    they run (a captured graph: what it holds at the replay), and which must
+    not change between a forward pass and its backward pass."""
+    return (_ext or extension()).dropout(x, p, seed, offset, residual)
+
+
+def block_join(x: torch.Tensor, o: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+               post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+               gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, p: float = 0.0,
+               seed: Union[int, torch.Tensor] = 0, offset: int = 0, eps: float = 1e-5,
+               post_eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The end of one block and the start of the next, in one pass:
+
+        x' = x + scale·drop(gate·LN(o; post_weight, post_bias, post_eps))
+        h  = LN(x'; weight, bias, eps)
+
+    differentiable in all eight tensors.  x [..., D] the residual stream
+    (float32 or o's type), o the block's result and gate [..., D] of one type
+    (float32, bfloat16 or float16), the vectors [D] of one type (float32 or
+    o's); D at most 8192.  Without post_weight o is not normed; gate, scale and
+    p = 0 leave their factors out; drop as `dropout` has it.  Returns (x' of x's
+    type, h of o's).  Statistics and sums are fp32; h comes from x' before its
+    rounding.  The backward pass keeps x' (the result), four numbers a row, and
+    o and gate where they reach a gradient."""
+    return (_ext or extension()).block_join(x, o, weight, bias, post_weight, post_bias, gate, scale, p, seed, offset, eps,
+                                            post_eps)
+
+
+def wkv_tail(o: torch.Tensor, r: torch.Tensor, k: torch.Tensor, v: torch.Tensor, r_k: torch.Tensor, gate: torch.Tensor,
+             weight: torch.Tensor, bias: torch.Tensor, eps: float = 64e-5) -> torch.Tensor:
+    """The time mix's tail (ln_x, the bonus and the gate, RWKVBlock.swift:249-270),
+    differentiable in all eight: (LN(o) of every head of 64 · weight + bias +
+    (Σ r·k·r_k)·v)·gate.
+
+    o [..., 64 H] the recurrence's result (float32 or r's type); r, k, v, gate
+    [..., 64 H] of one type (float32, bfloat16 or float16), which the result
+    has; r_k [64 H] or [H, 64], weight and bias [64 H] of one type (float32 or
+    r's).  H at most 1024.  Sums are fp32; the backward pass keeps the inputs
+    alone.  kernel.wkv_tail is the decode step's, fp32 without gradients."""
+    return (_ext or extension()).wkv_tail(o, r, k, v, r_k, gate, weight, bias, eps)
 
 
 # ───────────────────────────── together ─────────────────────────────
