@@ -442,6 +442,27 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
                             int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                             void* stream);
 
+/* act of a gated product: relu(z)²; σ(z) = 1/(1 + e^-z); z·σ(z); z·σ(2√(2/π)(z +
+ * 0.044715 z³)), the tanh form of the gelu. */
+typedef enum { RWKV_GATE_RELU2 = 0, RWKV_GATE_SIGMOID = 1, RWKV_GATE_SILU = 2, RWKV_GATE_GELU_TANH = 3 } rwkv_gate;
+
+/* h = act(zg)·zu [M, F], [zg | zu] = x·Wᵀ: x [M, K], w [2F, K] (the gate's F
+ * rows, then the other factor's) and h of dt (bf16 or f16).  fp32 sums, one rounding, ties to
+ * even.  For the backward pass, both or neither: aux [M, 2F] of dt receives
+ * zg and zu, rem [M, 2F] their next 8 bits.  F <= 2^19, K <= 2^20.  Workspace
+ * as rwkv_linear_fwd's. */
+int64_t rwkv_gated_fwd_workspace(int64_t M, int64_t F, int64_t K);
+rwkv_status rwkv_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* h, void* aux, uint8_t* rem,
+                           rwkv_gate act, rwkv_dtype dt, int64_t M, int64_t F, int64_t K, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* dz = [dy·zu·act'(zg) | dy·act(zg)] [M, ldz] of dt from the forward's aux
+ * (kept) and rem (2F <= ldz < 2F + 8; columns from 2F on are written as
+ * zeros).  The gradients of x and W are rwkv_linear_dgrad and _wgrad of dz
+ * with N = 2F. */
+rwkv_status rwkv_gated_dact(const void* dy, int64_t lddy, const void* kept, const uint8_t* rem, rwkv_gate act, void* dz,
+                            int64_t ldz, rwkv_dtype dt, int64_t M, int64_t F, void* stream);
+
 /* Rows [N, D] of 16-bit values into pitch D rounded up to 8, zeros behind, y
  * 16-byte aligned: the products above run several times as fast on rows that
  * are 16-byte aligned, and contracting over the zeros changes nothing. */

@@ -144,6 +144,9 @@ _SIGS = {
     "rwkv_linear_dgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
     "rwkv_linear_wgrad_workspace": (L, [L, L, L]),
     "rwkv_linear_wgrad": (I, [P, L, P, L, P, I, L, L, L, P, L, P]),
+    "rwkv_gated_fwd_workspace": (L, [L, L, L]),
+    "rwkv_gated_fwd": (I, [P, L, P, L, P, P, P, I, I, L, L, L, P, L, P]),
+    "rwkv_gated_dact": (I, [P, L, P, P, I, P, L, I, L, L, P]),
     "rwkv_dropout": (I, [P, I, L, P, L, P, I, ctypes.POINTER(Drop), L, L, P]),
     "rwkv_join_fwd": (I, [ctypes.POINTER(Join), P, P, P, P]),
     "rwkv_join_bwd_workspace": (L, [L, L]),

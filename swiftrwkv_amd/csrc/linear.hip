@@ -7,6 +7,8 @@
 //   dz        dz = dy·act'(z), db = Σ_rows dz
 //   input     dx = dz·W
 //   weight    dW = dzᵀ·x
+//   gated     h  = act(x·Wgᵀ)·(x·Wuᵀ), W = [Wg; Wu] [2F, K]; its gradients are
+//             the input's and the weight's of dz = [dzg | dzu]
 //
 // All three are C[m, n] = Σ_k A[m, k]·B[n, k] over operands that are either
 // k-contiguous (x and W of the forward pass, dz of the input gradient) or
@@ -268,20 +270,87 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t row, int step,
     }
 }
 
+// ───────────────────────────── gates ─────────────────────────────
+
+enum { GATE_RELU2 = RWKV_GATE_RELU2, GATE_SIGMOID = RWKV_GATE_SIGMOID, GATE_SILU = RWKV_GATE_SILU, GATE_GELU = RWKV_GATE_GELU_TANH };
+
+// The gelu's argument of σ, 2·√(2/π)·(z + 0.044715 z³), and its slope: the tanh
+// form is z·(1 + tanh(u/2))/2 = z·σ(u).
+constexpr float GELU_A = 1.5957691216057308f, GELU_B = 0.07135481627260025f;
+__device__ __forceinline__ float gelu_arg(float z) { return z * (GELU_A + GELU_B * z * z); }
+
+// act(z).  σ saturates: its 0 and 1 are right for any z (a z³ past fp32's range
+// is an infinity).
+__device__ __forceinline__ float gate_of(int act, float z) {
+    if (act == GATE_RELU2) {
+        const float r = z < 0.0f ? 0.0f : z;   // a NaN stays one
+        return r * r;
+    }
+    const float s = sigmoid_of(act == GATE_GELU ? gelu_arg(z) : z);
+    return act == GATE_SIGMOID ? s : z * s;
+}
+
+// act'(z): 2·relu(z); σσ'; σ + z·σσ'·u', with σσ' = σ(u)·σ(−u) by t = e^(−|u|) as
+// above.  From |z| = 100 on t is 0 in fp32 and so is the second term, which z²'s
+// infinity would make a NaN.
+__device__ __forceinline__ float gate_slope(int act, float z) {
+    if (act == GATE_RELU2) return z < 0.0f ? 0.0f : 2.0f * z;
+    const float c = fabsf(z) > 100.0f ? __builtin_copysignf(100.0f, z) : z;
+    const float u = act == GATE_GELU ? gelu_arg(c) : c;
+    if (act == GATE_SIGMOID) return sigmoid_slope(z);
+    return sigmoid_of(u) + c * sigmoid_slope(u) * (act == GATE_GELU ? GELU_A + 3.0f * GELU_B * c * c : 1.0f);
+}
+
+// Eight neighbouring columns of h = act(zg)·zu in each of C rows row, row +
+// step, ...; with aux and rem [M, 2F], zg and zu in 16 + 8 bits for the backward
+// pass, side by side as W's rows lie.
+template <typename T, int C>
+__device__ __forceinline__ void finish_gated(const Epilogue& e, int64_t row, int step, int col, float (&zg)[C][8], float (&zu)[C][8]) {
+    const int valid = e.N - col;
+    if (valid <= 0) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int64_t r = row + c * step;
+        if (r >= e.M) continue;
+        if (e.aux) {
+            const int64_t at = r * 2 * e.N + col;
+            const uint4 g = round8<T>(zg[c]), u = round8<T>(zu[c]);
+            store_raw(reinterpret_cast<T*>(e.aux) + at, valid, g);
+            store_raw(reinterpret_cast<T*>(e.aux) + at + e.N, valid, u);
+            store_raw(e.rem + at, valid, rem8<T>(zg[c], g));
+            store_raw(e.rem + at + e.N, valid, rem8<T>(zu[c], u));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zg[c][i] = gate_of(e.act, zg[c][i]) * zu[c][i];
+        store_raw(reinterpret_cast<T*>(e.y) + r * e.N + col, valid, round8<T>(zg[c]));
+    }
+}
+
+// Sixteen staged columns of a gated product: eight of zg, the same eight of zu.
+__device__ __forceinline__ void split16(float4 a, float4 b, float4 c, float4 d, float (&zg)[8], float (&zu)[8]) {
+    zg[0] = a.x; zg[1] = a.y; zg[2] = a.z; zg[3] = a.w;
+    zg[4] = b.x; zg[5] = b.y; zg[6] = b.z; zg[7] = b.w;
+    zu[0] = c.x; zu[1] = c.y; zu[2] = c.z; zu[3] = c.w;
+    zu[4] = d.x; zu[5] = d.y; zu[6] = d.z; zu[7] = d.w;
+}
+
 // ───────────────────────────── operand tiles ─────────────────────────────
 
 // ROWS output rows (or columns) × BK of an operand: how a workgroup loads a
 // stage of it into registers, writes it to LDS and reads operands back.  ODD:
 // rows that are not 16-byte aligned or a k-contiguous length that 8 does not
 // divide; elsewhere buffer loads, whose range check fills what lies outside
-// the operand with zeros.
-template <typename T, bool KM, int ROWS, int THREADS, bool ODD>
+// the operand with zeros.  GATED: a k-contiguous W of twice `total` rows, whose
+// halves the tile's rows take by turns of eight, so that a column of zg and the
+// same of zu end up in one lane; a wave's chunks are all of one half.
+template <typename T, bool KM, int ROWS, int THREADS, bool ODD, bool GATED = false>
 struct Tile {
     static constexpr int P = ROWS * 8 / THREADS;   // 16-byte chunks per thread and stage
     static constexpr int CPR = KM ? ROWS / 8 : 8;  // chunks per LDS row
     static constexpr int STEP = THREADS / CPR;     // LDS rows a thread's chunks are apart
     static constexpr int BYTES = ROWS * BK * 2;
     static_assert(P >= 1 && THREADS % CPR == 0, "tile shape");
+    static_assert(!GATED || (!KM && STEP % 16 == 0), "a wave's rows are one half's");
 
     const T* p;       // operand, at the tile's first row (k-contiguous) or column (k-major)
     int64_t ld;
@@ -291,9 +360,15 @@ struct Tile {
     bool whole;       // the operand's rows hold a chunk
 
     __device__ __forceinline__ Tile(const void* base, int64_t ld_, int64_t at, int64_t total, int K_, int tid)
-        : p(reinterpret_cast<const T*>(base) + (KM ? at : at * ld_)), ld(ld_),
-          rows((int)min(total - at, (int64_t)(KM ? (1 << 30) : ROWS))), K(K_), c(tid % CPR), r(tid / CPR),
+        : p(reinterpret_cast<const T*>(base) + (KM ? at : (at + half(tid) * total) * ld_)), ld(ld_),
+          rows((int)min(total - at, (int64_t)(KM ? (1 << 30) : GATED ? ROWS / 2 : ROWS))), K(K_), c(tid % CPR), r(tid / CPR),
           whole((KM ? total : (int64_t)K_) >= 8) {}
+
+    static __device__ __forceinline__ int half(int tid) { return GATED ? __builtin_amdgcn_readfirstlane(tid >> 6) & 1 : 0; }
+    // the operand's row that is LDS row r + STEP·i
+    __device__ __forceinline__ int source(int i) const {
+        return GATED ? (r >> 4) * 8 + (r & 7) + STEP / 2 * i : r + STEP * i;
+    }
 
     __device__ __forceinline__ void load(uint4 (&v)[P], int st) const {
         if constexpr (ODD) {
@@ -303,14 +378,14 @@ struct Tile {
             if (whole) {
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    const int row = r + STEP * i;
+                    const int row = source(i);
                     const T* q = p + (KM ? (int64_t)min(st * BK + row, K - 1) * ld : (int64_t)min(row, rows - 1) * ld) + from(st);
                     __builtin_memcpy(&v[i], q, 16);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    const int row = r + STEP * i;
+                    const int row = source(i);
                     const int k = KM ? st * BK + row : st * BK + 8 * c;
                     const int valid = KM ? (k < K ? rows - 8 * c : 0) : (row < rows ? K - k : 0);
                     const T* q = p + (KM ? (int64_t)k * ld + 8 * c : (int64_t)row * ld + k);
@@ -337,8 +412,8 @@ struct Tile {
                 const_cast<T*>(p), 0, (int)(((int64_t)(rows - 1) * ld + K) * 2), 0x00020000);
             const int k = st * BK + 8 * c;
             // past the last k: an offset outside the range (also after the row steps are added)
-            const uint32_t o = k < K ? (uint32_t)(r * (int)ld + k) * 2 : 0x80000000u;
-            const uint32_t step = (uint32_t)(STEP * (int)ld) * 2;
+            const uint32_t o = k < K ? (uint32_t)(source(0) * (int)ld + k) * 2 : 0x80000000u;
+            const uint32_t step = (uint32_t)((GATED ? STEP / 2 : STEP) * (int)ld) * 2;
 #pragma unroll
             for (int i = 0; i < P; ++i)
                 v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, o + i * step, 0, 0));
@@ -459,7 +534,7 @@ __device__ __forceinline__ int items_of(const GemmArgs& g, int ntm, int ntn) {
 template <int AN>
 constexpr int EROW = 16 * AN + 4;   // floats per staged row
 
-template <typename T, int AM, int AN, int RC>
+template <typename T, int AM, int AN, int RC, bool GATED>
 __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc)[AM][AN], float* stage, int64_t row0,
                                             int col0, int lane, float* part, int pitch) {
     static_assert(AM % RC == 0, "row tiles per pass");
@@ -476,6 +551,19 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc
                 for (int q = 0; q < 4; ++q)
                     stage[(16 * i + 4 * gq + q) * EROW<AN> + 16 * j + li] = acc[h * RC + i][j][q];
         __builtin_amdgcn_wave_barrier();
+        if (GATED && !part) {   // sixteen columns a lane
+            constexpr int GPP = 64 / AN, G = 16 * RC / GPP;
+            const int r0 = lane / AN, c0 = 16 * (lane % AN);
+            float zg[G][8], zu[G][8];
+#pragma unroll
+            for (int c = 0; c < G; ++c) {
+                const float4* at = reinterpret_cast<const float4*>(stage + (r0 + c * GPP) * EROW<AN> + c0);
+                split16(at[0], at[1], at[2], at[3], zg[c], zu[c]);
+            }
+            finish_gated<T, G>(g.e, row0 + h * 16 * RC + r0, GPP, (col0 + c0) / 2, zg, zu);
+            __builtin_amdgcn_wave_barrier();
+            continue;
+        }
         constexpr int C = 16 * RC / RPP < 4 ? 16 * RC / RPP : 4;   // rows of a lane per round
 #pragma unroll 1
         for (int rloc = lane / LPR; rloc < 16 * RC; rloc += C * RPP) {
@@ -492,7 +580,7 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc
 #pragma unroll
                 for (int c = 0; c < C; ++c)
                     if (row + c * RPP < g.M) store8(part + (h * 16 * RC + rloc + c * RPP) * pitch + cl, 8, v[c]);
-            } else {
+            } else if constexpr (!GATED) {
                 finish<T, C>(g.e, row, RPP, col, v);
             }
         }
@@ -500,11 +588,11 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, const f32x4 (&acc
     }
 }
 
-template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, bool ODD>
+template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, bool ODD, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     constexpr int BM = 16 * WM * AM, BN = 16 * WN * AN, THREADS = 64 * WM * WN;
     using TileA = Tile<T, AKM, BM, THREADS, ODD>;
-    using TileB = Tile<T, BKM, BN, THREADS, ODD>;
+    using TileB = Tile<T, BKM, BN, THREADS, ODD, GATED>;
     constexpr int STAGE = TileA::BYTES + TileB::BYTES;
     static_assert(WM * WN * 32 * EROW<AN> * 4 <= 2 * STAGE, "epilogue staging");
     __shared__ __align__(16) char lds[2 * STAGE];
@@ -516,7 +604,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     const int st0 = it.st0, st1 = it.st1;
 
     const TileA ta(g.a, g.lda, m0, g.M, g.K, tid);
-    const TileB tb(g.b, g.ldb, n0, g.N, g.KB, tid);
+    const TileB tb(g.b, g.ldb, GATED ? n0 / 2 : n0, GATED ? g.N / 2 : g.N, g.KB, tid);
     const int wm = wave % WM, wn = wave / WM;
     f32x4 acc[AM][AN];
 #pragma unroll
@@ -561,7 +649,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     }
 
     float* const part = it.part < 0 ? nullptr : g.part + (int64_t)it.part * BM * BN + wm * AM * 16 * BN + wn * AN * 16;
-    finish_tile<T, AM, AN, 2>(g, acc, reinterpret_cast<float*>(lds) + wave * 32 * EROW<AN>, m0 + wm * AM * 16,
+    finish_tile<T, AM, AN, 2, GATED>(g, acc, reinterpret_cast<float*>(lds) + wave * 32 * EROW<AN>, m0 + wm * AM * 16,
                               n0 + wn * AN * 16, lane, part, BN);
 }
 
@@ -594,13 +682,13 @@ __device__ __forceinline__ i32x4 rsrc_of(uint64_t base, uint32_t bytes) {
 // ROWS × BK of an operand with 16-byte aligned rows, as Tile lays it out.  A
 // load covers 1024 LDS bytes; the permutation of the LDS layout is applied to
 // the global addresses its lanes read.
-template <typename T, bool KM, int ROWS, int WAVES, bool FEW>
+template <typename T, bool KM, int ROWS, int WAVES, bool FEW, bool GATED = false>
 struct DmaTile {
     static constexpr int P = ROWS / 8 / WAVES;       // loads per wave and stage
     static constexpr int KR = KM ? 512 / ROWS : 0;   // k rows per load
     static constexpr int BYTES = ROWS * BK * 2;
-    static_assert(P >= 1, "tile shape");
-    using Read = Tile<T, KM, ROWS, 64 * WAVES, false>;
+    static_assert(P >= 1 && (!GATED || (!KM && WAVES % 2 == 0)), "tile shape");
+    using Read = Tile<T, KM, ROWS, 64 * WAVES, false, GATED>;
 
     i32x4 r;           // the stage's part of the tile
     int64_t ld;
@@ -622,7 +710,9 @@ struct DmaTile {
             } else {
                 const int row = (j * WAVES + wave) * 8 + (lane >> 3);
                 c = 8 * ((lane & 7) ^ (row & 7));   // the same for every j
-                off[j] = (uint32_t)(row * (int)ld + c) * 2;
+                // (of a wave's half of W)
+                const int from = GATED ? ((j * WAVES + wave) >> 1) * 8 + (lane >> 3) : row;
+                off[j] = (uint32_t)(from * (int)ld + c) * 2;
             }
         }
     }
@@ -634,7 +724,7 @@ struct DmaTile {
 
     // Row (column) `at` of `total`, stage st of an operand of K.
     __device__ __forceinline__ void start(const void* base, int64_t at, int64_t total, int K, int st) {
-        const int rows = (int)min(total - at, (int64_t)ROWS);
+        const int rows = (int)min(total - at, (int64_t)(GATED ? ROWS / 2 : ROWS));
         k = K - st * BK;
         // a dword that holds a last odd column may be read whole
         cols = (rows + 1) & ~1;
@@ -676,11 +766,11 @@ enum { EPI_PLAIN, EPI_PART, EPI_FULL };
 //
 // The products are taken as (B tile)·(A tile)ᵀ, so that a lane holds four
 // neighbouring columns of a row: columns 16j + 4g .. + 3 of row 16i + (l & 15).
-template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, int EPI>
+template <typename T, bool AKM, bool BKM, int WM, int WN, int AM, int AN, int EPI, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
     constexpr int BM = 16 * WM * AM, BN = 16 * WN * AN, W = WM * WN;
     using DA = DmaTile<T, AKM, BM, W, EPI == EPI_PART>;
-    using DB = DmaTile<T, BKM, BN, W, EPI == EPI_PART>;
+    using DB = DmaTile<T, BKM, BN, W, EPI == EPI_PART, GATED>;
     using TileA = typename DA::Read;
     using TileB = typename DB::Read;
     constexpr uint32_t STAGE = DA::BYTES + DB::BYTES;
@@ -710,7 +800,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
         if (l_item < items) {
             const Item it = item_of(g, l_item, ntm, ntn);
             da.start(g.a, (int64_t)it.tm * BM, g.M, g.K, it.st0);
-            db.start(g.b, (int64_t)it.tn * BN, g.N, g.KB, it.st0);
+            if constexpr (GATED)
+                db.start(reinterpret_cast<const T*>(g.b) + (wave & 1) * (int64_t)(g.N / 2) * g.ldb, (int64_t)it.tn * (BN / 2), g.N / 2, g.KB, it.st0);
+            else
+                db.start(g.b, (int64_t)it.tn * BN, g.N, g.KB, it.st0);
             l_left = it.st1 - it.st0;
         } else {
             da.end();
@@ -839,6 +932,20 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
                         own[li * CPR + ((4 * j + gq) ^ li)] = make_float4(acc[k][j][0], acc[k][j][1], acc[k][j][2], acc[k][j][3]);
                 }
                 __builtin_amdgcn_wave_barrier();
+                if constexpr (GATED) {   // sixteen columns a lane
+                    constexpr int LPR = CPR / 4, RPP = 64 / LPR, C = 16 / RPP;
+                    const int q = l % LPR;
+                    float zg[C][8], zu[C][8];
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const int r = c * RPP + l / LPR;
+                        const float4* at = own + r * CPR;
+                        split16(at[(4 * q) ^ r], at[(4 * q + 1) ^ r], at[(4 * q + 2) ^ r], at[(4 * q + 3) ^ r], zg[c], zu[c]);
+                    }
+                    finish_gated<T, C>(g.e, row0 + 16 * i + l / LPR, RPP, col0 / 2 + 8 * q, zg, zu);
+                    __builtin_amdgcn_wave_barrier();
+                    continue;
+                }
                 constexpr int LPR = CPR / 2, RPP = 64 / LPR, C = 16 / RPP;   // lanes per row, rows per step
                 const int q = l % LPR;
                 float v[C][8];
@@ -867,27 +974,34 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_dma_kernel(GemmArgs g) {
 }
 
 // Sums the K ranges of the tiles from g.full on, in order, and finishes them:
-// a thread per 8 columns.
-template <typename T>
+// a thread per 8 columns, or 16 of a gated product.
+template <typename T, bool GATED>
 __global__ __launch_bounds__(256) void split_reduce_kernel(GemmArgs g, int BM, int BN, int ntm, int ntn) {
-    const int rest = ntm * ntn - g.full, per = BM * BN / 8 / 256;   // blocks per tile
+    constexpr int W = GATED ? 16 : 8;
+    const int rest = ntm * ntn - g.full, per = BM * BN / W / 256;   // blocks per tile
     const int t = blockIdx.x / per, at = (blockIdx.x - t * per) * 256 + threadIdx.x;
     int tm, tn;
     tile_of(g.full + t, ntm, ntn, tm, tn);
-    const int r = at / (BN / 8), c = 8 * (at - r * (BN / 8));
+    const int r = at / (BN / W), c = W * (at - r * (BN / W));
     const int64_t row = (int64_t)tm * BM + r;
     if (row >= g.M) return;   // whole quads: a row's chunks
     const int col = tn * BN + c;
     const float* p = g.part + ((int64_t)t * BM + r) * BN + c;
-    float v[1][8] = {};
+    float v[1][8] = {}, u[1][8] = {};
 #pragma unroll 4
     for (int s = 0; s < g.splits; ++s) {
         float q[8];
         load8(p + (int64_t)s * rest * BM * BN, 8, q);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[0][k] += q[k];
+        if constexpr (GATED) {
+            load8(p + (int64_t)s * rest * BM * BN + 8, 8, q);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[0][k] += q[k];
+        }
     }
-    finish<T, 1>(g.e, row, 1, col, v);
+    if constexpr (GATED) finish_gated<T, 1>(g.e, row, 1, col / 2, v, u);
+    else finish<T, 1>(g.e, row, 1, col, v);
 }
 
 // ───────────────────────────── a few rows ─────────────────────────────
@@ -896,7 +1010,8 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(GemmArgs g, int BM, i
 // waves every eighth 32 of k, straight from memory into the products' operands
 // (any alignment), the next U of each on their way under U products; their
 // sums meet in LDS, in order.
-template <typename T, int NT>
+// GATED: eight rows of each half of W make the 16 columns.
+template <typename T, int NT, bool GATED>
 __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     constexpr int WAVES = 8, U = 8 / NT;
     __shared__ __align__(16) float sums[WAVES][16][16 * NT + 4];
@@ -905,7 +1020,10 @@ __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     const T* xr = reinterpret_cast<const T*>(g.a) + (int64_t)min(i, (int)g.M - 1) * g.lda;
     const T* wr[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) wr[t] = reinterpret_cast<const T*>(g.b) + (int64_t)min(n0 + 16 * t + i, g.N - 1) * g.ldb;
+    for (int t = 0; t < NT; ++t) {
+        const int row = GATED ? (i >> 3) * (g.N / 2) + min(n0 / 2 + 8 * t + (i & 7), g.N / 2 - 1) : min(n0 + 16 * t + i, g.N - 1);
+        wr[t] = reinterpret_cast<const T*>(g.b) + (int64_t)row * g.ldb;
+    }
     auto chunk = [&](const T* p, int k) {
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (k + 8 <= g.K) {
@@ -951,6 +1069,17 @@ __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     for (int t = 0; t < NT; ++t)
         *reinterpret_cast<f32x4*>(&sums[wave][i][16 * t + 4 * q]) = acc[t];
     __syncthreads();
+    if constexpr (GATED) {
+        if (threadIdx.x >= 16 * NT) return;
+        const int m = threadIdx.x / NT, c = 16 * (threadIdx.x % NT);
+        float zg[1][8] = {}, zu[1][8] = {};
+#pragma unroll
+        for (int r = 0; r < WAVES; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) zg[0][e] += sums[r][m][c + e], zu[0][e] += sums[r][m][c + 8 + e];
+        finish_gated<T, 1>(g.e, m, 1, (n0 + c) / 2, zg, zu);
+        return;
+    }
     if (threadIdx.x >= 32 * NT) return;
     const int m = threadIdx.x / (2 * NT), c = 8 * (threadIdx.x % (2 * NT));
     float v[1][8] = {};
@@ -1096,6 +1225,49 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
     if (valid > 0) store8(a.part + (int64_t)blockIdx.y * a.N + col, valid, s);
 }
 
+struct GatedArgs {
+    const void* dy;         // [M, lddy]
+    int64_t lddy;
+    const void* kept;       // [M, 2F]: zg, zu
+    const uint8_t* rem;     // [M, 2F]: their next 8 bits
+    int act;
+    void* dz;               // [M, ldz], ldz >= 2F; columns from 2F on are written as zeros
+    int64_t ldz;
+    int64_t M;
+    int F;
+};
+
+// dzg = dy·zu·act'(zg), dzu = dy·act(zg), rounded to the operands' type for the
+// products (as dact_kernel).  TX chunks of 8 columns across, 256/TX rows down a
+// block, rows strided over gridDim.y.
+template <typename T>
+__global__ __launch_bounds__(256) void gated_dact_kernel(GatedArgs a, int TX) {
+    const int tx = threadIdx.x % TX, TY = 256 / TX;
+    const int col = 8 * (blockIdx.x * TX + tx), valid = a.F - col;
+    if (valid <= 0) return;
+    const int64_t step = (int64_t)gridDim.y * TY;
+    for (int64_t row = (int64_t)blockIdx.y * TY + threadIdx.x / TX; row < a.M; row += step) {
+        float d[8], g[8], u[8];
+        const int64_t at = row * 2 * a.F + col;
+        load8(reinterpret_cast<const T*>(a.dy) + row * a.lddy + col, valid, d);
+        load8(reinterpret_cast<const T*>(a.kept) + at, valid, g);
+        load8(reinterpret_cast<const T*>(a.kept) + at + a.F, valid, u);
+        load_rem8<T>(a.rem + at, valid, g);
+        load_rem8<T>(a.rem + at + a.F, valid, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = g[i];
+            g[i] = d[i] * u[i] * gate_slope(a.act, v);
+            u[i] = d[i] * gate_of(a.act, v);
+        }
+        T* z = reinterpret_cast<T*>(a.dz) + row * a.ldz;
+        store8(z + col, valid, g);
+        store8(z + a.F + col, valid, u);
+        if (valid <= 8)
+            for (int64_t i = 2 * (int64_t)a.F; i < a.ldz; ++i) z[i] = (T)0.0f;
+    }
+}
+
 // Column sums of part [G][N], in order within 16 interleaved runs of rows.
 template <typename T>
 __global__ __launch_bounds__(256) void bias_reduce_kernel(const float* part, int G, int N, T* out) {
@@ -1187,34 +1359,35 @@ int64_t route_workspace(const Route& r, int64_t M, int64_t N) {
 
 // The whole tiles, then the pieces of the others, on at most `fit` workgroups
 // (what the LDS of 256 CUs holds).
-template <typename T, bool AKM, bool BKM, int AM, int AN>
+template <typename T, bool AKM, bool BKM, int AM, int AN, bool GATED>
 void gemm_launch_dma(int fit, const GemmArgs& g, int64_t items, hipStream_t s) {
     const dim3 whole((unsigned)std::min<int64_t>(g.full, fit)), pieces((unsigned)std::min<int64_t>(items - g.full, fit));
     if (g.full > 0) {
         if constexpr (!AKM && !BKM) {
-            if (g.e.plain) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN>, whole, dim3(256), s, g);
-            else rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_FULL>, whole, dim3(256), s, g);
+            if constexpr (!GATED)
+                if (g.e.plain) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN, false>, whole, dim3(256), s, g);
+            if (!g.e.plain) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_FULL, GATED>, whole, dim3(256), s, g);
         } else {
-            rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN>, whole, dim3(256), s, g);
+            rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PLAIN, false>, whole, dim3(256), s, g);
         }
     }
     if constexpr (!(AKM && BKM && AN == 8))
-        if (items > g.full) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PART>, pieces, dim3(256), s, g);
+        if (items > g.full) rwkv::launch(gemm_dma_kernel<T, AKM, BKM, 2, 2, AM, AN, EPI_PART, GATED>, pieces, dim3(256), s, g);
 }
 
-template <typename T, bool AKM, bool BKM, bool ODD>
+template <typename T, bool AKM, bool BKM, bool ODD, bool GATED>
 void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
     const int64_t items = g.full + (tiles_of(g.M, g.N, r.bm, r.bn) - g.full) * g.splits;
     const dim3 grid((unsigned)items);
     if constexpr (!ODD) {
-        if (r.bm == 256 && r.bn == 256) return gemm_launch_dma<T, AKM, BKM, 8, 8>(256, g, items, s);
-        if (r.bm == 256) return gemm_launch_dma<T, AKM, BKM, 8, 4>(256, g, items, s);
-        if (r.bm == 128) return gemm_launch_dma<T, AKM, BKM, 4, 4>(512, g, items, s);
+        if (r.bm == 256 && r.bn == 256) return gemm_launch_dma<T, AKM, BKM, 8, 8, GATED>(256, g, items, s);
+        if (r.bm == 256) return gemm_launch_dma<T, AKM, BKM, 8, 4, GATED>(256, g, items, s);
+        if (r.bm == 128) return gemm_launch_dma<T, AKM, BKM, 4, 4, GATED>(512, g, items, s);
     }
     if (r.bm == 128)
-        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 4, 4, true>, grid, dim3(256), s, g);
+        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 4, 4, true, GATED>, grid, dim3(256), s, g);
     else
-        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 2, 2, ODD>, grid, dim3(256), s, g);
+        rwkv::launch(gemm_kernel<T, AKM, BKM, 2, 2, 2, 2, ODD, GATED>, grid, dim3(256), s, g);
 }
 
 // Few rows with a short K (a wave's loads on their way at once hold 2048 of it,
@@ -1230,16 +1403,23 @@ void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
 // 2048 6.4 and 11.3), and from N = 6144 on a K of 512, or one of 8192, loses.
 bool rows16_applies(int64_t M, int64_t N, int64_t K) { return M <= 16 && (K <= 1024 || N >= 8192); }
 
-// C = A·Bᵀ by the route of its sizes, then the epilogue.
+// C = A·Bᵀ by the route of its sizes, then the epilogue.  gated: C's columns are
+// zg's and zu's by turns of eight (both operands k-contiguous).
 rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, void* workspace, int64_t bytes,
-                     hipStream_t s) {
+                     hipStream_t s, bool gated = false) {
+    if (gated && rows16_applies(g.M, g.N, g.K)) {
+        const dim3 grid((unsigned)((g.N + 15) / 16));
+        if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 1, true>, grid, dim3(512), s, g);
+        else rwkv::launch(rows16_kernel<f16, 1, true>, grid, dim3(512), s, g);
+        return status_of(what);
+    }
     if (!akm && !bkm && rows16_applies(g.M, g.N, g.K)) {
         const int nt = g.e.codes ? 2 : 1;   // a group of codes is 32 columns
         const dim3 grid((unsigned)((g.N + 16 * nt - 1) / (16 * nt)));
-        if (dt == RWKV_BF16 && nt == 1) rwkv::launch(rows16_kernel<bf16, 1>, grid, dim3(512), s, g);
-        else if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 2>, grid, dim3(512), s, g);
-        else if (nt == 1) rwkv::launch(rows16_kernel<f16, 1>, grid, dim3(512), s, g);
-        else rwkv::launch(rows16_kernel<f16, 2>, grid, dim3(512), s, g);
+        if (dt == RWKV_BF16 && nt == 1) rwkv::launch(rows16_kernel<bf16, 1, false>, grid, dim3(512), s, g);
+        else if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 2, false>, grid, dim3(512), s, g);
+        else if (nt == 1) rwkv::launch(rows16_kernel<f16, 1, false>, grid, dim3(512), s, g);
+        else rwkv::launch(rows16_kernel<f16, 2, false>, grid, dim3(512), s, g);
         return status_of(what);
     }
     const bool aligned = (uintptr_t)g.a % 16 == 0 && (uintptr_t)g.b % 16 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0;
@@ -1254,16 +1434,19 @@ rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, v
     g.splits = r.splits;
     g.per = r.per;
     g.part = (float*)workspace;
-    g.e.plain = !g.e.bias && !g.e.res && !g.e.wide && !g.e.aux && !g.e.rem && !g.e.codes && g.e.act == ACT_NONE;
+    g.e.plain = !gated && !g.e.bias && !g.e.res && !g.e.wide && !g.e.aux && !g.e.rem && !g.e.codes && g.e.act == ACT_NONE;
     auto by_layout = [&](auto type, auto o) {
         using T = decltype(type);
         constexpr bool O = decltype(o)::value;
-        if (!akm && !bkm) gemm_launch_tile<T, false, false, O>(r, g, s);
-        else if (!akm) gemm_launch_tile<T, false, true, O>(r, g, s);
-        else gemm_launch_tile<T, true, true, O>(r, g, s);
-        if (rest > 0)
-            rwkv::launch(split_reduce_kernel<T>, dim3((unsigned)(rest * (r.bm * r.bn / 2048))), dim3(256), s, g, r.bm, r.bn,
-                         (int)((g.M + r.bm - 1) / r.bm), (int)((g.N + r.bn - 1) / r.bn));
+        if (gated) gemm_launch_tile<T, false, false, O, true>(r, g, s);
+        else if (!akm && !bkm) gemm_launch_tile<T, false, false, O, false>(r, g, s);
+        else if (!akm) gemm_launch_tile<T, false, true, O, false>(r, g, s);
+        else gemm_launch_tile<T, true, true, O, false>(r, g, s);
+        const int ntm = (int)((g.M + r.bm - 1) / r.bm), ntn = (int)((g.N + r.bn - 1) / r.bn);
+        if (rest > 0 && gated)
+            rwkv::launch(split_reduce_kernel<T, true>, dim3((unsigned)(rest * (r.bm * r.bn / 4096))), dim3(256), s, g, r.bm, r.bn, ntm, ntn);
+        else if (rest > 0)
+            rwkv::launch(split_reduce_kernel<T, false>, dim3((unsigned)(rest * (r.bm * r.bn / 2048))), dim3(256), s, g, r.bm, r.bn, ntm, ntn);
     };
     if (dt == RWKV_BF16 && odd) by_layout(bf16{}, std::true_type{});
     else if (dt == RWKV_BF16) by_layout(bf16{}, std::false_type{});
@@ -1323,6 +1506,42 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)N, g.K = g.KB = (int)K;
     g.e = Epilogue{bias, residual, ldr, y, y_dt == RWKV_F32, aux, rem, codes, scales, (int)act, M, (int)N};
     return gemm_run("linear_fwd", false, false, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int64_t rwkv_gated_fwd_workspace(int64_t M, int64_t F, int64_t K) { return rwkv_linear_fwd_workspace(M, 2 * F, K); }
+
+rwkv_status rwkv_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* h, void* aux, uint8_t* rem,
+                           rwkv_gate act, rwkv_dtype dt, int64_t M, int64_t F, int64_t K, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    RWKV_REQUIRE(half_ok(dt), RWKV_E_DTYPE, "gated_fwd: dtype %d", (int)dt);
+    RWKV_REQUIRE((int)act >= GATE_RELU2 && (int)act <= GATE_GELU, RWKV_E_UNSUPPORTED, "gated_fwd: activation %d", (int)act);
+    RWKV_REQUIRE(F >= 1 && F <= (1 << 19) && shape_ok(M, 2 * F, K) && ld_ok(ldx, K) && ld_ok(ldw, K), RWKV_E_SHAPE,
+                 "gated_fwd: M=%lld F=%lld K=%lld ldx=%lld ldw=%lld", (long long)M, (long long)F, (long long)K, (long long)ldx,
+                 (long long)ldw);
+    RWKV_REQUIRE(M == 0 || (x && w && h), RWKV_E_NULL, "gated_fwd: null buffer");
+    RWKV_REQUIRE(!aux == !rem, RWKV_E_NULL, "gated_fwd: aux and its remainders go together");
+    if (M == 0) return RWKV_OK;
+    GemmArgs g{};
+    g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.M = M, g.N = (int)(2 * F), g.K = g.KB = (int)K;
+    g.e = Epilogue{nullptr, nullptr, 0, h, 0, aux, rem, nullptr, nullptr, (int)act, M, (int)F, false};
+    return gemm_run("gated_fwd", false, false, dt, g, workspace, workspace_bytes, (hipStream_t)stream, true);
+}
+
+rwkv_status rwkv_gated_dact(const void* dy, int64_t lddy, const void* kept, const uint8_t* rem, rwkv_gate act, void* dz,
+                            int64_t ldz, rwkv_dtype dt, int64_t M, int64_t F, void* stream) {
+    RWKV_REQUIRE(half_ok(dt), RWKV_E_DTYPE, "gated_dact: dtype %d", (int)dt);
+    RWKV_REQUIRE((int)act >= GATE_RELU2 && (int)act <= GATE_GELU, RWKV_E_UNSUPPORTED, "gated_dact: activation %d", (int)act);
+    RWKV_REQUIRE(F >= 1 && F <= (1 << 19) && shape_ok(M, 2 * F, 1) && lddy >= F && ldz >= 2 * F && ldz < 2 * F + 8, RWKV_E_SHAPE,
+                 "gated_dact: M=%lld F=%lld lddy=%lld ldz=%lld", (long long)M, (long long)F, (long long)lddy, (long long)ldz);
+    RWKV_REQUIRE(M == 0 || (dy && kept && rem && dz), RWKV_E_NULL, "gated_dact: null buffer");
+    if (M == 0) return RWKV_OK;
+    int TX, gx, gy;
+    dact_geometry(M, F, false, TX, gx, gy);
+    const GatedArgs a{dy, lddy, kept, rem, (int)act, dz, ldz, M, (int)F};
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (dt == RWKV_BF16) rwkv::launch(gated_dact_kernel<bf16>, grid, dim3(256), (hipStream_t)stream, a, TX);
+    else rwkv::launch(gated_dact_kernel<f16>, grid, dim3(256), (hipStream_t)stream, a, TX);
+    return status_of("gated_dact launch");
 }
 
 rwkv_status rwkv_linear_pad(const void* x, int64_t ldx, void* y, int64_t N, int64_t D, void* stream) {

@@ -574,6 +574,119 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ───────────────────────────── gated products ─────────────────────────────
+
+// Keeps x, W, and both pre-activations in 24 bits.
+struct GatedNode : Node {
+    SavedVariable x, w, kept, rem;
+    std::vector<int64_t> x_shape, y_shape;
+    at::ScalarType dt;
+    int64_t M, F, K;
+    rwkv_gate act;
+
+    std::string name() const override { return "GatedLinearBackward"; }
+
+    void release_variables() override {
+        for (SavedVariable* v : {&x, &w, &kept, &rem}) v->reset_data();
+    }
+
+    variable_list apply(variable_list&& grads) override {
+        const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1);
+        no_tangent("gated_linear", {&grads[0]});
+        const auto self = shared_from_this();
+        const Tensor wt = w.unpack(self), k = kept.unpack(self), r = rem.unpack(self);
+        const auto dev = wt.device();
+        const Guard guard(dev);
+        variable_list out(2);
+        if (!need_x && !need_w) return once(std::move(out), grads[0], *this, "gated_linear");
+        const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(y_shape, wt.options());
+        const Rows dy = rows_of(dyt), wr = product_rows(wt);
+        const int64_t N = 2 * F, ldz = (N + 7) / 8 * 8;
+        const Tensor dz = empty({M, ldz}, dt, dev);
+        const Ws ws(std::max(need_x ? rwkv_linear_dgrad_workspace(M, N, K) : 0,
+                             need_w && M > 0 ? rwkv_linear_wgrad_workspace(M, N, K) : 0), dev);
+        void* const s = stream_of(wt);
+        check(rwkv_gated_dact(dy.p(), dy.ld, cptr(k), ptr<uint8_t>(r), act, ptr(dz), ldz, dt_of(dt), M, F, s));
+        if (need_x) {
+            out[0] = empty(x_shape, dt, dev);
+            check(rwkv_linear_dgrad(cptr(dz), ldz, wr.p(), wr.ld, ptr(out[0]), dt_of(dt), M, N, K, ws.p(), ws.bytes, s));
+        }
+        if (need_w && M == 0) {
+            out[1] = at::zeros({N, K}, wt.options());
+        } else if (need_w) {
+            const Rows xr = product_rows(x.unpack(self));   // (columns from K on, of a padded x, are not asked for)
+            out[1] = empty({N, K}, dt, dev);
+            check(rwkv_linear_wgrad(cptr(dz), ldz, xr.p(), xr.ld, ptr(out[1]), dt_of(dt), M, N, K, ws.p(), ws.bytes, s));
+        }
+        return once(std::move(out), grads[0], *this, "gated_linear");
+    }
+};
+
+const char* const GATES[] = {"relu2", "sigmoid", "silu", "gelu_tanh"};
+
+// gated_linear(x, weight, activation)
+PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3) raise(PyExc_TypeError, "gated_linear: three arguments");
+    const Tensor x = tensor_arg(a[0], "gated_linear: x"), w = tensor_arg(a[1], "gated_linear: weight");
+    plain_call("gated_linear", {&x, &w});
+    no_tangent("gated_linear", {&x, &w});
+    const auto dt = x.scalar_type();
+    if (dt == at::kFloat) raise(PyExc_TypeError, "gated_linear: x must be bfloat16 or float16, got float32");
+    const char* name = PyUnicode_Check(a[2]) ? PyUnicode_AsUTF8(a[2]) : nullptr;
+    int act = -1;
+    for (int i = 0; name && i < 4; ++i)
+        if (std::strcmp(name, GATES[i]) == 0) act = i;
+    if (act < 0)
+        raise(PyExc_ValueError, std::string("gated_linear: activation '") + (name ? name : "?") + "' is none of relu2, sigmoid, silu, gelu_tanh");
+    if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1) || w.numel() == 0 || w.size(0) % 2)
+        raise(PyExc_ValueError, "gated_linear: x " + shape_of(x) + " and weight " + shape_of(w) + " must be [..., K] and [2F, K]");
+    const int64_t N = w.size(0), F = N / 2, K = w.size(1);
+    if (w.scalar_type() != dt)
+        raise(PyExc_TypeError, std::string("gated_linear: weight is ") + type_of(w.scalar_type()) + ", x " + type_of(dt));
+    need_device(x, "gated_linear: x");
+    same_device(x, w, "gated_linear: weight");
+
+    const bool train = at::GradMode::is_enabled() && (wants(x) || wants(w));
+    std::shared_ptr<GatedNode> node;
+    if (train) {
+        node = std::shared_ptr<GatedNode>(new GatedNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w));
+    }
+    const auto dev = x.device();
+    const Guard guard(dev);
+    const Rows x0 = product_rows(x), w0 = product_rows(w);
+    const bool pad = x0.N > 128 && (double)x0.N * N * K >= 1073741824.0;   // as linear's
+    const Rows xr = pad ? aligned_rows(x0) : x0, wr = pad ? aligned_rows(w0) : w0;
+    const int64_t M = xr.N, KK = xr.D;
+    c10::SmallVector<int64_t, 6> ysize(x.sizes().begin(), x.sizes().end());
+    ysize.back() = F;
+    Tensor y = empty(ysize, dt, dev), kept, rem;
+    if (train) {
+        kept = empty({M, N}, dt, dev);
+        rem = empty({M, N}, at::kByte, dev);
+    }
+    const Ws ws(rwkv_gated_fwd_workspace(M, F, KK), dev);
+    check(rwkv_gated_fwd(xr.p(), xr.ld, wr.p(), wr.ld, ptr(y), ptr(kept), ptr<uint8_t>(rem), (rwkv_gate)act, dt_of(dt), M, F, KK,
+                         ws.p(), ws.bytes, stream_of(x)));
+    if (train) {
+        node->x_shape = x.sizes().vec();
+        node->y_shape.assign(ysize.begin(), ysize.end());
+        node->dt = dt;
+        node->M = M;
+        node->F = F;
+        node->K = K;
+        node->act = (rwkv_gate)act;
+        node->w = SavedVariable(wr.t, false);
+        if (wants(w)) node->x = SavedVariable(xr.t, false);
+        node->kept = SavedVariable(kept, false);
+        node->rem = SavedVariable(rem, false);
+        torch::autograd::set_history(y, node);
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // ───────────────────────────── dropout ─────────────────────────────
 
 // A probability and the two numbers that name its draw; the seed from a tensor
@@ -1032,6 +1145,7 @@ PyObject* py_set_error(PyObject*, PyObject* type) {
 PyMethodDef methods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))py_layer_norm, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))py_linear, METH_FASTCALL, nullptr},
+    {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, nullptr},
     {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
     {"block_join", (PyCFunction)(void (*)(void))py_block_join, METH_FASTCALL, nullptr},
     {"wkv_tail", (PyCFunction)(void (*)(void))py_wkv_tail, METH_FASTCALL, nullptr},

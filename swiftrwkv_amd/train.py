@@ -24,6 +24,7 @@ import torch
 from . import _lib
 
 ACTIVATIONS = ("none", "relu2", "tanh", "sigmoid")
+GATES = ("relu2", "sigmoid", "silu", "gelu_tanh")
 
 _ext = None
 
@@ -109,6 +110,21 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     misaligned) are copied into such rows first, and a backward pass keeps the
     copies."""
     return (_ext or extension()).linear(x, weight, bias, activation, residual, keep8)
+
+
+def gated_linear(x: torch.Tensor, weight: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """act(x·Wgᵀ)·(x·Wuᵀ), differentiable in both: the gated half of a
+    feed-forward in one product.
+
+    x [..., K] and weight [2F, K], Wg's rows and then Wu's, bfloat16 or float16
+    alike; the result [..., F] has their type.  activation "silu" (z·σ(z)),
+    "gelu_tanh" (the gelu's tanh form), "sigmoid" or "relu2".  Products
+    accumulate in fp32 and the result is rounded once; of a backward pass's two
+    products the gradients of both factors are rounded to x's type.  For it 6
+    bytes per value of the result are kept (both pre-activations to 16 or 18
+    significant bits).  With no gradient needed nothing is kept.  Rows that are
+    not whole 16-byte chunks are copied as linear does."""
+    return (_ext or extension()).gated_linear(x, weight, activation)
 
 
 # ───────────────────────────── around a block ─────────────────────────────

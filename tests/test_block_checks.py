@@ -204,7 +204,7 @@ def test_wkv_tail_checks(kw, err, msg):
         train.wkv_tail(**args)
 
 
-CALLS = {"dropout": lambda a: train.dropout(a, 0.1, 1),
+CALLS = {"gated_linear": lambda a: train.gated_linear(a, t(4, 64)), "dropout": lambda a: train.dropout(a, 0.1, 1),
          "block_join": lambda a: train.block_join(a, t(2, 64), t(64))[0],
          "wkv_tail": lambda a: train.wkv_tail(t(2, 64), a, t(2, 64), t(2, 64), t(64), t(2, 64), t(64), t(64))}
 
@@ -224,3 +224,57 @@ def test_forward_mode_transforms_and_tracing_are_refused(name):
     with torch._subclasses.FakeTensorMode() as m:
         with pytest.raises(NotImplementedError, match=f"{name}: .*tracing"):
             f(m.from_tensor(t(2, 64)))
+
+
+# ───────────────────────────── gated products ─────────────────────────────
+
+def test_gated_entries_refuse():
+    lib = _lib.lib()
+    fwd = lambda **k: [k.get("x", D), k.get("ldx", 8), D, k.get("ldw", 8), k.get("h", D), k.get("aux"), k.get("rem"), k.get("act", 2),  # noqa: E731
+                       k.get("dt", 1), k.get("M", 2), k.get("F", 4), k.get("K", 8), k.get("ws"), k.get("wsn", 0), None]
+    refused(DTYPE, "rwkv_gated_fwd", *fwd(dt=0))
+    refused(UNSUP, "rwkv_gated_fwd", *fwd(act=4))
+    refused(UNSUP, "rwkv_gated_fwd", *fwd(act=-1))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(K=0))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(F=0))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(F=(1 << 19) + 1))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(F=1 << 62))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(M=-1))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(ldx=7))
+    refused(SHAPE, "rwkv_gated_fwd", *fwd(ldw=1 << 22))
+    refused(NULL, "rwkv_gated_fwd", *fwd(x=None))
+    refused(NULL, "rwkv_gated_fwd", *fwd(h=None))
+    refused(NULL, "rwkv_gated_fwd", *fwd(aux=D))
+    refused(NULL, "rwkv_gated_fwd", *fwd(rem=D))
+    refused(OK, "rwkv_gated_fwd", *fwd(M=0, x=None))
+    need = lib.rwkv_gated_fwd_workspace(256, 64, 16384)
+    assert need > 0 and lib.rwkv_gated_fwd_workspace(1, 64, 64) == 0 and lib.rwkv_gated_fwd_workspace(-1, 64, 64) == 0
+    for ws in ((None, need), (D, need - 1), (D + 4, need)):
+        refused(SHAPE, "rwkv_gated_fwd", *fwd(M=256, F=64, K=16384, ldx=16384, ldw=16384, ws=ws[0], wsn=ws[1]))
+    dact = lambda **k: [k.get("dy", D), k.get("lddy", 4), k.get("kept", D), k.get("rem", D), k.get("act", 2), k.get("dz", D),  # noqa: E731
+                        k.get("ldz", 8), k.get("dt", 1), k.get("M", 2), k.get("F", 4), None]
+    refused(DTYPE, "rwkv_gated_dact", *dact(dt=0))
+    refused(UNSUP, "rwkv_gated_dact", *dact(act=7))
+    refused(SHAPE, "rwkv_gated_dact", *dact(lddy=3))
+    refused(SHAPE, "rwkv_gated_dact", *dact(ldz=7))
+    refused(SHAPE, "rwkv_gated_dact", *dact(ldz=16))
+    refused(SHAPE, "rwkv_gated_dact", *dact(F=0))
+    for n in ("dy", "kept", "rem", "dz"):
+        refused(NULL, "rwkv_gated_dact", *dact(**{n: None}))
+    refused(OK, "rwkv_gated_dact", *dact(M=0, dy=None))
+
+
+@pytest.mark.parametrize("kw,err,msg", [
+    ({}, ValueError, DEVICE), (dict(x=t(8)), ValueError, DEVICE), (dict(activation="relu2"), ValueError, DEVICE),
+    (dict(x=t(2, 8, dtype=F32), weight=t(4, 8, dtype=F32)), TypeError, "x must be bfloat16 or float16, got float32"),
+    (dict(weight=t(5, 8)), ValueError, r"weight \(5, 8\) must be \[..., K\] and \[2F, K\]"),
+    (dict(weight=t(4, 7)), ValueError, r"weight \(4, 7\) must be"), (dict(weight=t(0, 8)), ValueError, r"weight \(0, 8\) must be"),
+    (dict(weight=t(4)), ValueError, r"weight \(4,\) must be"), (dict(x=t()), ValueError, "must be"),
+    (dict(weight=t(4, 8, dtype=HF)), TypeError, "weight is float16, x bfloat16"),
+    (dict(activation="gelu"), ValueError, "'gelu' is none of"), (dict(activation=None), ValueError, "is none of"),
+    (dict(weight=None), TypeError, "weight must be a tensor")])
+def test_gated_linear_checks(kw, err, msg):
+    args = dict(x=t(2, 8), weight=t(4, 8))
+    args.update(kw)
+    with pytest.raises(err, match=msg):
+        train.gated_linear(**args)

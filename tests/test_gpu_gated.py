@@ -1,0 +1,243 @@
+"""Gated products on the GPU against plain 64-bit forms.
+
+Tolerances.  A pre-activation z is an fp32 sum of K products: 2^-24·(K + 32) of
+their magnitudes' sum.  act and its slope carry that on by the largest slope and
+curvature there is, and add FUNC·(1 + |z|) of their size for the fp32 σ (as the
+dense products' tests take it).  The backward pass has z in 16 (bf16) or 18
+(fp16) bits, to one step where the remainder's byte clamps, and rounds dz to 16
+bits: half a step of its type."""
+import sys
+
+import pytest
+import torch
+
+from swiftrwkv_amd import _lib, train
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+E24, FUNC = 2.0 ** -24, 2.0 ** -20
+TINY = {BF: 2.0 ** -133, HF: 2.0 ** -25}
+KEPT = {BF: 2.0 ** -15, HF: 2.0 ** -17}
+GATES = train.GATES
+
+
+def case(msg):
+    print(f"[case] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (scale * torch.randn(shape, generator=g, device=DEV)).to(dtype)
+
+
+def act64(name, z):
+    """act, act' and act'' (its largest magnitude) in 64 bits."""
+    s = torch.sigmoid(z)
+    if name == "relu2":
+        return z.clamp(min=0) ** 2, 2 * z.clamp(min=0), 2.0
+    if name == "sigmoid":
+        return s, s * torch.sigmoid(-z), 0.1
+    if name == "silu":
+        return z * s, s + z * s * torch.sigmoid(-z), 0.5
+    a = 2 * (2 / torch.pi) ** 0.5
+    u, du = a * (z + 0.044715 * z ** 3), a * (1 + 3 * 0.044715 * z ** 2)
+    s = torch.sigmoid(u)
+    return z * s, s + z * s * torch.sigmoid(-u) * du, 0.81
+
+
+def act_off(name, z, ez):
+    """What act(z) in fp32 may be off by for a z off by ez."""
+    v, d, c = act64(name, z)
+    return (d.abs() + c * ez) * ez + FUNC * (1 + z.abs()) * v.abs() + (E24 * v.abs())
+
+
+def slope_off(name, z, ez):
+    v, d, c = act64(name, z)
+    if name == "relu2":
+        return 2 * ez + E24 * d
+    size = {"sigmoid": d, "silu": d.abs() + v.abs(), "gelu_tanh": d.abs() + v.abs() * (1 + z * z)}[name]
+    return c * ez + 2 * FUNC * (1 + z.abs()) * size + E24 * size
+
+
+def check(what, got, ref, off):
+    u = torch.finfo(got.dtype).eps / 2
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    bound = u * (ref.abs() + off) + off + TINY[got.dtype]
+    w = ((got.double() - ref).abs() / bound).nan_to_num(nan=float("inf")).max().item() if got.numel() else 0.0
+    print(f"  {what}: worst error {w:.3f} of its bound", flush=True)
+    assert w <= 1.0, (what, w)
+
+
+def run(M, F, K, dt, act, x=None, w=None, dy=None):
+    g = gen(M + 3 * F + 7 * K)
+    x = randn(g, M, K, dtype=dt) if x is None else x
+    w = randn(g, 2 * F, K, dtype=dt, scale=1.5 * K ** -0.5) if w is None else w
+    dy = randn(g, M, F, dtype=dt) if dy is None else dy
+    a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    y = train.gated_linear(a, b, act)
+    dx, dw = torch.autograd.grad(y, (a, b), dy)
+    with torch.no_grad():
+        assert torch.equal(train.gated_linear(x, w, act), y)
+    X, W, DY = x.double(), w.double(), dy.double()
+    z, ez = X @ W.t(), E24 * (K + 32) * (X.abs() @ W.abs().t())
+    (zg, zu), (eg, eu) = z.chunk(2, 1), ez.chunk(2, 1)
+    v, d, _ = act64(act, zg)
+    ev = act_off(act, zg, eg)
+    check("y", y.detach(), v * zu, ev * (zu.abs() + eu) + v.abs() * eu + E24 * (v * zu).abs())
+    u = torch.finfo(dt).eps / 2
+    eg, eu = eg + KEPT[dt] * zg.abs() + TINY[dt], eu + KEPT[dt] * zu.abs() + TINY[dt]
+    ev, ed = act_off(act, zg, eg), slope_off(act, zg, eg)
+    dz = torch.cat([DY * zu * d, DY * v], 1)
+    off = torch.cat([DY.abs() * (ed * (zu.abs() + eu) + d.abs() * eu), DY.abs() * ev], 1)
+    off = off + (u + 4 * E24) * (dz.abs() + off) + TINY[dt]
+    check("dx", dx, dz @ W, off @ W.abs() + E24 * (2 * F + 64) * ((dz.abs() + off) @ W.abs()))
+    check("dw", dw, dz.t() @ X, off.t() @ X.abs() + E24 * (M + 64) * ((dz.abs() + off).t() @ X.abs()))
+    return y, dx, dw
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("act", GATES)
+@pytest.mark.parametrize("M,F,K", [(1, 40, 64), (20, 72, 96), (150, 200, 333)])
+def test_gates(M, F, K, act, dt):
+    case(f"gated {M} x {F} x {K} {act} {dt}")
+    run(M, F, K, dt, act)
+
+
+@pytest.mark.parametrize("M,F,K", [(1, 1, 1), (1, 5, 8), (2, 8, 7), (3, 17, 33), (16, 40, 64), (16, 4099, 2056), (9, 4096, 1031), (17, 64, 64),
+                                   (17, 100, 1000), (40, 3, 4096), (64, 512, 512), (100, 96, 4096), (129, 257, 515), (300, 1000, 600),
+                                   (1000, 1001, 1000), (1024, 1024, 1024), (2048, 2048, 512), (4096, 4096, 256), (4096, 1037, 520),
+                                   (130, 2050, 4099), (700, 3001, 2001), (256, 64, 16384), (2500, 6000, 1024)])
+def test_gated_routes(M, F, K):
+    case(f"gated {M} x {F} x {K}")
+    a = run(M, F, K, BF, "silu")
+    b = run(M, F, K, BF, "silu")
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("M,F,K", [(20, 48, 64), (140, 520, 256), (600, 640, 512), (4096, 2048, 512)])
+def test_gated_is_two_products(M, F, K):
+    """Both halves of W where they belong, whatever the tile: W's rows one at a
+    time are zero but for one column, so each z is one value of x."""
+    case(f"gated columns {M} x {F} x {K}")
+    x = torch.randint(-8, 9, (M, K), generator=gen(1), device=DEV).to(HF)
+    at = torch.randint(0, K, (2 * F,), generator=gen(2), device=DEV)
+    w = torch.zeros(2 * F, K, device=DEV, dtype=HF)
+    w[torch.arange(2 * F, device=DEV), at] = 1.0
+    y = train.gated_linear(x, w, "relu2")
+    assert torch.equal(y, (x[:, at[:F]].float().clamp(min=0) ** 2 * x[:, at[F:]].float()).to(HF))
+
+
+def test_gated_layouts():
+    case("gated: views, one row, several axes, far rows, expanded dy")
+    g = gen(5)
+    big, wide = randn(g, 30, 500, dtype=BF), randn(g, 64, 700, dtype=BF, scale=0.1)
+    for x, w in ((big[:, 3:103], wide[:, :100]), (big[::3, :96], wide[:, 100:196]), (big.t()[:96], wide[::2, :30]),
+                 (big[:, ::5], wide[:, ::7]), (big.reshape(5, 6, 500)[..., :64], wide[:50, 1:65]), (big[4, :64], wide[:, :64]),
+                 (big[:1, :64].expand(9, 64), wide.t()[:64, :].t()[:, :64]), (big[:0, :64], wide[:, :64])):
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        c, d = x.detach().contiguous().requires_grad_(True), w.detach().contiguous().requires_grad_(True)
+        ya, yc = train.gated_linear(a, b), train.gated_linear(c, d)
+        F = w.shape[0] // 2
+        assert ya.shape == (*x.shape[:-1], F) and torch.equal(ya, yc)
+        dy = randn(gen(2), *ya.shape[:-1], 2 * F, dtype=BF)
+        ga = torch.autograd.grad(ya, (a, b), dy[..., F:])
+        gc = torch.autograd.grad(yc, (c, d), dy[..., F:].contiguous())
+        assert all(torch.equal(p, q) for p, q in zip(ga, gc))
+        y1, y2 = train.gated_linear(a, b), train.gated_linear(c, d)
+        e1, = torch.autograd.grad(y1.float().sum(), a)
+        e2, = torch.autograd.grad(y2, c, torch.ones_like(y2))
+        assert torch.equal(e1, e2)
+    step = (1 << 22) + 104   # rows further apart than the products reach
+    buf = torch.zeros(20 * step + 8, device=DEV, dtype=BF)
+    x = buf.as_strided((20, 64), (step, 1), 8)
+    x.copy_(big[:20, :64])
+    assert torch.equal(train.gated_linear(x, wide[:, :64]), train.gated_linear(big[:20, :64], wide[:, :64]))
+
+
+def test_gated_values():
+    """Infinities and NaN stay in their rows and columns; where σ saturates z passes or nothing does."""
+    case("gated: extremes")
+    K, F = 8, 12
+    for act in GATES:
+        w = torch.zeros(2 * F, K, device=DEV, dtype=BF)
+        w[:, 0] = 1.0
+        z = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 30.0, -30.0, 100.0, -100.0, 1e4, -1e4, 1e18, -1e18, float("nan")], device=DEV)
+        x = torch.zeros(z.numel(), K, device=DEV, dtype=BF)
+        x[:, 0] = z.to(BF)
+        w[F:, 0] = 0.0
+        w[F:, 1] = 1.0
+        x[:, 1] = 1.0
+        a, b = x.requires_grad_(True), w.requires_grad_(True)
+        y = train.gated_linear(a, b, act)
+        dx, dw = torch.autograd.grad(y, (a, b), torch.ones_like(y))
+        zz = x.detach()[:, 0].double()
+        v, d, _ = act64(act, zz.clamp(-1e15, 1e15))
+        v = torch.where(zz.abs() > 1e15, (zz ** 2 if act == "relu2" else zz if act != "sigmoid" else 1.0) * (zz > 0), v)
+        fin = slice(0, 12)
+        assert torch.isnan(y[12]).all() and torch.isfinite(dx[fin]).all() and torch.isnan(dx[12, 0])
+        off = FUNC * 64 * v.abs()[fin, None] + 1e-37
+        check(act, y.detach()[fin], v[fin, None].expand(-1, F), off.expand(-1, F))
+        d = torch.where(zz.abs() > 1e15, (2 * zz if act == "relu2" else 1.0 if act != "sigmoid" else 0.0) * (zz > 0), d)
+        # twelve equal columns; dz is rounded
+        check(act + " dz", dx[fin, 0], 12 * d[fin], 12 * ((2.0 ** -8 + FUNC * 64) * d.abs() + 2.0 ** -13 * (d.abs() > 0))[fin])
+
+
+def test_gated_in_a_graph():
+    case("gated products with their gradients captured, replayed between eager work")
+    x, w, dy = randn(gen(1), 40, 512, dtype=BF), randn(gen(2), 256, 512, dtype=BF, scale=0.05), randn(gen(3), 40, 128, dtype=BF)
+
+    def go():
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = train.gated_linear(a, b)
+        return (y.detach(), *torch.autograd.grad(y, (a, b), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        go()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = go()
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(4):
+        x.copy_(randn(gen(90 + k), 40, 512))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, go())), k
+
+
+def test_gated_refuses_second_and_forward_derivatives():
+    case("gated: derivatives of derivatives, tangents")
+    x, w = randn(gen(1), 4, 64, dtype=BF).requires_grad_(True), randn(gen(2), 16, 64, dtype=BF)
+    y = train.gated_linear(x, w)
+    v = torch.ones_like(y).requires_grad_(True)
+    dx, = torch.autograd.grad((v * y).float().sum(), x, create_graph=True)
+    for to in (x, v):
+        with pytest.raises(RuntimeError, match="gated_linear: gradients of its gradients"):
+            torch.autograd.grad(dx.float().sum() + v.float().sum(), to, retain_graph=True)
+    fa = torch.autograd.forward_ad
+    y = train.gated_linear(x, w)
+    with fa.dual_level():
+        with pytest.raises(NotImplementedError, match="gated_linear: forward-mode"):
+            torch.autograd.grad(y, x, fa.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("F", [1, 3, 4, 8, 37, 505, 512])
+def test_padding_columns_of_gated_dz_are_zeros(F):
+    """rwkv_gated_dact writes every column from 2F to its pitch, and nothing behind the last row."""
+    case(f"gated dact {F} columns, every pitch")
+    M = 37
+    dy, kept = randn(gen(F), M, F, dtype=BF), randn(gen(F + 1), M, 2 * F, dtype=BF)
+    rem = torch.zeros(M, 2 * F, device=DEV, dtype=torch.uint8)
+    want = torch.cat([2 * kept[:, :F].clamp(min=0) * kept[:, F:].float() * dy.float(), kept[:, :F].float().clamp(min=0) ** 2 * dy], 1)
+    for ldz in range(2 * F, 2 * F + 8):
+        dz = torch.full((M + 1, ldz), float("nan"), device=DEV, dtype=BF)
+        _lib.check(_lib.lib().rwkv_gated_dact(dy.data_ptr(), F, kept.data_ptr(), rem.data_ptr(), 0, dz.data_ptr(), ldz, _lib.BF16, M, F,
+                                              torch.cuda.current_stream().cuda_stream))
+        assert not dz[:M, 2 * F:].any() and torch.isnan(dz[M]).all(), ldz
+        assert ((dz[:M, :2 * F].double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs()).all(), ldz
