@@ -1,11 +1,13 @@
 """Differentiable operators around the WKV-7 recurrence, for training on
-MI355X: layer norm, dense products with bias / activation / residual, and
-8-bit activation checkpoints that their backward passes read.
+MI355X: layer norm, dense products with bias / activation / residual, gated
+products, 8-bit activation checkpoints that their backward passes read,
+dropout, the join of a block with the next, and the recurrence's tail.
 
 The reference forms these from MLX operations and differentiates them with
 MLX's autograd (RWKVBlock.rwkvTmixForward / rwkvCmixForward,
 Sources/RWKVModel/RWKVBlock.swift:163-307); here each is hand-written kernels
-behind the C ABI.  channel_mix runs them together as one block half.
+behind the C ABI.  channel_mix, mix_tail and gated_mix run them together as
+halves of a block.
 
 Tensors live on a ROCm device; results and gradients come back in the types
 of the arguments.  Leading axes are rows, at most 2^24; a last axis that is not
@@ -209,3 +211,35 @@ def channel_mix(x: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch.Tensor,
     xk = torch.lerp(xl, torch.cat([first, xl[:, :-1]], dim=1), x_k.to(xl.dtype))
     h = linear(xk, key, activation="relu2", keep8=keep8)
     return linear(h, value, residual=x, keep8=keep8), xl[:, -1]
+
+
+def gated_mix(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, next_weight: torch.Tensor,
+              next_bias: Optional[torch.Tensor] = None, *, activation: str = "silu", post_weight: Optional[torch.Tensor] = None,
+              post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+              scale: Optional[torch.Tensor] = None, p: float = 0.0, seed: Union[int, torch.Tensor] = 0, offset: int = 0,
+              eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A gated feed-forward half of a block, differentiable: from the stream x
+    [..., D] (float32 or h's type) and its norm h (as the join before returned
+    it), o = gated_linear(h, weight, activation)·downᵀ and the block_join of x
+    and o.  weight [2F, D], down [D, F] of h's type; the rest as block_join
+    has it, next_weight and next_bias the norm of what follows.  Returns
+    (x', h')."""
+    o = linear(gated_linear(h, weight, activation), down)
+    return block_join(x, o, next_weight, next_bias, post_weight=post_weight, post_bias=post_bias, gate=gate, scale=scale, p=p,
+                      seed=seed, offset=offset, eps=eps, post_eps=eps)
+
+
+def mix_tail(x: torch.Tensor, o: torch.Tensor, r: torch.Tensor, k: torch.Tensor, v: torch.Tensor, r_k: torch.Tensor,
+             gate: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch.Tensor, output: torch.Tensor,
+             next_weight: torch.Tensor, next_bias: Optional[torch.Tensor] = None, *, scale: Optional[torch.Tensor] = None,
+             p: float = 0.0, seed: Union[int, torch.Tensor] = 0, offset: int = 0, eps: float = 1e-5,
+             head_eps: float = 64e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The end of a time-mix half, differentiable (rwkvTmixForward from the
+    recurrence's result on, RWKVBlock.swift:249-273): wkv_tail, the output
+    projection, and the block_join with the stream x.  o [..., 64 H] from
+    kernel.wkv7_train (reshaped), r, k, v, gate [..., 64 H] and output
+    [D, 64 H] of one 16-bit type, ln_weight, ln_bias the heads' norm,
+    next_weight, next_bias the norm of the half that follows.  Returns
+    (x', h)."""
+    y = linear(wkv_tail(o, r, k, v, r_k, gate, ln_weight, ln_bias, head_eps), output)
+    return block_join(x, y, next_weight, next_bias, scale=scale, p=p, seed=seed, offset=offset, eps=eps)

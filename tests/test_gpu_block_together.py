@@ -1,0 +1,152 @@
+"""The operators around a block run together, as a training step uses them."""
+import sys
+
+import pytest
+import torch
+
+from swiftrwkv_amd import kernel, train
+
+from .philox import kept
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def case(msg):
+    print(f"[case] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+def norm(v, w, b, eps):
+    m = v.mean(-1, keepdim=True)
+    return (v - m) / torch.sqrt((v - m).square().mean(-1, keepdim=True) + eps) * w + b
+
+
+def inputs(B, T, H, F, dt, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s, scale=1.0, dtype=F32: (scale * torch.randn(s, generator=g, device=DEV)).to(dtype)  # noqa: E731
+    D = 64 * H
+    t = {"x": r(B, T, D)}
+    for n in ("r", "k", "v", "gate"):
+        t[n] = r(B, T, D, scale=0.5, dtype=dt)
+    t["r_k"] = r(H, 64, scale=0.3)
+    for n in ("ln", "next", "last"):
+        t[n + "_w"], t[n + "_b"] = 1 + 0.1 * r(D), 0.1 * r(D)
+    t["output"] = r(D, D, scale=D ** -0.5, dtype=dt)
+    t["weight"] = r(2 * F, D, scale=D ** -0.5, dtype=dt)
+    t["down"] = r(D, F, scale=F ** -0.5, dtype=dt)
+    t["scale"] = 0.5 + 0.1 * r(D)
+    t["w"] = torch.exp(-0.6 * torch.rand(B, T, H, 64, generator=g, device=DEV))
+    return t, r(B, T, D), r(B, T, D, dtype=dt)
+
+
+def step(t, B, T, H, p, seed):
+    """Recurrence, tail, output projection, join; gated feed-forward, join."""
+    heads = lambda v: v.reshape(B, T, H, 64).float()  # noqa: E731
+    kk = torch.nn.functional.normalize(heads(t["k"]), dim=-1)
+    o = kernel.wkv7_train(heads(t["r"]), t["w"], heads(t["k"]), heads(t["v"]), -kk, 0.5 * kk)
+    x, h = train.mix_tail(t["x"], o.reshape(B, T, -1), t["r"], t["k"], t["v"], t["r_k"], t["gate"], t["ln_w"], t["ln_b"], t["output"],
+                          t["next_w"], t["next_b"], p=p, seed=seed, offset=1)
+    return train.gated_mix(x, h, t["weight"], t["down"], t["last_w"], t["last_b"], scale=t["scale"], p=p, seed=seed, offset=2)
+
+
+def step64(t, B, T, H, p, seed):
+    heads = lambda v: v.reshape(B, T, H, 64)  # noqa: E731
+    r, w, k, v = heads(t["r"]), heads(t["w"]), heads(t["k"]), heads(t["v"])
+    kk = torch.nn.functional.normalize(k, dim=-1)
+    S = torch.zeros(B, H, 64, 64, dtype=torch.float64, device=DEV)
+    outs = []
+    for i in range(T):
+        sa = (S * -kk[:, i, :, None, :]).sum(-1)
+        S = S * w[:, i, :, None, :] + v[:, i, :, :, None] * k[:, i, :, None, :] + sa[..., None] * (0.5 * kk[:, i, :, None, :])
+        outs.append((S * r[:, i, :, None, :]).sum(-1))
+    o = torch.stack(outs, 1)
+    bonus = (r * k * t["r_k"]).sum(-1, keepdim=True) * v
+    m = o.mean(-1, keepdim=True)
+    oh = (o - m) / torch.sqrt((o - m).square().mean(-1, keepdim=True) + 64e-5)
+    y = (oh.flatten(2) * t["ln_w"] + t["ln_b"] + bonus.flatten(2)) * t["gate"]
+    D, q = 64 * H, round(65536 * p)
+    drop = lambda a, off: a * torch.from_numpy(kept(B * T, D, p, seed, off)).to(DEV).reshape(B, T, D) * 65536 / (65536 - q)  # noqa: E731
+    x = t["x"] + drop(y @ t["output"].t(), 1)
+    h = norm(x, t["next_w"], t["next_b"], 1e-5)
+    zg, zu = (h @ t["weight"].t()).chunk(2, -1)
+    x = x + t["scale"] * drop((zg * torch.sigmoid(zg) * zu) @ t["down"].t(), 2)
+    return x, norm(x, t["last_w"], t["last_b"], 1e-5)
+
+
+@pytest.mark.parametrize("B,T,H,F,dt", [(2, 32, 2, 320, BF), (1, 16, 3, 100, HF), (3, 48, 1, 96, HF)])
+@pytest.mark.parametrize("p", [0.0, 0.25])
+def test_block(B, T, H, F, dt, p):
+    """Both halves against 64-bit autograd of their formulas: relative 2-norms,
+    24 half steps of the 16-bit type for its at most twelve rounded values in a
+    row, each met on the way there and back."""
+    case(f"block {B} x {T} x {H} heads x {F} {dt} p {p}")
+    t, dx, dh = inputs(B, T, H, F, dt, B + T + F)
+    leaves = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+    out = step(leaves, B, T, H, p, 99)
+    grads = torch.autograd.grad(out, list(leaves.values()), (dx, dh))
+    big = {n: v.detach().double().requires_grad_(True) for n, v in t.items()}
+    ref = step64(big, B, T, H, p, 99)
+    want = torch.autograd.grad(ref, list(big.values()), (dx.double(), dh.double()))
+    tol = 24 * torch.finfo(dt).eps / 2
+    rel = lambda a, b: ((a.double() - b).norm() / b.norm()).item()  # noqa: E731
+    assert out[0].dtype == F32 and out[1].dtype == dt
+    assert rel(out[0].detach(), ref[0].detach()) <= tol and rel(out[1].detach(), ref[1].detach()) <= tol
+    for n, a, b in zip(leaves, grads, want):
+        print(f"  d{n}: {rel(a, b):.2e}", flush=True)
+        assert a.shape == b.shape and rel(a, b) <= tol, n
+
+
+def test_steps_with_a_seed_each():
+    """backward() into .grad, step after step, the seed in a tensor: each step's
+    gradients are those of a call with that seed as a number; a graph captured
+    with its own leaves replays the same."""
+    case("training steps of a block, eager and captured")
+    B, T, H, F, dt = 2, 16, 2, 128, BF
+    t, dx, dh = inputs(B, T, H, F, dt, 7)
+    leaves = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+    seed = torch.zeros(1, dtype=torch.int64, device=DEV)
+
+    def grads_of(sd):
+        own = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+        return torch.autograd.grad(step(own, B, T, H, 0.3, sd), list(own.values()), (dx, dh))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads_of(seed)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured = grads_of(seed)
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(3):
+        seed.fill_(40 + k)
+        out = step(leaves, B, T, H, 0.3, seed)
+        torch.autograd.backward(out, (dx, dh))
+        want = grads_of(40 + k)
+        assert all(torch.equal(leaf.grad, w) for leaf, w in zip(leaves.values(), want)), k
+        for leaf in leaves.values():
+            leaf.grad = None
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(captured, want)), k
+
+
+def test_a_token_at_a_time():
+    """With no gradient, a row alone gives what it gives in a batch."""
+    case("gated_mix and mix_tail, one token of a batch")
+    B, T, H, F, dt = 1, 5, 4, 512, HF
+    t, _, _ = inputs(B, T, H, F, dt, 3)
+    with torch.no_grad():
+        o = t["x"] * 0.3
+        go = lambda i: train.mix_tail(t["x"][0, i], o[0, i], t["r"][0, i], t["k"][0, i], t["v"][0, i], t["r_k"], t["gate"][0, i],  # noqa: E731
+                                      t["ln_w"], t["ln_b"], t["output"], t["next_w"])
+        x, h = go(slice(None))
+        for i in range(T):
+            a, b = go(slice(i, i + 1))
+            assert torch.equal(a[0], x[i]) and torch.equal(b[0], h[i])
+        x2, h2 = train.gated_mix(x, h, t["weight"], t["down"], t["last_w"])
+        for i in range(T):
+            a, b = train.gated_mix(x[i], h[i], t["weight"], t["down"], t["last_w"])
+            assert torch.equal(a, x2[i]) and torch.equal(b, h2[i])
