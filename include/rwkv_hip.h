@@ -527,8 +527,8 @@ typedef struct {
     int64_t N, D;
 } rwkv_join;
 
-/* xs = x' [N, D] of x_dt, h [N, D] of dt; stats [N, 4] fp32 (mean and rstd of o
- * and of x'; 16-byte aligned) where not NULL.  xs may be x where ldx = D; no
+/* xs = x' [N, D] of x_dt, h [N, D] of dt; stats [N, 4] fp32 (mean and rstd of
+ * o, 0 and 1 without its norm, and of x'; 16-byte aligned) where not NULL.  xs may be x where ldx = D; no
  * other output may alias an input. */
 rwkv_status rwkv_join_fwd(const rwkv_join* args, void* xs, void* h, float* stats, void* stream);
 

@@ -139,15 +139,28 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
 
 // ───────────────────────────── join ─────────────────────────────
 
-// Sums of two values over the TPR threads of a row, as row_sum of the layer
-// norm takes one: one wave, or the block through LDS, the waves in order.
-// Every thread has read a slot before the barrier of the next sum, so two
-// slots in turn are enough.
+// Sum over the TPR lanes of a row: sixteen, or a wave.
+template <int TPR>
+__device__ __forceinline__ float lanes_sum(float x) {
+    if constexpr (TPR != 16) return rwkv_wkv::wave_total(x);
+    auto turned = [](float v, auto ctrl) {
+        return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    x = turned(x, std::integral_constant<int, 0x128>{});   // row_ror:8, 4, 2, 1
+    x = turned(x, std::integral_constant<int, 0x124>{});
+    x = turned(x, std::integral_constant<int, 0x122>{});
+    return turned(x, std::integral_constant<int, 0x121>{});
+}
+
+// Sums over the TPR threads of a row, of one value or two, as the layer norm
+// takes one: its lanes, or the block through LDS, the waves in order.  Every
+// thread has read a slot before the barrier of the next sum, so two slots in
+// turn are enough.
 template <int TPR>
 __device__ __forceinline__ float2 row_sum2(float s, float q, float2 (*part)[16], int slot) {
-    s = rwkv_wkv::wave_total(s);
-    q = rwkv_wkv::wave_total(q);
-    if constexpr (TPR == 64) {
+    s = lanes_sum<TPR>(s);
+    q = lanes_sum<TPR>(q);
+    if constexpr (TPR <= 64) {
         return make_float2(s, q);
     } else {
         if ((threadIdx.x & 63) == 0) part[slot][threadIdx.x >> 6] = make_float2(s, q);
@@ -160,8 +173,8 @@ __device__ __forceinline__ float2 row_sum2(float s, float q, float2 (*part)[16],
 }
 template <int TPR>
 __device__ __forceinline__ float row_sum(float s, float2 (*part)[16], int slot) {
-    s = rwkv_wkv::wave_total(s);
-    if constexpr (TPR == 64) {
+    s = lanes_sum<TPR>(s);
+    if constexpr (TPR <= 64) {
         return s;
     } else {
         if ((threadIdx.x & 63) == 0) part[slot][threadIdx.x >> 6].x = s;
@@ -181,66 +194,154 @@ __device__ __forceinline__ void load_w(const void* w, int w32, int col, int vali
         load8(reinterpret_cast<const T*>(w) + col, valid, v);
 }
 
+// How a row of D columns falls into chunks of eight: WHOLE, D is a multiple of 8;
+// ENDS, it is not; FEW, D is under 8.
+enum { WHOLE, ENDS, FEW };
+
+// A thread's eight columns of a row.  Threads whose chunk passes the row's end,
+// or lies behind it, load the row's last eight columns, unconditionally (FEW:
+// one by one), and move them into place where they are used; WHOLE has none of
+// the former, and what the latter make of their load goes nowhere.  (Loads that
+// look at every value, in the same kernel, cost half of its time in branches
+// and moves.)
+template <int ROWS>
+struct Cols {
+    int col, valid;   // first column, and columns from there to the row's end
+    int at;           // where the thread loads
+    __device__ __forceinline__ Cols(int t, int D) : col(8 * t), valid(D - 8 * t), at(ROWS == FEW ? 8 * t : min(8 * t, D - 8)) {}
+    // A row's value at: a row's address is the same for all and stays in scalar
+    // registers, under a 32-bit offset of the thread's.
+    template <typename T>
+    static __device__ __forceinline__ T* place(T* row, int at) {
+        using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+        uint32_t off = (uint32_t)(at * (int)sizeof(T));
+        asm volatile("" : "+v"(off));   // (else the compiler keeps 64-bit addresses of every tensor over the loop)
+        return reinterpret_cast<T*>(reinterpret_cast<Byte*>(row) + off);
+    }
+    // value i is one of the row's; of a sum, whether the thread has any
+    __device__ __forceinline__ bool has(int i) const { return ROWS == WHOLE || i < valid; }
+    __device__ __forceinline__ float own(float s) const { return ROWS != WHOLE || valid > 0 ? s : 0.0f; }
+    template <typename T>
+    __device__ __forceinline__ void load(Raw8<T>& r, const void* p, int64_t row, int64_t ld) const {
+        const T* q = place(reinterpret_cast<const T*>(p) + row * ld, at);
+        if constexpr (ROWS == FEW) r.load(q, valid);
+        else __builtin_memcpy(r.q, q, sizeof(r.q));
+    }
+    // The values loaded, zeros past the row's end (WHOLE: any).
+    template <typename T>
+    __device__ __forceinline__ void get(Raw8<T> r, float (&v)[8]) const {
+        if constexpr (ROWS != ENDS) return r.get(v);
+        r.get(v);
+        if (col != at) {
+            const int moved = col - at;
+#pragma unroll
+            for (int k = 4; k >= 1; k /= 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (moved & k) v[i] = i + k < 8 ? v[i + k < 8 ? i + k : 7] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < valid ? v[i] : 0.0f;
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(void* p, int64_t row, int D, const float (&v)[8]) const {
+        if (valid > 0) store8(place(reinterpret_cast<T*>(p) + row * D, col), ROWS == WHOLE ? 8 : valid, v);
+    }
+    // The vector w's values of the columns, or `otherwise` without one.
+    template <typename T>
+    __device__ __forceinline__ void vector(const void* w, int w32, float otherwise, float (&v)[8]) const {
+        const int from = ROWS == WHOLE ? at : col, n = ROWS == WHOLE ? 8 : valid;
+        if (w && w32) load8(place(reinterpret_cast<const float*>(w), from), n, v);
+        else if (w) load8(place(reinterpret_cast<const T*>(w), from), n, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = otherwise;
+    }
+};
+
 struct JoinFwd {
     const void *x, *o, *gate;   // gate, post_w, post_b, scale, b may be null
     int64_t ldx, ldo, ldg;
     const void *post_w, *post_b, *scale, *w, *b;
     int w32;                    // the vectors are fp32 (else o's type)
     void *xs, *h;               // [N, D]
-    float* stats;               // [N, 4]: mean and rstd of o, of x'; or null
+    float* stats;               // [N, 4]: mean and rstd of o (0, 1 without its norm), of x'; or null
     int64_t N;
     int D;
     float post_eps, eps;
     Drop drop;
 };
 
-// Rows blockIdx.x·RPB + threadIdx.x / TPR, + gridDim.x·RPB, ...; a thread holds
-// one chunk of 8 columns of a row and the vectors' values for it.
-template <typename TS, typename T, int TPR>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fwd_kernel(JoinFwd a) {
-    constexpr int RPB = TPR == 64 ? 4 : 1;
-    __shared__ float2 part[2][16];
-    const int t = threadIdx.x % TPR, col = 8 * t, valid = a.D - col;
-    const int64_t step = (int64_t)gridDim.x * RPB;
-    int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-    if (row >= a.N) return;   // whole waves; rows that share a barrier end together
-    const float n = (float)a.D;
-    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
-    float pw[8], pb[8], sc[8], w[8], b[8];
-    if (a.post_w) load_w<T>(a.post_w, a.w32, col, valid, pw);
-    if (a.post_b) load_w<T>(a.post_b, a.w32, col, valid, pb);
-    if (a.scale) load_w<T>(a.scale, a.w32, col, valid, sc);
-    load_w<T>(a.w, a.w32, col, valid, w);
-    if (a.b) load_w<T>(a.b, a.w32, col, valid, b);
-    else
+// A block's threads, its rows at a time, and the row that TPR of its threads
+// begin with.
+constexpr int threads_of(int tpr) { return tpr < 256 ? (tpr == 128 ? 128 : 256) : tpr; }
+constexpr int rows_of(int tpr) { return threads_of(tpr) / tpr; }
+template <int TPR>
+__device__ __forceinline__ int64_t first_row() {
+    if constexpr (TPR == 16) return (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    else if constexpr (TPR == 64) return (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    else return blockIdx.x;
+}
+
+// A chunk of eight equal values: what stands for a part that is not there, so
+// that no value of a row has two ways to come about.
+template <typename T>
+__device__ __forceinline__ Raw8<T> filled(float x) {
+    T t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+    for (int i = 0; i < 8; ++i) t[i] = (T)x;
+    Raw8<T> r;
+    __builtin_memcpy(r.q, t, sizeof(r.q));
+    return r;
+}
+
+// Rows first_row(), + gridDim.x·RPB, ...; a thread holds one chunk of 8 columns
+// of a row, and the next row's is on its way.
+template <typename TS, typename T, int TPR, int ROWS>
+__global__ __launch_bounds__(threads_of(TPR)) void join_fwd_kernel(JoinFwd a) {
+    __shared__ float2 part[2][16];
+    const int t = threadIdx.x % TPR;
+    const Cols<ROWS> c(t, a.D);
+    const int64_t step = (int64_t)gridDim.x * rows_of(TPR);
+    int64_t row = first_row<TPR>();
+    if (row >= a.N) return;   // rows that share a barrier end together
+    const float per = 1.0f / (float)a.D;
+    const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
+    Raw8<TS> rx;
+    Raw8<T> ro, rg = filled<T>(1.0f);
+    auto load = [&](int64_t r) {
+        c.load(ro, a.o, r, a.ldo);
+        c.load(rx, a.x, r, a.ldx);
+        if (a.gate) c.load(rg, a.gate, r, a.ldg);
+    };
+    load(row);
+    float pw[8], pb[8], sc[8], w[8], b[8];
+    c.template vector<T>(a.post_w, a.w32, 1.0f, pw);
+    c.template vector<T>(a.post_b, a.w32, 0.0f, pb);
+    c.template vector<T>(a.scale, a.w32, 1.0f, sc);
+    c.template vector<T>(a.w, a.w32, 1.0f, w);
+    c.template vector<T>(a.b, a.w32, 0.0f, b);
     for (; row < a.N; row += step) {
         float v[8], u[8], g[8];
-        load8(reinterpret_cast<const T*>(a.o) + row * a.ldo + col, valid, u);
-        load8(reinterpret_cast<const TS*>(a.x) + row * a.ldx + col, valid, v);
-        if (a.gate) load8(reinterpret_cast<const T*>(a.gate) + row * a.ldg + col, valid, g);
-        float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        c.get(ro, u);
+        c.get(rx, v);
+        c.get(rg, g);
+        load(min(row + step, a.N - 1));   // (the last row again rather than a choice)
+        float4 st = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
         if (a.post_w) {
             float s = 0.0f, q = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) s += u[i];
-            st.x = row_sum<TPR>(s, part, 0) / n;
+            st.x = row_sum<TPR>(c.own(s), part, 0) * per;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float d = u[i] - st.x;
-                q += col + i < a.D ? d * d : 0.0f;
+                u[i] -= st.x;
+                q += c.has(i) ? u[i] * u[i] : 0.0f;
             }
-            st.y = 1.0f / sqrtf(row_sum<TPR>(q, part, 1) / n + a.post_eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = (u[i] - st.x) * st.y * pw[i];
-            if (a.post_b)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] += pb[i];
+            st.y = __builtin_amdgcn_rsqf(row_sum<TPR>(c.own(q), part, 1) * per + a.post_eps);
         }
-        if (a.gate)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] *= g[i];
+        for (int i = 0; i < 8; ++i) u[i] = (u[i] * st.y * pw[i] + pb[i]) * g[i];
         if (a.drop.threshold) {
             factors(a.drop, key, (uint32_t)t, (uint32_t)row, g);
 #pragma unroll
@@ -249,26 +350,25 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fwd_kernel(JoinFwd
         float s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[i] = col + i < a.D ? v[i] + (a.scale ? sc[i] * u[i] : u[i]) : 0.0f;
+            v[i] = c.has(i) ? v[i] + sc[i] * u[i] : 0.0f;
             s += v[i];
         }
-        if (valid > 0) store8(reinterpret_cast<TS*>(a.xs) + row * a.D + col, valid, v);
-        st.z = row_sum<TPR>(s, part, 0) / n;
+        c.template store<TS>(a.xs, row, a.D, v);
+        st.z = row_sum<TPR>(c.own(s), part, 0) * per;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float d = v[i] - st.z;
-            q += col + i < a.D ? d * d : 0.0f;
+            v[i] -= st.z;
+            q += c.has(i) ? v[i] * v[i] : 0.0f;
         }
-        st.w = 1.0f / sqrtf(row_sum<TPR>(q, part, 1) / n + a.eps);
+        st.w = __builtin_amdgcn_rsqf(row_sum<TPR>(c.own(q), part, 1) * per + a.eps);
         if (a.stats && t == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = st;
-        if (valid <= 0) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (v[i] - st.z) * st.w * w[i] + b[i];
-        store8(reinterpret_cast<T*>(a.h) + row * a.D + col, valid, v);
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * st.w * w[i] + b[i];
+        c.template store<T>(a.h, row, a.D, v);
     }
 }
 
-enum { DW, DB, DPW, DPB, DSC, SUMS };   // column sums of the join
+enum { DW, DB, DPW, DPB, DSC, SUMS };   // column sums of the join, the scale's last
 
 struct JoinBwd {
     const void *xs, *o, *gate;  // o null: it does not reach a gradient
@@ -286,121 +386,208 @@ struct JoinBwd {
     Drop drop;
 };
 
+// N times eight values of a thread in LDS slots that it alone writes and reads.
+template <int N, int THREADS>
+struct Slots {
+    float4 (&v)[2 * N][THREADS];
+    __device__ __forceinline__ void put(int k, const float (&x)[8]) const {
+        v[2 * k][threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
+        v[2 * k + 1][threadIdx.x] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+    __device__ __forceinline__ void get(int k, float (&x)[8]) const {
+        const float4 a = v[2 * k][threadIdx.x], b = v[2 * k + 1][threadIdx.x];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+};
+
 // With xh = (x' − μ)·r and G the whole gradient of x':
 //   G = dx' + LN'(dh·w; xh, r), dw = Σ dh·xh, db = Σ dh
 //   du = G·s·m, ds = Σ G·m·u, dg = du·n, dn = du·g
 //   do = LN'(dn·w1; oh, r1), dw1 = Σ dn·oh, db1 = Σ dn
 // LN'(y; h, r) = r·(y − mean y − h·mean(y·h)).
-template <typename TS, typename T, int TPR>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bwd_kernel(JoinBwd a) {
-    constexpr int RPB = TPR == 64 ? 4 : 1;
+//
+// A chunk is loaded as soon as the one before it has been taken apart, so the
+// next row is on its way under this one's two sums over the row.  The vectors
+// lie in LDS; with 1024 threads, which have 128 registers each, the column sums
+// do instead, and the vectors and rows are read where they are used.
+template <typename TS, typename T, int TPR, int ROWS>
+__global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
+    constexpr int RPB = rows_of(TPR);
     __shared__ float2 part[2][16];
-    __shared__ float sums[RPB > 1 ? 4 * 8 * 64 : 1];
-    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, col = 8 * t, valid = a.D - col;
+    __shared__ float sums[RPB > 1 ? 8 * 256 : 1];
+    __shared__ float4 slots[8][threads_of(TPR)];
+    constexpr bool AHEAD = TPR < 1024;
+    enum { PW, PB, SC, W };
+    const Slots<4, threads_of(TPR)> lds{slots};
+    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    const Cols<ROWS> at(t, a.D);
     const int64_t step = (int64_t)gridDim.x * RPB;
-    const float n = (float)a.D;
+    const float per = 1.0f / (float)a.D;
     const uint64_t key = a.drop.threshold ? a.drop.key() : 0;
-    float pw[8], pb[8], sc[8], w[8];
-    auto vectors = [&] {
-        if (a.post_w) load_w<T>(a.post_w, a.w32, col, valid, pw);
-        if (a.post_b) load_w<T>(a.post_b, a.w32, col, valid, pb);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pb[i] = 0.0f;
-        if (a.scale) load_w<T>(a.scale, a.w32, col, valid, sc);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sc[i] = 1.0f;
-        load_w<T>(a.w, a.w32, col, valid, w);
+    Raw8<TS> rdx = filled<TS>(0.0f), rx;
+    Raw8<T> rdh, ro = filled<T>(0.0f), rg = filled<T>(1.0f);
+    auto load_h = [&](int64_t r) {
+        if (!a.dh) return;
+        at.load(rdh, a.dh, r, a.D);
+        at.load(rx, a.xs, r, a.D);
     };
-    if constexpr (TPR < 1024) vectors();   // 1024 threads have 128 registers each: read row by row
+    auto load_o = [&](int64_t r) {
+        if (a.dxs) at.load(rdx, a.dxs, r, a.D);
+        if (a.o) at.load(ro, a.o, r, a.ldo);
+        if (a.gate) at.load(rg, a.gate, r, a.ldg);
+    };
+    int64_t row = first_row<TPR>();
+    float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (AHEAD && row < a.N) {
+        next = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+        load_h(row);
+        load_o(row);
+    }
+    const void* const vectors[4] = {a.post_w, a.post_b, a.scale, a.w};
+    auto vector = [&](int k, float (&x)[8]) {   // or, of a missing one, what changes nothing
+        if constexpr (AHEAD) lds.get(k, x);
+        else at.template vector<T>(vectors[k], a.w32, k == PB ? 0.0f : 1.0f, x);
+    };
     float acc[SUMS][8] = {};
+    auto add = [&](int k, const float (&x)[8]) {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[k][i] += x[i];
+        } else {
+            float s[8];
+            lds.get(k, s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += x[i];
+            lds.put(k, s);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float x[8] = {};
+        if constexpr (AHEAD) at.template vector<T>(vectors[k], a.w32, k == PB ? 0.0f : 1.0f, x);
+        lds.put(k, x);
+    }
     int slot = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPB + grp; row < a.N; row += step) {
-        float G[8], y[8], xh[8], u[8], g[8];
-        const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
-        if constexpr (TPR == 1024) vectors();
-        if (a.dxs) load8(reinterpret_cast<const TS*>(a.dxs) + row * a.D + col, valid, G);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) G[i] = 0.0f;
-        if (a.o) load8(reinterpret_cast<const T*>(a.o) + row * a.ldo + col, valid, u);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = 0.0f;
-        if (a.gate) load8(reinterpret_cast<const T*>(a.gate) + row * a.ldg + col, valid, g);
+    for (; row < a.N; row += step) {
+        const int64_t then = min(row + step, a.N - 1);   // (the last row again rather than a choice)
+        const float4 st = AHEAD ? next : *reinterpret_cast<const float4*>(a.stats + 4 * row);
+        if constexpr (!AHEAD) load_h(row);
+        float G[8], y[8], c[8], oh[8];
+        if constexpr (AHEAD) next = *reinterpret_cast<const float4*>(a.stats + 4 * then);
         if (a.dh) {
-            load8(reinterpret_cast<const T*>(a.dh) + row * a.D + col, valid, y);
-            load8(reinterpret_cast<const TS*>(a.xs) + row * a.D + col, valid, xh);
+            float xh[8];
+            at.get(rdh, y);
+            at.get(rx, xh);
+            if constexpr (AHEAD) load_h(then);
+            add(DB, y);
             float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                xh[i] = i < valid ? (xh[i] - st.z) * st.w : 0.0f;
-                acc[DW][i] += y[i] * xh[i];
-                acc[DB][i] += y[i];
-                y[i] *= w[i];
+                xh[i] = at.has(i) ? (xh[i] - st.z) * st.w : 0.0f;
+                c[i] = y[i] * xh[i];
+            }
+            add(DW, c);
+            vector(W, c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] *= c[i];
                 s1 += y[i];
                 s2 += y[i] * xh[i];
             }
-            const float2 s = row_sum2<TPR>(s1, s2, part, slot);
+            const float2 s = row_sum2<TPR>(at.own(s1), at.own(s2), part, slot);
             slot ^= 1;
-            s1 = s.x / n, s2 = s.y / n;
+            s1 = s.x * per, s2 = s.y * per;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) G[i] += (y[i] - s1 - xh[i] * s2) * st.w;
+            for (int i = 0; i < 8; ++i) y[i] = (y[i] - s1 - xh[i] * s2) * st.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = 0.0f;
         }
-        if (a.dx && valid > 0) store8(reinterpret_cast<TS*>(a.dx) + row * a.D + col, valid, G);
-        float m[8], oh[8];
-        if (a.drop.threshold) factors(a.drop, key, (uint32_t)t, (uint32_t)row, m);
-        else
+        if constexpr (!AHEAD) {
+            __builtin_amdgcn_sched_barrier(0);   // (not ahead: registers)
+            load_o(row);
+        }
+        at.get(rdx, G);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m[i] = 1.0f;
-        float p1 = 0.0f, p2 = 0.0f;
-        // u: n, then dn·w1; y: dg
+        for (int i = 0; i < 8; ++i) G[i] += y[i];
+        if (a.dx) at.template store<TS>(a.dx, row, a.D, G);
+        float nv[8];   // y: the gate
+        at.get(ro, oh);
+        at.get(rg, y);
+        if constexpr (AHEAD) load_o(then);
+        {
+            float b[8];
+            vector(PW, c);
+            vector(PB, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                oh[i] = at.has(i) ? (oh[i] - st.x) * st.y : 0.0f;
+                nv[i] = oh[i] * c[i] + b[i];
+            }
+        }
+        float u[8], sc[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            oh[i] = a.post_w ? (i < valid ? (u[i] - st.x) * st.y : 0.0f) : u[i];
-            const float nv = a.post_w ? oh[i] * pw[i] + pb[i] : u[i], gv = a.gate ? g[i] : 1.0f;
-            const float gm = dropped(m[i], i < valid ? G[i] : 0.0f);   // past the row's end G is not zero
-            acc[DSC][i] += m[i] > 0.0f ? gm * (gv * nv) : 0.0f;
-            const float du = gm * sc[i];
-            y[i] = du * nv;
-            const float dn = du * gv;
-            acc[DPW][i] += dn * oh[i];
-            acc[DPB][i] += dn;
-            u[i] = a.post_w ? dn * pw[i] : dn;
-            p1 += u[i];
-            p2 += u[i] * oh[i];
+            u[i] = y[i] * nv[i];
+            G[i] = at.has(i) ? G[i] : 0.0f;   // (not zero of itself past the row's end)
         }
-        if (a.dgate && valid > 0) store8(reinterpret_cast<T*>(a.dgate) + row * a.D + col, valid, y);
+        if (a.drop.threshold) {
+            float m[8];
+            factors(a.drop, key, (uint32_t)t, (uint32_t)row, m);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                u[i] = dropped(m[i], u[i]);   // m of G, for the sum
+                nv[i] = dropped(m[i], nv[i]);
+                y[i] = dropped(m[i], y[i]);
+            }
+        }
+        vector(SC, sc);
+        float p1 = 0.0f, p2 = 0.0f;
+        // u: dn·oh; y: dn; nv: dg; G: dn·w1
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            acc[DSC][i] += G[i] * u[i];
+            G[i] *= sc[i];
+            nv[i] *= G[i];
+            y[i] *= G[i];
+            u[i] = y[i] * oh[i];
+            G[i] = y[i] * c[i];
+            p1 += G[i];
+            p2 += G[i] * oh[i];
+        }
+        add(DPB, y);
+        add(DPW, u);
+        if (a.dgate) at.template store<T>(a.dgate, row, a.D, nv);
         if (!a.dout) continue;
         if (a.post_w) {
-            const float2 p = row_sum2<TPR>(p1, p2, part, slot);
+            const float2 p = row_sum2<TPR>(at.own(p1), at.own(p2), part, slot);
             slot ^= 1;
-            p1 = p.x / n, p2 = p.y / n;
+            p1 = p.x * per, p2 = p.y * per;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = (u[i] - p1 - oh[i] * p2) * st.y;
+            for (int i = 0; i < 8; ++i) G[i] = (G[i] - p1 - oh[i] * p2) * st.y;
         }
-        if (valid > 0) store8(reinterpret_cast<T*>(a.dout) + row * a.D + col, valid, u);
+        at.template store<T>(a.dout, row, a.D, G);
     }
     if (!a.part) return;
 #pragma unroll
     for (int k = 0; k < SUMS; ++k) {
         if (a.slot[k] < 0) continue;   // the same for all
+        if constexpr (!AHEAD)
+            if (k != DSC) lds.get(k, acc[k]);
         if constexpr (RPB > 1) {
             // the block's row groups meet in order
             __syncthreads();
             if (grp > 0)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sums[(grp * 8 + i) * 64 + t] = acc[k][i];
+                for (int i = 0; i < 8; ++i) sums[(grp * 8 + i) * TPR + t] = acc[k][i];
             __syncthreads();
             if (grp == 0)
-#pragma unroll
                 for (int r = 1; r < RPB; ++r)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[k][i] += sums[(r * 8 + i) * 64 + t];
+                    for (int i = 0; i < 8; ++i) acc[k][i] += sums[(r * 8 + i) * TPR + t];
         }
-        if (grp == 0 && valid > 0)
-            store8(a.part + ((int64_t)blockIdx.x * a.sums + a.slot[k]) * a.D + col, valid, acc[k]);
+        if (grp == 0) at.template store<float>(a.part, (int64_t)blockIdx.x * a.sums + a.slot[k], a.D, acc[k]);
     }
 }
 
@@ -409,29 +596,29 @@ struct Outs {
 };
 
 // Column sums of part [G][sums][D] (G may be 0) into out.p[0 .. sums): a block
-// owns 16 columns of one sum and splits the G rows over 16 thread rows, each in
-// order; the 16 partial sums meet in LDS, in order.
+// owns 32 columns (a cache line) of one sum and splits the G rows over 32 thread
+// rows, each in order, whose loads are all on their way at once up to 512; the 32
+// partial sums meet in LDS, by halves.
 template <typename T>
-__global__ __launch_bounds__(256) void join_reduce_kernel(const float* part, int G, int sums, int D, Outs out) {
-    __shared__ float s[16][17];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-    const int col = blockIdx.x * 16 + c, k = blockIdx.y;
+__global__ __launch_bounds__(1024) void join_reduce_kernel(const float* part, int G, int sums, int D, Outs out) {
+    __shared__ float s[32][33];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5, k = blockIdx.y;
+    const int col = min((int)blockIdx.x * 32 + c, D - 1);
     float t = 0.0f;
-    if (col < D) {
-#pragma unroll 8
-        for (int g = r; g < G; g += 16) t += part[((int64_t)g * sums + k) * D + col];
-    }
+#pragma unroll 16
+    for (int g = r; g < G; g += 32) t += part[((int64_t)g * sums + k) * D + col];
     s[r][c] = t;
     __syncthreads();
-    if (r != 0 || col >= D) return;
-    float sum = 0.0f;
+    t = s[c][r];   // row c's sum of column r
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += s[i][c];
+    for (int h = 16; h >= 1; h /= 2) t += __shfl_xor(t, h);
+    const int at = blockIdx.x * 32 + r;
+    if (c != 0 || at >= D) return;
     T* o = reinterpret_cast<T*>(out.p[0]);
 #pragma unroll
     for (int i = 1; i < SUMS; ++i)
         if (k == i) o = reinterpret_cast<T*>(out.p[i]);
-    o[col] = (T)sum;
+    o[at] = (T)t;
 }
 
 // ───────────────────────────── tail ─────────────────────────────
@@ -624,24 +811,37 @@ void by_types(int wide, int dt, F f) {
     }
 }
 
+// Threads of a row, and how it falls into chunks.
 template <typename F>
 void by_width(int64_t D, F f) {
-    if (D <= 512) f(std::integral_constant<int, 64>{});
-    else if (D <= 1024) f(std::integral_constant<int, 128>{});
-    else if (D <= 2048) f(std::integral_constant<int, 256>{});
-    else if (D <= 4096) f(std::integral_constant<int, 512>{});
-    else f(std::integral_constant<int, 1024>{});
+    auto by_ends = [&](auto tpr) {
+        if (D % 8 == 0) f(tpr, std::integral_constant<int, WHOLE>{});
+        else f(tpr, std::integral_constant<int, ENDS>{});
+    };
+    if (D < 8) f(std::integral_constant<int, 16>{}, std::integral_constant<int, FEW>{});
+    else if (D <= 128) by_ends(std::integral_constant<int, 16>{});
+    else if (D <= 512) by_ends(std::integral_constant<int, 64>{});
+    else if (D <= 1024) by_ends(std::integral_constant<int, 128>{});
+    else if (D <= 2048) by_ends(std::integral_constant<int, 256>{});
+    else if (D <= 4096) by_ends(std::integral_constant<int, 512>{});
+    else by_ends(std::integral_constant<int, 1024>{});
 }
 
-// Blocks of the join's passes: rows beyond a full chip's are walked.
+// Blocks of the join's passes: what the registers of 256 CUs hold at once (rows
+// beyond are walked).
+int64_t join_rows_at_once(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 4 : 1; }
 int join_fwd_blocks(int64_t N, int64_t D) {
-    const int full = D <= 512 ? 2048 : D <= 1024 ? 4096 : D <= 2048 ? 2048 : D <= 4096 ? 1024 : 512;
-    return (int)std::min<int64_t>(D <= 512 ? (N + 3) / 4 : N, full);
+    const int full = D <= 512 ? 1024 : D <= 1024 ? 2048 : D <= 2048 ? 1024 : D <= 4096 ? 512 : 256;
+    const int64_t rpb = join_rows_at_once(D);
+    return (int)std::min<int64_t>((N + rpb - 1) / rpb, full);
 }
-// Each block writes one partial row per column sum.
+// Each block writes one partial row per column sum: from 256 blocks on no more
+// than one for sixteen of its rows (4096 x 2048, all sums: 51 us by 256 blocks, 59
+// by 512; 16384 x 2048: 166 and 159, by 768 172).
 int join_bwd_blocks(int64_t N, int64_t D) {
-    const int full = D <= 512 ? 768 : D <= 1024 ? 1536 : D <= 2048 ? 768 : D <= 4096 ? 512 : 256;
-    return (int)std::min<int64_t>(D <= 512 ? (N + 3) / 4 : N, full);
+    const int64_t full = D <= 512 ? 512 : D <= 1024 ? 1024 : D <= 2048 ? 512 : 256;
+    const int64_t blocks = (N + join_rows_at_once(D) - 1) / join_rows_at_once(D);
+    return (int)std::min({blocks, full, std::max<int64_t>(256, blocks / 16)});
 }
 
 // Lanes across and the grid of the tail's passes.
@@ -705,9 +905,9 @@ rwkv_status rwkv_join_fwd(const rwkv_join* j, void* xs, void* h, float* stats, v
                     j->w_dt == RWKV_F32, xs, h, stats, j->N, (int)j->D, j->post_eps, j->eps, drop_of(j->drop)};
     const dim3 grid((unsigned)join_fwd_blocks(j->N, j->D));
     by_types(j->x_dt, j->dt, [&](auto ts, auto t) {
-        by_width(j->D, [&](auto tpr) {
+        by_width(j->D, [&](auto tpr, auto ends) {
             constexpr int TPR = decltype(tpr)::value;
-            rwkv::launch(join_fwd_kernel<decltype(ts), decltype(t), TPR>, grid, dim3(TPR == 64 ? 256 : TPR),
+            rwkv::launch(join_fwd_kernel<decltype(ts), decltype(t), TPR, decltype(ends)::value>, grid, dim3(threads_of(TPR)),
                          (hipStream_t)stream, a);
         });
     });
@@ -751,16 +951,16 @@ rwkv_status rwkv_join_bwd(const rwkv_join* j, const void* xs, const float* stats
     const hipStream_t s = (hipStream_t)stream;
     if (j->N > 0 && (a.sums || dx || dout || dgate)) {
         by_types(j->x_dt, j->dt, [&](auto ts, auto t) {
-            by_width(j->D, [&](auto tpr) {
+            by_width(j->D, [&](auto tpr, auto ends) {
                 constexpr int TPR = decltype(tpr)::value;
-                rwkv::launch(join_bwd_kernel<decltype(ts), decltype(t), TPR>, dim3((unsigned)G), dim3(TPR == 64 ? 256 : TPR), s, a);
+                rwkv::launch(join_bwd_kernel<decltype(ts), decltype(t), TPR, decltype(ends)::value>, dim3((unsigned)G), dim3(threads_of(TPR)), s, a);
             });
         });
     }
     if (a.sums) {
-        const dim3 grid((unsigned)((j->D + 15) / 16), (unsigned)a.sums);
+        const dim3 grid((unsigned)((j->D + 31) / 32), (unsigned)a.sums);
         by_types(j->w_dt, j->w_dt, [&](auto, auto t) {
-            rwkv::launch(join_reduce_kernel<decltype(t)>, grid, dim3(256), s, (const float*)workspace, G, a.sums, (int)j->D, outs);
+            rwkv::launch(join_reduce_kernel<decltype(t)>, grid, dim3(1024), s, (const float*)workspace, G, a.sums, (int)j->D, outs);
         });
     }
     return status_of("join_bwd launch");
@@ -830,9 +1030,9 @@ rwkv_status rwkv_tail_bwd(const rwkv_tail* j, const void* dy, int64_t lddy, void
         });
     if (sums) {
         const Outs outs{{dr_k, dweight, dbias, nullptr, nullptr}};
-        const dim3 grid((unsigned)((a.C + 15) / 16), 3);
+        const dim3 grid((unsigned)((a.C + 31) / 32), 3);
         by_types(j->w_dt, j->w_dt, [&](auto, auto t) {
-            rwkv::launch(join_reduce_kernel<decltype(t)>, grid, dim3(256), s, (const float*)workspace, a.N > 0 ? gy : 0, 3, a.C, outs);
+            rwkv::launch(join_reduce_kernel<decltype(t)>, grid, dim3(1024), s, (const float*)workspace, a.N > 0 ? gy : 0, 3, a.C, outs);
         });
     }
     return status_of("tail_bwd launch");
