@@ -648,7 +648,9 @@ struct TailArgs {
 };
 
 // A head is eight neighbouring lanes of 8 columns; TX lanes across, 256 / TX
-// rows down a block, rows strided over gridDim.y.
+// rows down a block, rows strided over gridDim.y, the next one on its way.
+// Bound by bytes: 32768 x 32 heads, o fp32, the rest bf16: 186 us (5.0 TB/s; a
+// large copy 5.1).
 template <typename TO, typename T>
 __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
     const int tx = threadIdx.x % TX, col = 8 * (blockIdx.x * TX + tx);
@@ -658,13 +660,26 @@ __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
     load_w<T>(a.rk, a.w32, col, 8, rk);
     load_w<T>(a.w, a.w32, col, 8, w);
     load_w<T>(a.b, a.w32, col, 8, b);
-    for (int64_t row = (int64_t)blockIdx.y * (256 / TX) + threadIdx.x / TX; row < a.N; row += step) {
+    int64_t row = (int64_t)blockIdx.y * (256 / TX) + threadIdx.x / TX;
+    if (row >= a.N) return;
+    Raw8<TO> ro;
+    Raw8<T> rr, rkk, rv, rg;
+    auto load = [&](int64_t at) {
+        ro.load(reinterpret_cast<const TO*>(a.o) + at * a.ldo + col, 8);
+        rr.load(reinterpret_cast<const T*>(a.r) + at * a.ldr + col, 8);
+        rkk.load(reinterpret_cast<const T*>(a.k) + at * a.ldk + col, 8);
+        rv.load(reinterpret_cast<const T*>(a.v) + at * a.ldv + col, 8);
+        rg.load(reinterpret_cast<const T*>(a.g) + at * a.ldg + col, 8);
+    };
+    load(row);
+    for (; row < a.N; row += step) {
         float o[8], r[8], k[8], v[8], g[8];
-        load8(reinterpret_cast<const TO*>(a.o) + row * a.ldo + col, 8, o);
-        load8(reinterpret_cast<const T*>(a.r) + row * a.ldr + col, 8, r);
-        load8(reinterpret_cast<const T*>(a.k) + row * a.ldk + col, 8, k);
-        load8(reinterpret_cast<const T*>(a.v) + row * a.ldv + col, 8, v);
-        load8(reinterpret_cast<const T*>(a.g) + row * a.ldg + col, 8, g);
+        ro.get(o);
+        rr.get(r);
+        rkk.get(k);
+        rv.get(v);
+        rg.get(g);
+        load(min(row + step, a.N - 1));
         float s = 0.0f, q = 0.0f, d = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -678,7 +693,7 @@ __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
             o[i] -= mean;
             q += o[i] * o[i];
         }
-        const float inv = 1.0f / sqrtf(sum8(q) * (1.0f / HEAD) + a.eps);
+        const float inv = __builtin_amdgcn_rsqf(sum8(q) * (1.0f / HEAD) + a.eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (o[i] * inv * w[i] + b[i] + d * v[i]) * g[i];
         store8(reinterpret_cast<T*>(a.y) + row * a.C + col, 8, o);
@@ -688,6 +703,8 @@ __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
 // With oh = (o − μ)·i, d = Σ r·k·r_k, q = oh·w + b + d·v:
 //   dg = dy·q, dq = dy·g, dv = dq·d, e = Σ dq·v, dr = e·k·r_k, dk = e·r·r_k
 //   do = LN'(dq·w; oh, i);  dr_k = Σ e·r·k, dw = Σ dq·oh, db = Σ dq
+// μ and i are formed again: o is read anyway.  Bound by bytes, 26 a value: the
+// same sizes in 330 us (5.3 TB/s), the sums' join 6 of them.
 template <typename TO, typename T>
 __global__ __launch_bounds__(256) void tail_bwd_kernel(TailArgs a, int TX) {
     __shared__ float sums[8 * 256];
@@ -723,7 +740,7 @@ __global__ __launch_bounds__(256) void tail_bwd_kernel(TailArgs a, int TX) {
                 o[i] -= mean;
                 q += o[i] * o[i];
             }
-            const float inv = 1.0f / sqrtf(sum8(q) * (1.0f / HEAD) + a.eps);
+            const float inv = __builtin_amdgcn_rsqf(sum8(q) * (1.0f / HEAD) + a.eps);
             float m1 = 0.0f, m2 = 0.0f, t[8];
             const int64_t at = row * a.C + col;
             // o: oh; g: dq; t: dg
@@ -847,13 +864,16 @@ int join_bwd_blocks(int64_t N, int64_t D) {
 // Lanes across and the grid of the tail's passes.
 void tail_geometry(int64_t N, int64_t C, int most, int& TX, int& gx, int& gy) {
     const int64_t chunks = C / 8;
-    TX = 8;
-    while (TX < 64 && TX < chunks) TX *= 2;
+    TX = 64;
+    // no more than an eighth of the lanes beyond the last head
+    while (TX > 8 && ((chunks + TX - 1) / TX * TX - chunks) * 8 > chunks) TX /= 2;
     gx = (int)((chunks + TX - 1) / TX);
     const int ty = 256 / TX;
     gy = (int)std::max<int64_t>(1, std::min<int64_t>((N + ty - 1) / ty, std::max(1, most / gx)));
 }
-constexpr int TAIL_FWD_BLOCKS = 4096, TAIL_BWD_BLOCKS = 1024;
+// (32768 x 32 heads: forward 183 us by 512 blocks, 186 by 1024, 185 by 4096, a few
+// rows 7.7 and 6.6; backward 330 by 512, whose partial rows are half of 1024's 342)
+constexpr int TAIL_FWD_BLOCKS = 1024, TAIL_BWD_BLOCKS = 512;
 
 bool join_ok(const rwkv_join* a) {
     return (a->x_dt == a->dt || a->x_dt == RWKV_F32) && rwkv::dtype_ok(a->dt) && (a->w_dt == RWKV_F32 || a->w_dt == a->dt);

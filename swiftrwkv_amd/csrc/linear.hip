@@ -1010,8 +1010,7 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(GemmArgs g, int BM, i
 // waves every eighth 32 of k, straight from memory into the products' operands
 // (any alignment), the next U of each on their way under U products; their
 // sums meet in LDS, in order.
-// GATED: eight rows of each half of W make the 16 columns.
-template <typename T, int NT, bool GATED>
+template <typename T, int NT>
 __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     constexpr int WAVES = 8, U = 8 / NT;
     __shared__ __align__(16) float sums[WAVES][16][16 * NT + 4];
@@ -1020,10 +1019,7 @@ __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     const T* xr = reinterpret_cast<const T*>(g.a) + (int64_t)min(i, (int)g.M - 1) * g.lda;
     const T* wr[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int row = GATED ? (i >> 3) * (g.N / 2) + min(n0 / 2 + 8 * t + (i & 7), g.N / 2 - 1) : min(n0 + 16 * t + i, g.N - 1);
-        wr[t] = reinterpret_cast<const T*>(g.b) + (int64_t)row * g.ldb;
-    }
+    for (int t = 0; t < NT; ++t) wr[t] = reinterpret_cast<const T*>(g.b) + (int64_t)min(n0 + 16 * t + i, g.N - 1) * g.ldb;
     auto chunk = [&](const T* p, int k) {
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (k + 8 <= g.K) {
@@ -1069,17 +1065,6 @@ __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
     for (int t = 0; t < NT; ++t)
         *reinterpret_cast<f32x4*>(&sums[wave][i][16 * t + 4 * q]) = acc[t];
     __syncthreads();
-    if constexpr (GATED) {
-        if (threadIdx.x >= 16 * NT) return;
-        const int m = threadIdx.x / NT, c = 16 * (threadIdx.x % NT);
-        float zg[1][8] = {}, zu[1][8] = {};
-#pragma unroll
-        for (int r = 0; r < WAVES; ++r)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) zg[0][e] += sums[r][m][c + e], zu[0][e] += sums[r][m][c + 8 + e];
-        finish_gated<T, 1>(g.e, m, 1, (n0 + c) / 2, zg, zu);
-        return;
-    }
     if (threadIdx.x >= 32 * NT) return;
     const int m = threadIdx.x / (2 * NT), c = 8 * (threadIdx.x % (2 * NT));
     float v[1][8] = {};
@@ -1088,6 +1073,108 @@ __global__ __launch_bounds__(512) void rows16_kernel(GemmArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[0][e] += sums[r][m][c + e];
     finish<T, 1>(g.e, m, 1, n0 + c, v);   // stores rows under M
+}
+
+// x [M <= 16, K] through a gated W, x in LDS: a block walks groups of 8 columns
+// of h (16 rows of W), its eight waves every eighth 64 of k, straight from
+// memory into the products' operands, DEPTH of those on their way all the time,
+// through the groups' ends: W's bytes are all there is to this product.  A
+// group's sums meet in LDS, in order, under the next group's loads; the two
+// halves of the waves take turns at it.  16 x 14336 x 4096 bf16: 49.6 us (4.75
+// TB/s), 1 row 41.7 (5.6); one group a block as rows16_kernel has it 71.4, 51.7.  R: units of 64 k between looks at the
+// group's end.  ODD: K is not a multiple of 8.
+constexpr int GATED_ROWS_X = 65536;   // values of x that fit
+template <typename T, int R, bool ODD>
+__global__ __launch_bounds__(512) void gated_rows_kernel(GemmArgs g) {
+    constexpr int WAVES = 8, DEPTH = 4;
+    __shared__ __align__(16) float sums[2][WAVES][16][20];
+    extern __shared__ __align__(16) uint4 xs[];   // [units][8 chunks][M]: chunk c of row m at c·M + m
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
+    const int M = (int)g.M, F = g.N / 2, groups = (F + 7) / 8;
+    const int per = ((g.K + 64 * WAVES - 1) / (64 * WAVES) + R - 1) / R * R;   // units of a wave and group
+    // eight values of a row from k on, zeros past its end
+    auto chunk = [&](const T* p, int k) {
+        uint4 v;
+        if constexpr (!ODD) {
+            __builtin_memcpy(&v, p + min(k, g.K - 8), 16);
+            if (k >= g.K) v = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            v = make_uint4(0u, 0u, 0u, 0u);
+            if (k + 8 <= g.K) {
+                __builtin_memcpy(&v, p + k, 16);
+            } else if (k < g.K) {
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+                for (int e = 0; e < 7; ++e)
+                    if (k + e < g.K) w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[k + e] << (16 * (e & 1));
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        return v;
+    };
+    // the loader: its group and unit
+    int l_group = blockIdx.x, l_unit = 0;
+    const T* wr = nullptr;
+    auto start = [&] {
+        const int col = min(8 * l_group + (i & 7), F - 1);   // (groups that do not come: the last columns again)
+        wr = reinterpret_cast<const T*>(g.b) + (int64_t)((i >> 3) * F + col) * g.ldb;
+    };
+    uint4 w[DEPTH][2];
+    auto load = [&](uint4 (&v)[2]) {
+        const int k = (l_unit * WAVES + wave) * 64 + 8 * q;
+        v[0] = chunk(wr, k);
+        v[1] = chunk(wr, k + 32);
+        if (++l_unit == per) {
+            l_unit = 0;
+            l_group = min(l_group + (int)gridDim.x, groups);
+            start();
+        }
+    };
+    start();
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) load(w[u]);
+    for (int c = threadIdx.x; c < per * WAVES * 8 * M; c += 512) {
+        const int m = c % M, k = 8 * (c / M);
+        xs[c] = chunk(reinterpret_cast<const T*>(g.a) + (int64_t)m * g.lda, k);
+    }
+    __syncthreads();
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int group = blockIdx.x, unit = 0, turn = 0;
+    const int row = min(i, M - 1);   // rows of x from M on are the last one again
+    while (group < groups) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+            uint4 cw[2] = {w[u][0], w[u][1]};
+            load(w[u]);
+            if (group < groups) {   // (a group's end may lie inside the unrolled units)
+                const int at = ((unit * WAVES + wave) * 8 + q) * M + row;
+                acc = mfma<T>(cw[0], xs[at], acc);
+                acc = mfma<T>(cw[1], xs[at + 4 * M], acc);
+                ++unit;
+                if ((u + 1) % R == 0 && unit == per) {
+                    *reinterpret_cast<f32x4*>(&sums[turn][wave][i][4 * q]) = acc;
+                    __syncthreads();
+                    if ((wave >> 2) == turn) {
+                        const int t = threadIdx.x & 255, m = t >> 4, c = t & 15;
+                        float s = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < WAVES; ++r) s += sums[turn][r][m][c];
+                        // columns of zg and zu, eight lanes apart
+                        float zg[1][8], zu[1][8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            zg[0][e] = __shfl(s, (lane & 48) + e);
+                            zu[0][e] = __shfl(s, (lane & 48) + 8 + e);
+                        }
+                        if (c == 0) finish_gated<T, 1>(g.e, m, 1, 8 * group, zg, zu);   // rows under M
+                    }
+                    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+                    unit = 0;
+                    turn ^= 1;
+                    group += gridDim.x;
+                }
+            }
+        }
+    }
 }
 
 // ───────────────────────────── rows of whole chunks ─────────────────────────────
@@ -1403,23 +1490,57 @@ void gemm_launch_tile(const Route& r, const GemmArgs& g, hipStream_t s) {
 // 2048 6.4 and 11.3), and from N = 6144 on a K of 512, or one of 8192, loses.
 bool rows16_applies(int64_t M, int64_t N, int64_t K) { return M <= 16 && (K <= 1024 || N >= 8192); }
 
+// Units of 512 k of gated_rows_kernel, and between looks at a group's end.
+int gated_rows_step(int64_t K) { return K <= 512 ? 1 : K <= 1024 ? 2 : 4; }
+int64_t gated_rows_units(int64_t K) {
+    const int64_t step = gated_rows_step(K);
+    return ((K + 511) / 512 + step - 1) / step * step;
+}
+// Few rows, whose x fits LDS; and not few columns with a long K, which the tiles
+// split over more CUs.  us by gated_rows_kernel, by tiles (bf16, W from memory;
+// rows x F x K):
+//   1 x 2048 x 16384   32.9, 38.6       8 x 2048 x 8192    20.8, 19.4
+//   1 x 1024 x 16384   22.1, 20.5       1 x 64 x 16384     18.3, 12.3
+//  16 x 2730 x 2048    12.4, 22.2      16 x 512 x 4096     11.9, 10.4
+bool gated_rows_applies(int64_t M, int64_t F, int64_t K) {
+    return M >= 1 && M <= 16 && gated_rows_units(K) * 512 * M <= GATED_ROWS_X && (K <= 4096 || F >= 2048);
+}
+
+template <typename T>
+void gated_rows_launch(const GemmArgs& g, hipStream_t s) {
+    const int groups = (g.N / 2 + 7) / 8, step = gated_rows_step(g.K);
+    const size_t lds = (size_t)gated_rows_units(g.K) * 512 * g.M * 2;
+    // Two blocks a CU where filling x twice costs little (1 x 4096 x 1024: 7.9 us, by
+    // one 8.5; 1 x 14336 x 4096 41.7 and 44.8; 16 x 8192 x 2048, 64 KB of x, 23.8 and 19.1).
+    const int blocks = lds <= 32768 ? 512 : 256;
+    auto launch = [&](auto r, auto odd) {
+        rwkv::launch_lds(gated_rows_kernel<T, decltype(r)::value, decltype(odd)::value>, dim3((unsigned)std::min(groups, blocks)), dim3(512), lds, s, g);
+    };
+    auto by_k = [&](auto odd) {
+        if (step == 1) launch(std::integral_constant<int, 1>{}, odd);
+        else if (step == 2) launch(std::integral_constant<int, 2>{}, odd);
+        else launch(std::integral_constant<int, 4>{}, odd);
+    };
+    if (g.K % 8 == 0) by_k(std::false_type{});
+    else by_k(std::true_type{});
+}
+
 // C = A·Bᵀ by the route of its sizes, then the epilogue.  gated: C's columns are
 // zg's and zu's by turns of eight (both operands k-contiguous).
 rwkv_status gemm_run(const char* what, bool akm, bool bkm, int dt, GemmArgs g, void* workspace, int64_t bytes,
                      hipStream_t s, bool gated = false) {
-    if (gated && rows16_applies(g.M, g.N, g.K)) {
-        const dim3 grid((unsigned)((g.N + 15) / 16));
-        if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 1, true>, grid, dim3(512), s, g);
-        else rwkv::launch(rows16_kernel<f16, 1, true>, grid, dim3(512), s, g);
+    if (gated && gated_rows_applies(g.M, g.N / 2, g.K)) {
+        if (dt == RWKV_BF16) gated_rows_launch<bf16>(g, s);
+        else gated_rows_launch<f16>(g, s);
         return status_of(what);
     }
-    if (!akm && !bkm && rows16_applies(g.M, g.N, g.K)) {
+    if (!gated && !akm && !bkm && rows16_applies(g.M, g.N, g.K)) {
         const int nt = g.e.codes ? 2 : 1;   // a group of codes is 32 columns
         const dim3 grid((unsigned)((g.N + 16 * nt - 1) / (16 * nt)));
-        if (dt == RWKV_BF16 && nt == 1) rwkv::launch(rows16_kernel<bf16, 1, false>, grid, dim3(512), s, g);
-        else if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 2, false>, grid, dim3(512), s, g);
-        else if (nt == 1) rwkv::launch(rows16_kernel<f16, 1, false>, grid, dim3(512), s, g);
-        else rwkv::launch(rows16_kernel<f16, 2, false>, grid, dim3(512), s, g);
+        if (dt == RWKV_BF16 && nt == 1) rwkv::launch(rows16_kernel<bf16, 1>, grid, dim3(512), s, g);
+        else if (dt == RWKV_BF16) rwkv::launch(rows16_kernel<bf16, 2>, grid, dim3(512), s, g);
+        else if (nt == 1) rwkv::launch(rows16_kernel<f16, 1>, grid, dim3(512), s, g);
+        else rwkv::launch(rows16_kernel<f16, 2>, grid, dim3(512), s, g);
         return status_of(what);
     }
     const bool aligned = (uintptr_t)g.a % 16 == 0 && (uintptr_t)g.b % 16 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0;
@@ -1508,7 +1629,9 @@ rwkv_status rwkv_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t l
     return gemm_run("linear_fwd", false, false, dt, g, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-int64_t rwkv_gated_fwd_workspace(int64_t M, int64_t F, int64_t K) { return rwkv_linear_fwd_workspace(M, 2 * F, K); }
+int64_t rwkv_gated_fwd_workspace(int64_t M, int64_t F, int64_t K) {
+    return F >= 1 && F <= (1 << 19) && shape_ok(M, 2 * F, K) && !gated_rows_applies(M, F, K) ? gemm_workspace(M, 2 * F, K, false) : 0;
+}
 
 rwkv_status rwkv_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* h, void* aux, uint8_t* rem,
                            rwkv_gate act, rwkv_dtype dt, int64_t M, int64_t F, int64_t K, void* workspace,

@@ -111,7 +111,10 @@ def test_gates(M, F, K, act, dt):
 @pytest.mark.parametrize("M,F,K", [(1, 1, 1), (1, 5, 8), (2, 8, 7), (3, 17, 33), (16, 40, 64), (16, 4099, 2056), (9, 4096, 1031), (17, 64, 64),
                                    (17, 100, 1000), (40, 3, 4096), (64, 512, 512), (100, 96, 4096), (129, 257, 515), (300, 1000, 600),
                                    (1000, 1001, 1000), (1024, 1024, 1024), (2048, 2048, 512), (4096, 4096, 256), (4096, 1037, 520),
-                                   (130, 2050, 4099), (700, 3001, 2001), (256, 64, 16384), (2500, 6000, 1024)])
+                                   (130, 2050, 4099), (700, 3001, 2001), (256, 64, 16384), (2500, 6000, 1024),
+                                   (16, 2100, 4096), (16, 2100, 4104), (13, 2200, 5000), (9, 2100, 7280), (5, 2100, 13100), (1, 2064, 32768),
+                                   (1, 2050, 65530), (2, 64, 16384), (7, 4100, 513), (16, 4200, 512), (3, 9000, 40), (12, 8200, 1027),
+                                   (4, 6000, 2040)])
 def test_gated_routes(M, F, K):
     case(f"gated {M} x {F} x {K}")
     a = run(M, F, K, BF, "silu")
