@@ -508,7 +508,9 @@ typedef struct {
 
 /* y = drop(x) + residual: x [N, D] of x_dt, residual (pitch ldr, may be NULL)
  * and y [N, D] of y_dt; the types are alike or one of them is f32.  The
- * gradient of x is the same call on dy.  D <= 2^22. */
+ * gradient of x is the same call on dy.  D <= 2^22, pitches at most
+ * RWKV_DROPOUT_MAX_PITCH. */
+#define RWKV_DROPOUT_MAX_PITCH ((1LL << 32) - 1)
 rwkv_status rwkv_dropout(const void* x, rwkv_dtype x_dt, int64_t ldx, const void* residual, int64_t ldr, void* y,
                          rwkv_dtype y_dt, const rwkv_drop* drop, int64_t N, int64_t D, void* stream);
 

@@ -77,63 +77,97 @@ __device__ __forceinline__ void factors(const Drop& d, uint64_t key, uint32_t c,
 // A dropped value is zero whatever it was, an infinity or a NaN too.
 __device__ __forceinline__ float dropped(float m, float v) { return m > 0.0f ? m * v : 0.0f; }
 
+// ───────────────────────────── chunks ─────────────────────────────
+
+// How a row of D columns falls into chunks of eight: WHOLE, D is a multiple of 8;
+// ENDS, it is not; FEW, D is under 8.
+enum { WHOLE, ENDS, FEW };
+
+// Eight values that were loaded `moved` columns before their place, into it:
+// zeros from `valid` on.
+__device__ __forceinline__ void move8(float (&v)[8], int moved, int valid) {
+#pragma unroll
+    for (int k = 4; k >= 1; k /= 2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (moved & k) v[i] = i + k < 8 ? v[i + k < 8 ? i + k : 7] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? v[i] : 0.0f;
+}
+
 // ───────────────────────────── dropout ─────────────────────────────
 
 struct DropoutArgs {
     const void* x;
-    int64_t ldx;
-    const void* res;   // of y's type, or null
-    int64_t ldr;
-    void* y;           // [N, D]
-    int64_t chunks;    // N·cpr
-    int cpr, D;        // chunks of 8 a row
-    uint32_t magic;    // ceil(2^32 / cpr) where cpr is at most a block's chunks
+    const void* res;     // of y's type, or null
+    void* y;             // [N, D]
+    uint32_t ldx, ldr;
+    int64_t chunks;      // N·cpr
+    int cpr, D;          // chunks of 8 a row
+    uint32_t magic;      // ceil(2^32 / cpr) where cpr is at most a block's chunks
     Drop drop;
 };
 
 // Chunks of 8 values, U a thread, a block's in one run; its first row is found
 // once (in 64 bits), the others from there: a quotient under 2·RUN by a divisor
-// of at most RUN is the high half of a 32-bit product with ceil(2^32 / cpr).
+// of at most RUN is the high half of a 32-bit product with ceil(2^32 / cpr), and
+// an address one product of 32 x 32 bits (products are a quarter of the rate of
+// other operations, and the generator has 20 of them a chunk).  A chunk that
+// passes its row's end is loaded as the row's last eight columns (FEW: one by
+// one), and moved.
+//
+// Bound by bytes, and with 4 a value by the generator too: 32768 x 4096 bf16
+// with an fp32 residual 235 us (5.7 TB/s), fp32 into bf16 143, bf16 96 (5.6).
 constexpr int DROP_U = 4, DROP_RUN = 256 * DROP_U;
 
-template <typename TX, typename TY>
+template <typename TX, typename TY, int ROWS>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
     const int64_t first = (int64_t)blockIdx.x * DROP_RUN;
     const int64_t row0 = first / a.cpr;
     const uint32_t rem = (uint32_t)(first - row0 * a.cpr);
     const int left = (int)min(a.chunks - first, (int64_t)DROP_RUN);
     const uint64_t key = a.drop.key();
+    const TX* const x0 = reinterpret_cast<const TX*>(a.x) + row0 * a.ldx;
+    const TY* const r0 = reinterpret_cast<const TY*>(a.res) + row0 * a.ldr;
+    TY* const y0 = reinterpret_cast<TY*>(a.y) + row0 * a.D;
     Raw8<TX> x[DROP_U];
     Raw8<TY> r[DROP_U];
-    int64_t row[DROP_U];
-    uint32_t c[DROP_U];
+    uint32_t row[DROP_U], col[DROP_U];   // from row0; the chunk's first column
+    auto valid = [&](int u) { return ROWS == WHOLE ? 8 : a.D - (int)col[u]; };
+    auto load = [&](auto& r, auto* p, uint32_t ld, int u) {
+        if constexpr (ROWS == FEW) r.load(p + (uint64_t)row[u] * ld, a.D);
+        else __builtin_memcpy(r.q, p + ((uint64_t)row[u] * ld + (ROWS == ENDS ? min(col[u], (uint32_t)a.D - 8) : col[u])), sizeof(r.q));
+    };
+    auto get = [&](const auto& r, int u, float (&v)[8]) {
+        r.get(v);
+        if constexpr (ROWS == ENDS)
+            if (valid(u) < 8) move8(v, 8 - valid(u), valid(u));
+    };
 #pragma unroll
     for (int u = 0; u < DROP_U; ++u) {
-        const int at = threadIdx.x + 256 * u;
-        const uint32_t n = rem + at;
-        const uint32_t q = a.cpr == 1 ? n : a.cpr > DROP_RUN ? (n >= (uint32_t)a.cpr) : __umulhi(n, a.magic);
-        row[u] = row0 + q;
-        c[u] = n - q * a.cpr;
-        if (at >= left) continue;
-        x[u].load(reinterpret_cast<const TX*>(a.x) + row[u] * a.ldx + 8 * c[u], a.D - 8 * (int)c[u]);
-        if (a.res) r[u].load(reinterpret_cast<const TY*>(a.res) + row[u] * a.ldr + 8 * c[u], a.D - 8 * (int)c[u]);
+        // (threads behind the last chunk have it again)
+        const uint32_t n = rem + min((int)threadIdx.x + 256 * u, left - 1);
+        row[u] = a.cpr == 1 ? n : a.cpr > DROP_RUN ? (n >= (uint32_t)a.cpr) : __umulhi(n, a.magic);
+        col[u] = 8 * (n - row[u] * a.cpr);
+        load(x[u], x0, a.ldx, u);
+        if (a.res) load(r[u], r0, a.ldr, u);
     }
 #pragma unroll
     for (int u = 0; u < DROP_U; ++u) {
         if ((int)threadIdx.x + 256 * u >= left) continue;
         float v[8], m[8];
-        x[u].get(v);
+        get(x[u], u, v);
         if (a.drop.threshold) {
-            factors(a.drop, key, c[u], (uint32_t)row[u], m);
+            factors(a.drop, key, col[u] / 8, (uint32_t)row0 + row[u], m);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = dropped(m[i], v[i]);
         }
         if (a.res) {
-            r[u].get(m);
+            get(r[u], u, m);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += m[i];
         }
-        store8(reinterpret_cast<TY*>(a.y) + row[u] * a.D + 8 * c[u], a.D - 8 * (int)c[u], v);
+        store8(y0 + ((uint64_t)row[u] * (uint32_t)a.D + col[u]), valid(u), v);
     }
 }
 
@@ -194,10 +228,6 @@ __device__ __forceinline__ void load_w(const void* w, int w32, int col, int vali
         load8(reinterpret_cast<const T*>(w) + col, valid, v);
 }
 
-// How a row of D columns falls into chunks of eight: WHOLE, D is a multiple of 8;
-// ENDS, it is not; FEW, D is under 8.
-enum { WHOLE, ENDS, FEW };
-
 // A thread's eight columns of a row.  Threads whose chunk passes the row's end,
 // or lies behind it, load the row's last eight columns, unconditionally (FEW:
 // one by one), and move them into place where they are used; WHOLE has none of
@@ -232,16 +262,7 @@ struct Cols {
     __device__ __forceinline__ void get(Raw8<T> r, float (&v)[8]) const {
         if constexpr (ROWS != ENDS) return r.get(v);
         r.get(v);
-        if (col != at) {
-            const int moved = col - at;
-#pragma unroll
-            for (int k = 4; k >= 1; k /= 2)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (moved & k) v[i] = i + k < 8 ? v[i + k < 8 ? i + k : 7] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < valid ? v[i] : 0.0f;
-        }
+        if (col != at) move8(v, col - at, valid);
     }
     template <typename T>
     __device__ __forceinline__ void store(void* p, int64_t row, int D, const float (&v)[8]) const {
@@ -886,26 +907,25 @@ extern "C" {
 rwkv_status rwkv_dropout(const void* x, rwkv_dtype x_dt, int64_t ldx, const void* residual, int64_t ldr, void* y,
                          rwkv_dtype y_dt, const rwkv_drop* drop, int64_t N, int64_t D, void* stream) {
     RWKV_REQUIRE(pair_ok(x_dt, y_dt), RWKV_E_DTYPE, "dropout: types x %d, y %d", (int)x_dt, (int)y_dt);
-    RWKV_REQUIRE(N >= 0 && N <= (1 << 24) && D >= 1 && D <= (1 << 22) && ldx >= D && (!residual || ldr >= D), RWKV_E_SHAPE,
-                 "dropout: N=%lld D=%lld ldx=%lld ldr=%lld", (long long)N, (long long)D, (long long)ldx, (long long)ldr);
+    RWKV_REQUIRE(N >= 0 && N <= (1 << 24) && D >= 1 && D <= (1 << 22) && ldx >= D && ldx <= RWKV_DROPOUT_MAX_PITCH &&
+                     (!residual || (ldr >= D && ldr <= RWKV_DROPOUT_MAX_PITCH)),
+                 RWKV_E_SHAPE, "dropout: N=%lld D=%lld ldx=%lld ldr=%lld", (long long)N, (long long)D, (long long)ldx, (long long)ldr);
     RWKV_REQUIRE(N == 0 || (x && y), RWKV_E_NULL, "dropout: null buffer");
     RWKV_REQUIRE(drop_ok(drop), RWKV_E_UNSUPPORTED, "dropout: threshold %d of 65536", drop ? drop->threshold : -1);
     if (N == 0) return RWKV_OK;
     const int64_t cpr = (D + 7) / 8, chunks = N * cpr, blocks = (chunks + DROP_RUN - 1) / DROP_RUN;
     RWKV_REQUIRE(blocks < (int64_t(1) << 31), RWKV_E_SHAPE, "dropout: %lld values", (long long)(N * D));
-    const DropoutArgs a{x, ldx, residual, ldr, y, chunks, (int)cpr, (int)D,
+    const DropoutArgs a{x, residual, y, (uint32_t)ldx, residual ? (uint32_t)ldr : 0u, chunks, (int)cpr, (int)D,
                         (uint32_t)(((uint64_t(1) << 32) + cpr - 1) / cpr), drop_of(*drop)};
     const hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)blocks);
-    if (y_dt == RWKV_F32 || x_dt == y_dt) {
-        by_types(y_dt, x_dt, [&](auto ty, auto tx) {
-            rwkv::launch(dropout_kernel<decltype(tx), decltype(ty)>, grid, dim3(256), s, a);
-        });
-    } else {
-        by_types(x_dt, y_dt, [&](auto tx, auto ty) {
-            rwkv::launch(dropout_kernel<decltype(tx), decltype(ty)>, grid, dim3(256), s, a);
-        });
-    }
+    auto launch = [&](auto tx, auto ty) {
+        if (D < 8) rwkv::launch(dropout_kernel<decltype(tx), decltype(ty), FEW>, grid, dim3(256), s, a);
+        else if (D % 8 == 0) rwkv::launch(dropout_kernel<decltype(tx), decltype(ty), WHOLE>, grid, dim3(256), s, a);
+        else rwkv::launch(dropout_kernel<decltype(tx), decltype(ty), ENDS>, grid, dim3(256), s, a);
+    };
+    if (y_dt == RWKV_F32 || x_dt == y_dt) by_types(y_dt, x_dt, [&](auto ty, auto tx) { launch(tx, ty); });
+    else by_types(x_dt, y_dt, [&](auto tx, auto ty) { launch(tx, ty); });
     return status_of("dropout launch");
 }
 

@@ -9,6 +9,7 @@
 // (RWKVBlock.swift:163-307).
 
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -170,6 +171,13 @@ Rows product_rows(const Tensor& x) {
     return r;
 }
 
+// Operands of dropout, likewise.
+Rows dropout_rows(const Tensor& x) {
+    Rows r = rows_of(x);
+    if (r.ld > RWKV_DROPOUT_MAX_PITCH) r = {r.t.detach().contiguous(), r.N, r.D, r.D};
+    return r;
+}
+
 // Rows for the products: 16-byte aligned ones as they lie, others as a copy
 // whose width is rounded up to 8, with zeros behind.
 Rows aligned_rows(Rows r) {
@@ -220,6 +228,23 @@ Tensor unpack(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, 
 }
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A leaf's gradient belongs to the stream under which its node came to be.  If
+// an eager graph still holds that node, a captured backward pass on another
+// stream would have the engine make the one wait for the other, which the
+// capture does not survive, nor the process.
+void capture_ok(const char* what, const Node& node, c10::Device dev) {
+    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const torch::autograd::Edge& e : node.next_edges()) {
+        if (!e.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
+        const std::optional<c10::Stream> leaf = e.function->stream();
+        TORCH_CHECK(!leaf || *leaf == stream.unwrap(), what,
+                    ": its captured backward pass reaches a leaf that an eager graph on another stream still holds; "
+                    "free that graph, or capture with leaves of their own");
+    }
+}
 
 // Gradients of gradients: the kernels leave no graph, so a graph through
 // their results raises instead of missing a term, on the way to every input
@@ -597,6 +622,7 @@ struct GatedNode : Node {
         const Tensor wt = w.unpack(self), k = kept.unpack(self), r = rem.unpack(self);
         const auto dev = wt.device();
         const Guard guard(dev);
+        capture_ok("gated_linear", *this, dev);
         variable_list out(2);
         if (!need_x && !need_w) return once(std::move(out), grads[0], *this, "gated_linear");
         const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(y_shape, wt.options());
@@ -697,12 +723,16 @@ struct DropArgs {
 };
 
 uint64_t count_arg(PyObject* o, const char* what) {
-    if (PyLong_Check(o)) {
-        const uint64_t v = PyLong_AsUnsignedLongLong(o);
-        if (!PyErr_Occurred()) return v;
-        PyErr_Clear();
+    // (numpy's integers too; not a tensor, whose value would have to be waited for)
+    PyObject* n = THPVariable_Check(o) ? nullptr : PyNumber_Index(o);
+    uint64_t v = 0;
+    if (n) {
+        v = PyLong_AsUnsignedLongLong(n);
+        Py_DECREF(n);
     }
-    raise(PyLong_Check(o) ? PyExc_ValueError : PyExc_TypeError, std::string(what) + " must be an integer of 0 to 2^64 - 1");
+    if (n && !PyErr_Occurred()) return v;
+    PyErr_Clear();
+    raise(n ? PyExc_ValueError : PyExc_TypeError, std::string(what) + " must be an integer of 0 to 2^64 - 1");
 }
 
 // p, seed and offset, before anything is known of the device
@@ -746,11 +776,12 @@ struct DropoutNode : Node {
         no_tangent("dropout", {&grads[0]});
         const Tensor st = seed.unpack(shared_from_this());
         const Guard guard(dev);
+        capture_ok("dropout", *this, dev);
         const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(shape, at::TensorOptions().dtype(y_dt).device(dev));
         variable_list out(num_outputs());
         if (need_r) out[1] = dyt;
         if (need_x) {
-            const Rows dy = rows_of(dyt);
+            const Rows dy = dropout_rows(dyt);
             out[0] = empty(shape, x_dt, dev);
             const rwkv_drop d = drop_of(drop, st);
             check(rwkv_dropout(dy.p(), dt_of(y_dt), dy.ld, nullptr, 0, ptr(out[0]), dt_of(x_dt), &d, dy.N, dy.D, stream_of(dyt)));
@@ -784,9 +815,9 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->set_next_edges(res.defined() ? torch::autograd::collect_next_edges(x, res) : torch::autograd::collect_next_edges(x));
     }
     const Guard guard(x.device());
-    const Rows xr = rows_of(x);
+    const Rows xr = dropout_rows(x);
     Rows rr{};
-    if (res.defined()) rr = rows_of(res);
+    if (res.defined()) rr = dropout_rows(res);
     Tensor y = empty(x.sizes(), yt, x.device());
     const rwkv_drop d = drop_of(drop.d, drop.seed);
     check(rwkv_dropout(xr.p(), dt_of(xt), xr.ld, rr.t.defined() ? rr.p() : nullptr, rr.ld, ptr(y), dt_of(yt), &d, xr.N, xr.D,
@@ -860,6 +891,7 @@ struct JoinNode : Node {
         for (int i = O; i < INPUTS; ++i) t[i] = in[i].unpack(self);
         const auto dev = st.device();
         const Guard guard(dev);
+        capture_ok("block_join", *this, dev);
         Rows o{}, g{}, dx{}, dh{};
         if (t[O].defined()) o = rows_of(t[O]);
         if (t[GATE].defined()) g = rows_of(t[GATE]);
@@ -996,6 +1028,7 @@ struct TailNode : Node {
         for (int i = 0; i < INPUTS; ++i) t[i] = in[i].unpack(self);
         const auto dev = t[O].device();
         const Guard guard(dev);
+        capture_ok("wkv_tail", *this, dev);
         for (int i = 0; i < RK; ++i) r[i] = rows_of(t[i]);
         const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(shape, t[R].options());
         const Rows dy = rows_of(dyt);

@@ -58,6 +58,8 @@ def test_dropout_entry_refuses():
     refused(SHAPE, "rwkv_dropout", *a(N=(1 << 24) + 1))
     refused(SHAPE, "rwkv_dropout", *a(N=-1))
     refused(SHAPE, "rwkv_dropout", *a(res=D, ldr=7))
+    refused(SHAPE, "rwkv_dropout", *a(ldx=1 << 32))
+    refused(SHAPE, "rwkv_dropout", *a(res=D, ldr=1 << 32))
     refused(NULL, "rwkv_dropout", *a(x=None))
     refused(NULL, "rwkv_dropout", *a(y=None))
     refused(UNSUP, "rwkv_dropout", *a(drop=None))
@@ -140,6 +142,7 @@ SEED2 = torch.zeros(2, dtype=torch.int64)
     ({}, ValueError, DEVICE), (dict(x=t(8)), ValueError, DEVICE), (dict(residual=t(2, 8, dtype=F32)), ValueError, DEVICE),
     (dict(p=0), ValueError, DEVICE), (dict(p=1.0), ValueError, DEVICE), (dict(seed=(1 << 64) - 1, offset=1 << 63), ValueError, DEVICE),
     (dict(seed=torch.zeros(1, dtype=torch.int64)), ValueError, DEVICE), (dict(seed=torch.tensor(5)), ValueError, DEVICE),
+    (dict(seed=np.int64(5), offset=np.uint64(7)), ValueError, DEVICE),
     (dict(p=-0.1), ValueError, "p must be 0 to 1"), (dict(p=1.01), ValueError, "p must be 0 to 1"),
     (dict(p=float("nan")), ValueError, "p must be 0 to 1"), (dict(p="a"), TypeError, "real number"),
     (dict(seed=-1), ValueError, "seed must be an integer of 0"), (dict(seed=1 << 64), ValueError, "seed must be an integer of 0"),

@@ -157,6 +157,51 @@ def test_dropout_of_more_than_2_32_bytes():
     torch.cuda.empty_cache()
 
 
+def test_dropout_of_rows_far_apart():
+    """Rows 2^32 values apart and more: copied first."""
+    case("dropout of rows 2^32 values apart")
+    for step in ((1 << 32) - 8, (1 << 32) + 8):
+        buf = torch.empty(step + 72, device=DEV, dtype=BF)
+        v = buf.as_strided((2, 64), (step, 1), 8)
+        v.copy_(randn(gen(1), 2, 64))
+        run_dropout(v, 0.4, v.float())
+        del buf, v
+    torch.cuda.empty_cache()
+
+
+def test_captured_backward_over_an_eager_graph_s_leaves():
+    """The leaves' gradient nodes belong to the eager graph's stream: a captured
+    backward pass that reaches them is refused, with a message, and the next
+    capture, with leaves of its own, runs."""
+    case("a captured backward pass while an eager graph of the same leaves lives")
+    x, w = randn(gen(1), 6, 128, dtype=BF).requires_grad_(True), randn(gen(2), 16, 128, dtype=BF)
+    one = torch.ones(128, device=DEV)
+    calls = {"dropout": lambda a: train.dropout(a, 0.1, 1), "block_join": lambda a: train.block_join(a, a, one)[1],
+             "wkv_tail": lambda a: train.wkv_tail(a, a, a, a, one, a, one, one), "gated_linear": lambda a: train.gated_linear(a, w)}
+    for name, f in calls.items():
+        eager = f(x)
+        dy = torch.ones_like(eager)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                y = f(x)
+                with pytest.raises(RuntimeError, match=f"{name}: its captured backward pass reaches a leaf"):
+                    torch.autograd.grad(y, x, dy)
+            own = x.detach().requires_grad_(True)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                dx, = torch.autograd.grad(f(own), own, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            want, = torch.autograd.grad(f(x), x, dy)
+            assert torch.equal(dx, want), name
+        torch.autograd.grad(eager, x, dy)
+
+
 def test_seed_tensor_in_a_graph():
     """Forward and backward captured once; each replay takes the seed that the tensor holds then."""
     case("dropout and block_join captured with their gradients, another seed each replay")
