@@ -1359,15 +1359,16 @@ struct GatedArgs {
 
 // dzg = dy·zu·act'(zg), dzu = dy·act(zg), rounded to the operands' type for the
 // products (as dact_kernel).  TX chunks of 8 columns across, 256/TX rows down a
-// block, rows strided over gridDim.y, two of them loaded at a time.  WHOLE: F is
-// a multiple of 8, and no chunk has to be looked at value by value.  Bound by
+// block, rows strided over gridDim.y, two of them loaded at a time.  A chunk that
+// passes F is the last eight columns, of which some are another thread's too: both
+// store the same.  FEW: F is under 8.  Bound by
 // bytes: 16384 x 14336 bf16 (2.8 GB) 581 us, 4.85 TB/s.
-template <typename T, bool WHOLE>
+template <typename T, bool FEW>
 __global__ __launch_bounds__(256) void gated_dact_kernel(GatedArgs a, int TX) {
     constexpr int U = 2;
     const int tx = threadIdx.x % TX, TY = 256 / TX;
-    const int col = 8 * (blockIdx.x * TX + tx), valid = WHOLE ? 8 : a.F - col;
-    if (col >= a.F) return;
+    const int place = 8 * (blockIdx.x * TX + tx), col = FEW ? place : min(place, a.F - 8), valid = FEW ? a.F : 8;
+    if (place >= a.F) return;
     const int64_t step = (int64_t)gridDim.y * TY;
     for (int64_t first = (int64_t)blockIdx.y * TY + threadIdx.x / TX; first < a.M; first += U * step) {
         float d[U][8], g[U][8], u[U][8];
@@ -1394,7 +1395,7 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(GatedArgs a, int TX) {
             T* z = reinterpret_cast<T*>(a.dz) + row * a.ldz;
             store8(z + col, valid, u[k]);
             store8(z + a.F + col, valid, v);
-            if (col + 8 >= a.F)
+            if (place + 8 >= a.F)
                 for (int64_t i = 2 * (int64_t)a.F; i < a.ldz; ++i) z[i] = (T)0.0f;
         }
     }
@@ -1708,7 +1709,7 @@ rwkv_status rwkv_gated_dact(const void* dy, int64_t lddy, const void* kept, cons
     const GatedArgs a{dy, lddy, kept, rem, (int)act, dz, ldz, M, (int)F};
     const dim3 grid((unsigned)gx, (unsigned)gy);
     auto launch = [&](auto t) {
-        if (F % 8 == 0) rwkv::launch(gated_dact_kernel<decltype(t), true>, grid, dim3(256), (hipStream_t)stream, a, TX);
+        if (F < 8) rwkv::launch(gated_dact_kernel<decltype(t), true>, grid, dim3(256), (hipStream_t)stream, a, TX);
         else rwkv::launch(gated_dact_kernel<decltype(t), false>, grid, dim3(256), (hipStream_t)stream, a, TX);
     };
     if (dt == RWKV_BF16) launch(bf16{});
