@@ -534,10 +534,11 @@ typedef struct {
  * other output may alias an input. */
 rwkv_status rwkv_join_fwd(const rwkv_join* args, void* xs, void* h, float* stats, void* stream);
 
-/* Gradients from x' as stored and the stats (args->x is not read, args->o only
- * with gate, post_weight or scale): dxs [N, D]
- * of x_dt and dh [N, D] of dt, each NULL for zeros; dx of x_dt, dout and dgate
- * of dt, vectors' gradients of w_dt, each NULL where not wanted.  For those of
+/* Gradients from the stats and, with an f32 x_dt, xs as the forward pass wrote it
+ * (args->x is not read, args->o only with gate, post_weight or scale); with a
+ * 16-bit x_dt from x and o, of which x' is formed again (xs is not read).  dxs
+ * [N, D] of x_dt and dh [N, D] of dt, each NULL for zeros; dx of x_dt, dout and
+ * dgate of dt, vectors' gradients of w_dt, each NULL where not wanted.  For those of
  * vectors a workspace of rwkv_join_bwd_workspace(N, D) bytes, 16-byte aligned.
  * The sums' order is fixed. */
 int64_t rwkv_join_bwd_workspace(int64_t N, int64_t D);

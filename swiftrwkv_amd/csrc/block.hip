@@ -395,8 +395,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_fwd_kernel(JoinFwd a) {
 enum { DW, DB, DPW, DPB, DSC, SUMS };   // column sums of the join, the scale's last
 
 struct JoinBwd {
-    const void *xs, *o, *gate;  // o null: it does not reach a gradient
-    int64_t ldo, ldg;
+    const void *xs, *o, *gate;  // x', or x where x' has 16 bits; o null: it does not reach a gradient
+    int64_t ldx, ldo, ldg;
     const float* stats;
     const void *post_w, *post_b, *scale, *w;
     int w32;
@@ -431,6 +431,10 @@ struct Slots {
 //   do = LN'(dn·w1; oh, r1), dw1 = Σ dn·oh, db1 = Σ dn
 // LN'(y; h, r) = r·(y − mean y − h·mean(y·h)).
 //
+// A stream of 16 bits holds x' rounded, which would put that rounding into xh and
+// so into sums of fp32: x' is formed again from x, o and the gate, which are read
+// anyway.
+//
 // A chunk is loaded as soon as the one before it has been taken apart, so the
 // next row is on its way under this one's two sums over the row.  The vectors
 // lie in LDS.  The sizes above: 146 us (5.1 TB/s) and the join of the sums 6; with
@@ -444,7 +448,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
     __shared__ float2 part[2][16];
     __shared__ float sums[RPB > 1 ? 8 * 256 : 1];
     __shared__ float4 slots[8][threads_of(TPR)];
-    constexpr bool AHEAD = TPR < 1024;
+    constexpr bool AHEAD = TPR < 1024, AGAIN = sizeof(TS) == 2;   // rows read ahead; x' formed again
     enum { PW, PB, SC, W };
     const Slots<4, threads_of(TPR)> lds{slots};
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
@@ -457,7 +461,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
     auto load_h = [&](int64_t r) {
         if (!a.dh) return;
         at.load(rdh, a.dh, r, a.D);
-        at.load(rx, a.xs, r, a.D);
+        at.load(rx, a.xs, r, a.ldx);
     };
     auto load_o = [&](int64_t r) {
         if (a.dxs) at.load(rdx, a.dxs, r, a.D);
@@ -500,13 +504,45 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
         const int64_t then = min(row + step, a.N - 1);   // (the last row again rather than a choice)
         const float4 st = AHEAD ? next : *reinterpret_cast<const float4*>(a.stats + 4 * row);
         if constexpr (!AHEAD) load_h(row);
-        float G[8], y[8], c[8], oh[8];
+        float G[8], y[8], c[8], oh[8], nv[8];
         if constexpr (AHEAD) next = *reinterpret_cast<const float4*>(a.stats + 4 * then);
+        // oh, n, the gate and, where something is dropped, m
+        float m[8];
+        auto branch = [&](float (&gate)[8]) {
+            if constexpr (!AHEAD) {
+                __builtin_amdgcn_sched_barrier(0);   // (not ahead: registers)
+                load_o(row);
+            }
+            float b[8];
+            at.get(ro, oh);
+            at.get(rg, gate);
+            vector(PW, c);
+            vector(PB, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                oh[i] = at.has(i) ? (oh[i] - st.x) * st.y : 0.0f;
+                nv[i] = oh[i] * c[i] + b[i];
+            }
+            if (a.drop.threshold) factors(a.drop, key, (uint32_t)t, (uint32_t)row, m);
+        };
+        float gate[8], sc[8];
+        if constexpr (AGAIN) {
+            branch(gate);
+            vector(SC, sc);
+        }
         if (a.dh) {
             float xh[8];
             at.get(rdh, y);
             at.get(rx, xh);
             if constexpr (AHEAD) load_h(then);
+            if constexpr (AGAIN) {   // as the forward pass forms x'
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float u = nv[i] * gate[i];
+                    if (a.drop.threshold) u = dropped(m[i], u);
+                    xh[i] = at.has(i) ? xh[i] + sc[i] * u : 0.0f;
+                }
+            }
             add(DB, y);
             float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -531,37 +567,20 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = 0.0f;
         }
-        if constexpr (!AHEAD) {
-            __builtin_amdgcn_sched_barrier(0);   // (not ahead: registers)
-            load_o(row);
-        }
+        if constexpr (!AGAIN) branch(gate);
         at.get(rdx, G);
 #pragma unroll
         for (int i = 0; i < 8; ++i) G[i] += y[i];
         if (a.dx) at.template store<TS>(a.dx, row, a.D, G);
-        float nv[8];   // y: the gate
-        at.get(ro, oh);
-        at.get(rg, y);
         if constexpr (AHEAD) load_o(then);
-        {
-            float b[8];
-            vector(PW, c);
-            vector(PB, b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                oh[i] = at.has(i) ? (oh[i] - st.x) * st.y : 0.0f;
-                nv[i] = oh[i] * c[i] + b[i];
-            }
-        }
-        float u[8], sc[8];
+        float u[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            u[i] = y[i] * nv[i];
+            u[i] = gate[i] * nv[i];
+            y[i] = gate[i];
             G[i] = at.has(i) ? G[i] : 0.0f;   // (not zero of itself past the row's end)
         }
         if (a.drop.threshold) {
-            float m[8];
-            factors(a.drop, key, (uint32_t)t, (uint32_t)row, m);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 u[i] = dropped(m[i], u[i]);   // m of G, for the sum
@@ -569,7 +588,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
                 y[i] = dropped(m[i], y[i]);
             }
         }
-        vector(SC, sc);
+        if constexpr (!AGAIN) vector(SC, sc);
+        vector(PW, c);
         float p1 = 0.0f, p2 = 0.0f;
         // u: dn·oh; y: dn; nv: dg; G: dn·w1
 #pragma unroll
@@ -974,15 +994,17 @@ rwkv_status rwkv_join_bwd(const rwkv_join* j, const void* xs, const float* stats
                      (!j->gate || j->ldg >= j->D),
                  RWKV_E_SHAPE, "join_bwd: N=%lld D=%lld ldo=%lld ldg=%lld (D <= %d)", (long long)j->N, (long long)j->D,
                  (long long)j->ldo, (long long)j->ldg, JOIN_MAX_D);
-    RWKV_REQUIRE(j->N == 0 || ((j->o || !(j->gate || j->post_weight || j->scale)) && j->weight && xs && stats), RWKV_E_NULL,
-                 "join_bwd: null buffer");
+    const bool again = j->x_dt != RWKV_F32;   // x' is formed again
+    RWKV_REQUIRE(!again || !j->x || j->ldx >= j->D, RWKV_E_SHAPE, "join_bwd: ldx=%lld", (long long)j->ldx);
+    RWKV_REQUIRE(j->N == 0 || ((again ? j->x && j->o : xs && (j->o || !(j->gate || j->post_weight || j->scale))) && j->weight && stats),
+                 RWKV_E_NULL, "join_bwd: null buffer");
     RWKV_REQUIRE((j->post_weight || (!j->post_bias && !dpost_weight && !dpost_bias)) && (j->gate || !dgate) &&
                      (j->scale || !dscale),
                  RWKV_E_NULL, "join_bwd: the gradient of a part that is not there");
     RWKV_REQUIRE((uintptr_t)stats % 16 == 0, RWKV_E_SHAPE, "join_bwd: misaligned stats");
     RWKV_REQUIRE(drop_ok(&j->drop), RWKV_E_UNSUPPORTED, "join_bwd: threshold %d of 65536", j->drop.threshold);
     void* const want[SUMS] = {dweight, dbias, dpost_weight, dpost_bias, dscale};
-    JoinBwd a{xs, j->o, j->gate, j->ldo, j->ldg, stats, j->post_weight, j->post_bias, j->scale, j->weight,
+    JoinBwd a{again ? j->x : xs, j->o, j->gate, again ? j->ldx : j->D, j->ldo, j->ldg, stats, j->post_weight, j->post_bias, j->scale, j->weight,
               j->w_dt == RWKV_F32, dxs, dh, dx, dout, dgate, nullptr, {}, 0, j->N, (int)j->D, drop_of(j->drop)};
     Outs outs{};
     for (int k = 0; k < SUMS; ++k) {

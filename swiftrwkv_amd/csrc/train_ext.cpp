@@ -865,10 +865,10 @@ at::ScalarType vectors_of(std::initializer_list<Vector*> all, const std::string&
 }
 
 // Keeps x' (its own result), the statistics, and o and gate where they reach a
-// gradient.
+// gradient; of a 16-bit stream x and o, from which x' is formed again.
 struct JoinNode : Node {
     enum { X, O, GATE, W, B, PW, PB, SC, INPUTS };
-    SavedVariable xs, stats, seed, in[INPUTS];   // (X unused)
+    SavedVariable xs, stats, seed, in[INPUTS];
     rwkv_drop drop;
     int at[INPUTS];                              // an input's gradient among the outputs, or -1
     std::vector<int64_t> shape;
@@ -888,11 +888,12 @@ struct JoinNode : Node {
         const auto self = shared_from_this();
         const Tensor x1 = xs.unpack(self), st = stats.unpack(self), sd = seed.unpack(self);
         Tensor t[INPUTS];
-        for (int i = O; i < INPUTS; ++i) t[i] = in[i].unpack(self);
+        for (int i = 0; i < INPUTS; ++i) t[i] = in[i].unpack(self);
         const auto dev = st.device();
         const Guard guard(dev);
         capture_ok("block_join", *this, dev);
-        Rows o{}, g{}, dx{}, dh{};
+        Rows x{}, o{}, g{}, dx{}, dh{};
+        if (t[X].defined()) x = rows_of(t[X]);
         if (t[O].defined()) o = rows_of(t[O]);
         if (t[GATE].defined()) g = rows_of(t[GATE]);
         if (grads[0].defined()) dx = rows_of(grads[0], true);
@@ -908,7 +909,7 @@ struct JoinNode : Node {
             d[i] = ptr(r);
             sums = sums || i >= W;
         }
-        const rwkv_join a{nullptr, opt(o), opt(g), 0, o.ld, g.ld, dt_of(x_dt), dt_of(dt), dt_of(w_dt), cptr(t[PW]), cptr(t[PB]),
+        const rwkv_join a{opt(x), opt(o), opt(g), x.ld, o.ld, g.ld, dt_of(x_dt), dt_of(dt), dt_of(w_dt), cptr(t[PW]), cptr(t[PB]),
                           cptr(t[SC]), cptr(t[W]), nullptr, post_eps, eps, drop_of(drop, sd), N, D};
         const Ws ws(sums ? rwkv_join_bwd_workspace(N, D) : 0, dev);
         check(rwkv_join_bwd(&a, cptr(x1), ptr<float>(st), opt(dx), opt(dh), d[X], d[O], d[GATE], d[W], d[B], d[PW], d[PB], d[SC],
@@ -987,14 +988,15 @@ PyObject* py_block_join(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->post_eps = (float)post_eps;
         if (drop.seed.defined()) node->seed = SavedVariable(drop.seed, false);
         node->stats = SavedVariable(st, false);
-        if (gate.defined() || pw.t.defined() || sc.t.defined()) node->in[JoinNode::O] = SavedVariable(orr.t, false);
+        if (xt != at::kFloat || gate.defined() || pw.t.defined() || sc.t.defined()) node->in[JoinNode::O] = SavedVariable(orr.t, false);
+        if (xt != at::kFloat) node->in[JoinNode::X] = SavedVariable(xr.t, false);
         if (gate.defined()) node->in[JoinNode::GATE] = SavedVariable(g.t, false);
         node->in[JoinNode::W] = SavedVariable(w.c, false);
         if (pw.c.defined()) node->in[JoinNode::PW] = SavedVariable(pw.c, false);
         if (pb.c.defined()) node->in[JoinNode::PB] = SavedVariable(pb.c, false);
         if (sc.c.defined()) node->in[JoinNode::SC] = SavedVariable(sc.c, false);
         torch::autograd::set_history(std::vector<Tensor>{xs, h}, node);
-        node->xs = SavedVariable(xs, true);
+        if (xt == at::kFloat) node->xs = SavedVariable(xs, true);
     }
     PyObject* r = PyTuple_New(2);
     if (!r) throw python_error();

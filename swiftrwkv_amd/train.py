@@ -167,7 +167,8 @@ def block_join(x: torch.Tensor, o: torch.Tensor, weight: torch.Tensor, bias: Opt
     p = 0 leave their factors out; drop as `dropout` has it.  Returns (x' of x's
     type, h of o's).  Statistics and sums are fp32; h comes from x' before its
     rounding.  The backward pass keeps x' (the result), four numbers a row, and
-    o and gate where they reach a gradient."""
+    o and gate where they reach a gradient; with an x of 16 bits x and o, from
+    which x' is formed again, unrounded."""
     return (_ext or extension()).block_join(x, o, weight, bias, post_weight, post_bias, gate, scale, p, seed, offset, eps,
                                             post_eps)
 

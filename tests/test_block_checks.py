@@ -101,6 +101,7 @@ def test_join_entries_refuse():
     assert bwd(join(), dw=D, wsn=one - 1) == SHAPE and bwd(join(), dw=D, ws=None) == SHAPE and bwd(join(), dw=D, ws=D + 4) == SHAPE
     assert bwd(join(), dg=D) == NULL and bwd(join(), dsc=D) == NULL and bwd(join(), dpw=D) == NULL and bwd(join(), dpb=D) == NULL
     assert bwd(join(o=None, scale=D), dw=D) == NULL and bwd(join(), xs=None, dw=D) == NULL and bwd(join(), st=None) == NULL
+    assert bwd(join(x_dt=1, x=None), dw=D) == NULL and bwd(join(x_dt=1, o=None), dw=D) == NULL and bwd(join(x_dt=1, ldx=7), dw=D) == SHAPE
     assert bwd(join(x_dt=2), dw=D) == DTYPE and bwd(join(ldo=7), dw=D) == SHAPE and bwd(None) == NULL
     assert bwd(join(), st=D + 8) == SHAPE
     assert [_lib.lib().rwkv_join_bwd_workspace(*a) for a in ((-1, 8), (2, 0), (2, 8193))] == [0, 0, 0]

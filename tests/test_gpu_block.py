@@ -265,7 +265,6 @@ def join_inputs(N, D, sdt, dt, wdt, parts, seed=0):
 def join_ref(v, p, dx, dh, N, D, eps=1e-5, post_eps=1e-5):
     """x', h and the gradients with their bounds."""
     t = {n: E(a) for n, a in v.items()}
-    sdt, dt = v["x"].dtype, v["o"].dtype
     row = 64 + 16   # a thread's 8 values, a wave's tree, 16 waves, a few more
     cols = max(1, N // 128) + 48   # a block's rows, the join of the blocks' partial rows
     m = mask_of(N, D, p) if round(65536 * p) else torch.ones(N, D, dtype=torch.bool, device=DEV)
@@ -281,10 +280,7 @@ def join_ref(v, p, dx, dh, N, D, eps=1e-5, post_eps=1e-5):
     xh, r2 = norm(xs, eps, row)
     h = xh * t["weight"]
     h = h + t["bias"] if "bias" in t else h
-    # the backward pass reads x' as stored, the statistics as they were
-    kept_x = xs.rounded(sdt)
-    mean = xs.mean(row)
-    xk = (kept_x - mean) * r2
+    xk = xh
     G = E(dx) if dx is not None else E(torch.zeros(N, D, device=DEV))
     out = {}
     zero = E(torch.zeros(D, device=DEV))
