@@ -441,7 +441,7 @@ struct Slots {
 // three waves a SIMD instead of two, by launch bounds, registers spilled (327 us
 // where two took 197).  With 1024 threads, which have 128 registers each, the
 // column sums lie in LDS instead, and the vectors and rows are read where they
-// are used: 4096 x 8192 213 us.
+// are used: 4096 x 8192 182 us.
 template <typename TS, typename T, int TPR, int ROWS>
 __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
     constexpr int RPB = rows_of(TPR);
@@ -464,6 +464,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
         at.load(rx, a.xs, r, a.ldx);
     };
     auto load_o = [&](int64_t r) {
+        if constexpr (!AHEAD) rdx = filled<TS>(0.0f), ro = filled<T>(0.0f), rg = filled<T>(1.0f);   // (not kept from row to row)
         if (a.dxs) at.load(rdx, a.dxs, r, a.D);
         if (a.o) at.load(ro, a.o, r, a.ldo);
         if (a.gate) at.load(rg, a.gate, r, a.ldg);
@@ -899,13 +900,14 @@ int join_fwd_blocks(int64_t N, int64_t D) {
     const int64_t rpb = join_rows_at_once(D);
     return (int)std::min<int64_t>((N + rpb - 1) / rpb, full);
 }
-// Each block writes one partial row per column sum: from 256 blocks on no more
-// than one for sixteen of its rows (4096 x 2048, all sums: 51 us by 256 blocks, 59
-// by 512; 16384 x 2048: 166 and 159, by 768 172).
+// What the registers hold, each block writing one partial row per column sum; and
+// from 256 blocks on no more than one for four of its rows.  us of the backward
+// pass by 256, 512 and 768 blocks (fp32 stream, bf16, every part): 600 x 2048 18.8,
+// 20.7, 24.7; 2048 x 2048 27.0, 26.4, 33.3; 16384 x 2048 160, 146, 172.
 int join_bwd_blocks(int64_t N, int64_t D) {
     const int64_t full = D <= 512 ? 512 : D <= 1024 ? 1024 : D <= 2048 ? 512 : 256;
     const int64_t blocks = (N + join_rows_at_once(D) - 1) / join_rows_at_once(D);
-    return (int)std::min({blocks, full, std::max<int64_t>(256, blocks / 16)});
+    return (int)std::min({blocks, full, std::max<int64_t>(256, blocks / 4)});
 }
 
 // Lanes across and the grid of the tail's passes.
