@@ -190,6 +190,50 @@ def test_gated_values():
         check(act + " dz", dx[fin, 0], 12 * d[fin], 12 * ((2.0 ** -8 + FUNC * 64) * d.abs() + 2.0 ** -13 * (d.abs() > 0))[fin])
 
 
+@pytest.mark.parametrize("dt,bits", [(BF, (0x7fc0, 0x7fff, -1, -64, 0x7f81)), (HF, (0x7e00, 0x7fff, -1, -512, 0x7c01))])
+def test_gated_nan_of_any_pattern(dt, bits):
+    """A NaN in x reaches the result and both gradients, whatever its bits and
+    sign, on the kernels for few rows and for tiles; other rows stay clean."""
+    case(f"gated: NaN patterns {dt}")
+    for M in (8, 200):
+        for act in GATES:
+            x, w = randn(gen(1), M, 64, dtype=dt), randn(gen(2), 48, 64, dtype=dt, scale=0.1)
+            for i, b in enumerate(bits):
+                x[i].view(torch.int16)[3 + i] = b
+            n = len(bits)
+            assert torch.isnan(x[:n]).any(1).all() and not torch.isnan(x[n:]).any()
+            a, c = x.requires_grad_(True), w.requires_grad_(True)
+            y = train.gated_linear(a, c, act)
+            dx, = torch.autograd.grad(y, a, torch.ones_like(y))
+            assert torch.isnan(y[:n]).all() and torch.isfinite(y[n:]).all()
+            assert torch.isnan(dx[:n]).all() and torch.isfinite(dx[n:]).all()
+
+
+@pytest.mark.parametrize("M,F,K", [(4, 512, 8), (300, 512, 8)])
+def test_kept_pre_activations_are_not_one_sided(M, F, K):
+    """bf16: the mean error of the kept 24 bits.  Values' errors are up to 2^-17
+    of their size either way (half a step of 2^-16), their mean over 2^11 values
+    and more under 2^-17/2^4; cut off they would all lie one way, 2^-17 in the
+    mean.  Seen through dzu = dy·act(zg) with relu², act = z²: twice that."""
+    case(f"kept bits of {M} x {F}")
+    L = _lib.lib()
+    x, w = randn(gen(1), M, K, dtype=BF), randn(gen(2), 2 * F, K, dtype=BF)
+    h, aux = torch.empty(M, F, device=DEV, dtype=BF), torch.empty(M, 2 * F, device=DEV, dtype=BF)
+    rem = torch.empty(M, 2 * F, device=DEV, dtype=torch.int8)
+    n = L.rwkv_gated_fwd_workspace(M, F, K)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=DEV)
+    _lib.check(L.rwkv_gated_fwd(x.data_ptr(), K, w.data_ptr(), K, h.data_ptr(), aux.data_ptr(), rem.data_ptr(), 0, _lib.BF16, M, F, K,
+                                ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    z = x.double() @ w.double().t()
+    bits = aux.float().view(torch.int32) + rem.int() * 256
+    kept = bits.view(torch.float32).double()
+    on = z.abs() > 0.5   # where the fp32 sum's own error, 2^-24·8 of its terms, says nothing
+    rel = ((kept - z) / z)[on]
+    off = 2.0 ** -17 + 2.0 ** -21 * 8 / 0.5
+    print(f"  mean {rel.mean().item() * 2 ** 17:.3f}, most {rel.abs().max().item() * 2 ** 17:.3f} of 2^-17", flush=True)
+    assert rel.abs().max() <= 2 * off and abs(rel.mean().item()) <= 2.0 ** -21
+
+
 def test_gated_in_a_graph():
     case("gated products with their gradients captured, replayed between eager work")
     x, w, dy = randn(gen(1), 40, 512, dtype=BF), randn(gen(2), 256, 512, dtype=BF, scale=0.05), randn(gen(3), 40, 128, dtype=BF)
