@@ -617,6 +617,48 @@ def test_on_another_stream():
     assert torch.equal(d1, d2)
 
 
+def test_two_threads_on_two_streams():
+    """Calls at the same time share nothing: each thread's results and gradients
+    are those of the calls one after the other."""
+    case("the operators from two threads, each on a stream of its own")
+    import threading
+
+    def inputs(k):
+        g = gen(100 + k)
+        D = (640, 1024)[k]
+        return {n: randn(g, 200, D, dtype=F32 if n == "x" else BF) for n in ("x", "o", "gate", "dy")}, torch.ones(D, device=DEV)
+
+    def go(v, w):
+        t = {n: a.detach().requires_grad_(n != "dy") for n, a in v.items()}
+        xs, h = train.block_join(t["x"], t["o"], w, post_weight=w, gate=t["gate"], scale=w, p=0.3, seed=11)
+        y = train.wkv_tail(xs, h, t["o"], t["gate"], w, t["o"], w, w)
+        z = train.dropout(y, 0.2, 12, residual=t["o"])
+        return [z.detach(), *torch.autograd.grad(z, [t["x"], t["o"], t["gate"]], v["dy"])]
+
+    data = [inputs(k) for k in range(2)]
+    want = [go(*d) for d in data]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[k] = go(*data[k])
+                    assert all(torch.equal(a, b) for a, b in zip(got[k], want[k])), k
+            s.synchronize()
+        except Exception as e:   # of the thread, told below
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not failed and all(g is not None for g in got), failed
+
+
 def test_second_and_forward_derivatives_are_refused():
     case("derivatives of derivatives, tangents of gradients")
     x, w = randn(gen(1), 4, 64).requires_grad_(True), torch.ones(64, device=DEV)
