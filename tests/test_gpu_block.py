@@ -566,6 +566,37 @@ def test_tail_layouts_and_needs():
         assert torch.equal(one, want), n
 
 
+# ───────────────────────────── many values ─────────────────────────────
+
+def test_join_and_tail_past_2_31_values():
+    """A row's results depend on no other row: the last rows of more than 2^31
+    values are those of a call on them alone (bitwise; nothing dropped)."""
+    N, D, n = 530000, 4096, 37   # 2.2e9 values
+    case(f"join {N} x {D}")
+    x = randn(gen(1), 1, D, dtype=BF).expand(N, D).contiguous()
+    o, w = x.clone(), ones(gen(2), D, F32)
+    x[-n:], o[-n:] = randn(gen(3), n, D), randn(gen(4), n, D)
+    x[0] = 7.0
+    def join(a, b):
+        la, lb = a.requires_grad_(True), b.requires_grad_(True)
+        xs, h = train.block_join(la, lb, w, post_weight=w, scale=w)
+        return (xs.detach(), h.detach(), *torch.autograd.grad((xs, h), (la, lb), (b.detach(), a.detach())))
+    big = join(x, o)
+    small = join(x.detach()[-n:].clone(), o.detach()[-n:].clone())
+    assert all(torch.equal(p[-n:], q) for p, q in zip(big, small))
+    del big
+    case(f"tail {N} x {D // 64} heads")
+    def tail(a, b):
+        la, lb = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        y = train.wkv_tail(la, lb, la, lb, w, la, w, w)
+        return (y.detach(), *torch.autograd.grad(y, (la, lb), b.detach()))
+    big = tail(x, o)
+    small = tail(x[-n:].clone(), o[-n:].clone())
+    assert all(torch.equal(p[-n:], q) for p, q in zip(big, small))
+    del big, x, o
+    torch.cuda.empty_cache()
+
+
 # ───────────────────────────── graphs, streams, derivatives ─────────────────────────────
 
 def test_tail_and_join_in_a_graph():

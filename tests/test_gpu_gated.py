@@ -135,6 +135,31 @@ def test_gated_is_two_products(M, F, K):
     assert torch.equal(y, (x[:, at[:F]].float().clamp(min=0) ** 2 * x[:, at[F:]].float()).to(HF))
 
 
+def test_gated_past_2_31_values():
+    """More than 2^31 pre-activations: small integers and W's rows of a single
+    one, so that every value of the last rows is exact."""
+    M, F, K, n = 76000, 14336, 64, 40
+    case(f"gated {M} x {F} x {K}")
+    x = torch.randint(-8, 9, (M, K), generator=gen(1), device=DEV).to(HF)
+    at = torch.randint(0, K, (2 * F,), generator=gen(2), device=DEV)
+    w = torch.zeros(2 * F, K, device=DEV, dtype=HF)
+    w[torch.arange(2 * F, device=DEV), at] = 1.0
+    a = x.detach().requires_grad_(True)
+    y = train.gated_linear(a, w, "relu2")
+    dy = torch.zeros(M, F, device=DEV, dtype=HF)
+    dy[-n:, 0], dy[-n:, F - 1], dy[-n:, F // 2 + 1] = 1.0, -2.0, 1.0
+    dx, = torch.autograd.grad(y, a, dy)
+    zg, zu = x[-n:, at[:F]].float(), x[-n:, at[F:]].float()
+    r = zg.clamp(min=0)
+    assert torch.equal(y[-n:], (r * r * zu).to(HF))
+    d = dy[-n:].float()
+    dz = torch.cat([d * zu * 2 * r, d * r * r], 1)
+    want = torch.zeros(n, K, device=DEV).index_add_(1, at, dz)
+    assert torch.equal(dx[-n:], want.to(HF)) and not dx[:-n].any()
+    del x, y, dy, dx, a
+    torch.cuda.empty_cache()
+
+
 def test_gated_layouts():
     case("gated: views, one row, several axes, far rows, expanded dy")
     g = gen(5)
