@@ -234,13 +234,19 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // stream would have the engine make the one wait for the other, which the
 // capture does not survive, nor the process.
 void capture_ok(const char* what, const Node& node, c10::Device dev) {
-    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index());
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    using Stream = c10::hip::HIPStreamMasqueradingAsCUDA;
+    const auto captured = [](const Stream& s) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        return hipStreamIsCapturing(s.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+    };
+    const Stream stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index());
+    if (!captured(stream)) return;
     for (const torch::autograd::Edge& e : node.next_edges()) {
         if (!e.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
         const std::optional<c10::Stream> leaf = e.function->stream();
-        TORCH_CHECK(!leaf || *leaf == stream.unwrap(), what,
+        if (!leaf || *leaf == stream.unwrap()) continue;
+        const Stream other(*leaf);   // (the default stream is not asked: that is an error while another is captured)
+        TORCH_CHECK(other.stream() && captured(other), what,
                     ": its captured backward pass reaches a leaf that an eager graph on another stream still holds; "
                     "free that graph, or capture with leaves of their own");
     }
