@@ -566,6 +566,24 @@ def test_tail_layouts_and_needs():
         assert torch.equal(one, want), n
 
 
+@pytest.mark.parametrize("N,H", [(1, 1), (5, 3), (37, 12), (3, 65)])
+def test_tail_writes_its_rows_alone(N, H):
+    case(f"tail {N} x {H} heads into the middle of buffers")
+    L, s, C = _lib.lib(), torch.cuda.current_stream().cuda_stream, 64 * H
+    o, r = randn(gen(1), N, C), randn(gen(2), N, C, dtype=BF)
+    w = torch.ones(C, device=DEV)
+    j = _lib.Tail(o=o.data_ptr(), r=r.data_ptr(), k=r.data_ptr(), v=r.data_ptr(), gate=r.data_ptr(), ldo=C, ldr=C, ldk=C, ldv=C, ldg=C,
+                  o_dt=_lib.F32, dt=_lib.BF16, w_dt=_lib.F32, r_k=w.data_ptr(), weight=w.data_ptr(), bias=w.data_ptr(), eps=64e-5, N=N, H=H)
+    put = lambda n, dt: torch.full((n + 64,), 7.0, device=DEV, dtype=dt)  # noqa: E731
+    at = lambda t: t[32:].data_ptr()  # noqa: E731
+    outs = [put(N * C, BF), put(N * C, F32), *(put(N * C, BF) for _ in range(4)), *(put(C, F32) for _ in range(3))]
+    ws = torch.empty(L.rwkv_tail_bwd_workspace(N, H), dtype=torch.uint8, device=DEV)
+    _lib.check(L.rwkv_tail_fwd(ctypes.byref(j), at(outs[0]), s))
+    _lib.check(L.rwkv_tail_bwd(ctypes.byref(j), r.data_ptr(), C, *(at(t) for t in outs[1:]), ws.data_ptr(), ws.numel(), s))
+    for t in outs:
+        assert (t[:32] == 7).all() and (t[-32:] == 7).all() and not (t[32:-32] == 7).all()
+
+
 # ───────────────────────────── many values ─────────────────────────────
 
 def test_join_and_tail_past_2_31_values():

@@ -160,6 +160,25 @@ def test_gated_past_2_31_values():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("M,F,K", [(1, 1, 1), (3, 5, 8), (16, 33, 40), (16, 4099, 64), (40, 100, 64), (130, 70, 72), (300, 1001, 600), (1030, 2055, 136),
+                                   (50, 60, 4096), (700, 1500, 2048)])
+def test_gated_writes_its_rows_alone(M, F, K):
+    """The result, both kept pre-activations and dz, into the middle of buffers."""
+    case(f"gated {M} x {F} x {K} into the middle of buffers")
+    L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    x, w, dy = randn(gen(1), M, K, dtype=BF), randn(gen(2), 2 * F, K, dtype=BF, scale=K ** -0.5), randn(gen(3), M, F, dtype=BF)
+    ldz = (2 * F + 7) // 8 * 8
+    put = lambda n, dt: torch.full((n + 128,), 7, device=DEV, dtype=dt)  # noqa: E731
+    h, aux, rem, dz = put(M * F, BF), put(2 * M * F, BF), put(2 * M * F, torch.uint8), put(M * ldz, BF)
+    ws = torch.empty(max(L.rwkv_gated_fwd_workspace(M, F, K), 16), dtype=torch.uint8, device=DEV)
+    at = lambda t: t[64:].data_ptr()  # noqa: E731
+    _lib.check(L.rwkv_gated_fwd(x.data_ptr(), K, w.data_ptr(), K, at(h), at(aux), at(rem), 2, _lib.BF16, M, F, K, ws.data_ptr(), ws.numel(), s))
+    _lib.check(L.rwkv_gated_dact(dy.data_ptr(), F, at(aux), at(rem), 2, at(dz), ldz, _lib.BF16, M, F, s))
+    for t in (h, aux, rem, dz):
+        assert (t[:64] == 7).all() and (t[-64:] == 7).all()
+    assert torch.equal(h[64:-64].reshape(M, F), train.gated_linear(x, w))
+
+
 def test_gated_layouts():
     case("gated: views, one row, several axes, far rows, expanded dy")
     g = gen(5)
