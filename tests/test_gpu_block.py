@@ -344,6 +344,14 @@ def test_join_widths(N, D):
     run_join(N, D, parts="bpgs" if D > 2 else "gs")   # a norm of one or two values says nothing
 
 
+@pytest.mark.parametrize("sdt,dt", [(BF, BF), (HF, HF), (F32, HF)])
+@pytest.mark.parametrize("N,D", [(4, 5), (2, 31), (70, 64), (9, 512), (7, 513), (6, 1025), (4, 2048), (3, 2049), (4, 4096), (3, 4097), (2, 8191),
+                                 (2, 8192), (300, 256), (5000, 33), (1030, 1024)])
+def test_join_widths_of_16_bit_types(N, D, sdt, dt):
+    case(f"join width {N} x {D} stream {sdt}, {dt}")
+    run_join(N, D, sdt, dt, dt)
+
+
 @pytest.mark.parametrize("parts", ["", "b", "p", "pb", "g", "s", "pg", "ps", "gs", "pgs"])
 @pytest.mark.parametrize("p", [0.0, 0.6])
 def test_join_parts(parts, p):

@@ -114,7 +114,8 @@ def test_gates(M, F, K, act, dt):
                                    (130, 2050, 4099), (700, 3001, 2001), (256, 64, 16384), (2500, 6000, 1024),
                                    (16, 2100, 4096), (16, 2100, 4104), (13, 2200, 5000), (9, 2100, 7280), (5, 2100, 13100), (1, 2064, 32768),
                                    (1, 2050, 65530), (2, 64, 16384), (7, 4100, 513), (16, 4200, 512), (3, 9000, 40), (12, 8200, 1027),
-                                   (4, 6000, 2040)])
+                                   (4, 6000, 2040), (200, 300, 8192), (1000, 1200, 8192), (700, 6000, 4096), (700, 3000, 8192), (1500, 6000, 4096),
+                                   (100, 1200, 4097), (1500, 3000, 1003)])
 def test_gated_routes(M, F, K):
     case(f"gated {M} x {F} x {K}")
     a = run(M, F, K, BF, "silu")
@@ -122,7 +123,8 @@ def test_gated_routes(M, F, K):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
-@pytest.mark.parametrize("M,F,K", [(20, 48, 64), (140, 520, 256), (600, 640, 512), (4096, 2048, 512)])
+@pytest.mark.parametrize("M,F,K", [(20, 48, 64), (140, 520, 256), (600, 640, 512), (4096, 2048, 512), (200, 300, 8192), (1000, 1200, 8192),
+                                   (700, 6000, 4096), (700, 3000, 8192), (1500, 6000, 4096), (100, 1200, 4097), (1500, 3000, 1003)])
 def test_gated_is_two_products(M, F, K):
     """Both halves of W where they belong, whatever the tile: W's rows one at a
     time are zero but for one column, so each z is one value of x."""
