@@ -448,9 +448,10 @@ typedef enum { RWKV_GATE_RELU2 = 0, RWKV_GATE_SIGMOID = 1, RWKV_GATE_SILU = 2, R
 
 /* h = act(zg)·zu [M, F], [zg | zu] = x·Wᵀ: x [M, K], w [2F, K] (the gate's F
  * rows, then the other factor's) and h of dt (bf16 or f16).  fp32 sums, one rounding, ties to
- * even.  For the backward pass, both or neither: aux [M, 2F] of dt receives
- * zg and zu, rem [M, 2F] their next 8 bits.  F <= 2^19, K <= 2^20.  Workspace
- * as rwkv_linear_fwd's. */
+ * even.  For the backward pass, both or neither: aux [M, 2F], 16 bits each
+ * whatever dt is, and rem [M, 2F] receive the upper 24 bits of zg and zu as fp32,
+ * rounded to nearest: aux·2^16 + rem·2^8 (rem signed) is the pattern.  F <= 2^19,
+ * K <= 2^20.  Workspace as rwkv_linear_fwd's. */
 int64_t rwkv_gated_fwd_workspace(int64_t M, int64_t F, int64_t K);
 rwkv_status rwkv_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* h, void* aux, uint8_t* rem,
                            rwkv_gate act, rwkv_dtype dt, int64_t M, int64_t F, int64_t K, void* workspace,

@@ -335,28 +335,26 @@ __device__ __forceinline__ void gate_slope8(int act, const float (&z)[8], float 
     }
 }
 
-// What is kept of eight pre-activations, as round8 and rem8 lay it out.  bf16: the
-// pattern's upper 24 bits, rounded to nearest (ties to even: sums of a few
-// products end in halves of a step often), are those 16 whose signed remainder the
-// next 8 are, without a clamp.  (bf16 operands' NaN have no low bits that could
-// carry beyond the exponent.)
-template <typename T>
+// What is kept of eight pre-activations for the backward pass: the upper 24 bits of
+// their fp32 patterns, rounded to nearest (ties to even: sums of a few products end
+// in halves of a step often), as the 16 bits whose signed remainder the next 8 are,
+// without a clamp.  For fp16 operands too: z outgrows that type (65504) where
+// act(zg)·zu and its gradients do not, and an infinity kept in its place makes them
+// infinities and NaN; 16 significant bits are still 5 more than dz keeps.  (A z
+// within 2^-17 of fp32's largest becomes an infinity.  16-bit operands' NaN have no
+// low bits that could carry beyond the exponent, and one that carries out of the 16
+// bits comes back with its remainder.)
 __device__ __forceinline__ void keep8(const float (&v)[8], uint4& a, uint2& rem) {
-    if constexpr (__is_same(T, bf16)) {
-        uint32_t q[8], w[4];
+    uint32_t q[8], w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __builtin_bit_cast(uint32_t, v[i]) + (__builtin_bit_cast(uint32_t, v[i]) >> 8 & 1u) + 0x7fu;
+    for (int i = 0; i < 8; ++i) q[i] = __builtin_bit_cast(uint32_t, v[i]) + (__builtin_bit_cast(uint32_t, v[i]) >> 8 & 1u) + 0x7fu;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(q[2 * i + 1] + 0x8000u, q[2 * i] + 0x8000u, 0x07060302u);
-        a = make_uint4(w[0], w[1], w[2], w[3]);
-        auto second = [&](int i) {   // second bytes of four
-            return __builtin_amdgcn_perm(q[i + 1], q[i], 0x0c0c0501u) | __builtin_amdgcn_perm(q[i + 3], q[i + 2], 0x05010c0cu);
-        };
-        rem = make_uint2(second(0), second(4));
-    } else {
-        a = round8<T>(v);
-        rem = rem8<T>(v, a);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(q[2 * i + 1] + 0x8000u, q[2 * i] + 0x8000u, 0x07060302u);
+    a = make_uint4(w[0], w[1], w[2], w[3]);
+    auto second = [&](int i) {   // second bytes of four
+        return __builtin_amdgcn_perm(q[i + 1], q[i], 0x0c0c0501u) | __builtin_amdgcn_perm(q[i + 3], q[i + 2], 0x05010c0cu);
+    };
+    rem = make_uint2(second(0), second(4));
 }
 
 // Eight neighbouring columns of h = act(zg)·zu in each of C rows row, row +
@@ -372,12 +370,12 @@ __device__ __forceinline__ void finish_gated(const Epilogue& e, int64_t row, int
         for (int c = 0; c < C; ++c) {
             uint4 g, u;
             uint2 gr, ur;
-            keep8<T>(zg[c], g, gr);
-            keep8<T>(zu[c], u, ur);
+            keep8(zg[c], g, gr);
+            keep8(zu[c], u, ur);
             if (row + c * step >= e.M) continue;
             const int64_t at = from + (row + 2 * c * step) * e.N;
-            store_raw(reinterpret_cast<T*>(e.aux) + at, valid, g);
-            store_raw(reinterpret_cast<T*>(e.aux) + at + e.N, valid, u);
+            store_raw(reinterpret_cast<uint16_t*>(e.aux) + at, valid, g);
+            store_raw(reinterpret_cast<uint16_t*>(e.aux) + at + e.N, valid, u);
             store_raw(e.rem + at, valid, gr);
             store_raw(e.rem + at + e.N, valid, ur);
         }
@@ -1380,7 +1378,7 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a, int TX) {
 struct GatedArgs {
     const void* dy;         // [M, lddy]
     int64_t lddy;
-    const void* kept;       // [M, 2F]: zg, zu
+    const void* kept;       // [M, 2F]: zg, zu, the upper 16 bits of 24
     const uint8_t* rem;     // [M, 2F]: their next 8 bits
     int act;
     void* dz;               // [M, ldz], ldz >= 2F; columns from 2F on are written as zeros
@@ -1408,10 +1406,10 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(GatedArgs a, int TX) {
         for (int k = 0; k < U; ++k) {
             const int64_t row = min(first + k * step, a.M - 1), at = row * 2 * a.F + col;
             load8(reinterpret_cast<const T*>(a.dy) + row * a.lddy + col, valid, d[k]);
-            load8(reinterpret_cast<const T*>(a.kept) + at, valid, g[k]);
-            load8(reinterpret_cast<const T*>(a.kept) + at + a.F, valid, u[k]);
-            load_rem8<T>(a.rem + at, valid, g[k]);
-            load_rem8<T>(a.rem + at + a.F, valid, u[k]);
+            load8(reinterpret_cast<const bf16*>(a.kept) + at, valid, g[k]);   // (upper halves of fp32, whatever T is)
+            load8(reinterpret_cast<const bf16*>(a.kept) + at + a.F, valid, u[k]);
+            load_rem8<bf16>(a.rem + at, valid, g[k]);
+            load_rem8<bf16>(a.rem + at + a.F, valid, u[k]);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {

@@ -607,7 +607,8 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ───────────────────────────── gated products ─────────────────────────────
 
-// Keeps x, W, and both pre-activations in 24 bits.
+// Keeps x, W, and both pre-activations in 24 bits: kept's 16 are no values of
+// its type but the upper half of fp32's.
 struct GatedNode : Node {
     SavedVariable x, w, kept, rem;
     std::vector<int64_t> x_shape, y_shape;

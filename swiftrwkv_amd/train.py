@@ -123,8 +123,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, activation: str = "silu"
     "gelu_tanh" (the gelu's tanh form), "sigmoid" or "relu2".  Products
     accumulate in fp32 and the result is rounded once; of a backward pass's two
     products the gradients of both factors are rounded to x's type.  For it 6
-    bytes per value of the result are kept (both pre-activations to 16 or 18
-    significant bits).  With no gradient needed nothing is kept.  Rows that are
+    bytes per value of the result are kept (both pre-activations to 16
+    significant bits, with fp32's range).  With no gradient needed nothing is kept.  Rows that are
     not whole 16-byte chunks are copied as linear does."""
     return (_ext or extension()).gated_linear(x, weight, activation)
 

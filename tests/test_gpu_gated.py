@@ -334,3 +334,82 @@ def test_padding_columns_of_gated_dz_are_zeros(F):
                                               torch.cuda.current_stream().cuda_stream))
         assert not dz[:M, 2 * F:].any() and torch.isnan(dz[M]).all(), ldz
         assert ((dz[:M, :2 * F].double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs()).all(), ldz
+
+
+@pytest.mark.parametrize("M", [1, 16, 200])
+@pytest.mark.parametrize("act", GATES)
+def test_pre_activations_past_the_type(act, M):
+    """fp16: pre-activations of 98304 (the type ends at 65504) under a gate that
+    leaves the result and both gradients inside it; the other rows are zeros.
+    Every z has a few bits, so what is kept of it is exact; from |zg| = 100 on
+    act and its slope are 0, 1 or powers of z.  dz is rounded once."""
+    case(f"gated: large pre-activations {act}, {M} rows")
+    K, F, big = 8, 12, 98304.0
+    x, w = torch.zeros(M, K, device=DEV, dtype=HF), torch.zeros(2 * F, K, device=DEV, dtype=HF)
+    w[:F, 0], w[F:, 1] = 2.0, 2.0
+    dy = torch.zeros(M, F, device=DEV, dtype=HF)
+    dy[0] = 2.0 ** -6
+    seen = 0
+    for g, u in ((-2.0, big), (-20.0, big), (-20.0, -big), (0.0, big), (0.0, -big), (-big, 2.0), (-big, big), (-big, -big), (big, 2.0 ** -7), (big, 0.0)):
+        x[0, 0], x[0, 1] = g / 2, u / 2
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = train.gated_linear(a, b, act)
+        dx, dw = torch.autograd.grad(y, (a, b), dy)
+        z = torch.tensor(g, dtype=torch.float64)
+        v, d, _ = act64(act, z)
+        far = abs(g) > 100
+        ev, ed = (E24 * v.abs(), E24 * d.abs()) if far else (act_off(act, z, 0.0), slope_off(act, z, 0.0))
+        half = 2.0 ** -11
+        dz = [t.item() for t in (2.0 ** -6 * u * d, 2.0 ** -6 * v)]
+        off = [t.item() for t in (2.0 ** -6 * abs(u) * ed, 2.0 ** -6 * ev)]
+        off = [half * (abs(t) + o) + o + TINY[HF] for t, o in zip(dz, off)]
+        row = lambda t: torch.tensor(t, dtype=torch.float64, device=DEV)  # noqa: E731
+        if abs(u * v) < 6e4:
+            check(f"{g} {u} y", y.detach()[0, :1], row([u * v.item()]), row([abs(u) * ev.item()]))
+        for k in range(2):
+            # An infinity by right: of dx, or of the other factor's dz, which is rounded to
+            # fp16 too (relu², zg = 98304: dzu = 2^-6·98304² = 1.5e8) and meets W's zeros in dx.
+            if abs(24 * dz[k]) >= 6e4 or abs(dz[1 - k]) >= 6e4:
+                continue
+            seen += 1
+            check(f"{g} {u} dx{k}", dx[0, k:k + 1], row([24 * dz[k]]), row([24 * off[k]]))
+            rows, other = dw[k * F:(k + 1) * F], 1 - k
+            for c, at in ((k, (g, u)[k] / 2), (other, (g, u)[other] / 2)):
+                if abs(dz[k] * at) < 6e4:
+                    check(f"{g} {u} dw{k}{c}", rows[:, c], row([dz[k] * at] * F), row([off[k] * abs(at)] * F))
+            assert not rows[:, 2:].any() and not dx[1:].any()
+    assert seen >= 14
+
+
+def test_what_is_kept_of_fp16_pre_activations():
+    """The upper 24 bits of the fp32 value, rounded to nearest: within 2^-16 of
+    it (half a step of 2^-15), past fp16's range as inside it; both kernels."""
+    case("kept bits of fp16")
+    L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for M, F, K in ((4, 512, 8), (300, 512, 8), (200, 300, 8192)):
+        x, w = randn(gen(1), M, K, dtype=HF, scale=400.0), randn(gen(2), 2 * F, K, dtype=HF, scale=400.0 * K ** -0.5)
+        h, aux = torch.empty(M, F, device=DEV, dtype=HF), torch.empty(M, 2 * F, device=DEV, dtype=torch.int16)
+        rem = torch.empty(M, 2 * F, device=DEV, dtype=torch.int8)
+        ws = torch.empty(max(L.rwkv_gated_fwd_workspace(M, F, K), 16), dtype=torch.uint8, device=DEV)
+        _lib.check(L.rwkv_gated_fwd(x.data_ptr(), K, w.data_ptr(), K, h.data_ptr(), aux.data_ptr(), rem.data_ptr(), 1, _lib.F16, M, F, K,
+                                    ws.data_ptr(), ws.numel(), s))
+        kept = (aux.int() * 65536 + rem.int() * 256).view(torch.float32).double()
+        z, ez = x.double() @ w.double().t(), E24 * (K + 32) * (x.double().abs() @ w.double().abs().t())
+        assert (z.abs() > 65520).float().mean() > 0.2
+        w_ = ((kept - z).abs() / (2.0 ** -16 * (z.abs() + ez) + ez)).nan_to_num(nan=float("inf")).max().item()
+        print(f"  {M} x {F} x {K}: worst error {w_:.3f} of its bound", flush=True)
+        assert w_ <= 1.0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_gates_far_below_zero_pass_nothing(act):
+    """act(z) = z·σ(..) of a z far below zero is under 2^-100 however large z is:
+    dzu = dy·act(zg) and with it dx are zeros."""
+    case(f"gated: {act} far below zero")
+    for z in (-101.0, -2.0 ** 60, -2.0 ** 126):
+        x, w = torch.zeros(2, 8, device=DEV, dtype=BF), torch.zeros(2, 8, device=DEV, dtype=BF)
+        x[:, 0], w[0, 0], x[:, 1], w[1, 1] = z, 1.0, 1.0, 1.0
+        a = x.requires_grad_(True)
+        y = train.gated_linear(a, w, act)
+        dx, = torch.autograd.grad(y, a, torch.ones_like(y))
+        assert (y.double().abs() <= 2.0 ** -100).all() and (dx.double().abs() <= 2.0 ** -100).all(), (z, y, dx)
