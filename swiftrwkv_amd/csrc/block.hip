@@ -587,6 +587,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
                 u[i] = dropped(m[i], u[i]);   // m of G, for the sum
                 nv[i] = dropped(m[i], nv[i]);
                 y[i] = dropped(m[i], y[i]);
+                G[i] = m[i] > 0.0f ? G[i] : 0.0f;   // (zeros times an infinity are none)
             }
         }
         if constexpr (!AGAIN) vector(SC, sc);

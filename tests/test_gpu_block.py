@@ -753,3 +753,43 @@ def test_gradients_against_differences():
     better = (4 * d2 - d1) / 3   # the step's square cancels
     print(f"  {want:.4f}, differences {d1:.4f} {d2:.4f}", flush=True)
     assert abs(better - want) <= 2.0 ** -4 + abs(d2 - d1) / 2 + 2.0 ** -10 * abs(want)
+
+
+# ───────────────────────────── values that leave their range ─────────────────────────────
+
+@pytest.mark.parametrize("parts", ["", "g", "s", "p", "bpgs"])
+@pytest.mark.parametrize("sdt,dt", [(F32, F32), (F32, BF), (BF, BF)])
+@pytest.mark.parametrize("N,D", [(6, 7), (9, 96), (5, 601), (3, 5000)])
+def test_join_dropped_places_pass_no_gradient(N, D, sdt, dt, parts):
+    """What the gradient of x' holds at dropped places, an infinity or a NaN too,
+    reaches dx there and nothing else: the bits of a call with zeros there."""
+    case(f"join {N} x {D} {sdt} {dt} '{parts}': bad gradients at dropped places")
+    v, dx, dh = join_inputs(N, D, sdt, dt, F32, parts)
+    m = mask_of(N, D, 0.4)
+    assert not m.all()
+    bad = torch.where(m, dx, torch.tensor([float("inf"), float("nan"), -float("inf")], device=DEV).repeat(D)[:D].to(sdt))
+    leaves = {n: a.detach().clone().requires_grad_(True) for n, a in v.items()}
+    xs, h = call_join(leaves, 0.4)
+    want = torch.autograd.grad((xs, h), list(leaves.values()), (dx.masked_fill(~m, 0), dh), retain_graph=True)
+    got = torch.autograd.grad((xs, h), list(leaves.values()), (bad, dh))
+    for n, a, b in zip(leaves, got, want):
+        if n == "x":
+            assert not torch.isfinite(a[~m]).any() and torch.equal(a[m], b[m])
+        else:
+            assert torch.isfinite(b).all() and torch.equal(a, b), n
+
+
+def test_join_dropped_places_of_a_bad_row():
+    case("join: a NaN in dh and o, nothing of it at dropped places")
+    for sdt in (F32, BF):
+        v, dx, dh = join_inputs(4, 300, sdt, BF, F32, "gs")
+        m = mask_of(4, 300, 0.4)
+        dh[1, 5] = float("nan")
+        v["gate"][2], v["o"][3] = v["gate"][2].masked_fill(~m[2], float("inf")), v["o"][3].masked_fill(~m[3], float("nan"))
+        leaves = {n: a.detach().requires_grad_(True) for n, a in v.items()}
+        xs, h = call_join(leaves, 0.4)
+        assert torch.isfinite(xs).all() and torch.isfinite(h).all()
+        g = dict(zip(leaves, torch.autograd.grad((xs, h), list(leaves.values()), (dx, dh))))
+        assert torch.isnan(g["x"][1]).all() and torch.isfinite(g["x"][[0, 2, 3]]).all()
+        for n in ("o", "gate"):
+            assert not g[n][~m].any() and torch.isnan(g[n][1][m[1]]).all() and torch.isfinite(g[n][[0, 2, 3]]).all(), n
