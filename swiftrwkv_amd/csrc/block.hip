@@ -77,6 +77,14 @@ __device__ __forceinline__ void factors(const Drop& d, uint64_t key, uint32_t c,
 // A dropped value is zero whatever it was, an infinity or a NaN too.
 __device__ __forceinline__ float dropped(float m, float v) { return m > 0.0f ? m * v : 0.0f; }
 
+// 1/sqrt of a variance, to one step of fp32.  The hardware's takes a subnormal for
+// zero (rows under 2^-63 with an eps of 0): those go in 2^64 times as large.
+__device__ __forceinline__ float rstd_of(float x) {
+    const bool small = x < 0x1p-126f;
+    const float r = __builtin_amdgcn_rsqf(small ? x * 0x1p64f : x);
+    return small ? r * 0x1p32f : r;
+}
+
 // ───────────────────────────── chunks ─────────────────────────────
 
 // How a row of D columns falls into chunks of eight: WHOLE, D is a multiple of 8;
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_fwd_kernel(JoinFwd a) {
                 u[i] -= st.x;
                 q += c.has(i) ? u[i] * u[i] : 0.0f;
             }
-            st.y = __builtin_amdgcn_rsqf(row_sum<TPR>(c.own(q), part, 1) * per + a.post_eps);
+            st.y = rstd_of(row_sum<TPR>(c.own(q), part, 1) * per + a.post_eps);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = (u[i] * st.y * pw[i] + pb[i]) * g[i];
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void join_fwd_kernel(JoinFwd a) {
             v[i] -= st.z;
             q += c.has(i) ? v[i] * v[i] : 0.0f;
         }
-        st.w = __builtin_amdgcn_rsqf(row_sum<TPR>(c.own(q), part, 1) * per + a.eps);
+        st.w = rstd_of(row_sum<TPR>(c.own(q), part, 1) * per + a.eps);
         if (a.stats && t == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = st;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * st.w * w[i] + b[i];
@@ -742,7 +750,7 @@ __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
             o[i] -= mean;
             q += o[i] * o[i];
         }
-        const float inv = __builtin_amdgcn_rsqf(sum8(q) * (1.0f / HEAD) + a.eps);
+        const float inv = rstd_of(sum8(q) * (1.0f / HEAD) + a.eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (o[i] * inv * w[i] + b[i] + d * v[i]) * g[i];
         store8(reinterpret_cast<T*>(a.y) + row * a.C + col, 8, o);
@@ -789,7 +797,7 @@ __global__ __launch_bounds__(256) void tail_bwd_kernel(TailArgs a, int TX) {
                 o[i] -= mean;
                 q += o[i] * o[i];
             }
-            const float inv = __builtin_amdgcn_rsqf(sum8(q) * (1.0f / HEAD) + a.eps);
+            const float inv = rstd_of(sum8(q) * (1.0f / HEAD) + a.eps);
             float m1 = 0.0f, m2 = 0.0f, t[8];
             const int64_t at = row * a.C + col;
             // o: oh; g: dq; t: dg

@@ -793,3 +793,29 @@ def test_join_dropped_places_of_a_bad_row():
         assert torch.isnan(g["x"][1]).all() and torch.isfinite(g["x"][[0, 2, 3]]).all()
         for n in ("o", "gate"):
             assert not g[n][~m].any() and torch.isnan(g[n][1][m[1]]).all() and torch.isfinite(g[n][[0, 2, 3]]).all(), n
+
+
+def test_rows_of_tiny_values():
+    """eps = 0 and rows around 2^-66, whose variance is subnormal in fp32: what
+    the layer norm makes of them.  The variance, 1024 squares around 2^-132 in
+    steps of 2^-149 each off by up to half of one, is right to 2^-17 and its
+    root's inverse to 2^-18; sums and products are far below that."""
+    case("join and tail: rows around 2^-66 without eps")
+    x = randn(gen(1), 5, 1024, scale=2.0 ** -66)
+    w, b = ones(gen(2), 1024, F32), randn(gen(3), 1024)
+    _, h = train.block_join(x, torch.zeros_like(x), w, b, eps=0.0)
+    _, n = train.block_join(torch.zeros_like(x), x, w, b, post_weight=w, post_bias=b, post_eps=0.0)
+    xs, _ = train.block_join(torch.zeros_like(x), x, w, b, post_weight=w, post_bias=b, post_eps=0.0)
+    X, W, B = x.double(), w.double(), b.double()
+    xh = (X - X.mean(-1, keepdim=True)) / X.var(-1, correction=0, keepdim=True).sqrt()
+    ref = xh * W + B
+    off = 2.0 ** -17 * (xh * W).abs() + 2.0 ** -22 * ref.abs()
+    assert torch.isfinite(n).all()
+    for t in (h, xs, train.layer_norm(x, w, b, 0.0)):
+        assert ((t.double() - ref).abs() <= off).all()
+    one, zero = torch.ones(1024, device=DEV), torch.zeros(1024, device=DEV)
+    y = train.wkv_tail(x, zero.expand_as(x), zero.expand_as(x), zero.expand_as(x), zero, one.expand_as(x), w, b, eps=0.0)
+    X = X.reshape(5, 16, 64)
+    xh = ((X - X.mean(-1, keepdim=True)) / X.var(-1, correction=0, keepdim=True).sqrt()).reshape(5, 1024)
+    # 64 squares of a head: right to 2^-15, were they all at the mean's size; a head's largest row of errors is half a step each
+    assert ((y.double() - xh * W - B).abs() <= 2.0 ** -15 * (xh * W).abs() + 2.0 ** -22 * (xh * W + B).abs()).all()
