@@ -232,21 +232,25 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // A leaf's gradient belongs to the stream under which its node came to be.  If
 // an eager graph still holds that node, a captured backward pass on another
 // stream would have the engine make the one wait for the other, which the
-// capture does not survive, nor the process.
+// capture does not survive, nor the process.  Looked at are the leaves next to a
+// node, those alone that the pass goes to.
 void capture_ok(const char* what, const Node& node, c10::Device dev) {
     using Stream = c10::hip::HIPStreamMasqueradingAsCUDA;
     const auto captured = [](const Stream& s) {
+        if (!s.stream()) return false;   // (the default stream never is; to ask it while another is captured is an error)
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
         return hipStreamIsCapturing(s.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
     };
     const Stream stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index());
     if (!captured(stream)) return;
-    for (const torch::autograd::Edge& e : node.next_edges()) {
-        if (!e.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
+    const torch::autograd::edge_list& edges = node.next_edges();
+    for (size_t i = 0; i < edges.size(); ++i) {
+        const torch::autograd::Edge& e = edges[i];
+        if (!e.function || !node.task_should_compute_output(i)) continue;
+        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
         const std::optional<c10::Stream> leaf = e.function->stream();
         if (!leaf || *leaf == stream.unwrap()) continue;
-        const Stream other(*leaf);   // (the default stream is not asked: that is an error while another is captured)
-        TORCH_CHECK(other.stream() && captured(other), what,
+        TORCH_CHECK(captured(Stream(*leaf)), what,
                     ": its captured backward pass reaches a leaf that an eager graph on another stream still holds; "
                     "free that graph, or capture with leaves of their own");
     }
@@ -296,8 +300,8 @@ struct NormNode : Node {
         const auto self = shared_from_this();
         const Tensor st = stats.unpack(self), wt = w.unpack(self), xt = x.unpack(self), ct = codes.unpack(self),
                      sc = scales.unpack(self);
-        const Guard guard(st.device());
         const auto dev = st.device();
+        const Guard guard(dev);
         Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(shape, st.options().dtype(y_dt));
         const Rows dy = rows_of(dyt, true);
         int64_t ld = D;

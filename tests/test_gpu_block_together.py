@@ -150,3 +150,48 @@ def test_a_token_at_a_time():
         for i in range(T):
             a, b = train.gated_mix(x[i], h[i], t["weight"], t["down"], t["last_w"])
             assert torch.equal(a, x2[i]) and torch.equal(b, h2[i])
+
+
+def captured(f):
+    """f() in a graph on a stream of its own: its results and the graph."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = f()
+    torch.cuda.current_stream().wait_stream(side)
+    return out, graph
+
+
+def leaves_of(dt=BF, D=128):
+    g = torch.Generator(device=DEV).manual_seed(1)
+    r = lambda *s, dtype=dt: (0.3 * torch.randn(s, generator=g, device=DEV)).to(dtype)  # noqa: E731
+    return {"x": r(24, D), "m": r(D, D), "w2": r(64, D), "down": r(D, 32), "v": 1 + r(D, dtype=F32), "key": r(160, D), "value": r(D, 160)}
+
+
+def test_captured_backward_past_leaves_that_it_does_not_reach():
+    """A leaf that another graph holds, and whose gradient is not asked for, is no reason to refuse."""
+    case("captured backward passes beside held leaves")
+    t = leaves_of()
+    held = {n: a.detach().requires_grad_(True) for n, a in t.items()}
+    x, m, w2, v = (held[n] for n in ("x", "m", "w2", "v"))
+    calls = {"layer_norm": lambda a: train.layer_norm(a, v, v), "linear": lambda a: train.linear(a, m, activation="sigmoid", residual=x),
+             "gated_linear": lambda a: train.gated_linear(a, w2), "dropout": lambda a: train.dropout(a, 0.3, 5, residual=x),
+             "block_join": lambda a: train.block_join(x, a, v, v, post_weight=v, gate=x, scale=v)[1],
+             "wkv_tail": lambda a: train.wkv_tail(x, a, x, x, v, x, v, v)}
+    for name, f in calls.items():
+        print(f"  {name}", flush=True)
+        eager = f(t["x"])   # holds the nodes of the other leaves
+        assert eager.requires_grad
+        dy = torch.ones_like(eager)
+
+        def go():
+            own = t["x"].detach().requires_grad_(True)
+            return torch.autograd.grad(f(own), own, dy)[0]
+
+        got, graph = captured(go)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, go()), name
+        del eager
