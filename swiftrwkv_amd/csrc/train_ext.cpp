@@ -232,8 +232,8 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // A leaf's gradient belongs to the stream under which its node came to be.  If
 // an eager graph still holds that node, a captured backward pass on another
 // stream would have the engine make the one wait for the other, which the
-// capture does not survive, nor the process.  Looked at are the leaves next to a
-// node, those alone that the pass goes to.
+// capture does not survive, nor the process.  Every node here looks at the leaves
+// next to it, those alone that the pass goes to.
 void capture_ok(const char* what, const Node& node, c10::Device dev) {
     using Stream = c10::hip::HIPStreamMasqueradingAsCUDA;
     const auto captured = [](const Stream& s) {
@@ -302,6 +302,7 @@ struct NormNode : Node {
                      sc = scales.unpack(self);
         const auto dev = st.device();
         const Guard guard(dev);
+        capture_ok("layer_norm", *this, dev);
         Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(shape, st.options().dtype(y_dt));
         const Rows dy = rows_of(dyt, true);
         int64_t ld = D;
@@ -437,6 +438,7 @@ struct LinearNode : Node {
                     "linear: its result has been modified by an inplace operation before the backward pass");
         const auto dev = wt.device();
         const Guard guard(dev);
+        capture_ok("linear", *this, dev);
         const Tensor dyt = grads[0].defined() ? grads[0] : at::zeros(y_shape, wt.options().dtype(y_dt));
         variable_list out(num_outputs());
         if (need_r) out[res_at] = dyt;

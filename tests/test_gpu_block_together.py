@@ -169,6 +169,51 @@ def leaves_of(dt=BF, D=128):
     return {"x": r(24, D), "m": r(D, D), "w2": r(64, D), "down": r(D, 32), "v": 1 + r(D, dtype=F32), "key": r(160, D), "value": r(D, 160)}
 
 
+def test_captured_backward_refuses_every_held_leaf():
+    """Each operator, and the halves of a block where the held leaf is next to a
+    product in their middle: refused by the operator that meets it."""
+    case("captured backward passes over held leaves")
+    t = leaves_of()
+    x, m, w2, down, v = (t[n] for n in ("x", "m", "w2", "down", "v"))
+    on = lambda a: a.detach().requires_grad_(True)  # noqa: E731
+    stream = x.float()
+    calls = {
+        "layer_norm x": ("layer_norm", x, lambda a: train.layer_norm(a, v, v)),
+        "layer_norm bias": ("layer_norm", v, lambda a: train.layer_norm(x, v, a)),
+        "linear x": ("linear", x, lambda a: train.linear(a, m, activation="tanh")),
+        "linear weight": ("linear", m, lambda a: train.linear(x, a)),
+        "linear residual": ("linear", x, lambda a: train.linear(x, m, residual=a)),
+        "gated_mix down": ("linear", down, lambda a: train.gated_mix(stream, x, w2, a, v)[0]),
+        "gated_mix weight": ("gated_linear", w2, lambda a: train.gated_mix(stream, x, a, down, v)[1]),
+        "mix_tail output": ("linear", m, lambda a: train.mix_tail(stream, x, x, x, x, v, x, v, v, a, v)[0]),
+        "mix_tail gate": ("wkv_tail", x, lambda a: train.mix_tail(stream, x, x, x, x, v, a, v, v, m, v)[1]),
+        "channel_mix key": ("linear", t["key"], lambda a: train.channel_mix(stream.reshape(2, 12, 128), v, v, v, a, t["value"])[0]),
+        "channel_mix norm": ("layer_norm", v, lambda a: train.channel_mix(stream.reshape(2, 12, 128), a, v, v, t["key"], t["value"])[0])}
+    for name, (what, leaf, f) in calls.items():
+        print(f"  {name}", flush=True)
+        held = on(leaf)
+        eager = f(held)
+        dy = torch.ones_like(eager)
+
+        def refused():
+            y = f(held)
+            with pytest.raises(RuntimeError, match=f"^{what}: its captured backward pass reaches a leaf"):
+                torch.autograd.grad(y, held, dy)
+
+        captured(refused)
+
+        def go():
+            own = on(leaf)
+            return torch.autograd.grad(f(own), own, dy)[0]
+
+        got, graph = captured(go)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, go()), name
+        assert torch.equal(torch.autograd.grad(eager, held, dy)[0], got), name
+
+
 def test_captured_backward_past_leaves_that_it_does_not_reach():
     """A leaf that another graph holds, and whose gradient is not asked for, is no reason to refuse."""
     case("captured backward passes beside held leaves")
