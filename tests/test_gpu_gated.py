@@ -413,3 +413,47 @@ def test_gates_far_below_zero_pass_nothing(act):
         y = train.gated_linear(a, w, act)
         dx, = torch.autograd.grad(y, a, torch.ones_like(y))
         assert (y.double().abs() <= 2.0 ** -100).all() and (dx.double().abs() <= 2.0 ** -100).all(), (z, y, dx)
+
+
+FEW = [(1, 2050, 65530), (1, 2064, 32768), (2, 2050, 32760), (16, 45, 40), (16, 517, 513), (7, 99, 1027), (1, 33, 2056), (16, 2101, 4096),
+       (10, 2053, 5000), (7, 2059, 7280), (5, 2099, 13099), (16, 300, 8), (3, 5, 7), (1, 4096, 1024), (13, 8200, 1031), (2, 4100, 2055)]
+
+
+def gate_of_whole_numbers(zg, zu, dt):
+    r = zg.clamp(min=0)
+    return ((r * r) * zu).to(dt)   # two fp32 products, as the kernel takes them, and the rounding
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("M,F,K", FEW)
+def test_few_rows_are_two_products(M, F, K, dt):
+    """The kernel of up to sixteen rows, exactly.  First, each z is one value of
+    x: rows of W are zero but for one column, among them the last one, those of
+    the last chunk of 8, of the last 64 and of the last 512."""
+    case(f"gated columns, few rows: {M} x {F} x {K} {dt}")
+    x = torch.randint(-8, 9, (M, K), generator=gen(1), device=DEV).to(dt)
+    at = torch.randint(0, K, (2 * F,), generator=gen(2), device=DEV)
+    for part, size in enumerate((1, 8, 64, 512)):
+        lo = max(0, (K - 1) // size * size)
+        some = torch.arange(part, 2 * F, 8, device=DEV)
+        at[some] = lo + torch.arange(some.numel(), device=DEV) % (K - lo)
+    w = torch.zeros(2 * F, K, device=DEV, dtype=dt)
+    w[torch.arange(2 * F, device=DEV), at] = 1.0
+    y = train.gated_linear(x, w, "relu2")
+    assert torch.equal(y, gate_of_whole_numbers(x[:, at[:F]].float(), x[:, at[F:]].float(), dt))
+
+
+@pytest.mark.parametrize("M,F,K", FEW + [(17, 300, 4096), (40, 100, 16384), (100, 96, 8200), (200, 300, 8192), (700, 3000, 8192), (129, 70, 4099)])
+def test_every_value_of_k_counts(M, F, K):
+    """Whole numbers, whose sums fp32 holds exactly (under 2^24: K·8): a range of K
+    that is left out or taken twice changes them.  bf16, whose range the products
+    stay in; every row and column depends on every k, as nothing is zero."""
+    case(f"gated whole numbers: {M} x {F} x {K}")
+    assert 8 * K < 2 ** 24
+    sign = lambda *s, seed: torch.randint(0, 2, s, generator=gen(seed), device=DEV) * 2 - 1  # noqa: E731
+    x = (torch.randint(1, 9, (M, K), generator=gen(1), device=DEV) * sign(M, K, seed=2)).to(BF)
+    w = sign(2 * F, K, seed=3).to(BF)
+    z = (x.double() @ w.double().t()).float()
+    assert z.abs().max() < 2 ** 24
+    for f in (lambda: train.gated_linear(x, w, "relu2"), lambda: train.gated_linear(x, w.detach().requires_grad_(True), "relu2").detach()):
+        assert torch.equal(f(), gate_of_whole_numbers(z[:, :F], z[:, F:], BF))
