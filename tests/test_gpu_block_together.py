@@ -240,3 +240,52 @@ def test_captured_backward_past_leaves_that_it_does_not_reach():
             torch.cuda.synchronize()
             assert torch.equal(got, go()), name
         del eager
+
+
+@pytest.mark.parametrize("B,T,H,F,dt", [(2, 32, 2, 320, BF), (1, 16, 3, 100, HF)])
+@pytest.mark.parametrize("act", train.GATES)
+def test_every_part_of_both_halves(B, T, H, F, dt, act):
+    """mix_tail and gated_mix with every argument they take, an eps of their own
+    for each norm, large enough that one in another's place shows.  Relative
+    2-norms: at most 24 values are rounded on the way there and back, each off by
+    0.43 half steps in the quadratic mean (a third of the square, over a
+    mantissa's octave); independent, √24·0.43 = 2.1 half steps together.  Twice
+    that, as norms and activations pass some of it on enlarged: 4 half steps."""
+    case(f"block, every part: {B} x {T} x {H} heads x {F} {dt} {act}")
+    D, p, seed = 64 * H, 0.25, 123
+    eps = {"head": 0.3, "next": 0.05, "last": 0.6}
+    t, dx, dh = inputs(B, T, H, F, dt, 5)
+    del t["w"]
+    g = torch.Generator(device=DEV).manual_seed(6)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    t["o"] = 0.4 * r(B, T, D)
+    t["post_w"], t["post_b"], t["scale1"] = 1 + 0.1 * r(D), 0.1 * r(D), 0.5 + 0.1 * r(D)
+    t["gate2"] = torch.sigmoid(r(B, T, D)).to(dt)
+    leaves = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+    a = leaves
+    x, h = train.mix_tail(a["x"], a["o"], a["r"], a["k"], a["v"], a["r_k"], a["gate"], a["ln_w"], a["ln_b"], a["output"], a["next_w"],
+                          a["next_b"], scale=a["scale1"], p=p, seed=seed, offset=3, eps=eps["next"], head_eps=eps["head"])
+    out = train.gated_mix(x, h, a["weight"], a["down"], a["last_w"], a["last_b"], activation=act, post_weight=a["post_w"],
+                          post_bias=a["post_b"], gate=a["gate2"], scale=a["scale"], p=p, seed=seed, offset=4, eps=eps["last"])
+    grads = torch.autograd.grad(out, list(leaves.values()), (dx, dh))
+
+    b = {n: v.detach().double().requires_grad_(True) for n, v in t.items()}
+    q = round(65536 * p)
+    drop = lambda v, off: v * torch.from_numpy(kept(B * T, D, p, seed, off)).to(DEV).reshape(B, T, D) * 65536 / (65536 - q)  # noqa: E731
+    heads = lambda v: v.reshape(B, T, H, 64)  # noqa: E731
+    y = norm(heads(b["o"]), 1.0, 0.0, eps["head"]).flatten(2) * b["ln_w"] + b["ln_b"]
+    y = (y + ((heads(b["r"]) * heads(b["k"]) * b["r_k"]).sum(-1, keepdim=True) * heads(b["v"])).flatten(2)) * b["gate"]
+    x = b["x"] + b["scale1"] * drop(y @ b["output"].t(), 3)
+    zg, zu = (norm(x, b["next_w"], b["next_b"], eps["next"]) @ b["weight"].t()).chunk(2, -1)
+    f = {"relu2": lambda v: v.clamp(min=0) ** 2, "sigmoid": torch.sigmoid, "silu": torch.nn.functional.silu,
+         "gelu_tanh": lambda v: torch.nn.functional.gelu(v, approximate="tanh")}[act]
+    n = norm((f(zg) * zu) @ b["down"].t(), b["post_w"], b["post_b"], eps["last"])
+    x = x + b["scale"] * drop(b["gate2"] * n, 4)
+    ref = x, norm(x, b["last_w"], b["last_b"], eps["last"])
+    want = torch.autograd.grad(ref, list(b.values()), (dx.double(), dh.double()))
+    tol = 4 * torch.finfo(dt).eps / 2
+    rel = lambda a, b: ((a.double() - b).norm() / b.norm()).item()  # noqa: E731
+    for n, got, w in (("x", out[0].detach(), ref[0].detach()), ("h", out[1].detach(), ref[1].detach()),
+                      *(("d" + n, got, w) for n, got, w in zip(leaves, grads, want))):
+        print(f"  {n}: {rel(got, w):.2e} of {tol:.2e}", flush=True)
+        assert got.shape == w.shape and rel(got, w) <= tol, n
