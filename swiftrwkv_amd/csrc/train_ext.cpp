@@ -92,7 +92,7 @@ Tensor tensor_arg(PyObject* o, const char* what, bool optional = false) {
     Tensor t = THPVariable_Unpack(o);
     if (!float_ok(t.scalar_type()))
         raise(PyExc_TypeError, std::string(what) + " must be float32, bfloat16 or float16, got " + type_of(t.scalar_type()));
-    return t;
+    return t.is_neg() ? t.resolve_neg() : t;   // (a view whose memory holds its negative)
 }
 
 // A result without a tangent would read as a derivative of zero; for a
@@ -147,6 +147,7 @@ struct Rows {
 };
 
 Rows rows_of(const Tensor& x, bool dense = false) {
+    if (x.is_neg()) return rows_of(x.detach().resolve_neg(), dense);   // (a gradient; arguments are none)
     const at::IntArrayRef size = x.sizes(), stride = x.strides();
     const int64_t k = x.dim(), D = size[k - 1];
     int64_t N = 1;

@@ -268,3 +268,37 @@ def test_few_rows_copy_no_weights():
         z = x.double() @ w.double().t()
         off = 2.0 ** -24 * (8195 + 32) * (x.double().abs() @ w.double().abs().t())
         assert ((y.double() - z).abs() <= 2.0 ** -8 * z.abs() + off * (1 + 2.0 ** -8)).all()
+
+
+# ───────────────────────────── views that negate ─────────────────────────────
+
+def negating(t):
+    """A tensor of t's values whose memory holds them negated (as the imaginary part of a conjugate does)."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_negating_views():
+    """Arguments and gradients whose memory holds the negated values: results and gradients of plain tensors."""
+    case("views that negate")
+    g = gen(12)
+    t = {n: randn(g, 6, 128, dtype=BF) for n in ("x", "o")}
+    m, w2, v = randn(g, 64, 128, dtype=BF, scale=0.1), randn(g, 64, 128, dtype=BF, scale=0.1), randn(g, 128)
+    res = randn(g, 6, 64)
+    # a leaf for every argument: torch sums the gradients of one that is used thrice in an order of its own
+    calls = {"layer_norm": (train.layer_norm, t["x"], v, v), "gated_linear": (train.gated_linear, t["x"], w2),
+             "linear": (lambda x, m, b, r: train.linear(x, m, b, "tanh", r), t["x"], m, m[:, 0].contiguous(), res),
+             "dropout": (lambda x, r: train.dropout(x, 0.3, 9, residual=r), t["x"], t["o"].float()),
+             "block_join": (lambda x, o, w, b, p, g, s: train.block_join(x, o, w, b, post_weight=p, gate=g, scale=s)[1], t["x"], t["o"], v, v, v,
+                            t["x"], v),
+             "wkv_tail": (train.wkv_tail, *(t["x"], t["o"]) * 2, v.reshape(2, 64), t["o"], v, v)}
+    for name, (f, *args) in calls.items():
+        plain = [a.detach().requires_grad_(True) for a in args]
+        odd = [negating(a).detach().requires_grad_(True) for a in args]
+        y, z = f(*plain), f(*odd)
+        assert torch.equal(y, z), name
+        dy = randn(gen(3), *y.shape, dtype=y.dtype)
+        for a, b in zip(torch.autograd.grad(y, plain, dy), torch.autograd.grad(z, odd, negating(dy))):
+            assert torch.equal(a, b), name
+    assert torch.equal(train.checkpoint8(negating(v[None])).restore(), train.checkpoint8(v[None]).restore())
