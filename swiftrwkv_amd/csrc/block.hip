@@ -1,9 +1,10 @@
 // What a training block does around its recurrence and products, each in one
-// pass over the rows (RWKVBlock.swift:163-307, which the reference forms from
-// MLX operations): dropout from a counter-based generator, the join of one
+// pass over the rows: dropout from a counter-based generator, the join of one
 // block with the next (norm, gate, dropout and scale of the branch, the
 // residual sum, the next norm), and the recurrence's tail (head norm, bonus,
-// gate) with its gradients.
+// gate) with its gradients.  The reference has the tail, the residual sum and
+// the next norm, from MLX operations (RWKVBlock.swift:163-307); dropout and
+// what may stand before the sum in a join are for blocks beside its own.
 //
 //   dropout   y = res + m·x,  dx = m·dy
 //   join      n = LN(o; w1, b1), x' = x + s·m·(g·n), h = LN(x'; w, b)
@@ -326,9 +327,10 @@ __device__ __forceinline__ Raw8<T> filled(float x) {
 
 // Rows first_row(), + gridDim.x·RPB, ...; a thread holds one chunk of 8 columns
 // of a row, and the next row's is on its way.  Bound by bytes: 16384 x 2048, fp32
-// stream, bf16 o and gate, every part: 90 us (5.2 TB/s; a large copy 5.1).  With
-// the next row's loads under a choice, 64-bit addresses and a look at every
-// value of a chunk 112.
+// stream, bf16 o and gate, every part: 90 us (5.2 TB/s; a large copy 5.1); a bf16
+// stream 65 (5.1), and without gate, post norm, scale and dropout 43.  With the
+// next row's loads under a choice, 64-bit addresses and a look at every value of a
+// chunk the first took 112.
 template <typename TS, typename T, int TPR, int ROWS>
 __global__ __launch_bounds__(threads_of(TPR)) void join_fwd_kernel(JoinFwd a) {
     __shared__ float2 part[2][16];
@@ -445,11 +447,12 @@ struct Slots {
 //
 // A chunk is loaded as soon as the one before it has been taken apart, so the
 // next row is on its way under this one's two sums over the row.  The vectors
-// lie in LDS.  The sizes above: 146 us (5.1 TB/s) and the join of the sums 6; with
-// three waves a SIMD instead of two, by launch bounds, registers spilled (327 us
-// where two took 197).  With 1024 threads, which have 128 registers each, the
-// column sums lie in LDS instead, and the vectors and rows are read where they
-// are used: 4096 x 8192 182 us.
+// lie in LDS.  The sizes above, back to back and with the sums' join, 6 us of it: 145
+// us (5.1 TB/s), a bf16 stream 114 (4.7); without gate, post norm, scale and dropout
+// 112 (4.8) and 82 (4.9).  With three waves a SIMD instead of two, by launch bounds,
+// registers spilled (327 us where two took 197).  With 1024 threads, which have 128
+// registers each, the column sums lie in LDS instead, and the vectors and rows are
+// read where they are used: 4096 x 8192 184 us.
 template <typename TS, typename T, int TPR, int ROWS>
 __global__ __launch_bounds__(threads_of(TPR)) void join_bwd_kernel(JoinBwd a) {
     constexpr int RPB = rows_of(TPR);
@@ -706,8 +709,8 @@ struct TailArgs {
 
 // A head is eight neighbouring lanes of 8 columns; TX lanes across, 256 / TX
 // rows down a block, rows strided over gridDim.y, the next one on its way.
-// Bound by bytes: 32768 x 32 heads, o fp32, the rest bf16: 186 us (5.0 TB/s; a
-// large copy 5.1).
+// Bound by bytes: 32768 x 32 heads, o fp32, the rest bf16: 186 us back to back
+// (5.05 TB/s; a large copy 5.1), 200 between a training pass's other kernels.
 template <typename TO, typename T>
 __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
     const int tx = threadIdx.x % TX, col = 8 * (blockIdx.x * TX + tx);
@@ -761,7 +764,8 @@ __global__ __launch_bounds__(256) void tail_fwd_kernel(TailArgs a, int TX) {
 //   dg = dy·q, dq = dy·g, dv = dq·d, e = Σ dq·v, dr = e·k·r_k, dk = e·r·r_k
 //   do = LN'(dq·w; oh, i);  dr_k = Σ e·r·k, dw = Σ dq·oh, db = Σ dq
 // μ and i are formed again: o is read anyway.  Bound by bytes, 26 a value: the
-// same sizes in 330 us (5.3 TB/s), the sums' join 6 of them.
+// same sizes in 313 us (5.6 TB/s) and 5 of the sums' join in a training pass, 324
+// for both back to back.
 template <typename TO, typename T>
 __global__ __launch_bounds__(256) void tail_bwd_kernel(TailArgs a, int TX) {
     __shared__ float sums[8 * 256];
@@ -912,7 +916,8 @@ int join_fwd_blocks(int64_t N, int64_t D) {
 // What the registers hold, each block writing one partial row per column sum; and
 // from 256 blocks on no more than one for four of its rows.  us of the backward
 // pass by 256, 512 and 768 blocks (fp32 stream, bf16, every part): 600 x 2048 18.8,
-// 20.7, 24.7; 2048 x 2048 27.0, 26.4, 33.3; 16384 x 2048 160, 146, 172.
+// 20.7, 24.7; 2048 x 2048 27.0, 26.4, 33.3; 16384 x 2048 160, 146, 172.  (Measured at
+// 2048 columns with every part alone, and taken over for the others.)
 int join_bwd_blocks(int64_t N, int64_t D) {
     const int64_t full = D <= 512 ? 512 : D <= 1024 ? 1024 : D <= 2048 ? 512 : 256;
     const int64_t blocks = (N + join_rows_at_once(D) - 1) / join_rows_at_once(D);

@@ -9,8 +9,9 @@
 //   weight    dW = dzᵀ·x
 //   gated     h  = act(x·Wgᵀ)·(x·Wuᵀ), W = [Wg; Wu] [2F, K]; its gradients are
 //             the input's and the weight's of dz = [dzg | dzu].  16384 x 14336 x
-//             4096 bf16: 2.98 ms forward (1290 TFLOP/s; the tiles' 262 KB each, z in
-//             24 bits, leave all CUs at once and no product runs beside them)
+//             4096 bf16: 2.95 ms forward (1300 TFLOP/s; the tiles' 262 KB each, z in
+//             24 bits, leave all CUs at once and no product runs beside them).  Its
+//             tiles are chosen by the plain product's fitted cost.
 //
 // All three are C[m, n] = Σ_k A[m, k]·B[n, k] over operands that are either
 // k-contiguous (x and W of the forward pass, dz of the input gradient) or
@@ -1578,6 +1579,8 @@ int64_t gated_rows_units(int64_t K) {
 //   1 x 2048 x 16384   32.9, 38.6       8 x 2048 x 8192    20.8, 19.4
 //   1 x 1024 x 16384   22.1, 20.5       1 x 64 x 16384     18.3, 12.3
 //  16 x 2730 x 2048    12.4, 22.2      16 x 512 x 4096     11.9, 10.4
+// (Of these 8 x 2048 x 8192 and 16 x 512 x 4096 go the way that is slower by 1.4 and
+// 1.5 us.)  17 to 128 rows take the tiles: 14336 x 4096 55 to 58 us, W's bytes 46.
 bool gated_rows_applies(int64_t M, int64_t F, int64_t K) {
     return M >= 1 && M <= 16 && gated_rows_units(K) * 512 * M <= GATED_ROWS_X && (K <= 4096 || F >= 2048);
 }

@@ -5,7 +5,8 @@
 // without; here 32 or 55 to 67, by process, most of it torch's engine and its
 // threads, and 5.
 //
-// The reference forms these operators from MLX operations under valueAndGrad
+// Of these operators the reference forms the norms, the dense products, the
+// residual sums and the recurrence's tail from MLX operations under valueAndGrad
 // (RWKVBlock.swift:163-307).
 
 #include <torch/csrc/autograd/function.h>

@@ -3,11 +3,13 @@ MI355X: layer norm, dense products with bias / activation / residual, gated
 products, 8-bit activation checkpoints that their backward passes read,
 dropout, the join of a block with the next, and the recurrence's tail.
 
-The reference forms these from MLX operations and differentiates them with
-MLX's autograd (RWKVBlock.rwkvTmixForward / rwkvCmixForward,
+The reference forms the norms, the dense products, the residual sums and the
+recurrence's tail from MLX operations and differentiates them with MLX's autograd
+(RWKVBlock.rwkvTmixForward / rwkvCmixForward,
 Sources/RWKVModel/RWKVBlock.swift:163-307); here each is hand-written kernels
-behind the C ABI.  channel_mix, mix_tail and gated_mix run them together as
-halves of a block.
+behind the C ABI.  The others are for training on blocks beside the reference's own.
+channel_mix and mix_tail run them together as the halves of RWKV-7's block,
+gated_mix as the half of one with a gated feed-forward.
 
 Tensors live on a ROCm device; results and gradients come back in the types
 of the arguments.  Leading axes are rows, at most 2^24; a last axis that is not
@@ -105,7 +107,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     without one).  Products accumulate in fp32 and the result is rounded once.
     The gradient of z is rounded to x's type before its two products, as they
     run on the matrix cores.  For it an activation keeps 3 bytes per value
-    (bfloat16 relu² without a residual 1, beside y).  keep8:
+    (bfloat16 relu² without a residual 1, beside y); float16 pre-activations past
+    65504 are infinities there, as is their relu²'s gradient.  keep8:
     x and, under an activation, z are kept in 8 bits instead.  With no gradient
     needed nothing is kept.  With more than 128 rows and from M·N·K = 2^30 on, x and
     weight whose rows are not whole 16-byte chunks (K not a multiple of 8, or
