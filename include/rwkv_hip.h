@@ -531,8 +531,9 @@ typedef struct {
 } rwkv_join;
 
 /* xs = x' [N, D] of x_dt, h [N, D] of dt; stats [N, 4] fp32 (mean and rstd of
- * o, 0 and 1 without its norm, and of x'; 16-byte aligned) where not NULL.  xs may be x where ldx = D; no
- * other output may alias an input. */
+ * o, 0 and 1 without its norm, and of x'; 16-byte aligned) where not NULL.  xs may be x where ldx = D,
+ * but not before a backward pass with a 16-bit x_dt, which reads x; no other
+ * output may alias an input. */
 rwkv_status rwkv_join_fwd(const rwkv_join* args, void* xs, void* h, float* stats, void* stream);
 
 /* Gradients from the stats and, with an f32 x_dt, xs as the forward pass wrote it

@@ -819,3 +819,23 @@ def test_rows_of_tiny_values():
     xh = ((X - X.mean(-1, keepdim=True)) / X.var(-1, correction=0, keepdim=True).sqrt()).reshape(5, 1024)
     # 64 squares of a head: right to 2^-15, were they all at the mean's size; a head's largest row of errors is half a step each
     assert ((y.double() - xh * W - B).abs() <= 2.0 ** -15 * (xh * W).abs() + 2.0 ** -22 * (xh * W + B).abs()).all()
+
+
+@pytest.mark.parametrize("sdt,dt", [(F32, BF), (HF, HF)])
+@pytest.mark.parametrize("N,D", [(5, 7), (700, 9), (1500, 1531), (2100, 1000), (1100, 2048), (600, 5001)])
+def test_join_into_its_own_stream(N, D, sdt, dt):
+    """Through the C entry, x' where x is: the same bits."""
+    case(f"join {N} x {D} {sdt} {dt}, x' over x")
+    L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    of = {F32: _lib.F32, BF: _lib.BF16, HF: _lib.F16}
+    x, o, w = randn(gen(1), N, D, dtype=sdt), randn(gen(2), N, D, dtype=dt), ones(gen(3), D, F32)
+    buf, got = [], []
+    for alias in (False, True):
+        a = x.clone()
+        xs, h, st = a if alias else torch.empty_like(x), torch.empty_like(o), torch.empty(N, 4, device=DEV)
+        j = _lib.Join(x=a.data_ptr(), o=o.data_ptr(), ldx=D, ldo=D, x_dt=of[sdt], dt=of[dt], w_dt=_lib.F32, weight=w.data_ptr(),
+                      post_weight=w.data_ptr(), scale=w.data_ptr(), eps=1e-5, post_eps=1e-5, drop=_lib.Drop(SEED, None, OFF, 6554), N=N, D=D)
+        buf.append((a, j))
+        _lib.check(L.rwkv_join_fwd(ctypes.byref(j), xs.data_ptr(), h.data_ptr(), st.data_ptr(), s))
+        got.append((xs, h, st))
+    assert all(torch.equal(p, q) for p, q in zip(*got)) and not torch.equal(got[0][0], x)
