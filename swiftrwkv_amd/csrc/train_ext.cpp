@@ -615,8 +615,8 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ───────────────────────────── gated products ─────────────────────────────
 
-// Keeps x, W, and both pre-activations in 24 bits: kept's 16 are no values of
-// its type but the upper half of fp32's.
+// Keeps x, W, and both pre-activations in 24 bits, as whole numbers: a hook that
+// keeps floating point tensors in another type has no business with patterns.
 struct GatedNode : Node {
     SavedVariable x, w, kept, rem;
     std::vector<int64_t> x_shape, y_shape;
@@ -704,7 +704,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     ysize.back() = F;
     Tensor y = empty(ysize, dt, dev), kept, rem;
     if (train) {
-        kept = empty({M, N}, dt, dev);
+        kept = empty({M, N}, at::kShort, dev);
         rem = empty({M, N}, at::kByte, dev);
     }
     const Ws ws(rwkv_gated_fwd_workspace(M, F, KK), dev);

@@ -457,3 +457,30 @@ def test_every_value_of_k_counts(M, F, K):
     assert z.abs().max() < 2 ** 24
     for f in (lambda: train.gated_linear(x, w, "relu2"), lambda: train.gated_linear(x, w.detach().requires_grad_(True), "relu2").detach()):
         assert torch.equal(f(), gate_of_whole_numbers(z[:, :F], z[:, F:], BF))
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_saved_tensor_hooks(dt):
+    """Hooks that keep floating point tensors in another type leave the kept bits
+    of the pre-activations alone, which are no numbers of x's type: with lossless
+    hooks (float64) nothing changes, with x and W kept in 8 bits behind the point
+    (bfloat16) dx, which reads W, is off by half a step of it, 2^-8, a term."""
+    case(f"gated: saved tensor hooks {dt}")
+    x, w, dy = randn(gen(1), 40, 96, dtype=dt), randn(gen(2), 128, 96, dtype=dt, scale=0.1), randn(gen(3), 40, 64, dtype=dt)
+
+    def grads(to):
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        pack = lambda t: (t.to(to), t.dtype) if to and t.is_floating_point() else (t, t.dtype)  # noqa: E731
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda p: p[0].to(p[1])):
+            y = train.gated_linear(a, b)
+        return torch.autograd.grad(y, (a, b), dy)
+
+    want, same, low = grads(None), grads(torch.float64), grads(torch.bfloat16)
+    assert all(torch.equal(p, q) for p, q in zip(want, same))
+    X, W, DY = x.double(), w.double(), dy.double()
+    zg, zu = (X @ W.t()).chunk(2, 1)
+    v, d, _ = act64("silu", zg)
+    dz = torch.cat([DY * zu * d, DY * v], 1).abs()
+    for p, q, terms in ((want[0], low[0], dz @ W.abs()), (want[1], low[1], dz.t() @ X.abs())):
+        # each side rounds its result too; 2^-7 of the terms holds the operand's half step and theirs
+        assert ((p.double() - q.double()).abs() <= 2.0 ** -7 * terms + 2.0 ** -24).all()
