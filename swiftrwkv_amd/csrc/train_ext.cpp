@@ -229,6 +229,23 @@ Tensor unpack(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, 
     return y;
 }
 
+// What a node keeps of a call.
+struct Saved {
+    Saved() = default;
+    explicit Saved(const Tensor& t, bool output = false) : v(t, output) {}
+    void reset_data() { v.reset_data(); }
+    Tensor unpack(const std::shared_ptr<Node>& node) const { return v.unpack(node); }
+    // for what the kernels take as it lies, as a hook on saved tensors may lay it out
+    // otherwise (rows_of sees to the rest)
+    Tensor dense(const std::shared_ptr<Node>& node) const {
+        const Tensor t = unpack(node);
+        return t.defined() && (!t.is_contiguous() || t.is_neg()) ? t.detach().resolve_neg().contiguous() : t;
+    }
+
+private:
+    SavedVariable v;
+};
+
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // A leaf's gradient belongs to the stream under which its node came to be.  If
@@ -283,7 +300,7 @@ variable_list once(variable_list&& g, const Tensor& dy, const Node& node, const 
 // ───────────────────────────── layer norm ─────────────────────────────
 
 struct NormNode : Node {
-    SavedVariable x, codes, scales, stats, w;
+    Saved x, codes, scales, stats, w;
     std::vector<int64_t> shape;
     at::ScalarType x_dt, y_dt;
     int64_t N, D;
@@ -292,7 +309,7 @@ struct NormNode : Node {
     std::string name() const override { return "LayerNormBackward"; }
 
     void release_variables() override {
-        for (SavedVariable* v : {&x, &codes, &scales, &stats, &w}) v->reset_data();
+        for (Saved* v : {&x, &codes, &scales, &stats, &w}) v->reset_data();
     }
 
     variable_list apply(variable_list&& grads) override {
@@ -300,8 +317,8 @@ struct NormNode : Node {
                    need_b = num_outputs() > 2 && task_should_compute_output(2);
         no_tangent("layer_norm", {&grads[0]});
         const auto self = shared_from_this();
-        const Tensor st = stats.unpack(self), wt = w.unpack(self), xt = x.unpack(self), ct = codes.unpack(self),
-                     sc = scales.unpack(self);
+        const Tensor st = stats.dense(self), wt = w.dense(self), xt = x.unpack(self), ct = codes.dense(self),
+                     sc = scales.dense(self);
         const auto dev = st.device();
         const Guard guard(dev);
         capture_ok("layer_norm", *this, dev);
@@ -389,13 +406,13 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->N = xr.N;
         node->D = D;
         node->keep8 = keep8;
-        if (!keep8) node->x = SavedVariable(xr.t, false);
+        if (!keep8) node->x = Saved(xr.t);
         if (keep8) {
-            node->codes = SavedVariable(c.codes, false);
-            node->scales = SavedVariable(c.scales, false);
+            node->codes = Saved(c.codes);
+            node->scales = Saved(c.scales);
         }
-        node->stats = SavedVariable(st, false);
-        node->w = SavedVariable(wc, false);
+        node->stats = Saved(st);
+        node->w = Saved(wc);
         torch::autograd::set_history(y, node);
     }
     return THPVariable_Wrap(std::move(y));
@@ -414,7 +431,7 @@ constexpr int RELU2 = RWKV_ACT_RELU2;
 // that was changed in place is refused, as torch does for its own, though only
 // the count of its changes is kept.
 struct LinearNode : Node {
-    SavedVariable x, xc, xs, w, kept, rem, zc, zs;
+    Saved x, xc, xs, w, kept, rem, zc, zs;
     c10::VariableVersion y_version;
     int64_t y_was = -1;   // its value after the forward pass, if it is looked at
     std::vector<int64_t> x_shape, y_shape, res_shape;
@@ -426,7 +443,7 @@ struct LinearNode : Node {
     std::string name() const override { return "LinearBackward"; }
 
     void release_variables() override {
-        for (SavedVariable* v : {&x, &xc, &xs, &w, &kept, &rem, &zc, &zs}) v->reset_data();
+        for (Saved* v : {&x, &xc, &xs, &w, &kept, &rem, &zc, &zs}) v->reset_data();
     }
 
     variable_list apply(variable_list&& grads) override {
@@ -466,7 +483,7 @@ struct LinearNode : Node {
         void* const s = stream_of(wt);
         if (need_b) out[bias_at] = empty({N}, dt, dev);
         if (own_z || need_b) {
-            const Tensor k = kept.unpack(self), r = rem.unpack(self), c = zc.unpack(self), sc = zs.unpack(self);
+            const Tensor k = kept.dense(self), r = rem.dense(self), c = zc.dense(self), sc = zs.dense(self);
             check(rwkv_linear_dact(dy.p(), dy.ld, dt_of(y_dt), cptr(k), ptr<uint8_t>(r), from_y,
                                    ptr<int8_t>(c), ptr<uint8_t>(sc), (rwkv_activation)act, own_z ? ptr(dzt) : nullptr,
                                    ldz, need_b ? ptr(out[bias_at]) : nullptr, dt_of(dt), M, N, ws.p(), ws.bytes, s));
@@ -479,7 +496,7 @@ struct LinearNode : Node {
             out[1] = at::zeros({N, K}, wt.options());
         } else if (need_w) {
             // codes hold zeros up to a multiple of 32
-            const Tensor xt = x8 ? unpack(xc.unpack(self), xs.unpack(self), {M, (K + 7) / 8 * 8}, dt) : x.unpack(self);
+            const Tensor xt = x8 ? unpack(xc.dense(self), xs.dense(self), {M, (K + 7) / 8 * 8}, dt) : x.unpack(self);
             const Rows xr = product_rows(xt);   // (columns from K on, of a padded x, are not asked for)
             out[1] = empty({N, K}, dt, dev);
             check(rwkv_linear_wgrad(cptr(dzt), ldz, xr.p(), xr.ld, ptr(out[1]), dt_of(dt), M, N, K, ws.p(), ws.bytes, s));
@@ -586,24 +603,24 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->act = act;
         node->from_y = from_y;
         node->x8 = keep8;
-        node->w = SavedVariable(wr.t, false);
+        node->w = Saved(wr.t);
         if (wants(w)) {
             if (keep8) {
                 const Codes c = pack(x0);
-                node->xc = SavedVariable(c.codes, false);
-                node->xs = SavedVariable(c.scales, false);
+                node->xc = Saved(c.codes);
+                node->xs = Saved(c.scales);
             } else {
-                node->x = SavedVariable(xr.t, false);
+                node->x = Saved(xr.t);
             }
         }
         if (z8) {
-            node->zc = SavedVariable(z.codes, false);
-            node->zs = SavedVariable(z.scales, false);
+            node->zc = Saved(z.codes);
+            node->zs = Saved(z.scales);
         }
-        if (rem.defined()) node->rem = SavedVariable(rem, false);
-        if (aux.defined()) node->kept = SavedVariable(aux, false);
+        if (rem.defined()) node->rem = Saved(rem);
+        if (aux.defined()) node->kept = Saved(aux);
         torch::autograd::set_history(y, node);
-        if (from_y) node->kept = SavedVariable(y, true);
+        if (from_y) node->kept = Saved(y, true);
         if (aux.defined() && act != RELU2 && !res.defined()) {
             node->y_version = y.unsafeGetTensorImpl()->version_counter();
             node->y_was = node->y_version.current_version();
@@ -618,7 +635,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // Keeps x, W, and both pre-activations in 24 bits, as whole numbers: a hook that
 // keeps floating point tensors in another type has no business with patterns.
 struct GatedNode : Node {
-    SavedVariable x, w, kept, rem;
+    Saved x, w, kept, rem;
     std::vector<int64_t> x_shape, y_shape;
     at::ScalarType dt;
     int64_t M, F, K;
@@ -627,14 +644,14 @@ struct GatedNode : Node {
     std::string name() const override { return "GatedLinearBackward"; }
 
     void release_variables() override {
-        for (SavedVariable* v : {&x, &w, &kept, &rem}) v->reset_data();
+        for (Saved* v : {&x, &w, &kept, &rem}) v->reset_data();
     }
 
     variable_list apply(variable_list&& grads) override {
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1);
         no_tangent("gated_linear", {&grads[0]});
         const auto self = shared_from_this();
-        const Tensor wt = w.unpack(self), k = kept.unpack(self), r = rem.unpack(self);
+        const Tensor wt = w.unpack(self), k = kept.dense(self), r = rem.dense(self);
         const auto dev = wt.device();
         const Guard guard(dev);
         capture_ok("gated_linear", *this, dev);
@@ -718,10 +735,10 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->F = F;
         node->K = K;
         node->act = (rwkv_gate)act;
-        node->w = SavedVariable(wr.t, false);
-        if (wants(w)) node->x = SavedVariable(xr.t, false);
-        node->kept = SavedVariable(kept, false);
-        node->rem = SavedVariable(rem, false);
+        node->w = Saved(wr.t);
+        if (wants(w)) node->x = Saved(xr.t);
+        node->kept = Saved(kept);
+        node->rem = Saved(rem);
         torch::autograd::set_history(y, node);
     }
     return THPVariable_Wrap(std::move(y));
@@ -777,7 +794,7 @@ const rwkv_drop drop_of(const rwkv_drop& d, const Tensor& t) {
 
 // Keeps nothing but the numbers' names: the backward pass draws them again.
 struct DropoutNode : Node {
-    SavedVariable seed;
+    Saved seed;
     rwkv_drop drop;
     std::vector<int64_t> shape;
     at::ScalarType x_dt, y_dt;
@@ -838,7 +855,7 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(rwkv_dropout(xr.p(), dt_of(xt), xr.ld, rr.t.defined() ? rr.p() : nullptr, rr.ld, ptr(y), dt_of(yt), &d, xr.N, xr.D,
                        stream_of(x)));
     if (node) {
-        if (drop.seed.defined()) node->seed = SavedVariable(drop.seed, false);
+        if (drop.seed.defined()) node->seed = Saved(drop.seed);
         node->drop = drop.d;
         node->shape = x.sizes().vec();
         node->x_dt = xt;
@@ -883,7 +900,7 @@ at::ScalarType vectors_of(std::initializer_list<Vector*> all, const std::string&
 // gradient; of a 16-bit stream x and o, from which x' is formed again.
 struct JoinNode : Node {
     enum { X, O, GATE, W, B, PW, PB, SC, INPUTS };
-    SavedVariable xs, stats, seed, in[INPUTS];
+    Saved xs, stats, seed, in[INPUTS];
     rwkv_drop drop;
     int at[INPUTS];                              // an input's gradient among the outputs, or -1
     std::vector<int64_t> shape;
@@ -894,16 +911,16 @@ struct JoinNode : Node {
     std::string name() const override { return "BlockJoinBackward"; }
 
     void release_variables() override {
-        for (SavedVariable* v : {&xs, &stats, &seed}) v->reset_data();
-        for (SavedVariable& v : in) v.reset_data();
+        for (Saved* v : {&xs, &stats, &seed}) v->reset_data();
+        for (Saved& v : in) v.reset_data();
     }
 
     variable_list apply(variable_list&& grads) override {
         no_tangent("block_join", {&grads[0], &grads[1]});
         const auto self = shared_from_this();
-        const Tensor x1 = xs.unpack(self), st = stats.unpack(self), sd = seed.unpack(self);
+        const Tensor x1 = xs.dense(self), st = stats.dense(self), sd = seed.unpack(self);
         Tensor t[INPUTS];
-        for (int i = 0; i < INPUTS; ++i) t[i] = in[i].unpack(self);
+        for (int i = 0; i < INPUTS; ++i) t[i] = i < W ? in[i].unpack(self) : in[i].dense(self);
         const auto dev = st.device();
         const Guard guard(dev);
         capture_ok("block_join", *this, dev);
@@ -1001,17 +1018,17 @@ PyObject* py_block_join(PyObject*, PyObject* const* a, Py_ssize_t n) {
         node->D = D;
         node->eps = (float)eps;
         node->post_eps = (float)post_eps;
-        if (drop.seed.defined()) node->seed = SavedVariable(drop.seed, false);
-        node->stats = SavedVariable(st, false);
-        if (xt != at::kFloat || gate.defined() || pw.t.defined() || sc.t.defined()) node->in[JoinNode::O] = SavedVariable(orr.t, false);
-        if (xt != at::kFloat) node->in[JoinNode::X] = SavedVariable(xr.t, false);
-        if (gate.defined()) node->in[JoinNode::GATE] = SavedVariable(g.t, false);
-        node->in[JoinNode::W] = SavedVariable(w.c, false);
-        if (pw.c.defined()) node->in[JoinNode::PW] = SavedVariable(pw.c, false);
-        if (pb.c.defined()) node->in[JoinNode::PB] = SavedVariable(pb.c, false);
-        if (sc.c.defined()) node->in[JoinNode::SC] = SavedVariable(sc.c, false);
+        if (drop.seed.defined()) node->seed = Saved(drop.seed);
+        node->stats = Saved(st);
+        if (xt != at::kFloat || gate.defined() || pw.t.defined() || sc.t.defined()) node->in[JoinNode::O] = Saved(orr.t);
+        if (xt != at::kFloat) node->in[JoinNode::X] = Saved(xr.t);
+        if (gate.defined()) node->in[JoinNode::GATE] = Saved(g.t);
+        node->in[JoinNode::W] = Saved(w.c);
+        if (pw.c.defined()) node->in[JoinNode::PW] = Saved(pw.c);
+        if (pb.c.defined()) node->in[JoinNode::PB] = Saved(pb.c);
+        if (sc.c.defined()) node->in[JoinNode::SC] = Saved(sc.c);
         torch::autograd::set_history(std::vector<Tensor>{xs, h}, node);
-        if (xt == at::kFloat) node->xs = SavedVariable(xs, true);
+        if (xt == at::kFloat) node->xs = Saved(xs, true);
     }
     PyObject* r = PyTuple_New(2);
     if (!r) throw python_error();
@@ -1025,7 +1042,7 @@ PyObject* py_block_join(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 struct TailNode : Node {
     enum { O, R, K, V, GATE, RK, W, B, INPUTS };
-    SavedVariable in[INPUTS];
+    Saved in[INPUTS];
     std::vector<int64_t> shape, rk_shape;
     at::ScalarType o_dt, dt, w_dt;
     int64_t N, H;
@@ -1034,7 +1051,7 @@ struct TailNode : Node {
     std::string name() const override { return "WkvTailBackward"; }
 
     void release_variables() override {
-        for (SavedVariable& v : in) v.reset_data();
+        for (Saved& v : in) v.reset_data();
     }
 
     variable_list apply(variable_list&& grads) override {
@@ -1042,7 +1059,7 @@ struct TailNode : Node {
         const auto self = shared_from_this();
         Tensor t[INPUTS];
         Rows r[RK];
-        for (int i = 0; i < INPUTS; ++i) t[i] = in[i].unpack(self);
+        for (int i = 0; i < INPUTS; ++i) t[i] = i < RK ? in[i].unpack(self) : in[i].dense(self);
         const auto dev = t[O].device();
         const Guard guard(dev);
         capture_ok("wkv_tail", *this, dev);
@@ -1118,10 +1135,10 @@ PyObject* py_wkv_tail(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       rows[0].N, C / 64};
     check(rwkv_tail_fwd(&j, ptr(y), stream_of(o)));
     if (train) {
-        for (int i = 0; i < 5; ++i) node->in[i] = SavedVariable(rows[i].t, false);
-        node->in[TailNode::RK] = SavedVariable(rk.c, false);
-        node->in[TailNode::W] = SavedVariable(w.c, false);
-        node->in[TailNode::B] = SavedVariable(b.c, false);
+        for (int i = 0; i < 5; ++i) node->in[i] = Saved(rows[i].t);
+        node->in[TailNode::RK] = Saved(rk.c);
+        node->in[TailNode::W] = Saved(w.c);
+        node->in[TailNode::B] = Saved(b.c);
         node->shape = o.sizes().vec();
         node->rk_shape = rk0.sizes().vec();
         node->o_dt = ot;

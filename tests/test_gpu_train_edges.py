@@ -302,3 +302,31 @@ def test_negating_views():
         for a, b in zip(torch.autograd.grad(y, plain, dy), torch.autograd.grad(z, odd, negating(dy))):
             assert torch.equal(a, b), name
     assert torch.equal(train.checkpoint8(negating(v[None])).restore(), train.checkpoint8(v[None]).restore())
+
+
+# ───────────────────────────── saved tensors laid out anew ─────────────────────────────
+
+def test_saved_tensors_of_other_strides():
+    """A hook gives back what was saved, equal but with its values two apart in memory: the same gradients."""
+    case("hooks that return other strides")
+    g = gen(14)
+    x, o, dy = (randn(g, 40, 128, dtype=BF) for _ in range(3))
+    m, w2, v = randn(g, 128, 128, dtype=BF, scale=0.1), randn(g, 256, 128, dtype=BF, scale=0.1), randn(g, 128)
+    apart = lambda t: torch.stack([t, torch.ones_like(t)], -1)[..., 0]  # noqa: E731
+    calls = {"layer_norm": (train.layer_norm, x, v, v), "layer_norm keep8": (lambda *a: train.layer_norm(*a, keep8=True), x, v, v),
+             **{f"linear {act} {k8}": (lambda x, m, act=act, k8=k8: train.linear(x, m, None, act, keep8=k8), x, m)
+                for act in train.ACTIVATIONS for k8 in (False, True)},
+             "gated_linear": (train.gated_linear, x, w2), "dropout": (lambda x: train.dropout(x, 0.3, torch.tensor(3, device=DEV)), x),
+             "block_join": (lambda x, o, w, b, p, q, g, s: train.block_join(x, o, w, b, post_weight=p, post_bias=q, gate=g, scale=s, p=0.2)[1],
+                            x.float(), o, v, v, v, v, o, v),
+             "block_join bf16": (lambda x, o, w, s: train.block_join(x, o, w, scale=s)[1], x, o, v, v),
+             "wkv_tail": (train.wkv_tail, x, o, x, o, v, o, v, v)}
+    for name, (f, *args) in calls.items():
+        def grads(unpack):
+            leaves = [a.detach().requires_grad_(True) for a in args]
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = f(*leaves)
+            return torch.autograd.grad(y, leaves, dy)
+
+        for a, b in zip(grads(lambda t: t), grads(apart)):
+            assert torch.equal(a, b), name
