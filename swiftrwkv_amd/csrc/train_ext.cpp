@@ -229,14 +229,21 @@ Tensor unpack(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, 
     return y;
 }
 
-// What a node keeps of a call.
+// What a node keeps of a call.  A hook on saved tensors may give it back laid out
+// otherwise; of another type, shape or device it is refused, before a kernel reads
+// past it.
 struct Saved {
     Saved() = default;
-    explicit Saved(const Tensor& t, bool output = false) : v(t, output) {}
+    explicit Saved(const Tensor& t, bool output = false) : v(t, output), size(t.sizes()), dt(t.scalar_type()), dev(t.device()) {}
     void reset_data() { v.reset_data(); }
-    Tensor unpack(const std::shared_ptr<Node>& node) const { return v.unpack(node); }
-    // for what the kernels take as it lies, as a hook on saved tensors may lay it out
-    // otherwise (rows_of sees to the rest)
+    Tensor unpack(const std::shared_ptr<Node>& node) const {
+        Tensor t = v.unpack(node);
+        TORCH_CHECK(!t.defined() || (t.sizes() == at::IntArrayRef(size) && t.scalar_type() == dt && t.device() == dev), node->name(),
+                    ": a saved tensor came back as ", type_of(t.scalar_type()), " ", shape_of(t), " on ", t.device().str(), ", not ", type_of(dt), " ",
+                    shape_of(size), " on ", dev.str());
+        return t;
+    }
+    // for what the kernels take as it lies (rows_of sees to the rest)
     Tensor dense(const std::shared_ptr<Node>& node) const {
         const Tensor t = unpack(node);
         return t.defined() && (!t.is_contiguous() || t.is_neg()) ? t.detach().resolve_neg().contiguous() : t;
@@ -244,6 +251,9 @@ struct Saved {
 
 private:
     SavedVariable v;
+    c10::SmallVector<int64_t, 4> size;
+    at::ScalarType dt{};
+    c10::Device dev{at::kCPU};
 };
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }

@@ -330,3 +330,24 @@ def test_saved_tensors_of_other_strides():
 
         for a, b in zip(grads(lambda t: t), grads(apart)):
             assert torch.equal(a, b), name
+
+
+def test_saved_tensors_of_another_kind_are_refused():
+    """By the host, before a launch: a saved tensor that a hook gives back on the CPU, shorter or of another type."""
+    case("hooks that return something else")
+    g = gen(15)
+    x, o = randn(g, 6, 128, dtype=BF), randn(g, 6, 128, dtype=BF)
+    m, v = randn(g, 128, 128, dtype=BF), randn(g, 128)
+    calls = {"LayerNorm": lambda a: train.layer_norm(a, v, v), "Linear": lambda a: train.linear(a, m), "GatedLinear": lambda a: train.gated_linear(a, m),
+             "Dropout": lambda a: train.dropout(a, 0.3, torch.tensor(3, device=DEV)), "BlockJoin": lambda a: train.block_join(a, o, v, scale=v)[1],
+             "WkvTail": lambda a: train.wkv_tail(o, a, o, o, v, o, v, v)}
+    others = {"on cpu": lambda t: t.cpu(), "a saved": lambda t: t.reshape(-1)[:1], "came back": lambda t: t.to(torch.float64)}
+    for name, f in calls.items():
+        for msg, unpack in others.items():
+            if name == "Dropout" and msg == "a saved":
+                continue   # the seed is one value anyway
+            a = x.detach().requires_grad_(True)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = f(a)
+            with pytest.raises(RuntimeError, match=f"{name}Backward: a saved tensor came back.*{'on cpu' if msg == 'on cpu' else ''}"):
+                torch.autograd.grad(y, a, torch.ones_like(y))
